@@ -18,6 +18,7 @@ ERR_RUNTIME = 2
 ERR_CUDA = 3
 ERR_DEVICE_TIMEOUT = 4
 ERR_OUT_OF_MEMORY = 5
+ERR_INDEX = 6
 
 PREC = {None: -1, "default": -1, "3xtf32": 0, "tf32": 1}
 
@@ -36,6 +37,8 @@ EXPORTED = [
     "attnb_kv_cache_create", "attnb_kv_cache_destroy", "attnb_kv_cache_length",
     "attnb_kv_cache_truncate", "attnb_kv_cache_append", "attnb_kv_cache_step",
     "attnb_kv_cache_step_dev",
+    "attnb_seq_workspace", "attnb_attn_packed_dev", "attnb_attn_paged_dev",
+    "attnb_kv_pages_append_dev", "attnb_kv_pages_read_dev",
 ]
 
 
@@ -44,6 +47,27 @@ class Tensor(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("H", ctypes.c_int), ("T", ctypes.c_int),
                 ("Dh", ctypes.c_int), ("strideH", ctypes.c_int64), ("strideT", ctypes.c_int64),
                 ("strideDh", ctypes.c_int64)]
+
+
+class Rows(ctypes.Structure):
+    """attnb_rows: data, type, tokens, heads, Dh, strideT, strideH."""
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int), ("tokens", ctypes.c_int),
+                ("heads", ctypes.c_int), ("Dh", ctypes.c_int), ("strideT", ctypes.c_int64),
+                ("strideH", ctypes.c_int64)]
+
+
+class KvPages(ctypes.Structure):
+    """attnb_kv_pages: k, v, k_scale, v_scale, type, num_pages, H, page_size, Dh."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("type", ctypes.c_int), ("num_pages", ctypes.c_int),
+                ("H", ctypes.c_int), ("page_size", ctypes.c_int), ("Dh", ctypes.c_int)]
+
+
+class Seqs(ctypes.Structure):
+    """attnb_seqs: cu, batch, table, table_stride, max_pages, lens."""
+    _fields_ = [("cu", ctypes.c_void_p), ("batch", ctypes.c_int), ("table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int),
+                ("lens", ctypes.c_void_p)]
 
 
 class AttnbError(RuntimeError):
@@ -110,6 +134,12 @@ def lib() -> ctypes.CDLL:
         L.attnb_kv_cache_append.argtypes = [vp, vp, vp, i, vp]
         L.attnb_kv_cache_step.argtypes = [vp, vp, vp, vp, vp]
         L.attnb_kv_cache_step_dev.argtypes = [vp, vp, vp, vp, vp, vp]
+        R, P, S = (ctypes.POINTER(x) for x in (Rows, KvPages, Seqs))
+        L.attnb_seq_workspace.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_size_t)]
+        L.attnb_attn_packed_dev.argtypes = [R, R, R, R, vp, vp, i, i, f, vp, ctypes.c_size_t, vp]
+        L.attnb_attn_paged_dev.argtypes = [R, P, R, S, i, i, f, vp, ctypes.c_size_t, vp]
+        L.attnb_kv_pages_append_dev.argtypes = [R, R, P, S, vp]
+        L.attnb_kv_pages_read_dev.argtypes = [P, R, R, S, vp]
         for name in EXPORTED:
             if name not in ("attnb_last_error", "attnb_version"):
                 getattr(L, name).restype = ctypes.c_int
@@ -424,3 +454,299 @@ class KVCacheDev:
             self.close()
         except Exception:  # interpreter shutdown: the library may be gone
             pass
+
+
+# ------------------------------------------------- ragged sequences, paged KV cache
+_TYPES = None  # torch dtype -> ATTNB_TYPE_*
+
+
+def _type_of(t, name: str) -> int:
+    global _TYPES
+    if _TYPES is None:
+        import torch
+
+        _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
+                  torch.int8: 4}
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{name}: {t.dtype} is not supported") from None
+
+
+def _rows(t, name: str, device) -> Rows:
+    """attnb_rows view of a CUDA tensor [tokens, heads, Dh]."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, Dh]")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    sT, sH, sD = t.stride()
+    if sD != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name} needs a unit stride of the head size")
+    n, h, d = t.shape
+    return Rows(t.data_ptr(), _type_of(t, name), n, h, d, sT, sH)
+
+
+def _offsets(t, name: str, device, n=None) -> int:
+    """Device address of a contiguous int32 vector (of n entries)."""
+    if t.dim() != 1 or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+        raise ValueError(f"{name} must be a contiguous int32 vector")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, one more than sequences for offsets")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr()
+
+
+def _pages(k_pages, v_pages, k_scale, v_scale, device) -> KvPages:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must be [pages, H, page_size, Dh] of one type")
+    n, H, page, Dh = k_pages.shape
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale),
+                    ("v_scale", v_scale)):
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if name.endswith("scale") and (tuple(t.shape) != (n, H, page)
+                                       or str(t.dtype) != "torch.float32"):
+            raise ValueError(f"{name} must be float32 [pages, H, page_size]")
+    return KvPages(k_pages.data_ptr(), v_pages.data_ptr(),
+                   None if k_scale is None else k_scale.data_ptr(),
+                   None if v_scale is None else v_scale.data_ptr(), _type_of(k_pages, "k_pages"),
+                   n, H, page, Dh)
+
+
+def _seqs(cu, table, lens, device) -> Seqs:
+    if table.dim() != 2 or str(table.dtype) != "torch.int32" or table.device != device or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"table must be int32 [sequences, pages] on {device}, rows contiguous")
+    batch = table.shape[0]
+    return Seqs(_offsets(cu, "cu", device, batch + 1), batch, table.data_ptr(), table.stride(0),
+                table.shape[1], _offsets(lens, "lens", device, batch))
+
+
+class _On:
+    """Makes `device` the current one, and `stream` torch's current stream, for
+    the length of a call; .stream is the raw stream to enqueue on.  A workspace
+    that is allocated inside belongs to that stream."""
+
+    def __init__(self, device, stream):
+        import torch
+
+        if device.type != "cuda":
+            raise ValueError("CUDA tensors expected")
+        self._ctx = None
+        if stream is not None:
+            if stream.device != device:
+                raise ValueError(f"stream is on {stream.device}, not on {device}")
+            self._ctx = torch.cuda.stream(stream)
+        elif device.index != torch.cuda.current_device():
+            self._ctx = torch.cuda.device(device)
+
+    def __enter__(self):
+        import torch
+
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        self.stream = torch.cuda.current_stream().cuda_stream
+        return self
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+
+
+_workspace_bytes: dict = {}
+
+
+def _workspace(device, q_heads: int, kv_heads: int, Dh: int):
+    """A fresh workspace from torch's allocator: calls in flight at the same
+    time, and captured graphs, each have their own."""
+    import torch
+
+    key = (device.index, q_heads, kv_heads, Dh)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        size = ctypes.c_size_t()
+        check(lib().attnb_seq_workspace(q_heads, kv_heads, Dh, ctypes.byref(size)))
+        n = _workspace_bytes[key] = size.value
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def attn_packed_dev(Q, K, V, O, cu_q, cu_k=None, causal=False, scale=None, stream=None) -> None:
+    """O = attention of packed sequences (attnb_attn_packed_dev): Q, O [tokens,
+    heads, Dh], K, V [tokens, kv_heads, Dh], float32, bfloat16 or float16 CUDA
+    tensors; sequence b is rows cu_q[b]:cu_q[b+1] of Q and O and cu_k[b]:cu_k[b+1]
+    of K and V (int32; cu_k defaults to cu_q).  causal: the last row of a
+    sequence sees all its keys, each row before it one less.  heads is a
+    multiple of kv_heads.  Rows of O behind cu_q[-1] stay as they are."""
+    dev = Q.device
+    with _On(dev, stream) as on:
+        q, k, v, o = (_rows(t, n, dev) for t, n in ((Q, "Q"), (K, "K"), (V, "V"), (O, "O")))
+        if cu_q.dim() != 1 or cu_q.shape[0] < 1:
+            raise ValueError("cu_q must have one entry more than there are sequences")
+        batch = cu_q.shape[0] - 1
+        cq = _offsets(cu_q, "cu_q", dev)
+        ck = cq if cu_k is None else _offsets(cu_k, "cu_k", dev, batch + 1)
+        if k.heads == 0 or q.heads % k.heads:
+            raise ValueError("Q heads must be a multiple of the KV heads")
+        ws, n = _workspace(dev, q.heads, k.heads, q.Dh)
+        check(lib().attnb_attn_packed_dev(q, k, v, o, cq, ck, batch, int(causal),
+                                          0.0 if scale is None else _scale(scale), ws.data_ptr(),
+                                          n, on.stream))
+
+
+def _scale(scale) -> float:
+    if not scale > 0:
+        raise ValueError("scale must be positive")
+    return float(scale)
+
+
+def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=True, scale=None,
+                   k_scale=None, v_scale=None, stream=None) -> None:
+    """O = attention of new tokens over a paged cache (attnb_attn_paged_dev): Q,
+    O [tokens, heads, Dh]; k_pages, v_pages [pages, kv_heads, page_size, Dh] of
+    Q's type, or float8_e4m3fn or int8 codes with k_scale, v_scale [pages,
+    kv_heads, page_size]; sequence b is rows cu[b]:cu[b+1] of Q, the last of the
+    lens[b] tokens in pages table[b] (all int32).  max_new: the most rows of one
+    sequence, where the caller knows it; it only steers the choice of kernel."""
+    dev = Q.device
+    with _On(dev, stream) as on:
+        q, o = _rows(Q, "Q", dev), _rows(O, "O", dev)
+        pg = _pages(k_pages, v_pages, k_scale, v_scale, dev)
+        sq = _seqs(cu, table, lens, dev)
+        if pg.H == 0 or q.heads % pg.H:
+            raise ValueError("Q heads must be a multiple of the KV heads")
+        ws, n = _workspace(dev, q.heads, pg.H, q.Dh)
+        check(lib().attnb_attn_paged_dev(q, pg, o, sq, max_new, int(causal),
+                                         0.0 if scale is None else _scale(scale), ws.data_ptr(),
+                                         n, on.stream))
+
+
+def kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale=None, v_scale=None,
+                        stream=None) -> None:
+    """Write new tokens K, V [tokens, kv_heads, Dh] into the pages, quantising
+    them for float8_e4m3fn and int8 pages (attnb_kv_pages_append_dev); lens
+    counts them already.  Other arguments as in attn_paged_dev."""
+    dev = K.device
+    with _On(dev, stream) as on:
+        check(lib().attnb_kv_pages_append_dev(
+            _rows(K, "K", dev), _rows(V, "V", dev), _pages(k_pages, v_pages, k_scale, v_scale, dev),
+            _seqs(cu, table, lens, dev), on.stream))
+
+
+def kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale=None, v_scale=None,
+                      stream=None) -> None:
+    """Read the last cu[b+1] - cu[b] tokens of each sequence out of the pages
+    into K, V [tokens, kv_heads, Dh] (attnb_kv_pages_read_dev)."""
+    dev = K.device
+    with _On(dev, stream) as on:
+        check(lib().attnb_kv_pages_read_dev(
+            _pages(k_pages, v_pages, k_scale, v_scale, dev), _rows(K, "K", dev),
+            _rows(V, "V", dev), _seqs(cu, table, lens, dev), on.stream))
+
+
+class PagedKVCacheDev:
+    """A K/V cache for `batch` sequences in one pool of pages, the ragged
+    counterpart of KVCacheDev: ``append`` gives each sequence the pages it needs
+    and writes its new tokens (quantising them for dtype torch.float8_e4m3fn or
+    torch.int8), ``attend`` runs the new tokens' queries over everything held.
+    Page numbers and lengths are kept on the host and copied to the device when
+    they change; work is enqueued on ``stream`` (default: torch's current one)."""
+
+    def __init__(self, batch: int, H: int, Dh: int, num_pages: int, page_size: int = 64,
+                 dtype=None, max_tokens: int | None = None, device=None):
+        import torch
+
+        if batch <= 0 or num_pages <= 0:
+            raise ValueError("batch and num_pages must be positive")
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError("page_size must be 16, 32, 64 or 128")
+        dtype = torch.bfloat16 if dtype is None else dtype
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None \
+            else torch.device(device)
+        self.batch, self.H, self.Dh, self.page_size = batch, H, Dh, page_size
+        self.k_pages, self.v_pages = (torch.empty(num_pages, H, page_size, Dh, dtype=dtype,
+                                                  device=device) for _ in range(2))
+        self.k_scale = self.v_scale = None
+        if dtype in (torch.float8_e4m3fn, torch.int8):
+            self.k_scale, self.v_scale = (torch.empty(num_pages, H, page_size, device=device)
+                                          for _ in range(2))
+        most = num_pages * page_size if max_tokens is None else max_tokens
+        width = max(1, -(-most // page_size))
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._held = [[] for _ in range(batch)]
+        self.lengths = [0] * batch
+        self.table = torch.zeros(batch, width, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._new = None
+
+    def append(self, k, v, new, stream=None) -> None:
+        """k, v: the new tokens of all sequences, packed [sum(new), H, Dh]; new:
+        how many each sequence brings (a list of ints)."""
+        import torch
+
+        new = [int(n) for n in new]
+        if len(new) != self.batch or any(n < 0 for n in new):
+            raise ValueError("new must give a count for each sequence")
+        if k.shape[0] != sum(new) or v.shape[0] != sum(new):
+            raise ValueError("k and v must hold sum(new) tokens")
+        want = [-(-(n + m) // self.page_size) for n, m in zip(self.lengths, new)]
+        if any(w > self.table.shape[1] for w in want):
+            raise ValueError("a sequence would outgrow max_tokens")
+        if sum(want) - sum(len(h) for h in self._held) > len(self._free):
+            raise ValueError("the pool has too few free pages")
+        with _On(self.table.device, stream):
+            grew = False
+            for held, w in zip(self._held, want):
+                while len(held) < w:
+                    held.append(self._free.pop())
+                    grew = True
+            self.lengths = [n + m for n, m in zip(self.lengths, new)]
+            dev = self.table.device
+            if grew:
+                width = self.table.shape[1]
+                self.table.copy_(torch.tensor([h + [0] * (width - len(h)) for h in self._held],
+                                              dtype=torch.int32))
+            self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+            cu = [0]
+            for n in new:
+                cu.append(cu[-1] + n)
+            self._new, self.cu = new, torch.tensor(cu, dtype=torch.int32, device=dev)
+            if cu[-1]:
+                kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
+                                    self.lens, self.k_scale, self.v_scale)
+
+    def attend(self, q, o, causal=True, scale=None, stream=None) -> None:
+        """o = attention of q [sum(new), heads, Dh], the queries of the tokens
+        appended last, over their sequences."""
+        if self._new is None:
+            raise ValueError("append first: the queries belong to the tokens appended last")
+        if q.shape[0] != sum(self._new):
+            raise ValueError("q must hold one row for each token appended last")
+        attn_paged_dev(q, self.k_pages, self.v_pages, o, self.cu, self.table, self.lens,
+                       max(self._new), causal, scale, self.k_scale, self.v_scale, stream)
+
+    def read(self, b: int, k, v, stream=None) -> None:
+        """The tokens of sequence b into k, v [lengths[b], H, Dh]."""
+        import torch
+
+        if k.shape[0] != self.lengths[b] or v.shape[0] != self.lengths[b]:
+            raise ValueError("k and v must hold the sequence's tokens")
+        with _On(self.table.device, stream):
+            cu = torch.tensor([0, self.lengths[b]], dtype=torch.int32, device=self.table.device)
+            kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1],
+                              self.lens[b:b + 1], self.k_scale, self.v_scale)
+
+    def truncate(self, b: int, length: int) -> None:
+        """Keep the first `length` tokens of sequence b (0 gives all its pages
+        back); takes effect with the next append."""
+        if not 0 <= length <= self.lengths[b]:
+            raise ValueError("length must be in [0, current length]")
+        keep = -(-length // self.page_size)
+        self._free.extend(reversed(self._held[b][keep:]))
+        del self._held[b][keep:]
+        self.lengths[b] = length
+        self._new = None

@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "entry.h"
 #include "kernels.h"
 #include "runtime.h"
 
@@ -22,26 +23,6 @@ int profile_read(const char* kernel, double* total_ms, int* launches);
 using namespace attnb;
 
 namespace {
-
-// Runs an entry point's body inside an NVTX range named after the entry point
-// (visible in Nsight timelines; free when no tool is attached) and turns its
-// exceptions into a status code plus the thread's last-error message.
-template <class F>
-int guarded(const char* name, F&& f) {
-  NvtxRange range(name);
-  try {
-    f();
-    return ATTNB_OK;
-  } catch (const Error& e) {
-    return set_last_error(e.code, e.msg);
-  } catch (const std::exception& e) {
-    return set_last_error(ATTNB_ERR_RUNTIME, e.what());
-  } catch (...) {
-    return set_last_error(ATTNB_ERR_RUNTIME, "unknown error");
-  }
-}
-
-cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 // ------------------------------------------------------------- validation
 // attn::validate_dense_shapes, include/attn.h:54-83 of the reference.
@@ -422,8 +403,12 @@ int attnb_host_free(void* ptr) {
 int attnb_stream_status(void* stream) {
   return guarded(__func__, [&] {
     DeviceCtx& c = current_ctx();
-    if (consume_status(c, as_stream(stream)) != ATTNB_OK)
-      fail(ATTNB_ERR_DEVICE_TIMEOUT, "a bounded device wait expired");
+    const int rc = consume_status(c, as_stream(stream));
+    const bool index = consume_index_status(c);  // both words are cleared
+    if (rc != ATTNB_OK) fail(ATTNB_ERR_DEVICE_TIMEOUT, "a bounded device wait expired");
+    if (index)
+      fail(ATTNB_ERR_INDEX, "a page number or a sequence length was out of range; the places it "
+                            "names were left alone or read as zeros");
   });
 }
 

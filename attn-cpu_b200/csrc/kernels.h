@@ -197,4 +197,75 @@ size_t gemm_packed_bytes(int rows, int K, bool split3);
 void gemm_pack_b(const float* B, int64_t ldb, bool b_kmajor, int N, int K, bool split3,
                  float* hi, float* lo, int num_sms, cudaStream_t s);
 
+// ------------------------------- ragged sequences and the paged KV cache
+// Element types (the values of ATTNB_TYPE_* in attnb.h).
+enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2, kE4M3 = 3, kI8 = 4 };
+inline int elem_bytes(int t) { return t == kF32 ? 4 : (t == kBF16 || t == kF16) ? 2 : 1; }
+inline bool elem_coded(int t) { return t == kE4M3 || t == kI8; }  // codes with a scale per vector
+
+// Pages [num_pages, H, 1 << page_shift, Dh] of K and of V; for coded types the
+// scales are [num_pages, H, 1 << page_shift].
+struct KvPages {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int type, num_pages, H, page_shift, Dh;
+};
+// Sequence b owns rows [cu[b], cu[b+1]) of the packed tokens, its tokens'
+// pages are table[b * table_stride + i], i < max_pages, and it holds lens[b]
+// tokens, the packed ones last.
+struct SeqTable {
+  const int32_t* cu;
+  int batch, total;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages;
+  const int32_t* lens;
+};
+// Packed rows [tokens, heads, Dh] (element strides; Dh contiguous).
+struct RowsView {
+  void* data;
+  int type;
+  int tokens, heads, Dh;
+  int64_t sT, sH;
+};
+
+// K5 (kv_pages.cu): write the packed tokens K, V into their pages, quantising
+// for coded types; read the packed tokens' places back into K, V.
+void kv_pages_append_launch(const RowsView& K, const RowsView& V, const KvPages& pg,
+                            const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s);
+void kv_pages_read_launch(const KvPages& pg, const RowsView& K, const RowsView& V,
+                          const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s);
+
+// Attention of packed query rows over packed keys (pages.k == nullptr) or over
+// pages.  One launch of a K6-K8 kernel works through the items of the schedule
+// in seq.cuh, a second one joins the items that several CTAs shared.
+struct SeqAttnArgs {
+  RowsView q, o, k, v;  // k, v: packed keys only
+  const int32_t* cu_k;  // packed keys only
+  KvPages pages;
+  SeqTable seqs;        // seqs.cu: the query rows; table and lens with pages
+  int G;                // query heads per KV head
+  int causal;
+  float scale_log2;     // softmax scale times log2(e)
+  // Schedule: rows per item, log2 of the keys per tile, fewest tiles per CTA.
+  int rows, kt_shift, min_tiles;
+  // Workspace: partial O [2 * ctas][rows][Dh], (m, l) [2 * ctas][rows], one
+  // SeqSplit per CTA.
+  float* ws_o;
+  float* ws_ml;
+  void* ws_split;
+  int* index_status;
+  int* status;
+};
+// Bytes of workspace that any attention call with these heads may need.
+size_t seq_workspace_bytes(int G, int Dh, int num_sms);
+// max_new: the caller's bound on the query rows of one sequence (0: unknown);
+// it only steers the choice of kernel.
+void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
+                  cudaStream_t s);
+
+// The kernels (K6: any type, stride and head size up to 256).
+void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+void seq_merge_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+
 }  // namespace attnb

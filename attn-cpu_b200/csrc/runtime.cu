@@ -107,10 +107,12 @@ DeviceCtx& current_ctx() {
   // the bus, and the host reads it once the stream is synchronised -- no copy
   // on the normal path (a 4-byte device-to-host copy cost each host-pointer
   // call about 6 us).
-  ATTNB_CUDA(cudaHostAlloc(&c->status_host, sizeof(int),
+  ATTNB_CUDA(cudaHostAlloc(&c->status_host, 2 * sizeof(int),
                            cudaHostAllocMapped | cudaHostAllocPortable));
-  *c->status_host = 0;
+  c->index_status_host = c->status_host + 1;
+  *c->status_host = *c->index_status_host = 0;
   ATTNB_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&c->status), c->status_host, 0));
+  c->index_status = c->status + 1;
   DeviceCtx& ref = *c;
   g_ctx.emplace(dev, std::move(c));
   return ref;
@@ -302,6 +304,14 @@ int consume_status(DeviceCtx& c, cudaStream_t stream) {
     return ATTNB_ERR_DEVICE_TIMEOUT;
   }
   return ATTNB_OK;
+}
+
+bool consume_index_status(DeviceCtx& c) {
+  std::lock_guard<std::mutex> g(c.status_mu);
+  volatile int* word = c.index_status_host;
+  const bool met = *word != 0;
+  if (met) *word = 0;
+  return met;
 }
 
 // ------------------------------------------------------ pinned host pool

@@ -49,7 +49,9 @@ struct DeviceCtx {
   cudaStream_t stream = nullptr;  // used by the host-pointer entry points
   int* status = nullptr;          // status word as kernels see it (1: a wait timed out)
   int* status_host = nullptr;     // the same word: page-locked host memory, mapped
-  std::mutex status_mu;           // guards reading and clearing it
+  int* index_status = nullptr;    // second status word: a kernel met an index out of range
+  int* index_status_host = nullptr;
+  std::mutex status_mu;           // guards reading and clearing them
   std::mutex mu;                  // serialises host-pointer calls on this device
   DeviceBuffer io;                // device copies of host inputs/outputs
   DeviceBuffer scratch_host_path; // kernel scratch for host-pointer calls
@@ -123,6 +125,9 @@ void selftest_wait_timeout(DeviceCtx& c, int limit_us, cudaStream_t s);
 
 // Reads and clears the device status word of ctx (synchronises `stream`).
 int consume_status(DeviceCtx& c, cudaStream_t stream);
+// Reads and clears the index word (the caller has synchronised): whether a
+// kernel met a page number or a length out of range since the last call.
+bool consume_index_status(DeviceCtx& c);
 
 // Page-locked host blocks for results handed to callers (attnb_host_alloc):
 // power-of-two size classes from 4 KiB, recycled on free, at most

@@ -42,6 +42,7 @@ extern "C" {
 #define ATTNB_ERR_CUDA 3             /* a CUDA runtime/driver call failed */
 #define ATTNB_ERR_DEVICE_TIMEOUT 4   /* a bounded in-kernel wait expired */
 #define ATTNB_ERR_OUT_OF_MEMORY 5    /* device memory could not be had: std::bad_alloc */
+#define ATTNB_ERR_INDEX 6            /* a kernel met a page number or length out of range */
 
 /* Device memory.  Scratch (packed operands, split partials) and the device
  * copies of host-pointer calls' data live in per-device arenas that grow on
@@ -84,8 +85,8 @@ typedef struct attnb_mtensor {
 ATTNB_API const char* attnb_last_error(void);
 /* Library version string, e.g. "attnb 0.1 sm_100a". */
 ATTNB_API const char* attnb_version(void);
-/* Device status word of `stream`'s device: ATTNB_OK or ATTNB_ERR_DEVICE_TIMEOUT
- * (and clears it).  Synchronises the stream. */
+/* Device status of `stream`'s device: ATTNB_OK, ATTNB_ERR_DEVICE_TIMEOUT or
+ * ATTNB_ERR_INDEX (and clears it).  Synchronises the stream. */
 ATTNB_API int attnb_stream_status(void* stream);
 /* Self-test of the failure path (no counterpart in the reference): enqueues a
  * kernel whose bounded wait on a barrier that nothing arrives on expires after
@@ -325,6 +326,96 @@ ATTNB_API int attnb_mha_block_dense(const float* x, int T, int D, const float* W
 ATTNB_API int attnb_mha_block_dense_dev(const float* x, int batch, int T, int D, const float* W_in,
                               const float* b_in, const float* W_out, const float* b_out,
                               int H, int causal, float* y, int precision, void* stream);
+
+/* ------------------------------------- ragged sequences, paged KV cache */
+/* Serving operators over sequences of different lengths (no counterpart in
+ * the reference, which takes one dense fp32 problem per call).  Device
+ * pointers only; every length, offset and page number below is read on the
+ * device, so the calls can be captured into a CUDA graph and replayed with
+ * other values.  What is out of range there leads to no access out of range:
+ * offsets are clamped to the packed rows, and a page number outside
+ * [0, num_pages), or a length that is negative or more than the table's pages
+ * hold, reads as zeros or is not written, and the next attnb_stream_status
+ * reports ATTNB_ERR_INDEX. */
+#define ATTNB_TYPE_F32 0
+#define ATTNB_TYPE_BF16 1
+#define ATTNB_TYPE_F16 2
+#define ATTNB_TYPE_E4M3 3 /* pages only: 8-bit floating-point codes with a scale per vector */
+#define ATTNB_TYPE_I8 4   /* pages only: 8-bit integer codes with a scale per vector */
+
+/* Packed rows [tokens, heads, Dh] of F32, BF16 or F16, Dh contiguous
+ * (1 <= Dh <= 256); strides in elements.  Outputs need rows that do not
+ * overlap. */
+typedef struct attnb_rows {
+  void* data;
+  int type;
+  int tokens, heads, Dh;
+  int64_t strideT, strideH;
+} attnb_rows;
+
+/* The pages of a KV cache: k and v are [num_pages, H, page_size, Dh], dense,
+ * page_size 16, 32, 64 or 128.  E4M3 and I8 pages hold codes; their scales are
+ * [num_pages, H, page_size], NULL for the other types. */
+typedef struct attnb_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int type;
+  int num_pages, H, page_size, Dh;
+} attnb_kv_pages;
+
+/* `batch` sequences: packed rows [cu[b], cu[b+1]) belong to sequence b (cu has
+ * batch + 1 entries; rows behind cu[batch] belong to none and are neither read
+ * nor written).  Sequence b holds lens[b] tokens, its packed rows the last of
+ * them; token p lies in page table[b * table_stride + p / page_size], which
+ * must be one of the first max_pages entries of the row. */
+typedef struct attnb_seqs {
+  const int32_t* cu;
+  int batch;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages;
+  const int32_t* lens;
+} attnb_seqs;
+
+/* Bytes of device workspace for the two attention calls below, enough for any
+ * number of sequences and tokens with these head counts on the current device.
+ * Calls that may run at the same time need workspaces of their own. */
+ATTNB_API int attnb_seq_workspace(int q_heads, int kv_heads, int Dh, size_t* bytes);
+
+/* Attention over packed sequences: query row i of sequence b attends to that
+ * sequence's keys, rows [cu_k[b], cu_k[b+1]) of K and V.  With causal != 0 its
+ * last row sees every key and each row before it one key less.  Query head h
+ * reads KV head h / (Q.heads / K.heads); a row that sees no key gives zeros.
+ * Q, K, V and O have one type; scale <= 0 means 1 / sqrt(Dh). */
+ATTNB_API int attnb_attn_packed_dev(const attnb_rows* Q, const attnb_rows* K, const attnb_rows* V,
+                                    const attnb_rows* O, const int32_t* cu_q,
+                                    const int32_t* cu_k, int batch, int causal, float scale,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Writes the packed rows K and V (one type, page H heads each) to their places
+ * in the pages.  Pages of the rows' own type take them as they are.  E4M3 and
+ * I8 pages take round(x * C / a) with a = max|x| over the vector and C = 448
+ * or 127, ties to even, and the scale a / C; a vector of zeros has scale 0, and
+ * one that holds an infinity or a NaN has scale NaN. */
+ATTNB_API int attnb_kv_pages_append_dev(const attnb_rows* K, const attnb_rows* V,
+                                        const attnb_kv_pages* pages, const attnb_seqs* seqs,
+                                        void* stream);
+/* Reads the places of the packed rows (the last cu[b+1] - cu[b] tokens of each
+ * sequence) out of the pages into K and V. */
+ATTNB_API int attnb_kv_pages_read_dev(const attnb_kv_pages* pages, const attnb_rows* K,
+                                      const attnb_rows* V, const attnb_seqs* seqs, void* stream);
+
+/* Attention of the packed rows (new tokens, one and up per sequence) over the
+ * lens[b] tokens that the pages hold, their own among them (append first);
+ * otherwise as attnb_attn_packed_dev.  Q and O have one type; the pages have
+ * that type or are E4M3 or I8.  max_new: the most rows of one sequence, as far
+ * as the caller knows (0: unknown); it steers the choice of kernel only. */
+ATTNB_API int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pages,
+                                   const attnb_rows* O, const attnb_seqs* seqs, int max_new,
+                                   int causal, float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
