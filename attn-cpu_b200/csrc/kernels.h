@@ -266,6 +266,12 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
 
 // The kernels (K6: any type, stride and head size up to 256).
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
-void seq_merge_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+// K7: 16-bit queries over 16-bit or coded pages, 16 rows per item.
+bool seq_mma_supported(const SeqAttnArgs& a);
+void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+// Whether TMA can read the pages, and the map of one of the two pools with
+// copies of up to `rows` rows of one page.
+bool seq_pages_tma(const SeqAttnArgs& a);
+CUtensorMap seq_pages_map(const KvPages& p, const void* base, int rows);
 
 }  // namespace attnb

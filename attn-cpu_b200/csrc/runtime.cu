@@ -223,6 +223,36 @@ CUtensorMap make_tmap_3d(const float* base, uint64_t depth, uint64_t rows, uint6
   return m;
 }
 
+CUtensorMap make_tmap_nd(const void* base, int elem_bytes, int rank, const uint64_t* dims,
+                         const uint64_t* strides, const uint32_t* box) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
+    fail(ATTNB_ERR_RUNTIME, "TMA base address is not 16-byte aligned");
+  if (box[0] * elem_bytes != 128 || rank < 2 || rank > 5)
+    fail(ATTNB_ERR_RUNTIME, "TMA box must be 128 bytes wide, of rank 2 to 5");
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    es[i] = 1;
+    if (box[i] == 0 || box[i] > 256) fail(ATTNB_ERR_RUNTIME, "TMA box out of range");
+    if (i + 1 < rank) {
+      st[i] = strides[i];
+      if (strides[i] % 16 != 0) fail(ATTNB_ERR_RUNTIME, "TMA pitch is not 16-byte aligned");
+    }
+  }
+  CUtensorMap m;
+  std::memset(&m, 0, sizeof(m));
+  const CUresult r = encode_fn()(
+      &m, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, rank,
+      const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    fail(ATTNB_ERR_CUDA, "cuTensorMapEncodeTiled (n-D) failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
 static std::atomic<bool> g_prof_on{false};
 static std::mutex g_prof_mu;
 static std::map<std::string, std::vector<std::pair<cudaEvent_t, cudaEvent_t>>> g_prof;

@@ -105,6 +105,12 @@ CUtensorMap make_tmap_2d(const float* base, uint64_t rows, uint64_t cols, uint64
 CUtensorMap make_tmap_3d(const float* base, uint64_t depth, uint64_t rows, uint64_t cols,
                          uint64_t ld, uint64_t ld_depth, uint32_t box_rows, uint32_t box_cols);
 
+// Tensor map of `rank` dimensions (innermost first; strides in bytes, of every
+// dimension but the innermost) for elements of 1 or 2 bytes, 128-byte swizzle;
+// out-of-range elements read as 0.
+CUtensorMap make_tmap_nd(const void* base, int elem_bytes, int rank, const uint64_t* dims,
+                         const uint64_t* strides, const uint32_t* box);
+
 // CUDA-event timing of the dominant kernel of each call (attnb_profile_*):
 // construct before the launch, destroy after it, on the launching stream.
 class ProfScope {

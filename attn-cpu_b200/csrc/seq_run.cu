@@ -1,0 +1,90 @@
+// seq_run.cu -- choice of kernel and workspace for attention over ragged
+// sequences, and the join of the items that several CTAs shared.
+#include <algorithm>
+#include <cmath>
+
+#include "runtime.h"
+#include "seq.cuh"
+#include "seq_elem.cuh"
+
+namespace attnb {
+namespace {
+
+// Joins the pieces of each item that a cut fell into: block c the item that
+// goes on in CTA c, if it began in CTA c - 1.
+template <int T>
+__global__ void __launch_bounds__(128) seq_merge_kernel(const SeqAttnArgs a) {
+  using E = elem_t<T>;
+  grid_dep_wait();
+  const int c = blockIdx.x + 1;
+  const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];
+  if (!d.continues || d.item0 < (c - 1) * d.quota) return;
+  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1;
+  const int slot0 = 2 * (c - 1) + (d.item0 == (c - 1) * d.quota ? 0 : 1);
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
+  const int Dh = a.q.Dh;
+  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
+    float top = ml[(int64_t)slot0 * a.rows + r].x;
+    for (int i = c; i <= last; ++i) top = fmaxf(top, ml[(int64_t)2 * i * a.rows + r].x);
+    const int row = d.first_row + r;
+    E* o = static_cast<E*>(a.o.data) + (int64_t)(d.row_token + row / a.G) * a.o.sT +
+           (int64_t)(d.kv_head * a.G + row % a.G) * a.o.sH;
+    for (int x = threadIdx.x; x < Dh; x += blockDim.x) {
+      float sum = 0.f, acc = 0.f;
+      for (int i = c - 1; i <= last; ++i) {
+        const int64_t at = (int64_t)(i < c ? slot0 : 2 * i) * a.rows + r;
+        const float2 p = ml[at];
+        const float f = p.x == -INFINITY ? 0.f : fast_exp2(p.x - top);
+        sum = fmaf(f, p.y, sum);
+        acc = fmaf(f, a.ws_o[at * Dh + x], acc);
+      }
+      from_float(sum == 0.f ? 0.f : acc / sum, o[x]);
+    }
+  }
+}
+
+// What a kernel takes from the workspace: two partial results and a SeqSplit
+// per CTA.
+struct Space {
+  int rows, ctas;
+  size_t bytes(int Dh) const {
+    return (size_t)ctas * (2 * rows * ((size_t)Dh * 4 + 8) + sizeof(SeqSplit)) + 64;
+  }
+};
+Space simt_space(int Dh, int num_sms) { return {Dh <= 128 ? 4 : 2, 2 * num_sms}; }
+Space mma_space(int num_sms) { return {16, 2 * num_sms}; }
+
+}  // namespace
+
+size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
+  (void)G;
+  return std::max(simt_space(Dh, num_sms).bytes(Dh), mma_space(num_sms).bytes(Dh)) + 256;
+}
+
+void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
+                  cudaStream_t s) {
+  (void)max_new;
+  if (a.seqs.batch == 0 || a.seqs.total == 0) return;
+  const bool mma = seq_mma_supported(a);
+  const Space sp = mma ? mma_space(num_sms) : simt_space(a.q.Dh, num_sms);
+  a.rows = sp.rows;
+  a.kt_shift = 6;
+  a.min_tiles = 2;
+  uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
+  if (p + sp.bytes(a.q.Dh) > reinterpret_cast<uintptr_t>(ws) + ws_bytes)
+    fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
+  a.ws_split = reinterpret_cast<void*>(p);
+  p += sp.ctas * sizeof(SeqSplit);
+  a.ws_ml = reinterpret_cast<float*>(p);
+  p += (size_t)2 * sp.ctas * sp.rows * 8;
+  a.ws_o = reinterpret_cast<float*>(p);
+  if (mma) seq_mma_launch(a, sp.ctas, s);
+  else seq_simt_launch(a, sp.ctas, s);
+  // Joins what the cuts between CTAs split.
+  with_value_type(a.o.type, [&](auto t) {
+    ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
+                          dim3(sp.ctas - 1, std::min(a.rows, 16)), dim3(128), 0, s, a));
+  });
+}
+
+}  // namespace attnb

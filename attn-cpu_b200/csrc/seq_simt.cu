@@ -227,39 +227,6 @@ __global__ void __launch_bounds__(kThreads) seq_simt_kernel(const SeqAttnArgs a,
   }
 }
 
-// Joins the pieces of each item that a cut fell into: block c the item that
-// goes on in CTA c, if it began in CTA c - 1.
-template <int T>
-__global__ void __launch_bounds__(128) seq_merge_kernel(const SeqAttnArgs a) {
-  using E = elem_t<T>;
-  grid_dep_wait();
-  const int c = blockIdx.x + 1;
-  const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];
-  if (!d.continues || d.item0 < (c - 1) * d.quota) return;
-  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1;
-  const int slot0 = 2 * (c - 1) + (d.item0 == (c - 1) * d.quota ? 0 : 1);
-  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
-  const int Dh = a.q.Dh;
-  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
-    float top = ml[(int64_t)slot0 * a.rows + r].x;
-    for (int i = c; i <= last; ++i) top = fmaxf(top, ml[(int64_t)2 * i * a.rows + r].x);
-    const int row = d.first_row + r;
-    E* o = static_cast<E*>(a.o.data) + (int64_t)(d.row_token + row / a.G) * a.o.sT +
-           (int64_t)(d.kv_head * a.G + row % a.G) * a.o.sH;
-    for (int x = threadIdx.x; x < Dh; x += blockDim.x) {
-      float sum = 0.f, acc = 0.f;
-      for (int i = c - 1; i <= last; ++i) {
-        const int64_t at = (int64_t)(i < c ? slot0 : 2 * i) * a.rows + r;
-        const float2 p = ml[at];
-        const float f = p.x == -INFINITY ? 0.f : fast_exp2(p.x - top);
-        sum = fmaf(f, p.y, sum);
-        acc = fmaf(f, a.ws_o[at * Dh + x], acc);
-      }
-      from_float(sum == 0.f ? 0.f : acc / sum, o[x]);
-    }
-  }
-}
-
 bool rows_aligned(const void* p, int64_t sT, int64_t sH, int Dh, int type) {
   const int b = 4 * elem_bytes(type);
   return (reinterpret_cast<uintptr_t>(p) % b) == 0 && sT % 4 == 0 && sH % 4 == 0 && Dh % 4 == 0;
@@ -292,43 +259,6 @@ void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
     else if (tk == kI8) go(tq, std::integral_constant<int, kI8>{});
     else go(tq, tq);
   });
-}
-
-void seq_merge_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
-  if (ctas < 2) return;
-  with_value_type(a.o.type, [&](auto t) {
-    ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
-                          dim3(ctas - 1, std::min(a.rows, 16)), dim3(128), 0, s, a));
-  });
-}
-
-size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
-  // Two CTAs per SM with 4 rows.
-  (void)G;
-  const size_t ctas = 2 * num_sms;
-  return ctas * (2 * 4 * ((size_t)Dh * 4 + 8) + sizeof(SeqSplit)) + 1024;
-}
-
-void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
-                  cudaStream_t s) {
-  (void)max_new;
-  if (a.seqs.batch == 0 || a.seqs.total == 0) return;
-  a.rows = a.q.Dh <= 128 ? 4 : 2;
-  a.kt_shift = 6;
-  a.min_tiles = 2;
-  const int ctas = 2 * num_sms;
-  char* p = static_cast<char*>(ws);
-  a.ws_o = reinterpret_cast<float*>(p);
-  p += (size_t)2 * ctas * a.rows * a.q.Dh * 4;
-  a.ws_ml = reinterpret_cast<float*>(p);
-  p += (size_t)2 * ctas * a.rows * 8;
-  p += (16 - reinterpret_cast<uintptr_t>(p) % 16) % 16;
-  a.ws_split = p;
-  p += ctas * sizeof(SeqSplit);
-  if (p > static_cast<char*>(ws) + ws_bytes)
-    fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
-  seq_simt_launch(a, ctas, s);
-  seq_merge_launch(a, ctas, s);
 }
 
 }  // namespace attnb
