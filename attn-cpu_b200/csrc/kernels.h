@@ -269,6 +269,11 @@ void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // K7: 16-bit queries over 16-bit or coded pages, 16 rows per item.
 bool seq_mma_supported(const SeqAttnArgs& a);
 void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+// K8: 16-bit queries over packed keys or pages, two tiles of up to 128 rows per
+// item (seq_tc_rows in all).
+bool seq_tc_supported(const SeqAttnArgs& a);
+int seq_tc_rows(int G);
+void seq_tc_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // Whether TMA can read the pages, and the map of one of the two pools with
 // copies of up to `rows` rows of one page.
 bool seq_pages_tma(const SeqAttnArgs& a);

@@ -53,22 +53,31 @@ struct Space {
 };
 Space simt_space(int Dh, int num_sms) { return {Dh <= 128 ? 4 : 2, 2 * num_sms}; }
 Space mma_space(int num_sms) { return {16, 2 * num_sms}; }
+Space tc_space(int G, int num_sms) { return {seq_tc_rows(G), num_sms}; }
 
 }  // namespace
 
 size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
-  (void)G;
-  return std::max(simt_space(Dh, num_sms).bytes(Dh), mma_space(num_sms).bytes(Dh)) + 256;
+  size_t n = std::max(simt_space(Dh, num_sms).bytes(Dh), mma_space(num_sms).bytes(Dh));
+  if (G <= 128 && Dh <= 128) n = std::max(n, tc_space(G, num_sms).bytes(Dh));
+  return n + 256;
 }
 
 void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
                   cudaStream_t s) {
-  (void)max_new;
   if (a.seqs.batch == 0 || a.seqs.total == 0) return;
-  const bool mma = seq_mma_supported(a);
-  const Space sp = mma ? mma_space(num_sms) : simt_space(a.q.Dh, num_sms);
+  // New tokens of one sequence: the caller's bound, or the mean.
+  const int64_t rows =
+      (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
+  enum { kSimt, kMma, kTc } kind = kSimt;
+  if (seq_mma_supported(a) && rows <= 32) kind = kMma;
+  else if (seq_tc_supported(a)) kind = kTc;
+  else if (seq_mma_supported(a)) kind = kMma;
+  const Space sp = kind == kTc    ? tc_space(a.G, num_sms)
+                   : kind == kMma ? mma_space(num_sms)
+                                  : simt_space(a.q.Dh, num_sms);
   a.rows = sp.rows;
-  a.kt_shift = 6;
+  a.kt_shift = kind == kTc ? 7 : 6;
   a.min_tiles = 2;
   uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
   if (p + sp.bytes(a.q.Dh) > reinterpret_cast<uintptr_t>(ws) + ws_bytes)
@@ -78,7 +87,8 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   a.ws_ml = reinterpret_cast<float*>(p);
   p += (size_t)2 * sp.ctas * sp.rows * 8;
   a.ws_o = reinterpret_cast<float*>(p);
-  if (mma) seq_mma_launch(a, sp.ctas, s);
+  if (kind == kTc) seq_tc_launch(a, sp.ctas, s);
+  else if (kind == kMma) seq_mma_launch(a, sp.ctas, s);
   else seq_simt_launch(a, sp.ctas, s);
   // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {

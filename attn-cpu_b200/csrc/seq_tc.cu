@@ -1,0 +1,753 @@
+// seq_tc.cu -- K8: attention of packed query rows over packed keys or pages with
+// tcgen05, for 16-bit queries and 16-bit or coded keys: whole prompts and chunks
+// of new tokens.
+//
+// Bound by the tensor cores (4 * Dh operations per visible key and query head)
+// and, next to them, by the exponentials: a 128 x 128 tile of weights takes 1024
+// cycles of the SM's 16 exponentials a cycle, as many as its two products.
+//
+//   A CTA takes two tiles A, B of up to 128 rows of one KV head (the query heads
+//   that share it lie side by side) and streams tiles of 128 keys by TMA; each
+//   K and V tile serves both.  The two tiles run as chains, so that one's
+//   products run under the other's softmax:
+//       S = Q K^T (TMEM)  ->  softmax writes P over S (16 bits, TMEM)  ->  O += P V
+//   with O in TMEM as well: 2 x (128 + 128) columns.  V is read as it lies in
+//   memory, keys by rows (an N-major operand).
+//   Warp 0 loads; warps 1 and 2 issue the chains' products; warp 3 clears masked
+//   V values; warps 4-7 and 8-11 own one row of A or B per thread.  With codes,
+//   warps 12-15 turn them into f16 tiles (exact for e4m3 and int8), and the
+//   register file is dealt out anew: the softmax warps need theirs for a whole
+//   row of S.
+//   CTAs are persistent and walk the pieces of the schedule in seq.cuh.
+//
+// The running maximum moves only when it grows by more than 8 (weights stay
+// below 2^8, which f16 and bf16 hold); O and the sum are rescaled then.  Weights
+// are rounded to 16 bits once, to nearest; maxima, sums and O are fp32.  Codes:
+// scales as in K7 (seq_mma.cu).
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+
+#include "runtime.h"
+#include "seq_elem.cuh"
+#include "seq_pages.cuh"
+
+namespace attnb {
+namespace {
+
+constexpr int BM = 128;
+constexpr int BN = 128;
+constexpr float kRescaleGap = 8.f;
+constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
+
+template <bool CODED, int DHP>
+struct TcCfg {
+  static constexpr int THREADS = CODED ? 512 : 384;
+  static constexpr int CHUNKS = DHP / 64;        // 128-byte pieces of a 16-bit row
+  static constexpr int CHUNK = BN * 128;         // 16 KB: 128 rows x 64 columns
+  static constexpr int TILE = CHUNKS * CHUNK;    // Q, K or V
+  static constexpr int K_ST = DHP == 128 ? 2 : 4;
+  static constexpr int V_ST = DHP == 128 ? 2 : 4;
+  static constexpr int RAW_ST = 3;               // codes: half tiles of 64 keys
+  static constexpr int RAW = 64 * 128 + 1024;    // codes, then K and V scales
+  static constexpr int OFF_K = 2 * TILE;
+  static constexpr int OFF_V = OFF_K + K_ST * TILE;
+  static constexpr int OFF_RAW = OFF_V + V_ST * TILE;
+  static constexpr int OFF_X = OFF_RAW + (CODED ? RAW_ST * RAW : 0);
+  // Codes: {K scale, log2 V scale, 1 / V scale} of as many tiles as K tiles may
+  // be ahead of the softmax that reads them; else poison.
+  static constexpr int SCALES = K_ST + 2;
+  static constexpr int SMEM =
+      OFF_X + (CODED ? SCALES * 3 * BN * 4 : kPoison * 3 * DHP * 4) + 1024;
+  static_assert(SMEM <= 227 * 1024 - 1024, "shared memory budget");
+};
+
+template <int TQ>
+__device__ __forceinline__ bool any_not_finite(const uint4& x) {
+  constexpr uint32_t mask = TQ == kBF16 ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t unit = TQ == kBF16 ? 0x00800080u : 0x04000400u;
+  return ((((x.x & mask) + unit) | ((x.y & mask) + unit) | ((x.z & mask) + unit) |
+           ((x.w & mask) + unit)) &
+          0x80008000u) != 0;
+}
+
+template <int TQ, int TK, int DHP>
+__global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS, 1)
+    seq_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ SeqAttnArgs a, const bool qvec, const bool ovec) {
+  constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  using Cfg = TcCfg<CODED, DHP>;
+  using EQ = elem_t<TQ>;
+  constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
+  constexpr int KST = Cfg::K_ST, VST = Cfg::V_ST, RST = Cfg::RAW_ST;
+  constexpr uint32_t IDESC_S = idesc_f16(BM, BN, BF16, false);
+  constexpr uint32_t IDESC_PV = idesc_f16(BM, DHP, BF16, true);
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
+  __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
+  __shared__ __align__(8) uint64_t q_bar[2], s_bar[2], p_bar[2], pv_bar[2], done_bar[2];
+  __shared__ SeqShared sh;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ int poison_set[kPoison];
+  __shared__ int outputs[2];  // warps' outputs written, per chain
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const mem = smem_raw + (base - smem_addr(smem_raw));
+  volatile int* abort_p = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    outputs[0] = outputs[1] = 0;
+    for (int i = 0; i < KST; ++i) {
+      mbar_init(smem_addr(&kfull[i]), CODED ? 4 : 1);
+      mbar_init(smem_addr(&kempty[i]), 2);
+    }
+    for (int i = 0; i < VST; ++i) {
+      mbar_init(smem_addr(&vfull[i]), CODED ? 4 : 1);
+      mbar_init(smem_addr(&vempty[i]), 2);
+      mbar_init(smem_addr(&vfix[i]), 1);
+    }
+    for (int i = 0; i < RST; ++i) {
+      mbar_init(smem_addr(&rfull[i]), 1);
+      mbar_init(smem_addr(&rempty[i]), 4);
+    }
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(smem_addr(&q_bar[c]), 4);
+      mbar_init(smem_addr(&s_bar[c]), 1);
+      mbar_init(smem_addr(&p_bar[c]), 4);
+      mbar_init(smem_addr(&pv_bar[c]), 1);
+      mbar_init(smem_addr(&done_bar[c]), 1);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (threadIdx.x < kPoison) poison_set[threadIdx.x] = 0;
+  if constexpr (!CODED) {
+    int* ps = reinterpret_cast<int*>(mem + Cfg::OFF_X);
+    for (int i = threadIdx.x; i < kPoison * 3 * DHP; i += Cfg::THREADS) ps[i] = INT_MAX;
+  }
+  grid_dep_wait();
+  SeqPlace place;
+  const bool any = seq_locate(a, sh, place);  // synchronises the block
+  if (threadIdx.x == 0) seq_write_split(a, any, place);
+  if (!any) return;
+  if (warp == 1) {
+    tmem_alloc(smem_addr(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  const int half = a.rows >> 1;  // rows of chain A's tile
+  SeqIter it;
+  it.start(place);
+  SeqPiece w{};
+  // Tiles of the piece that chain c takes: the first ones.
+  auto tiles_of = [&](int c) {
+    const int rows = min(w.rows - c * half, half);
+    if (rows <= 0) return 0;
+    int seen = w.s.L;
+    if (a.causal) seen = seq_row_seen(a, w.s, w.row0 + c * half + rows - 1);
+    const int nt = max(1, (max(seen, 0) + BN - 1) / BN);
+    return min(nt, w.j1) - min(nt, w.j0);
+  };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+    int got = 0;
+    if (lane == 0) got = mbar_wait(smem_addr(bar), parity, abort_p, a.status) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, got, 0) != 0;
+  };
+
+  if (warp < 4) {
+    if constexpr (CODED) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  }
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loader
+    const bool paged = a.pages.k != nullptr;
+    const int shift = a.pages.page_shift, mask = (1 << shift) - 1;
+    PageWindow win;
+    bool ok = true;
+    if constexpr (CODED) {
+      Ring<RST> ring;
+      const int box = min(1 << shift, 64), copies = 64 / box;
+      while (ok && it.next(a, w)) {
+        const int used = (w.s.L + mask) >> shift;
+        for (int hj = 4 * w.j0; ok && hj < 4 * w.j1; ++hj) {
+          // Half tiles: K, K, V, V of each tile.
+          const bool is_v = (hj & 2) != 0;
+          ok = warp_wait(&rempty[ring.stage], ring.phase ^ 1u);
+          if (!ok) break;
+          const uint32_t st = base + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
+          const uint32_t bar = smem_addr(&rfull[ring.stage]);
+          const int key0 = (hj >> 2) * BN + (hj & 1) * 64;
+          int page = 0;  // of this lane's copy
+          uint32_t bytes = 64 * 128;
+          for (int i = 0; i < copies; ++i) {
+            const int p = win.get(a, w.b, (key0 + i * box) >> shift, used);
+            if (lane == i) page = p;
+            if (!is_v && p < a.pages.num_pages) bytes += 2 * box * 4;
+          }
+          const int my_key = key0 + lane * box;
+          const bool there = page < a.pages.num_pages;
+          if (lane < copies && !is_v && !there) {  // no such page: codes 0 with scales of 1
+            float* sc = reinterpret_cast<float*>(mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW +
+                                                 64 * 128);
+            for (int k = 0; k < box; ++k) sc[lane * box + k] = sc[64 + lane * box + k] = 1.f;
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
+          if (lane < copies) {
+            tma_load_4d(st + lane * box * 128, is_v ? &tmV : &tmK, bar, 0, my_key & mask, w.h, page);
+            if (!is_v && there) {
+              const int64_t at = (((int64_t)page * a.pages.H + w.h) << shift) + (my_key & mask);
+              bulk_load(st + 64 * 128 + lane * box * 4, a.pages.k_scale + at, box * 4, bar);
+              bulk_load(st + 64 * 128 + 256 + lane * box * 4, a.pages.v_scale + at, box * 4, bar);
+            }
+          }
+          ring.note_issue();
+          ring.advance();
+        }
+      }
+      if (lane == 0)
+        for (int i = 0; i < RST; ++i)
+          if (ring.issued_mask & (1u << i))
+            drain_wait(smem_addr(&rfull[i]), (ring.issued_parity >> i) & 1u, a.status);
+    } else {
+      Ring<KST> rk;
+      Ring<VST> rv;
+      const int box = paged ? min(1 << shift, BN) : BN, copies = BN / box;
+      // One tile of K or V: `copies` lanes issue their copies.
+      auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int j, int used) {
+        int page = 0;
+        if (paged)
+          for (int i = 0; i < copies; ++i) {
+            const int p = win.get(a, w.b, (j * BN + i * box) >> shift, used);
+            if (lane == i) page = p;
+          }
+        if (lane == 0) mbar_arrive_expect_tx(bar, Cfg::TILE);
+        __syncwarp();
+        if (lane < copies) {
+          const int key = j * BN + lane * box;
+#pragma unroll
+          for (int c = 0; c < Cfg::CHUNKS; ++c) {
+            const uint32_t to = dst + c * Cfg::CHUNK + lane * box * 128;
+            if (paged) tma_load_4d(to, map, bar, c * 64, key & mask, w.h, page);
+            else tma_load_3d(to, map, bar, c * 64, w.h, w.s.k0 + key);
+          }
+        }
+      };
+      while (ok && it.next(a, w)) {
+        const int used = paged ? (w.s.L + mask) >> shift : 0;
+        for (int j = w.j0; ok && j < w.j1; ++j) {
+          ok = warp_wait(&kempty[rk.stage], rk.phase ^ 1u);
+          if (!ok) break;
+          load(&tmK, base + Cfg::OFF_K + rk.stage * Cfg::TILE, smem_addr(&kfull[rk.stage]), j, used);
+          rk.note_issue();
+          rk.advance();
+          ok = warp_wait(&vempty[rv.stage], rv.phase ^ 1u);
+          if (!ok) break;
+          load(&tmV, base + Cfg::OFF_V + rv.stage * Cfg::TILE, smem_addr(&vfull[rv.stage]), j, used);
+          rv.note_issue();
+          rv.advance();
+        }
+      }
+      // Every copy issued lands before the CTA may exit.
+      if (lane == 0) {
+        for (int i = 0; i < KST; ++i)
+          if (rk.issued_mask & (1u << i))
+            drain_wait(smem_addr(&kfull[i]), (rk.issued_parity >> i) & 1u, a.status);
+        for (int i = 0; i < VST; ++i)
+          if (rv.issued_mask & (1u << i))
+            drain_wait(smem_addr(&vfull[i]), (rv.issued_parity >> i) & 1u, a.status);
+      }
+    }
+  } else if (warp <= 2) {
+    // -------------------------------------------------- products of chain c
+    if (lane == 0) {
+      const int c = warp - 1;
+      const uint32_t sbuf = tmem + c * BN;
+      const uint32_t obuf = tmem + 2 * BN + c * 128;
+      const uint32_t qbase = base + c * Cfg::TILE;
+      Ring<KST> rk;
+      Ring<VST> rv;
+      uint32_t tiles = 0, qphase = 0;  // tiles done, whose parity the chain's barriers have
+      bool ok = true;
+      while (ok && it.next(a, w)) {
+        const int n = tiles_of(c);
+        if (n > 0) {
+          if (!(ok = mbar_wait(smem_addr(&q_bar[c]), qphase, abort_p, a.status))) break;
+          qphase ^= 1;
+        }
+        for (int j = 0; j < w.j1 - w.j0; ++j) {
+          const bool use = j < n;
+          if (!(ok = mbar_wait(smem_addr(&kfull[rk.stage]), rk.phase, abort_p, a.status))) break;
+          if (use) {
+            // S overwrites P of the tile before, whose product has to be done.
+            if (tiles > 0 && !(ok = mbar_wait(smem_addr(&pv_bar[c]), (tiles - 1) & 1, abort_p, a.status)))
+              break;
+            tc_fence_after();
+            const uint32_t kb = base + Cfg::OFF_K + rk.stage * Cfg::TILE;
+#pragma unroll
+            for (int k = 0; k < DHP / 16; ++k)
+              mma_f16(sbuf, sdesc_kmajor_sw128(qbase + (k >> 2) * Cfg::CHUNK + (k & 3) * 32),
+                      sdesc_kmajor_sw128(kb + (k >> 2) * Cfg::CHUNK + (k & 3) * 32), IDESC_S,
+                      k != 0 ? 1u : 0u);
+            mma_commit(smem_addr(&kempty[rk.stage]));
+            mma_commit(smem_addr(&s_bar[c]));
+          } else {
+            mbar_arrive(smem_addr(&kempty[rk.stage]));
+          }
+          rk.advance();
+          if (!(ok = mbar_wait(smem_addr(&vfull[rv.stage]), rv.phase, abort_p, a.status))) break;
+          if constexpr (!CODED)
+            if (!(ok = mbar_wait(smem_addr(&vfix[rv.stage]), rv.phase, abort_p, a.status))) break;
+          if (use) {
+            if (!(ok = mbar_wait(smem_addr(&p_bar[c]), tiles & 1, abort_p, a.status))) break;
+            tc_fence_after();
+            const uint32_t vb = base + Cfg::OFF_V + rv.stage * Cfg::TILE;
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              mma_f16_ts(obuf, sbuf + k * 8, sdesc_mnmajor_sw128(vb + k * 2048, Cfg::CHUNK),
+                         IDESC_PV, (j | k) != 0 ? 1u : 0u);
+            mma_commit(smem_addr(&vempty[rv.stage]));
+            mma_commit(smem_addr(&pv_bar[c]));
+            ++tiles;
+          } else {
+            mbar_arrive(smem_addr(&vempty[rv.stage]));
+          }
+          rv.advance();
+        }
+      }
+      // Every product issued completes before TMEM is released.
+      mma_commit(smem_addr(&done_bar[c]));
+      drain_wait(smem_addr(&done_bar[c]), 0, a.status);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------ values of V that a mask hides
+    if constexpr (!CODED) {
+      Ring<VST> rv;
+      bool ok = true;
+      int piece = 0;
+      while (ok && it.next(a, w)) {
+        const int at = piece % kPoison;
+        int* ps = reinterpret_cast<int*>(mem + Cfg::OFF_X) + at * 3 * DHP;
+        if (poison_set[at]) {  // set by piece - kPoison, whose outputs come first
+          const uint64_t t0 = globaltimer();
+          const int want = 4 * (piece - kPoison + 1);
+          while (*(volatile int*)&outputs[0] < want || *(volatile int*)&outputs[1] < want) {
+            if (*abort_p) break;
+            if (globaltimer() - t0 > ATTNB_WAIT_LIMIT_NS) {
+              *abort_p = 1;
+              raise_timeout(a.status);
+              break;
+            }
+          }
+          __syncwarp();
+          for (int i = lane; i < 3 * DHP; i += 32) ps[i] = INT_MAX;
+          if (lane == 0) poison_set[at] = 0;
+          __syncwarp();
+        }
+        const int seen_min = seq_row_seen(a, w.s, w.row0);
+        for (int j = w.j0; j < w.j1; ++j) {
+          ok = warp_wait(&vfull[rv.stage], rv.phase);
+          if (!ok) break;
+          const int key0 = j * BN;
+          if (key0 + BN > seen_min) {
+            uint8_t* v = mem + Cfg::OFF_V + rv.stage * Cfg::TILE;
+            const int from = max(0, seen_min - key0);
+            bool hit = false;
+            for (int i = lane; i < (BN - from) * 8; i += 32) {
+              const int r = from + (i >> 3), u = i & 7;
+#pragma unroll
+              for (int ch = 0; ch < Cfg::CHUNKS; ++ch) {
+                uint4* p = reinterpret_cast<uint4*>(v + ch * Cfg::CHUNK + sw128(r, u));
+                if (key0 + r >= w.s.L) {
+                  *p = make_uint4(0, 0, 0, 0);
+                  continue;
+                }
+                uint4 x = *p;
+                if (!any_not_finite<TQ>(x)) continue;
+                EQ* e = reinterpret_cast<EQ*>(&x);
+#pragma unroll
+                for (int b = 0; b < 8; ++b) {
+                  const float f = to_float(e[b]);
+                  if (fabsf(f) <= 3.402823466e38f) continue;
+                  const int kind = f != f ? 0 : (f > 0.f ? 1 : 2);
+                  atomicMin(&ps[kind * DHP + ch * 64 + u * 8 + b], key0 + r);
+                  from_float(0.f, e[b]);
+                }
+                *p = x;
+                hit = true;
+              }
+            }
+            if (hit) poison_set[at] = 1;
+            fence_proxy_async_smem();  // the products read V through the async proxy
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&vfix[rv.stage]));
+          rv.advance();
+        }
+        ++piece;
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------ codes to f16 tiles
+    if constexpr (CODED) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+      const int t = threadIdx.x - 384, row = t & 63, part = t >> 6;  // half the row's units
+      Ring<RST> ring;
+      Ring<KST> rk;
+      Ring<VST> rv;
+      bool ok = true;
+      uint32_t tile = 0;
+      while (ok && it.next(a, w)) {
+        for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            ok = ok && (kv ? warp_wait(&vempty[rv.stage], rv.phase ^ 1u)
+                           : warp_wait(&kempty[rk.stage], rk.phase ^ 1u));
+            uint8_t* to = mem + (kv ? Cfg::OFF_V + rv.stage * Cfg::TILE
+                                    : Cfg::OFF_K + rk.stage * Cfg::TILE);
+#pragma unroll 1
+            for (int hf = 0; hf < 2; ++hf) {
+              ok = ok && warp_wait(&rfull[ring.stage], ring.phase);
+              if (!ok) break;
+              const uint8_t* from = mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
+              const int r = hf * 64 + row, key = j * BN + r;
+              const bool gone = key >= w.s.L;  // stale: K is masked later, V is zeroed here
+#pragma unroll
+              for (int i = 0; i < DHP / 32; ++i) {
+                const int u = part * (DHP / 32) + i;  // 16 codes
+                uint4 x = *reinterpret_cast<const uint4*>(from + sw128(row, u));
+                if (gone) x = make_uint4(0, 0, 0, 0);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                uint32_t y[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  y[2 * k] = codes_to_f16<TK>(xs[k] & 0xffffu);
+                  y[2 * k + 1] = codes_to_f16<TK>(xs[k] >> 16);
+                }
+                uint8_t* ch = to + (u >> 2) * Cfg::CHUNK;
+                *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2)) =
+                    make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2 + 1)) =
+                    make_uint4(y[4], y[5], y[6], y[7]);
+              }
+              if (kv == 0 && part == 0) {
+                // Scales of a key past the sequence may be anything.
+                const float* sc = reinterpret_cast<const float*>(from + 64 * 128);
+                const float ks = gone ? 0.f : sc[row], vs = gone ? 1.f : sc[64 + row];
+                const float use = vs < 0x1p-60f ? 0x1p-60f : vs;  // see seq_mma.cu
+                float* out = reinterpret_cast<float*>(mem + Cfg::OFF_X) + (tile % Cfg::SCALES) * 3 * BN;
+                out[r] = ks;
+                out[BN + r] = __log2f(use);
+                out[2 * BN + r] = 1.f / use;
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_addr(&rempty[ring.stage]));
+              ring.advance();
+            }
+            if (!ok) break;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kv ? smem_addr(&vfull[rv.stage]) : smem_addr(&kfull[rk.stage]));
+            if (kv) rv.advance();
+            else rk.advance();
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------ softmax / output, chain c
+    if constexpr (CODED) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int c = warp >= 8 ? 1 : 0;
+    const int quarter = warp & 3;  // TMEM lanes [32 * quarter, +32)
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t srow = tmem + lane_off + c * BN;
+    const uint32_t orow = tmem + lane_off + 2 * BN + c * 128;
+    uint32_t tiles = 0, tile0 = 0;  // of this chain; of the CTA
+    bool ok = true;
+    int piece = 0;
+    for (bool first = true; it.next(a, w); first = false, ++piece) {
+      const int n = tiles_of(c);
+      const int rows = min(w.rows - c * half, half);  // of this chain, <= 0: none
+      const bool mine = r < rows;
+      const int row = w.row0 + c * half + r;
+      const int seen = mine ? seq_row_seen(a, w.s, row) : 0;
+      const int64_t token = w.s.q0 + row / a.G;
+      const int head = w.h * a.G + row % a.G;
+      float m = -INFINITY, l = 0.f, scale = a.scale_log2;
+      if (ok && n > 0) {
+        // ---- Q: this thread's row into its tile (the products that read the
+        // row before are done: the last S of the piece before has been seen)
+        uint8_t* qt = mem + c * Cfg::TILE;
+        const EQ* p = static_cast<const EQ*>(a.q.data) + token * a.q.sT + (int64_t)head * a.q.sH;
+        auto unit = [&](int u) {  // 8 values
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (mine) {
+            if (qvec) {
+              if (u * 8 < a.q.Dh) x = __ldg(reinterpret_cast<const uint4*>(p) + u);
+            } else {
+              EQ* e = reinterpret_cast<EQ*>(&x);
+#pragma unroll
+              for (int b = 0; b < 8; ++b)
+                if (u * 8 + b < a.q.Dh) e[b] = p[u * 8 + b];
+            }
+          }
+          return x;
+        };
+        float f = 1.f;
+        if constexpr (CODED) {
+          float top = 0.f;
+#pragma unroll 4
+          for (int u = 0; u < DHP / 8; ++u) {
+            const uint4 x = unit(u);
+            const EQ* e = reinterpret_cast<const EQ*>(&x);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) top = fmaxf(top, fabsf(to_float(e[b])));
+          }
+          f = row_scale(top);
+          scale = a.scale_log2 / f;
+        }
+#pragma unroll 4
+        for (int u = 0; u < DHP / 8; ++u) {
+          uint4 x = unit(u);
+          if constexpr (CODED) {
+            const EQ* e = reinterpret_cast<const EQ*>(&x);
+            x = make_uint4(pack_f16(to_float(e[0]) * f, to_float(e[1]) * f),
+                           pack_f16(to_float(e[2]) * f, to_float(e[3]) * f),
+                           pack_f16(to_float(e[4]) * f, to_float(e[5]) * f),
+                           pack_f16(to_float(e[6]) * f, to_float(e[7]) * f));
+          }
+          *reinterpret_cast<uint4*>(qt + (u >> 3) * Cfg::CHUNK + sw128(r, u & 7)) = x;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&q_bar[c]));
+      }
+      for (int j = 0; j < n; ++j, ++tiles) {
+        if (ok) ok = warp_wait(&s_bar[c], tiles & 1);
+        if (!ok) continue;
+        tc_fence_after();
+        uint32_t s[BN];
+        tmem_ld32x2(srow, *reinterpret_cast<uint32_t(*)[32]>(s), srow + 32,
+                    *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        tmem_ld32x2(srow + 64, *reinterpret_cast<uint32_t(*)[32]>(s + 64), srow + 96,
+                    *reinterpret_cast<uint32_t(*)[32]>(s + 96));
+        const int kb0 = (w.j0 + j) * BN;
+        const float* sc = reinterpret_cast<const float*>(mem + Cfg::OFF_X) +
+                          ((tile0 + j) % Cfg::SCALES) * 3 * BN;
+        if constexpr (CODED) {
+#pragma unroll
+          for (int i = 0; i < BN; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
+            const float4 v4 = *reinterpret_cast<const float4*>(sc + BN + i);
+            s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]) * k4.x, scale, v4.x));
+            s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]) * k4.y, scale, v4.y));
+            s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]) * k4.z, scale, v4.z));
+            s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]) * k4.w, scale, v4.w));
+          }
+        }
+        // Masks only occur in some tiles; a warp applies them only there.
+        if (__any_sync(0xffffffffu, kb0 + BN > seen)) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (kb0 + i >= seen) s[i] = __float_as_uint(-INFINITY);
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < BN; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s[i]));
+        const float mul = CODED ? 1.f : scale;
+        const float top = fmaxf(mx[0], mx[1]) * mul;
+        const bool need = top > m + kRescaleGap;
+        const bool rescale = __any_sync(0xffffffffu, need);
+        float alpha = 1.f;
+        if (need) {
+          alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
+          m = top;
+        }
+        const float use = m == -INFINITY ? 0.f : m;
+        float ls[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < BN; i += 2) {
+          const float p0 = fast_exp2(fmaf(__uint_as_float(s[i]), mul, -use));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(s[i + 1]), mul, -use));
+          if constexpr (CODED) {
+            const float2 v2 = *reinterpret_cast<const float2*>(sc + 2 * BN + i);
+            ls[0] = fmaf(p0, v2.x, ls[0]);
+            ls[1] = fmaf(p1, v2.y, ls[1]);
+          } else {
+            ls[0] += p0;
+            ls[1] += p1;
+          }
+          s[i >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
+        }
+        l = l * alpha + (ls[0] + ls[1]);
+        tmem_st32(srow, *reinterpret_cast<const uint32_t(*)[32]>(s));
+        tmem_st32(srow + 32, *reinterpret_cast<const uint32_t(*)[32]>(s + 32));
+        if (rescale && j > 0) {
+          // O holds the products up to the tile before (complete: S of this
+          // tile was issued after them).
+#pragma unroll 1
+          for (int d = 0; d < DHP; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(orow + d, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(orow + d, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&p_bar[c]));
+      }
+      tile0 += w.j1 - w.j0;
+      if (ok && n > 0) ok = warp_wait(&pv_bar[c], (tiles - 1) & 1);
+      // ---- output: O / l, or the piece's partial result
+      const int slot = seq_slot(w, first);
+      if (ok && rows > 0) {
+        tc_fence_after();
+        const float mulo = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        const int* ps = reinterpret_cast<const int*>(mem + Cfg::OFF_X) + (piece % kPoison) * 3 * DHP;
+        const bool hit = !CODED && *(volatile int*)&poison_set[piece % kPoison] != 0;
+        const int64_t prow = (int64_t)slot * a.rows + c * half + r;
+        if (slot >= 0 && mine)
+          reinterpret_cast<float2*>(a.ws_ml)[prow] = make_float2(m, l);
+        EQ* out = static_cast<EQ*>(a.o.data) + token * a.o.sT + (int64_t)head * a.o.sH;
+#pragma unroll 1
+        for (int d = 0; d < DHP; d += 32) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld32(orow + d, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (!mine) continue;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mulo);
+          if (hit) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(poisoned(__uint_as_float(o[i]), ps, ps + DHP, ps + 2 * DHP,
+                                              d + i, seen));
+          }
+          if (slot >= 0) {
+            float* to = a.ws_o + prow * a.q.Dh + d;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (d + i < a.q.Dh)  // Dh is a multiple of 8
+                *reinterpret_cast<uint4*>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (d + i >= a.q.Dh) continue;
+              if (ovec) {
+                uint4 x;
+                EQ* e = reinterpret_cast<EQ*>(&x);
+#pragma unroll
+                for (int b = 0; b < 8; ++b) from_float(__uint_as_float(o[i + b]), e[b]);
+                *reinterpret_cast<uint4*>(out + d + i) = x;
+              } else {
+#pragma unroll
+                for (int b = 0; b < 8; ++b) from_float(__uint_as_float(o[i + b]), out[d + i + b]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      if constexpr (!CODED) {
+        __syncwarp();
+        if (lane == 0) atomicAdd(&outputs[c], 1);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int TQ, int TK, int DHP>
+void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensorMap& v, bool qvec,
+            bool ovec, cudaStream_t s) {
+  using Cfg = TcCfg<TK == kE4M3 || TK == kI8, DHP>;
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  ATTNB_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    ATTNB_CUDA(cudaFuncSetAttribute(seq_tc_kernel<TQ, TK, DHP>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    configured.fetch_or(bit);
+  }
+  ATTNB_CUDA(launch_pdl(seq_tc_kernel<TQ, TK, DHP>, dim3(ctas), dim3(Cfg::THREADS), Cfg::SMEM, s, k,
+                        v, a, qvec, ovec));
+}
+
+bool aligned16(const RowsView& r) {
+  return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.sT % 8 == 0 && r.sH % 8 == 0;
+}
+
+// Packed keys [tokens, heads, Dh] as (Dh, heads, tokens).
+CUtensorMap rows_map(const RowsView& r) {
+  const uint64_t dims[3] = {(uint64_t)r.Dh, (uint64_t)r.heads, (uint64_t)r.tokens};
+  const uint64_t any = ((uint64_t)r.Dh * 2 + 15) / 16 * 16;  // of a dimension of one
+  const uint64_t strides[2] = {r.heads > 1 ? (uint64_t)r.sH * 2 : any,
+                               r.tokens > 1 ? (uint64_t)r.sT * 2 : any * r.heads};
+  const uint32_t box[3] = {64, 1, BN};
+  return make_tmap_nd(r.data, 2, 3, dims, strides, box);
+}
+
+}  // namespace
+
+bool seq_tc_supported(const SeqAttnArgs& a) {
+  if (a.q.type == kF32 || a.G > BM || a.q.Dh > 128 || a.q.Dh % 8 != 0) return false;
+  if (a.pages.k) return seq_pages_tma(a);
+  if (a.k.tokens == 0) return false;
+  for (const RowsView* r : {&a.k, &a.v}) {
+    if (!aligned16(*r)) return false;
+    if ((r->tokens > 1 && r->sT <= 0) || (r->heads > 1 && r->sH <= 0)) return false;
+    if (r->sT >= (1ll << 38) || r->sH >= (1ll << 38)) return false;  // the map's stride limit
+  }
+  return true;
+}
+
+int seq_tc_rows(int G) { return 2 * (BM / G) * G; }
+
+void seq_tc_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
+  const CUtensorMap k = a.pages.k ? seq_pages_map(a.pages, a.pages.k, elem_coded(a.pages.type) ? 64 : BN)
+                                  : rows_map(a.k);
+  const CUtensorMap v = a.pages.k ? seq_pages_map(a.pages, a.pages.v, elem_coded(a.pages.type) ? 64 : BN)
+                                  : rows_map(a.v);
+  const bool qvec = aligned16(a.q), ovec = aligned16(a.o);
+  auto go = [&](auto tq, auto tk) {
+    constexpr int TQ = decltype(tq)::value, TK = decltype(tk)::value;
+    if constexpr (TQ != kF32) {
+      if (a.q.Dh <= 64) launch<TQ, TK, 64>(a, ctas, k, v, qvec, ovec, s);
+      else launch<TQ, TK, 128>(a, ctas, k, v, qvec, ovec, s);
+    }
+  };
+  with_value_type(a.q.type, [&](auto tq) {
+    if (a.pages.k && a.pages.type == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});
+    else if (a.pages.k && a.pages.type == kI8) go(tq, std::integral_constant<int, kI8>{});
+    else go(tq, tq);
+  });
+}
+
+}  // namespace attnb
