@@ -15,15 +15,20 @@
 //   memory, keys by rows (an N-major operand).
 //   Warp 0 loads; warps 1 and 2 issue the chains' products; warp 3 clears masked
 //   V values; warps 4-7 and 8-11 own one row of A or B per thread.  With codes,
-//   warps 12-15 turn them into f16 tiles (exact for e4m3 and int8), and the
-//   register file is dealt out anew: the softmax warps need theirs for a whole
-//   row of S.
+//   warps 12-15 turn them into f16 tiles.
 //   CTAs are persistent and walk the pieces of the schedule in seq.cuh.
 //
 // The running maximum moves only when it grows by more than 8 (weights stay
 // below 2^8, which f16 and bf16 hold); O and the sum are rescaled then.  Weights
-// are rounded to 16 bits once, to nearest; maxima, sums and O are fp32.  Codes:
-// scales as in K7 (seq_mma.cu).
+// are rounded to 16 bits once, to nearest; maxima, sums and O are fp32.
+//
+// Codes: both products run in f16.  Q is brought to [1, 2) by a power of two per
+// row, and 64 keys at a time K becomes code * scale / 2^E with 2^E the largest
+// scale's power of two, rounded to f16 once (2^-11 of a value, where the codes
+// themselves are 2^-4 or 2^-8 off); keys whose scale is 2^14 below the largest
+// lose bits that are 2^-25 of the largest.  2^E goes into the rows' scale, and
+// V's 2^F into the exponent, s' = s + F, with 2^-F on the sum: nothing is left
+// to do for single keys in the softmax.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -55,11 +60,13 @@ struct TcCfg {
   static constexpr int OFF_V = OFF_K + K_ST * TILE;
   static constexpr int OFF_RAW = OFF_V + V_ST * TILE;
   static constexpr int OFF_X = OFF_RAW + (CODED ? RAW_ST * RAW : 0);
-  // Codes: {K scale, log2 V scale, 1 / V scale} of as many tiles as K tiles may
+  // Codes: four powers of two, of as many tiles as K tiles may
   // be ahead of the softmax that reads them; else poison.
   static constexpr int SCALES = K_ST + 2;
-  static constexpr int SMEM =
-      OFF_X + (CODED ? SCALES * 3 * BN * 4 : kPoison * 3 * DHP * 4) + 1024;
+  static constexpr int XTILE = 16;
+  // 2 KB per softmax warp to write outputs through; with codes Q's place serves.
+  static constexpr int OFF_OUT = OFF_X + (CODED ? SCALES * XTILE : kPoison * 3 * DHP * 4);
+  static constexpr int SMEM = OFF_OUT + (CODED ? 0 : 8 * 2048) + 1024;
   static_assert(SMEM <= 227 * 1024 - 1024, "shared memory budget");
 };
 
@@ -74,8 +81,9 @@ __device__ __forceinline__ bool any_not_finite(const uint4& x) {
 
 template <int TQ, int TK, int DHP>
 __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS, 1)
-    seq_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const __grid_constant__ SeqAttnArgs a, const bool qvec, const bool ovec) {
+    seq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ SeqAttnArgs a,
+                  const bool qtma, const bool qvec, const bool ovec) {
   constexpr bool CODED = TK == kE4M3 || TK == kI8;
   using Cfg = TcCfg<CODED, DHP>;
   using EQ = elem_t<TQ>;
@@ -87,7 +95,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
   __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
-  __shared__ __align__(8) uint64_t q_bar[2], s_bar[2], p_bar[2], pv_bar[2], done_bar[2];
+  __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2], p_bar[2], pv_bar[2], done_bar[2];
   __shared__ SeqShared sh;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -116,7 +124,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       mbar_init(smem_addr(&rempty[i]), 4);
     }
     for (int c = 0; c < 2; ++c) {
-      mbar_init(smem_addr(&q_bar[c]), 4);
+      mbar_init(smem_addr(&q_bar[c]), qtma ? 1 : 4);
+      mbar_init(smem_addr(&q_free[c]), 1);
       mbar_init(smem_addr(&s_bar[c]), 1);
       mbar_init(smem_addr(&p_bar[c]), 4);
       mbar_init(smem_addr(&pv_bar[c]), 1);
@@ -159,14 +168,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     return min(nt, w.j1) - min(nt, w.j0);
   };
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
-    int got = 0;
-    if (lane == 0) got = mbar_wait(smem_addr(bar), parity, abort_p, a.status) ? 1 : 0;
-    return __shfl_sync(0xffffffffu, got, 0) != 0;
+    const bool got = mbar_wait_quick(smem_addr(bar), parity, abort_p, a.status);
+    return __all_sync(0xffffffffu, got) != 0;
   };
 
-  if (warp < 4) {
-    if constexpr (CODED) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  }
   if (warp == 0) {
     // ---------------------------------------------------------------- loader
     const bool paged = a.pages.k != nullptr;
@@ -244,6 +249,21 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           }
         }
       };
+      // Q of chain c, once the products of the piece before are done with it.
+      uint32_t qloads[2] = {0, 0};
+      auto load_q = [&](int c) {
+        if (!warp_wait(&q_free[c], (qloads[c] & 1) ^ 1)) return false;
+        ++qloads[c];
+        if (lane == 0) {
+          const uint32_t bar = smem_addr(&q_bar[c]);
+          mbar_arrive_expect_tx(bar, Cfg::CHUNKS * half * 128);
+          const int token = w.s.q0 + (w.row0 + c * half) / a.G;
+#pragma unroll
+          for (int k = 0; k < Cfg::CHUNKS; ++k)
+            tma_load_3d(base + c * Cfg::TILE + k * Cfg::CHUNK, &tmQ, bar, k * 64, w.h * a.G, token);
+        }
+        return true;
+      };
       while (ok && it.next(a, w)) {
         const int used = paged ? (w.s.L + mask) >> shift : 0;
         for (int j = w.j0; ok && j < w.j1; ++j) {
@@ -252,6 +272,11 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           load(&tmK, base + Cfg::OFF_K + rk.stage * Cfg::TILE, smem_addr(&kfull[rk.stage]), j, used);
           rk.note_issue();
           rk.advance();
+          if (qtma && j == w.j0) {
+            for (int c = 0; ok && c < 2; ++c)
+              if (tiles_of(c) > 0) ok = load_q(c);
+            if (!ok) break;
+          }
           ok = warp_wait(&vempty[rv.stage], rv.phase ^ 1u);
           if (!ok) break;
           load(&tmV, base + Cfg::OFF_V + rv.stage * Cfg::TILE, smem_addr(&vfull[rv.stage]), j, used);
@@ -267,6 +292,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         for (int i = 0; i < VST; ++i)
           if (rv.issued_mask & (1u << i))
             drain_wait(smem_addr(&vfull[i]), (rv.issued_parity >> i) & 1u, a.status);
+        for (int c = 0; c < 2; ++c)
+          if (qloads[c] > 0) drain_wait(smem_addr(&q_bar[c]), (qloads[c] - 1) & 1u, a.status);
       }
     }
   } else if (warp <= 2) {
@@ -283,15 +310,15 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       while (ok && it.next(a, w)) {
         const int n = tiles_of(c);
         if (n > 0) {
-          if (!(ok = mbar_wait(smem_addr(&q_bar[c]), qphase, abort_p, a.status))) break;
+          if (!(ok = mbar_wait_quick(smem_addr(&q_bar[c]), qphase, abort_p, a.status))) break;
           qphase ^= 1;
         }
         for (int j = 0; j < w.j1 - w.j0; ++j) {
           const bool use = j < n;
-          if (!(ok = mbar_wait(smem_addr(&kfull[rk.stage]), rk.phase, abort_p, a.status))) break;
+          if (!(ok = mbar_wait_quick(smem_addr(&kfull[rk.stage]), rk.phase, abort_p, a.status))) break;
           if (use) {
             // S overwrites P of the tile before, whose product has to be done.
-            if (tiles > 0 && !(ok = mbar_wait(smem_addr(&pv_bar[c]), (tiles - 1) & 1, abort_p, a.status)))
+            if (tiles > 0 && !(ok = mbar_wait_quick(smem_addr(&pv_bar[c]), (tiles - 1) & 1, abort_p, a.status)))
               break;
             tc_fence_after();
             const uint32_t kb = base + Cfg::OFF_K + rk.stage * Cfg::TILE;
@@ -302,15 +329,16 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                       k != 0 ? 1u : 0u);
             mma_commit(smem_addr(&kempty[rk.stage]));
             mma_commit(smem_addr(&s_bar[c]));
+            if (j == n - 1) mma_commit(smem_addr(&q_free[c]));
           } else {
             mbar_arrive(smem_addr(&kempty[rk.stage]));
           }
           rk.advance();
-          if (!(ok = mbar_wait(smem_addr(&vfull[rv.stage]), rv.phase, abort_p, a.status))) break;
+          if (!(ok = mbar_wait_quick(smem_addr(&vfull[rv.stage]), rv.phase, abort_p, a.status))) break;
           if constexpr (!CODED)
-            if (!(ok = mbar_wait(smem_addr(&vfix[rv.stage]), rv.phase, abort_p, a.status))) break;
+            if (!(ok = mbar_wait_quick(smem_addr(&vfix[rv.stage]), rv.phase, abort_p, a.status))) break;
           if (use) {
-            if (!(ok = mbar_wait(smem_addr(&p_bar[c]), tiles & 1, abort_p, a.status))) break;
+            if (!(ok = mbar_wait_quick(smem_addr(&p_bar[c]), tiles & 1, abort_p, a.status))) break;
             tc_fence_after();
             const uint32_t vb = base + Cfg::OFF_V + rv.stage * Cfg::TILE;
 #pragma unroll
@@ -401,7 +429,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
   } else if (warp >= 12) {
     // ------------------------------------------------------ codes to f16 tiles
     if constexpr (CODED) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
       const int t = threadIdx.x - 384, row = t & 63, part = t >> 6;  // half the row's units
       Ring<RST> ring;
       Ring<KST> rk;
@@ -410,19 +437,48 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       uint32_t tile = 0;
       while (ok && it.next(a, w)) {
         for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
+          float vmul[2];  // of this thread's two keys
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             ok = ok && (kv ? warp_wait(&vempty[rv.stage], rv.phase ^ 1u)
                            : warp_wait(&kempty[rk.stage], rk.phase ^ 1u));
             uint8_t* to = mem + (kv ? Cfg::OFF_V + rv.stage * Cfg::TILE
                                     : Cfg::OFF_K + rk.stage * Cfg::TILE);
-#pragma unroll 1
+#pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               ok = ok && warp_wait(&rfull[ring.stage], ring.phase);
               if (!ok) break;
               const uint8_t* from = mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
-              const int r = hf * 64 + row, key = j * BN + r;
-              const bool gone = key >= w.s.L;  // stale: K is masked later, V is zeroed here
+              float* xt = reinterpret_cast<float*>(mem + Cfg::OFF_X +
+                                                   (tile % Cfg::SCALES) * Cfg::XTILE);
+              const int r = hf * 64 + row, left = w.s.L - j * BN - hf * 64;
+              const bool gone = row >= left;  // stale: K is masked later, V is zeroed here
+              float mul = 0.f;
+              if (kv == 0) {
+                // Scales of a key past the sequence may be anything.
+                const float* sc = reinterpret_cast<const float*>(from + 64 * 128);
+                float km = fmaxf(lane < left ? sc[lane] : 0.f, lane + 32 < left ? sc[lane + 32] : 0.f);
+                float vm = fmaxf(lane < left ? sc[64 + lane] : 0.f,
+                                 lane + 32 < left ? sc[96 + lane] : 0.f);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                  km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+                  vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+                }
+                // The largest scales' powers of two (as in row_scale, kept to
+                // 2^-60 .. 2^60: sums carry their inverses).
+                const float ke = fminf(fmaxf(1.f / row_scale(km), 0x1p-60f), 0x1p60f);
+                const float ve = fminf(fmaxf(1.f / row_scale(vm), 0x1p-60f), 0x1p60f);
+                if (!gone) mul = sc[row] / ke;
+                vmul[hf] = gone ? 0.f : sc[64 + row] / ve;
+                if (t == 0) {
+                  xt[hf] = ke;
+                  xt[2 + hf] = (float)((int)(__float_as_uint(ve) >> 23) - 127);
+                }
+              } else {
+                mul = vmul[hf];
+              }
+              const uint64_t mul2 = pack_f32x2(mul, mul);
 #pragma unroll
               for (int i = 0; i < DHP / 32; ++i) {
                 const int u = part * (DHP / 32) + i;  // 16 codes
@@ -431,25 +487,18 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
                 uint32_t y[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  y[2 * k] = codes_to_f16<TK>(xs[k] & 0xffffu);
-                  y[2 * k + 1] = codes_to_f16<TK>(xs[k] >> 16);
+                for (int k = 0; k < 8; ++k) {
+                  const uint32_t h = codes_to_f16<TK>((xs[k >> 1] >> (16 * (k & 1))) & 0xffffu);
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                  float lo, hi;
+                  unpack_f32x2(mul_f32x2(pack_f32x2(f.x, f.y), mul2), lo, hi);
+                  y[k] = pack_f16(lo, hi);
                 }
                 uint8_t* ch = to + (u >> 2) * Cfg::CHUNK;
                 *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2)) =
                     make_uint4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2 + 1)) =
                     make_uint4(y[4], y[5], y[6], y[7]);
-              }
-              if (kv == 0 && part == 0) {
-                // Scales of a key past the sequence may be anything.
-                const float* sc = reinterpret_cast<const float*>(from + 64 * 128);
-                const float ks = gone ? 0.f : sc[row], vs = gone ? 1.f : sc[64 + row];
-                const float use = vs < 0x1p-60f ? 0x1p-60f : vs;  // see seq_mma.cu
-                float* out = reinterpret_cast<float*>(mem + Cfg::OFF_X) + (tile % Cfg::SCALES) * 3 * BN;
-                out[r] = ks;
-                out[BN + r] = __log2f(use);
-                out[2 * BN + r] = 1.f / use;
               }
               __syncwarp();
               if (lane == 0) mbar_arrive(smem_addr(&rempty[ring.stage]));
@@ -467,7 +516,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     }
   } else {
     // ------------------------------------------------ softmax / output, chain c
-    if constexpr (CODED) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int c = warp >= 8 ? 1 : 0;
     const int quarter = warp & 3;  // TMEM lanes [32 * quarter, +32)
     const int r = quarter * 32 + lane;
@@ -486,7 +534,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       const int64_t token = w.s.q0 + row / a.G;
       const int head = w.h * a.G + row % a.G;
       float m = -INFINITY, l = 0.f, scale = a.scale_log2;
-      if (ok && n > 0) {
+      if (ok && n > 0 && !qtma) {
         // ---- Q: this thread's row into its tile (the products that read the
         // row before are done: the last S of the piece before has been seen)
         uint8_t* qt = mem + c * Cfg::TILE;
@@ -538,36 +586,48 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         if (ok) ok = warp_wait(&s_bar[c], tiles & 1);
         if (!ok) continue;
         tc_fence_after();
-        uint32_t s[BN];
-        tmem_ld32x2(srow, *reinterpret_cast<uint32_t(*)[32]>(s), srow + 32,
-                    *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-        tmem_ld32x2(srow + 64, *reinterpret_cast<uint32_t(*)[32]>(s + 64), srow + 96,
-                    *reinterpret_cast<uint32_t(*)[32]>(s + 96));
         const int kb0 = (w.j0 + j) * BN;
-        const float* sc = reinterpret_cast<const float*>(mem + Cfg::OFF_X) +
-                          ((tile0 + j) % Cfg::SCALES) * 3 * BN;
-        if constexpr (CODED) {
-#pragma unroll
-          for (int i = 0; i < BN; i += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
-            const float4 v4 = *reinterpret_cast<const float4*>(sc + BN + i);
-            s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]) * k4.x, scale, v4.x));
-            s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]) * k4.y, scale, v4.y));
-            s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]) * k4.z, scale, v4.z));
-            s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]) * k4.w, scale, v4.w));
-          }
-        }
         // Masks only occur in some tiles; a warp applies them only there.
-        if (__any_sync(0xffffffffu, kb0 + BN > seen)) {
-#pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (kb0 + i >= seen) s[i] = __float_as_uint(-INFINITY);
+        const bool masked = __any_sync(0xffffffffu, kb0 + BN > seen);
+        // Score to exponent: times mul, plus add (codes: per 64 keys).
+        float mul[2] = {scale, scale}, add[2] = {0.f, 0.f}, linv[2] = {1.f, 1.f};
+        if constexpr (CODED) {
+          const float4 x = *reinterpret_cast<const float4*>(
+              mem + Cfg::OFF_X + ((tile0 + j) % Cfg::SCALES) * Cfg::XTILE);
+          mul[0] = scale * x.x;
+          mul[1] = scale * x.y;
+          add[0] = x.z;
+          add[1] = x.w;
+          linv[0] = fast_exp2(-x.z);
+          linv[1] = fast_exp2(-x.w);
         }
-        float mx[2] = {-INFINITY, -INFINITY};
+        // The row of S: at once, or (codes, with fewer registers) 64 columns at
+        // a time, read again for the weights; those take the columns that are
+        // done with.
+        constexpr int W = CODED ? 64 : BN;
+        uint32_t s[W];
+        auto load = [&](int part) {
+          if constexpr (CODED) tmem_ld64(srow + part * W, s);
+          else tmem_ld128(srow, s);
+          if (masked) {
 #pragma unroll
-        for (int i = 0; i < BN; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s[i]));
-        const float mul = CODED ? 1.f : scale;
-        const float top = fmaxf(mx[0], mx[1]) * mul;
+            for (int i = 0; i < W; ++i)
+              if (kb0 + part * W + i >= seen) s[i] = __float_as_uint(-INFINITY);
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int part = 0; part < BN / W; ++part) {
+          load(part);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < W; i += 8)  // three operands an instruction
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])),
+                            __uint_as_float(s[i + 2 * k + 1]));
+          top = fmaxf(top, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), mul[part], add[part]));
+        }
         const bool need = top > m + kRescaleGap;
         const bool rescale = __any_sync(0xffffffffu, need);
         float alpha = 1.f;
@@ -576,24 +636,30 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           m = top;
         }
         const float use = m == -INFINITY ? 0.f : m;
-        float ls[2] = {0.f, 0.f};
+        l *= alpha;
 #pragma unroll
-        for (int i = 0; i < BN; i += 2) {
-          const float p0 = fast_exp2(fmaf(__uint_as_float(s[i]), mul, -use));
-          const float p1 = fast_exp2(fmaf(__uint_as_float(s[i + 1]), mul, -use));
-          if constexpr (CODED) {
-            const float2 v2 = *reinterpret_cast<const float2*>(sc + 2 * BN + i);
-            ls[0] = fmaf(p0, v2.x, ls[0]);
-            ls[1] = fmaf(p1, v2.y, ls[1]);
-          } else {
-            ls[0] += p0;
-            ls[1] += p1;
+        for (int part = 0; part < BN / W; ++part) {
+          if constexpr (CODED) load(part);
+          uint64_t ls[2] = {0, 0};
+          const float off = add[part] - use;
+          const uint64_t mul2 = pack_f32x2(mul[part], mul[part]), off2 = pack_f32x2(off, off);
+#pragma unroll
+          for (int i = 0; i < W; i += 2) {
+            float p0, p1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                                   mul2, off2),
+                         p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            ls[(i >> 1) & 1] = add_f32x2(ls[(i >> 1) & 1], pack_f32x2(p0, p1));
+            s[i >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
           }
-          s[i >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
+          float l0, l1;
+          unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
+          l = fmaf(l0 + l1, linv[part], l);
+          if constexpr (CODED) tmem_st32(srow + part * 32, *reinterpret_cast<const uint32_t(*)[32]>(s));
+          else tmem_st64(srow, s);
         }
-        l = l * alpha + (ls[0] + ls[1]);
-        tmem_st32(srow, *reinterpret_cast<const uint32_t(*)[32]>(s));
-        tmem_st32(srow + 32, *reinterpret_cast<const uint32_t(*)[32]>(s + 32));
         if (rescale && j > 0) {
           // O holds the products up to the tile before (complete: S of this
           // tile was issued after them).
@@ -623,7 +689,12 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         const int64_t prow = (int64_t)slot * a.rows + c * half + r;
         if (slot >= 0 && mine)
           reinterpret_cast<float2*>(a.ws_ml)[prow] = make_float2(m, l);
-        EQ* out = static_cast<EQ*>(a.o.data) + token * a.o.sT + (int64_t)head * a.o.sH;
+        // Through shared memory, 64 bytes of each row at a time, so that four
+        // lanes write one row's piece side by side.
+        uint8_t* stage = CODED ? mem + c * Cfg::TILE + quarter * 4096
+                               : mem + Cfg::OFF_OUT + (warp - 4) * 2048;
+        const int64_t out = token * a.o.sT + (int64_t)head * a.o.sH;
+        const int row0 = quarter * 32;  // of the chain
 #pragma unroll 1
         for (int d = 0; d < DHP; d += 32) {
           uint32_t o[32];
@@ -633,7 +704,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-          if (!mine) continue;
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mulo);
           if (hit) {
@@ -642,25 +712,53 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               o[i] = __float_as_uint(poisoned(__uint_as_float(o[i]), ps, ps + DHP, ps + 2 * DHP,
                                               d + i, seen));
           }
+          const int unit = lane & 3;
           if (slot >= 0) {
-            float* to = a.ws_o + prow * a.q.Dh + d;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (d + i < a.q.Dh)  // Dh is a multiple of 8
-                *reinterpret_cast<uint4*>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int hf = 0; hf < 2; ++hf) {  // 16 values are 64 bytes
+              __syncwarp();
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(o[hf * 16 + u * 4], o[hf * 16 + u * 4 + 1], o[hf * 16 + u * 4 + 2],
+                               o[hf * 16 + u * 4 + 3]);
+              __syncwarp();
+              const int dd = d + hf * 16 + unit * 4;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int rr = k * 8 + (lane >> 2);
+                const uint4 x = *reinterpret_cast<const uint4*>(
+                    stage + rr * 64 + ((unit ^ ((rr >> 1) & 3)) << 4));
+                if (row0 + rr < rows && dd < a.q.Dh)  // Dh is a multiple of 8
+                  *reinterpret_cast<uint4*>(
+                      a.ws_o + ((int64_t)slot * a.rows + c * half + row0 + rr) * a.q.Dh + dd) = x;
+              }
+            }
           } else {
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              if (d + i >= a.q.Dh) continue;
+            for (int u = 0; u < 4; ++u) {
+              uint4 x;
+              EQ* e = reinterpret_cast<EQ*>(&x);
+#pragma unroll
+              for (int b = 0; b < 8; ++b) from_float(__uint_as_float(o[u * 8 + b]), e[b]);
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = x;
+            }
+            __syncwarp();
+            const int dd = d + unit * 8;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int rr = k * 8 + (lane >> 2);
+              const uint4 x = *reinterpret_cast<const uint4*>(
+                  stage + rr * 64 + ((unit ^ ((rr >> 1) & 3)) << 4));
+              EQ* to = static_cast<EQ*>(a.o.data) + __shfl_sync(0xffffffffu, out, rr) + dd;
+              if (row0 + rr >= rows || dd >= a.q.Dh) continue;
               if (ovec) {
-                uint4 x;
-                EQ* e = reinterpret_cast<EQ*>(&x);
-#pragma unroll
-                for (int b = 0; b < 8; ++b) from_float(__uint_as_float(o[i + b]), e[b]);
-                *reinterpret_cast<uint4*>(out + d + i) = x;
+                *reinterpret_cast<uint4*>(to) = x;
               } else {
+                const EQ* e = reinterpret_cast<const EQ*>(&x);
 #pragma unroll
-                for (int b = 0; b < 8; ++b) from_float(__uint_as_float(o[i + b]), out[d + i + b]);
+                for (int b = 0; b < 8; ++b) to[b] = e[b];
               }
             }
           }
@@ -684,8 +782,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 }
 
 template <int TQ, int TK, int DHP>
-void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensorMap& v, bool qvec,
-            bool ovec, cudaStream_t s) {
+void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& q, const CUtensorMap& k,
+            const CUtensorMap& v, bool qtma, bool qvec, bool ovec, cudaStream_t s) {
   using Cfg = TcCfg<TK == kE4M3 || TK == kI8, DHP>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
@@ -696,21 +794,26 @@ void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensor
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     configured.fetch_or(bit);
   }
-  ATTNB_CUDA(launch_pdl(seq_tc_kernel<TQ, TK, DHP>, dim3(ctas), dim3(Cfg::THREADS), Cfg::SMEM, s, k,
-                        v, a, qvec, ovec));
+  ATTNB_CUDA(launch_pdl(seq_tc_kernel<TQ, TK, DHP>, dim3(ctas), dim3(Cfg::THREADS), Cfg::SMEM, s, q,
+                        k, v, a, qtma, qvec, ovec));
 }
 
 bool aligned16(const RowsView& r) {
   return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.sT % 8 == 0 && r.sH % 8 == 0;
 }
 
-// Packed keys [tokens, heads, Dh] as (Dh, heads, tokens).
-CUtensorMap rows_map(const RowsView& r) {
+// Packed rows [tokens, heads, Dh] as (Dh, heads, tokens), copied `heads` by
+// `tokens` rows at a time.
+bool map_allowed(const RowsView& r) {
+  return r.tokens > 0 && aligned16(r) && (r.tokens == 1 || r.sT > 0) &&
+         (r.heads == 1 || r.sH > 0) && r.sT < (1ll << 38) && r.sH < (1ll << 38);
+}
+CUtensorMap rows_map(const RowsView& r, int heads, int tokens) {
   const uint64_t dims[3] = {(uint64_t)r.Dh, (uint64_t)r.heads, (uint64_t)r.tokens};
   const uint64_t any = ((uint64_t)r.Dh * 2 + 15) / 16 * 16;  // of a dimension of one
   const uint64_t strides[2] = {r.heads > 1 ? (uint64_t)r.sH * 2 : any,
                                r.tokens > 1 ? (uint64_t)r.sT * 2 : any * r.heads};
-  const uint32_t box[3] = {64, 1, BN};
+  const uint32_t box[3] = {64, (uint32_t)heads, (uint32_t)tokens};
   return make_tmap_nd(r.data, 2, 3, dims, strides, box);
 }
 
@@ -719,28 +822,25 @@ CUtensorMap rows_map(const RowsView& r) {
 bool seq_tc_supported(const SeqAttnArgs& a) {
   if (a.q.type == kF32 || a.G > BM || a.q.Dh > 128 || a.q.Dh % 8 != 0) return false;
   if (a.pages.k) return seq_pages_tma(a);
-  if (a.k.tokens == 0) return false;
-  for (const RowsView* r : {&a.k, &a.v}) {
-    if (!aligned16(*r)) return false;
-    if ((r->tokens > 1 && r->sT <= 0) || (r->heads > 1 && r->sH <= 0)) return false;
-    if (r->sT >= (1ll << 38) || r->sH >= (1ll << 38)) return false;  // the map's stride limit
-  }
-  return true;
+  return map_allowed(a.k) && map_allowed(a.v);
 }
 
 int seq_tc_rows(int G) { return 2 * (BM / G) * G; }
 
 void seq_tc_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
-  const CUtensorMap k = a.pages.k ? seq_pages_map(a.pages, a.pages.k, elem_coded(a.pages.type) ? 64 : BN)
-                                  : rows_map(a.k);
-  const CUtensorMap v = a.pages.k ? seq_pages_map(a.pages, a.pages.v, elem_coded(a.pages.type) ? 64 : BN)
-                                  : rows_map(a.v);
+  const bool paged = a.pages.k != nullptr, coded = paged && elem_coded(a.pages.type);
+  const int box = coded ? 64 : BN;
+  const CUtensorMap k = paged ? seq_pages_map(a.pages, a.pages.k, box) : rows_map(a.k, 1, BN);
+  const CUtensorMap v = paged ? seq_pages_map(a.pages, a.pages.v, box) : rows_map(a.v, 1, BN);
+  // Over codes Q is scaled on its way in, by threads.
+  const bool qtma = !coded && map_allowed(a.q);
+  const CUtensorMap q = qtma ? rows_map(a.q, a.G, BM / a.G) : k;
   const bool qvec = aligned16(a.q), ovec = aligned16(a.o);
   auto go = [&](auto tq, auto tk) {
     constexpr int TQ = decltype(tq)::value, TK = decltype(tk)::value;
     if constexpr (TQ != kF32) {
-      if (a.q.Dh <= 64) launch<TQ, TK, 64>(a, ctas, k, v, qvec, ovec, s);
-      else launch<TQ, TK, 128>(a, ctas, k, v, qvec, ovec, s);
+      if (a.q.Dh <= 64) launch<TQ, TK, 64>(a, ctas, q, k, v, qtma, qvec, ovec, s);
+      else launch<TQ, TK, 128>(a, ctas, q, k, v, qtma, qvec, ovec, s);
     }
   };
   with_value_type(a.q.type, [&](auto tq) {
