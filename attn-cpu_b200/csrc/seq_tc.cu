@@ -11,8 +11,10 @@
 //   K and V tile serves both.  The two tiles run as chains, so that one's
 //   products run under the other's softmax:
 //       S = Q K^T (TMEM)  ->  softmax writes P over S (16 bits, TMEM)  ->  O += P V
-//   with O in TMEM as well: 2 x (128 + 128) columns.  V is read as it lies in
-//   memory, keys by rows (an N-major operand).
+//   with O in TMEM as well: 2 x (128 + 128) columns.  The chain goes in steps of
+//   64 keys through two halves of its S columns, so that the scores of a step
+//   are there before the softmax of the one before has ended.  V is read as it
+//   lies in memory, keys by rows (an N-major operand).
 //   Warp 0 loads; warps 1 and 2 issue the chains' products; warp 3 clears masked
 //   V values; warps 4-7 and 8-11 own one row of A or B per thread.  With codes,
 //   warps 12-15 turn them into f16 tiles.
@@ -42,8 +44,13 @@ namespace attnb {
 namespace {
 
 constexpr int BM = 128;
-constexpr int BN = 128;
+constexpr int BN = 128;  // keys of a tile in shared memory
+constexpr int BS = 64;   // keys of a step
 constexpr float kRescaleGap = 8.f;
+#ifndef POLY
+#define POLY 2
+#endif
+constexpr int kPolyPairs = POLY;  // of 8 pairs, how many exponentials the FMA units take
 constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
 
 template <bool CODED, int DHP>
@@ -79,6 +86,42 @@ __device__ __forceinline__ bool any_not_finite(const uint4& x) {
           0x80008000u) != 0;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of a pair on the FMA units: x = n + f with n the nearest whole number (the
+// last bits of x + 1.5 * 2^23), 2^f as a polynomial on [-1/2, 1/2] with the
+// least largest relative error (2^-13.7 of degree 3, 2^-18.6 of degree 4; fitted
+// by linear programming), n added to the exponent.  x below -126 counts as -126.
+template <int DEG>
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpack_f32x2(x, x0, x1);
+  x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  auto both = [](float v) { return pack_f32x2(v, v); };
+  const uint64_t t = add_f32x2(x, both(12582912.f));
+  const uint64_t f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
+  uint64_t p;
+  if constexpr (DEG == 3) {
+    p = fma_f32x2(both(0.0551714189350605f), f, both(0.24261116981506348f));
+    p = fma_f32x2(p, f, both(0.6932610273361206f));
+    p = fma_f32x2(p, f, both(0.9999280571937561f));
+  } else {
+    p = fma_f32x2(both(0.009567738510668278f), f, both(0.05591749772429466f));
+    p = fma_f32x2(p, f, both(0.24024811387062073f));
+    p = fma_f32x2(p, f, both(0.6931219100952148f));
+    p = fma_f32x2(p, f, both(0.9999992251396179f));
+  }
+  float t0, t1;
+  unpack_f32x2(t, t0, t1);
+  unpack_f32x2(p, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
 template <int TQ, int TK, int DHP>
 __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS, 1)
     seq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -89,13 +132,14 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
   using EQ = elem_t<TQ>;
   constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
   constexpr int KST = Cfg::K_ST, VST = Cfg::V_ST, RST = Cfg::RAW_ST;
-  constexpr uint32_t IDESC_S = idesc_f16(BM, BN, BF16, false);
+  constexpr uint32_t IDESC_S = idesc_f16(BM, BS, BF16, false);
   constexpr uint32_t IDESC_PV = idesc_f16(BM, DHP, BF16, true);
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
   __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
-  __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2], p_bar[2], pv_bar[2], done_bar[2];
+  __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2][2], p_bar[2][2], pv_bar[2][2],
+      done_bar[2];
   __shared__ SeqShared sh;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -126,9 +170,11 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     for (int c = 0; c < 2; ++c) {
       mbar_init(smem_addr(&q_bar[c]), qtma ? 1 : 4);
       mbar_init(smem_addr(&q_free[c]), 1);
-      mbar_init(smem_addr(&s_bar[c]), 1);
-      mbar_init(smem_addr(&p_bar[c]), 4);
-      mbar_init(smem_addr(&pv_bar[c]), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_addr(&s_bar[c][i]), 1);
+        mbar_init(smem_addr(&p_bar[c][i]), 4);
+        mbar_init(smem_addr(&pv_bar[c][i]), 1);
+      }
       mbar_init(smem_addr(&done_bar[c]), 1);
     }
     fence_barrier_init();
@@ -158,14 +204,14 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
   SeqIter it;
   it.start(place);
   SeqPiece w{};
-  // Tiles of the piece that chain c takes: the first ones.
-  auto tiles_of = [&](int c) {
+  // Steps of the piece that chain c takes: the first ones.
+  auto steps_of = [&](int c) {
     const int rows = min(w.rows - c * half, half);
     if (rows <= 0) return 0;
     int seen = w.s.L;
     if (a.causal) seen = seq_row_seen(a, w.s, w.row0 + c * half + rows - 1);
-    const int nt = max(1, (max(seen, 0) + BN - 1) / BN);
-    return min(nt, w.j1) - min(nt, w.j0);
+    const int n = max(1, (max(seen, 0) + BS - 1) / BS);
+    return min(n, 2 * w.j1) - min(n, 2 * w.j0);
   };
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
     const bool got = mbar_wait_quick(smem_addr(bar), parity, abort_p, a.status);
@@ -274,7 +320,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           rk.advance();
           if (qtma && j == w.j0) {
             for (int c = 0; ok && c < 2; ++c)
-              if (tiles_of(c) > 0) ok = load_q(c);
+              if (steps_of(c) > 0) ok = load_q(c);
             if (!ok) break;
           }
           ok = warp_wait(&vempty[rv.stage], rv.phase ^ 1u);
@@ -305,52 +351,69 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       const uint32_t qbase = base + c * Cfg::TILE;
       Ring<KST> rk;
       Ring<VST> rv;
-      uint32_t tiles = 0, qphase = 0;  // tiles done, whose parity the chain's barriers have
+      uint32_t g = 0, qphase = 0;  // g: steps done; step g uses half g & 1 of S
       bool ok = true;
-      while (ok && it.next(a, w)) {
-        const int n = tiles_of(c);
-        if (n > 0) {
-          if (!(ok = mbar_wait_quick(smem_addr(&q_bar[c]), qphase, abort_p, a.status))) break;
-          qphase ^= 1;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && mbar_wait_quick(smem_addr(bar), parity, abort_p, a.status);
+        return ok;
+      };
+      // Scores of step i (of n) of the piece, step s of the chain.
+      auto scores = [&](int i, int n, uint32_t s) {
+        // They overwrite the weights of step s - 2, whose product has to be done.
+        if (s >= 2 && !wait(&pv_bar[c][s & 1], ((s >> 1) - 1) & 1)) return;
+        if (!(i & 1) && !wait(&kfull[rk.stage], rk.phase)) return;
+        tc_fence_after();
+        const uint64_t qd = sdesc_kmajor_sw128(qbase);
+        const uint64_t kd = sdesc_kmajor_sw128(base + Cfg::OFF_K + rk.stage * Cfg::TILE +
+                                               (i & 1) * BS * 128);
+#pragma unroll
+        for (int k = 0; k < DHP / 16; ++k) {
+          const uint64_t at = ((k >> 2) * Cfg::CHUNK + (k & 3) * 32) >> 4;
+          mma_f16(sbuf + (s & 1) * BS, qd + at, kd + at, IDESC_S, k != 0 ? 1u : 0u);
         }
-        for (int j = 0; j < w.j1 - w.j0; ++j) {
-          const bool use = j < n;
-          if (!(ok = mbar_wait_quick(smem_addr(&kfull[rk.stage]), rk.phase, abort_p, a.status))) break;
-          if (use) {
-            // S overwrites P of the tile before, whose product has to be done.
-            if (tiles > 0 && !(ok = mbar_wait_quick(smem_addr(&pv_bar[c]), (tiles - 1) & 1, abort_p, a.status)))
-              break;
-            tc_fence_after();
-            const uint32_t kb = base + Cfg::OFF_K + rk.stage * Cfg::TILE;
-#pragma unroll
-            for (int k = 0; k < DHP / 16; ++k)
-              mma_f16(sbuf, sdesc_kmajor_sw128(qbase + (k >> 2) * Cfg::CHUNK + (k & 3) * 32),
-                      sdesc_kmajor_sw128(kb + (k >> 2) * Cfg::CHUNK + (k & 3) * 32), IDESC_S,
-                      k != 0 ? 1u : 0u);
-            mma_commit(smem_addr(&kempty[rk.stage]));
-            mma_commit(smem_addr(&s_bar[c]));
-            if (j == n - 1) mma_commit(smem_addr(&q_free[c]));
-          } else {
-            mbar_arrive(smem_addr(&kempty[rk.stage]));
-          }
+        mma_commit(smem_addr(&s_bar[c][s & 1]));
+        if ((i & 1) || i == n - 1) {
+          mma_commit(smem_addr(&kempty[rk.stage]));
           rk.advance();
-          if (!(ok = mbar_wait_quick(smem_addr(&vfull[rv.stage]), rv.phase, abort_p, a.status))) break;
-          if constexpr (!CODED)
-            if (!(ok = mbar_wait_quick(smem_addr(&vfix[rv.stage]), rv.phase, abort_p, a.status))) break;
-          if (use) {
-            if (!(ok = mbar_wait_quick(smem_addr(&p_bar[c]), tiles & 1, abort_p, a.status))) break;
-            tc_fence_after();
-            const uint32_t vb = base + Cfg::OFF_V + rv.stage * Cfg::TILE;
-#pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-              mma_f16_ts(obuf, sbuf + k * 8, sdesc_mnmajor_sw128(vb + k * 2048, Cfg::CHUNK),
-                         IDESC_PV, (j | k) != 0 ? 1u : 0u);
-            mma_commit(smem_addr(&vempty[rv.stage]));
-            mma_commit(smem_addr(&pv_bar[c]));
-            ++tiles;
-          } else {
-            mbar_arrive(smem_addr(&vempty[rv.stage]));
+        }
+        if (i == n - 1) mma_commit(smem_addr(&q_free[c]));
+      };
+      while (ok && it.next(a, w)) {
+        const int n = steps_of(c);
+        if (n > 0) {
+          if (!wait(&q_bar[c], qphase)) break;
+          qphase ^= 1;
+          scores(0, n, g);
+        }
+        for (int i = 0; ok && i < n; ++i, ++g) {
+          if (i + 1 < n) scores(i + 1, n, g + 1);
+          if (!ok) break;
+          if (!(i & 1)) {
+            if (!wait(&vfull[rv.stage], rv.phase)) break;
+            if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
           }
+          if (!wait(&p_bar[c][g & 1], (g >> 1) & 1)) break;
+          tc_fence_after();
+          const uint64_t vd = sdesc_mnmajor_sw128(
+              base + Cfg::OFF_V + rv.stage * Cfg::TILE + (i & 1) * BS * 128, Cfg::CHUNK);
+#pragma unroll
+          for (int k = 0; k < BS / 16; ++k)
+            mma_f16_ts(obuf, sbuf + (g & 1) * BS + k * 8, vd + k * (2048 >> 4), IDESC_PV,
+                       (i | k) != 0 ? 1u : 0u);
+          mma_commit(smem_addr(&pv_bar[c][g & 1]));
+          if ((i & 1) || i == n - 1) {
+            mma_commit(smem_addr(&vempty[rv.stage]));
+            rv.advance();
+          }
+        }
+        // Tiles that only the other chain takes.
+        for (int j = (n + 1) / 2; ok && j < w.j1 - w.j0; ++j) {
+          if (!wait(&kfull[rk.stage], rk.phase)) break;
+          mbar_arrive(smem_addr(&kempty[rk.stage]));
+          rk.advance();
+          if (!wait(&vfull[rv.stage], rv.phase)) break;
+          if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
+          mbar_arrive(smem_addr(&vempty[rv.stage]));
           rv.advance();
         }
       }
@@ -522,11 +585,11 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t srow = tmem + lane_off + c * BN;
     const uint32_t orow = tmem + lane_off + 2 * BN + c * 128;
-    uint32_t tiles = 0, tile0 = 0;  // of this chain; of the CTA
+    uint32_t g = 0, tile0 = 0;  // steps of this chain; tiles of the CTA
     bool ok = true;
     int piece = 0;
     for (bool first = true; it.next(a, w); first = false, ++piece) {
-      const int n = tiles_of(c);
+      const int n = steps_of(c);
       const int rows = min(w.rows - c * half, half);  // of this chain, <= 0: none
       const bool mine = r < rows;
       const int row = w.row0 + c * half + r;
@@ -582,52 +645,37 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&q_bar[c]));
       }
-      for (int j = 0; j < n; ++j, ++tiles) {
-        if (ok) ok = warp_wait(&s_bar[c], tiles & 1);
+      for (int i = 0; i < n; ++i, ++g) {
+        if (ok) ok = warp_wait(&s_bar[c][g & 1], (g >> 1) & 1);
         if (!ok) continue;
         tc_fence_after();
-        const int kb0 = (w.j0 + j) * BN;
-        // Masks only occur in some tiles; a warp applies them only there.
-        const bool masked = __any_sync(0xffffffffu, kb0 + BN > seen);
-        // Score to exponent: times mul, plus add (codes: per 64 keys).
-        float mul[2] = {scale, scale}, add[2] = {0.f, 0.f}, linv[2] = {1.f, 1.f};
+        const uint32_t sb = srow + (g & 1) * BS;
+        const int kb0 = w.j0 * BN + i * BS;
+        // Masks only occur in some steps; a warp applies them only there.
+        const bool masked = __any_sync(0xffffffffu, kb0 + BS > seen);
+        // Score to exponent: times mul, plus add.
+        float mul = scale, add = 0.f, linv = 1.f;
         if constexpr (CODED) {
-          const float4 x = *reinterpret_cast<const float4*>(
-              mem + Cfg::OFF_X + ((tile0 + j) % Cfg::SCALES) * Cfg::XTILE);
-          mul[0] = scale * x.x;
-          mul[1] = scale * x.y;
-          add[0] = x.z;
-          add[1] = x.w;
-          linv[0] = fast_exp2(-x.z);
-          linv[1] = fast_exp2(-x.w);
+          const float* x = reinterpret_cast<const float*>(
+              mem + Cfg::OFF_X + ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE) + (i & 1);
+          mul = scale * x[0];
+          add = x[2];
+          linv = fast_exp2(-add);
         }
-        // The row of S: at once, or (codes, with fewer registers) 64 columns at
-        // a time, read again for the weights; those take the columns that are
-        // done with.
-        constexpr int W = CODED ? 64 : BN;
-        uint32_t s[W];
-        auto load = [&](int part) {
-          if constexpr (CODED) tmem_ld64(srow + part * W, s);
-          else tmem_ld128(srow, s);
-          if (masked) {
+        uint32_t s[BS];
+        tmem_ld64(sb, s);
+        if (masked) {
 #pragma unroll
-            for (int i = 0; i < W; ++i)
-              if (kb0 + part * W + i >= seen) s[i] = __float_as_uint(-INFINITY);
-          }
-        };
-        float top = -INFINITY;
-#pragma unroll
-        for (int part = 0; part < BN / W; ++part) {
-          load(part);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < W; i += 8)  // three operands an instruction
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])),
-                            __uint_as_float(s[i + 2 * k + 1]));
-          top = fmaxf(top, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), mul[part], add[part]));
+          for (int k = 0; k < BS; ++k)
+            if (kb0 + k >= seen) s[k] = __float_as_uint(-INFINITY);
         }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < BS; k += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
+        const float top = fmaf(max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]), mul, add);
         const bool need = top > m + kRescaleGap;
         const bool rescale = __any_sync(0xffffffffu, need);
         float alpha = 1.f;
@@ -636,49 +684,50 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           m = top;
         }
         const float use = m == -INFINITY ? 0.f : m;
-        l *= alpha;
+        const float off = add - use;
+        const uint64_t mul2 = pack_f32x2(mul, mul), off2 = pack_f32x2(off, off);
+        uint64_t ls[2] = {0, 0};
 #pragma unroll
-        for (int part = 0; part < BN / W; ++part) {
-          if constexpr (CODED) load(part);
-          uint64_t ls[2] = {0, 0};
-          const float off = add[part] - use;
-          const uint64_t mul2 = pack_f32x2(mul[part], mul[part]), off2 = pack_f32x2(off, off);
-#pragma unroll
-          for (int i = 0; i < W; i += 2) {
-            float p0, p1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
-                                   mul2, off2),
-                         p0, p1);
+        for (int k = 0; k < BS; k += 2) {
+          const uint64_t x = fma_f32x2(
+              pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), mul2, off2);
+          float p0, p1;
+          if (k % 16 < kPolyPairs * 2 && !masked) {
+            exp2_poly<BF16 ? 3 : 4>(x, p0, p1);
+          } else {
+            unpack_f32x2(x, p0, p1);
             p0 = fast_exp2(p0);
             p1 = fast_exp2(p1);
-            ls[(i >> 1) & 1] = add_f32x2(ls[(i >> 1) & 1], pack_f32x2(p0, p1));
-            s[i >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
           }
-          float l0, l1;
-          unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
-          l = fmaf(l0 + l1, linv[part], l);
-          if constexpr (CODED) tmem_st32(srow + part * 32, *reinterpret_cast<const uint32_t(*)[32]>(s));
-          else tmem_st64(srow, s);
+          ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
+          s[k >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
         }
-        if (rescale && j > 0) {
-          // O holds the products up to the tile before (complete: S of this
-          // tile was issued after them).
+        tmem_st32(sb, *reinterpret_cast<const uint32_t(*)[32]>(s));
+        float l0, l1;
+        unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
+        l = fmaf(l0 + l1, linv, l * alpha);
+        // A score that is NaN or +inf makes the whole row NaN.
+        if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
+        if (rescale && i > 0) {
+          // O holds the products up to the step before, which has to be done.
+          ok = warp_wait(&pv_bar[c][(g - 1) & 1], ((g - 1) >> 1) & 1);
+          tc_fence_after();
 #pragma unroll 1
-          for (int d = 0; d < DHP; d += 32) {
+          for (int d = 0; ok && d < DHP; d += 32) {
             uint32_t o[32];
             tmem_ld32(orow + d, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
             tmem_st32(orow + d, o);
           }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&p_bar[c]));
+        if (lane == 0) mbar_arrive(smem_addr(&p_bar[c][g & 1]));
       }
       tile0 += w.j1 - w.j0;
-      if (ok && n > 0) ok = warp_wait(&pv_bar[c], (tiles - 1) & 1);
+      if (ok && n > 0) ok = warp_wait(&pv_bar[c][(g - 1) & 1], ((g - 1) >> 1) & 1);
       // ---- output: O / l, or the piece's partial result
       const int slot = seq_slot(w, first);
       if (ok && rows > 0) {
