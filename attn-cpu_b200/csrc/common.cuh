@@ -175,6 +175,20 @@ __device__ __forceinline__ void grid_dep_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// True in one lane of a converged warp.  Instructions that take their operands
+// from uniform registers (tcgen05.mma and its commit, TMA copies) are issued
+// plainly under this condition; under one on the lane number the compiler has to
+// allow for several lanes, which cost 80 cycles for each tcgen05.mma.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Barrier among the `nthreads` threads (a multiple of 32) that use barrier `id`.
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

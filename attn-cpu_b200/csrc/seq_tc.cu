@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     }
   } else if (warp <= 2) {
     // -------------------------------------------------- products of chain c
-    if (lane == 0) {
+    // The whole warp keeps step, one lane issues.
+    {
       const int c = warp - 1;
       const uint32_t sbuf = tmem + c * BN;
       const uint32_t obuf = tmem + 2 * BN + c * 128;
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       uint32_t g = 0, qphase = 0;  // g: steps done; step g uses half g & 1 of S
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait_quick(smem_addr(bar), parity, abort_p, a.status);
+        ok = ok && warp_wait(bar, parity);
         return ok;
       };
       // Scores of step i (of n) of the piece, step s of the chain.
@@ -366,17 +367,19 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         const uint64_t qd = sdesc_kmajor_sw128(qbase);
         const uint64_t kd = sdesc_kmajor_sw128(base + Cfg::OFF_K + rk.stage * Cfg::TILE +
                                                (i & 1) * BS * 128);
+        const bool tile_end = (i & 1) || i == n - 1;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < DHP / 16; ++k) {
-          const uint64_t at = ((k >> 2) * Cfg::CHUNK + (k & 3) * 32) >> 4;
-          mma_f16(sbuf + (s & 1) * BS, qd + at, kd + at, IDESC_S, k != 0 ? 1u : 0u);
+          for (int k = 0; k < DHP / 16; ++k) {
+            const uint64_t at = ((k >> 2) * Cfg::CHUNK + (k & 3) * 32) >> 4;
+            mma_f16(sbuf + (s & 1) * BS, qd + at, kd + at, IDESC_S, k != 0 ? 1u : 0u);
+          }
+          mma_commit(smem_addr(&s_bar[c][s & 1]));
+          if (tile_end) mma_commit(smem_addr(&kempty[rk.stage]));
+          if (i == n - 1) mma_commit(smem_addr(&q_free[c]));
         }
-        mma_commit(smem_addr(&s_bar[c][s & 1]));
-        if ((i & 1) || i == n - 1) {
-          mma_commit(smem_addr(&kempty[rk.stage]));
-          rk.advance();
-        }
-        if (i == n - 1) mma_commit(smem_addr(&q_free[c]));
+        __syncwarp();
+        if (tile_end) rk.advance();
       };
       while (ok && it.next(a, w)) {
         const int n = steps_of(c);
@@ -396,29 +399,33 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           tc_fence_after();
           const uint64_t vd = sdesc_mnmajor_sw128(
               base + Cfg::OFF_V + rv.stage * Cfg::TILE + (i & 1) * BS * 128, Cfg::CHUNK);
+          const bool tile_end = (i & 1) || i == n - 1;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BS / 16; ++k)
-            mma_f16_ts(obuf, sbuf + (g & 1) * BS + k * 8, vd + k * (2048 >> 4), IDESC_PV,
-                       (i | k) != 0 ? 1u : 0u);
-          mma_commit(smem_addr(&pv_bar[c][g & 1]));
-          if ((i & 1) || i == n - 1) {
-            mma_commit(smem_addr(&vempty[rv.stage]));
-            rv.advance();
+            for (int k = 0; k < BS / 16; ++k)
+              mma_f16_ts(obuf, sbuf + (g & 1) * BS + k * 8, vd + k * (2048 >> 4), IDESC_PV,
+                         (i | k) != 0 ? 1u : 0u);
+            mma_commit(smem_addr(&pv_bar[c][g & 1]));
+            if (tile_end) mma_commit(smem_addr(&vempty[rv.stage]));
           }
+          __syncwarp();
+          if (tile_end) rv.advance();
         }
         // Tiles that only the other chain takes.
         for (int j = (n + 1) / 2; ok && j < w.j1 - w.j0; ++j) {
           if (!wait(&kfull[rk.stage], rk.phase)) break;
-          mbar_arrive(smem_addr(&kempty[rk.stage]));
+          if (lane == 0) mbar_arrive(smem_addr(&kempty[rk.stage]));
           rk.advance();
           if (!wait(&vfull[rv.stage], rv.phase)) break;
           if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
-          mbar_arrive(smem_addr(&vempty[rv.stage]));
+          if (lane == 0) mbar_arrive(smem_addr(&vempty[rv.stage]));
           rv.advance();
         }
       }
       // Every product issued completes before TMEM is released.
-      mma_commit(smem_addr(&done_bar[c]));
+      __syncwarp();
+      if (elect_one()) mma_commit(smem_addr(&done_bar[c]));
+      __syncwarp();
       drain_wait(smem_addr(&done_bar[c]), 0, a.status);
     }
   } else if (warp == 3) {
