@@ -247,8 +247,9 @@ struct SeqAttnArgs {
   int G;                // query heads per KV head
   int causal;
   float scale_log2;     // softmax scale times log2(e)
-  // Schedule: rows per item, log2 of the keys per tile, fewest tiles per CTA.
-  int rows, kt_shift, min_tiles;
+  // Schedule: rows per item, log2 of the keys per tile, fewest tiles per CTA,
+  // tiles that an item counts for besides its own.
+  int rows, kt_shift, min_tiles, extra;
   // Workspace: partial O [2 * ctas][rows][Dh], (m, l) [2 * ctas][rows], one
   // SeqSplit per CTA.
   float* ws_o;

@@ -10,7 +10,8 @@
 // in the order (sequence, KV head, item), form one line that is cut into equal
 // pieces, one for each CTA: ragged batches, causal triangles and single long
 // contexts all load the CTAs evenly, and nothing about the lengths has to be
-// known on the host.  An item that a cut falls into is joined afterwards
+// known on the host.  An item counts `extra` tiles more than it has, ahead of
+// its first, for what it costs besides (its queries, its output).  An item that a cut falls into is joined afterwards
 // (seq_merge.cu) from the pieces' running maximum, sum and accumulator; a CTA
 // has at most two such pieces, its first and its last, so the workspace does
 // not grow with the batch.
@@ -32,8 +33,9 @@ struct SeqInfo {
 
 // One CTA's first piece, for the merge.
 struct SeqSplit {
-  long long item0, item1;  // the item's tiles on the line
+  long long item0, item1;  // the item's own tiles on the line
   long long quota;         // tiles per CTA
+  int extra;
   int row_token, rows;     // the item's first row is row `first_row` of its sequence
   int first_row, kv_head;
   int continues;           // the piece is not the item's first
@@ -119,8 +121,8 @@ __device__ __forceinline__ int seq_tiles(const SeqAttnArgs& a, const SeqInfo& i,
   return max(1, (int)(((long long)max(seen, 0) + (1 << a.kt_shift) - 1) >> a.kt_shift));
 }
 
-// Tiles of the items before item m (m <= items) of one KV head.
-__device__ __forceinline__ long long seq_tiles_before(const SeqAttnArgs& a, const SeqInfo& i,
+// Tiles on the line of the items before item m (m <= items) of one KV head.
+__device__ __forceinline__ long long seq_own_tiles_before(const SeqAttnArgs& a, const SeqInfo& i,
                                                       int m) {
   if (m <= 0) return 0;
   const int M = seq_items(a, i);
@@ -143,11 +145,16 @@ __device__ __forceinline__ long long seq_tiles_before(const SeqAttnArgs& a, cons
   return s;
 }
 
+__device__ __forceinline__ long long seq_tiles_before(const SeqAttnArgs& a, const SeqInfo& i,
+                                                      int m) {
+  return seq_own_tiles_before(a, i, m) + (long long)a.extra * max(m, 0);
+}
+
 // Where a CTA stands on the line.
 struct SeqPlace {
   long long t0, t1, quota;
-  long long item0;  // the first tile of the item that t0 lies in
-  int b, h, m, j;   // the item, and the tile of it that t0 is
+  long long item0;  // the place of the item that t0 lies in
+  int b, h, m, j;   // the item, and how far into it t0 is
 };
 
 // Sum over the block (all threads, blockDim.x a multiple of 32); excl: of the
@@ -270,36 +277,39 @@ struct SeqIter {
     fresh = true;
   }
   __device__ __forceinline__ bool next(const SeqAttnArgs& a, SeqPiece& w) {
-    if (t >= t1) return false;
-    if (fresh) {
-      s = seq_info(a, b);
-      items = seq_items(a, s);
-      fresh = false;
-    }
-    w.s = s;
-    w.b = b;
-    w.h = h;
-    w.m = m;
-    w.nt = seq_tiles(a, s, m);
-    w.j0 = j;
-    w.j1 = (int)min((long long)w.nt, j + (t1 - t));
-    w.row0 = m * a.rows;
-    w.rows = min(a.rows, s.n * a.G - w.row0);
-    t += w.j1 - w.j0;
-    j = 0;
-    if (++m == items) {
-      m = 0;
-      if (++h == a.pages.H) {
-        h = 0;
-        // The next sequence that has rows.
-        while (t < t1 && ++b < a.seqs.batch) {
-          s = seq_info(a, b);
-          items = seq_items(a, s);
-          if (items > 0) break;
+    while (t < t1) {
+      if (fresh) {
+        s = seq_info(a, b);
+        items = seq_items(a, s);
+        fresh = false;
+      }
+      w.s = s;
+      w.b = b;
+      w.h = h;
+      w.m = m;
+      w.nt = seq_tiles(a, s, m);
+      const int end = (int)min((long long)w.nt + a.extra, j + (t1 - t));
+      w.j0 = max(0, j - a.extra);
+      w.j1 = max(0, end - a.extra);
+      w.row0 = m * a.rows;
+      w.rows = min(a.rows, s.n * a.G - w.row0);
+      t += end - j;
+      j = 0;
+      if (++m == items) {
+        m = 0;
+        if (++h == a.pages.H) {
+          h = 0;
+          // The next sequence that has rows.
+          while (t < t1 && ++b < a.seqs.batch) {
+            s = seq_info(a, b);
+            items = seq_items(a, s);
+            if (items > 0) break;
+          }
         }
       }
+      if (w.j1 > w.j0) return true;  // the cut may leave an item's extra alone
     }
-    return true;
+    return false;
   }
 };
 
@@ -318,11 +328,12 @@ __device__ __forceinline__ int seq_slot(const SeqPiece& w, bool first) {
 __device__ __forceinline__ void seq_write_split(const SeqAttnArgs& a, bool any,
                                                 const SeqPlace& p) {
   SeqSplit d{};
-  if (any && p.j > 0) {
+  d.extra = a.extra;
+  if (any && p.j > a.extra) {
     const SeqInfo s = seq_info(a, p.b);
     d.continues = 1;
-    d.item0 = p.item0;
-    d.item1 = p.item0 + seq_tiles(a, s, p.m);
+    d.item0 = p.item0 + a.extra;
+    d.item1 = d.item0 + seq_tiles(a, s, p.m);
     d.quota = p.quota;
     d.first_row = p.m * a.rows;
     d.rows = min(a.rows, s.n * a.G - d.first_row);

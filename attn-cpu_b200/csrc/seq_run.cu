@@ -20,7 +20,8 @@ __global__ void __launch_bounds__(128) seq_merge_kernel(const SeqAttnArgs a) {
   const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];
   if (!d.continues || d.item0 < (c - 1) * d.quota) return;
   const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1;
-  const int slot0 = 2 * (c - 1) + (d.item0 == (c - 1) * d.quota ? 0 : 1);
+  // The first piece of CTA c - 1, or a later one.
+  const int slot0 = 2 * (c - 1) + (d.item0 - d.extra <= (c - 1) * d.quota ? 0 : 1);
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
   const int Dh = a.q.Dh;
   for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
@@ -79,6 +80,7 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   a.rows = sp.rows;
   a.kt_shift = kind == kTc ? 7 : 6;
   a.min_tiles = 2;
+  a.extra = kind == kTc ? 2 : 1;
   uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
   if (p + sp.bytes(a.q.Dh) > reinterpret_cast<uintptr_t>(ws) + ws_bytes)
     fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");

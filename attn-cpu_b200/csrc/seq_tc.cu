@@ -15,9 +15,10 @@
 //   64 keys through two halves of its S columns, so that the scores of a step
 //   are there before the softmax of the one before has ended.  V is read as it
 //   lies in memory, keys by rows (an N-major operand).
-//   Warp 0 loads; warps 1 and 2 issue the chains' products; warp 3 clears masked
-//   V values; warps 4-7 and 8-11 own one row of A or B per thread.  With codes,
-//   warps 12-15 turn them into f16 tiles.
+//   Warp 0 loads; warps 1 and 2 issue the chains' scores and two others their
+//   P V (a thread that waits for the one would hold up the other); warps 4-7 and
+//   8-11 own one row of A or B per thread; one warp clears masked V values.
+//   With codes, warps 12-15 turn them into f16 tiles.
 //   CTAs are persistent and walk the pieces of the schedule in seq.cuh.
 //
 // The running maximum moves only when it grows by more than 8 (weights stay
@@ -26,8 +27,8 @@
 //
 // Codes: both products run in f16.  Q is brought to [1, 2) by a power of two per
 // row, and 64 keys at a time K becomes code * scale / 2^E with 2^E the largest
-// scale's power of two, rounded to f16 once (2^-11 of a value, where the codes
-// themselves are 2^-4 or 2^-8 off); keys whose scale is 2^14 below the largest
+// scale's power of two, rounded to f16 twice (2^-11 of a value each, where the
+// codes themselves are 2^-4 or 2^-8 off); keys whose scale is 2^14 below the largest
 // lose bits that are 2^-25 of the largest.  2^E goes into the rows' scale, and
 // V's 2^F into the exponent, s' = s + F, with 2^-F on the sum: nothing is left
 // to do for single keys in the softmax.
@@ -47,15 +48,12 @@ constexpr int BM = 128;
 constexpr int BN = 128;  // keys of a tile in shared memory
 constexpr int BS = 64;   // keys of a step
 constexpr float kRescaleGap = 8.f;
-#ifndef POLY
-#define POLY 2
-#endif
-constexpr int kPolyPairs = POLY;  // of 8 pairs, how many exponentials the FMA units take
 constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
 
 template <bool CODED, int DHP>
 struct TcCfg {
-  static constexpr int THREADS = CODED ? 512 : 384;
+  static constexpr int THREADS = CODED ? 544 : 448;
+  static constexpr int PV_A = CODED ? 3 : 12, PV_B = CODED ? 16 : 13;  // warps that issue P V
   static constexpr int CHUNKS = DHP / 64;        // 128-byte pieces of a 16-bit row
   static constexpr int CHUNK = BN * 128;         // 16 KB: 128 rows x 64 columns
   static constexpr int TILE = CHUNKS * CHUNK;    // Q, K or V
@@ -92,36 +90,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// 2^x of a pair on the FMA units: x = n + f with n the nearest whole number (the
-// last bits of x + 1.5 * 2^23), 2^f as a polynomial on [-1/2, 1/2] with the
-// least largest relative error (2^-13.7 of degree 3, 2^-18.6 of degree 4; fitted
-// by linear programming), n added to the exponent.  x below -126 counts as -126.
-template <int DEG>
-__device__ __forceinline__ void exp2_poly(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  unpack_f32x2(x, x0, x1);
-  x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  auto both = [](float v) { return pack_f32x2(v, v); };
-  const uint64_t t = add_f32x2(x, both(12582912.f));
-  const uint64_t f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
-  uint64_t p;
-  if constexpr (DEG == 3) {
-    p = fma_f32x2(both(0.0551714189350605f), f, both(0.24261116981506348f));
-    p = fma_f32x2(p, f, both(0.6932610273361206f));
-    p = fma_f32x2(p, f, both(0.9999280571937561f));
-  } else {
-    p = fma_f32x2(both(0.009567738510668278f), f, both(0.05591749772429466f));
-    p = fma_f32x2(p, f, both(0.24024811387062073f));
-    p = fma_f32x2(p, f, both(0.6931219100952148f));
-    p = fma_f32x2(p, f, both(0.9999992251396179f));
-  }
-  float t0, t1;
-  unpack_f32x2(t, t0, t1);
-  unpack_f32x2(p, p0, p1);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 template <int TQ, int TK, int DHP>
 __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS, 1)
     seq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -139,7 +107,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
   __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
   __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
   __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2][2], p_bar[2][2], pv_bar[2][2],
-      done_bar[2];
+      done_bar[4];
   __shared__ SeqShared sh;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -176,6 +144,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         mbar_init(smem_addr(&pv_bar[c][i]), 1);
       }
       mbar_init(smem_addr(&done_bar[c]), 1);
+      mbar_init(smem_addr(&done_bar[2 + c]), 1);
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
@@ -343,28 +312,29 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       }
     }
   } else if (warp <= 2) {
-    // -------------------------------------------------- products of chain c
-    // The whole warp keeps step, one lane issues.
-    {
-      const int c = warp - 1;
-      const uint32_t sbuf = tmem + c * BN;
-      const uint32_t obuf = tmem + 2 * BN + c * 128;
-      const uint32_t qbase = base + c * Cfg::TILE;
-      Ring<KST> rk;
-      Ring<VST> rv;
-      uint32_t g = 0, qphase = 0;  // g: steps done; step g uses half g & 1 of S
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && warp_wait(bar, parity);
-        return ok;
-      };
-      // Scores of step i (of n) of the piece, step s of the chain.
-      auto scores = [&](int i, int n, uint32_t s) {
-        // They overwrite the weights of step s - 2, whose product has to be done.
-        if (s >= 2 && !wait(&pv_bar[c][s & 1], ((s >> 1) - 1) & 1)) return;
-        if (!(i & 1) && !wait(&kfull[rk.stage], rk.phase)) return;
+    // ------------------------------------ scores of chain c: the whole warp keeps
+    // step, one lane issues
+    const int c = warp - 1;
+    const uint32_t sbuf = tmem + c * BN;
+    Ring<KST> rk;
+    uint32_t g = 0, qphase = 0;  // step g uses half g & 1 of S
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && warp_wait(bar, parity);
+      return ok;
+    };
+    const uint64_t qd = sdesc_kmajor_sw128(base + c * Cfg::TILE);
+    while (ok && it.next(a, w)) {
+      const int n = steps_of(c);
+      if (n > 0) {
+        if (!wait(&q_bar[c], qphase)) break;
+        qphase ^= 1;
+      }
+      for (int i = 0; i < n; ++i, ++g) {
+        if (!(i & 1) && !wait(&kfull[rk.stage], rk.phase)) break;
+        // They overwrite the weights of step g - 2, whose product has to be done.
+        if (g >= 2 && !wait(&pv_bar[c][g & 1], ((g >> 1) - 1) & 1)) break;
         tc_fence_after();
-        const uint64_t qd = sdesc_kmajor_sw128(qbase);
         const uint64_t kd = sdesc_kmajor_sw128(base + Cfg::OFF_K + rk.stage * Cfg::TILE +
                                                (i & 1) * BS * 128);
         const bool tile_end = (i & 1) || i == n - 1;
@@ -372,62 +342,76 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 #pragma unroll
           for (int k = 0; k < DHP / 16; ++k) {
             const uint64_t at = ((k >> 2) * Cfg::CHUNK + (k & 3) * 32) >> 4;
-            mma_f16(sbuf + (s & 1) * BS, qd + at, kd + at, IDESC_S, k != 0 ? 1u : 0u);
+            mma_f16(sbuf + (g & 1) * BS, qd + at, kd + at, IDESC_S, k != 0 ? 1u : 0u);
           }
-          mma_commit(smem_addr(&s_bar[c][s & 1]));
+          mma_commit(smem_addr(&s_bar[c][g & 1]));
           if (tile_end) mma_commit(smem_addr(&kempty[rk.stage]));
           if (i == n - 1) mma_commit(smem_addr(&q_free[c]));
         }
         __syncwarp();
         if (tile_end) rk.advance();
-      };
-      while (ok && it.next(a, w)) {
-        const int n = steps_of(c);
-        if (n > 0) {
-          if (!wait(&q_bar[c], qphase)) break;
-          qphase ^= 1;
-          scores(0, n, g);
-        }
-        for (int i = 0; ok && i < n; ++i, ++g) {
-          if (i + 1 < n) scores(i + 1, n, g + 1);
-          if (!ok) break;
-          if (!(i & 1)) {
-            if (!wait(&vfull[rv.stage], rv.phase)) break;
-            if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
-          }
-          if (!wait(&p_bar[c][g & 1], (g >> 1) & 1)) break;
-          tc_fence_after();
-          const uint64_t vd = sdesc_mnmajor_sw128(
-              base + Cfg::OFF_V + rv.stage * Cfg::TILE + (i & 1) * BS * 128, Cfg::CHUNK);
-          const bool tile_end = (i & 1) || i == n - 1;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < BS / 16; ++k)
-              mma_f16_ts(obuf, sbuf + (g & 1) * BS + k * 8, vd + k * (2048 >> 4), IDESC_PV,
-                         (i | k) != 0 ? 1u : 0u);
-            mma_commit(smem_addr(&pv_bar[c][g & 1]));
-            if (tile_end) mma_commit(smem_addr(&vempty[rv.stage]));
-          }
-          __syncwarp();
-          if (tile_end) rv.advance();
-        }
-        // Tiles that only the other chain takes.
-        for (int j = (n + 1) / 2; ok && j < w.j1 - w.j0; ++j) {
-          if (!wait(&kfull[rk.stage], rk.phase)) break;
-          if (lane == 0) mbar_arrive(smem_addr(&kempty[rk.stage]));
-          rk.advance();
+      }
+      // Tiles that only the other chain takes.
+      for (int j = (n + 1) / 2; ok && j < w.j1 - w.j0; ++j) {
+        if (!wait(&kfull[rk.stage], rk.phase)) break;
+        if (lane == 0) mbar_arrive(smem_addr(&kempty[rk.stage]));
+        rk.advance();
+      }
+    }
+    // Every product issued completes before TMEM is released.
+    __syncwarp();
+    if (elect_one()) mma_commit(smem_addr(&done_bar[c]));
+    __syncwarp();
+    drain_wait(smem_addr(&done_bar[c]), 0, a.status);
+  } else if (warp == Cfg::PV_A || warp == Cfg::PV_B) {
+    // ------------------------------------------------------- P V of chain c
+    const int c = warp == Cfg::PV_A ? 0 : 1;
+    const uint32_t sbuf = tmem + c * BN;
+    const uint32_t obuf = tmem + 2 * BN + c * 128;
+    Ring<VST> rv;
+    uint32_t g = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && warp_wait(bar, parity);
+      return ok;
+    };
+    while (ok && it.next(a, w)) {
+      const int n = steps_of(c);
+      const int seen_max = seq_row_seen(a, w.s, w.row0 + w.rows - 1);
+      for (int i = 0; i < n; ++i, ++g) {
+        if (!(i & 1)) {
           if (!wait(&vfull[rv.stage], rv.phase)) break;
           if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
-          if (lane == 0) mbar_arrive(smem_addr(&vempty[rv.stage]));
-          rv.advance();
         }
+        if (!wait(&p_bar[c][g & 1], (g >> 1) & 1)) break;
+        tc_fence_after();
+        const uint64_t vd = sdesc_mnmajor_sw128(
+            base + Cfg::OFF_V + rv.stage * Cfg::TILE + (i & 1) * BS * 128, Cfg::CHUNK);
+        const bool tile_end = (i & 1) || i == n - 1;
+        // Keys behind the last one that a row of the item sees are not read.
+        const int left = seen_max - w.j0 * BN - i * BS;
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BS / 16; ++k)
+            if (k == 0 || k * 16 < left) mma_f16_ts(obuf, sbuf + (g & 1) * BS + k * 8, vd + k * (2048 >> 4), IDESC_PV,
+                       (i | k) != 0 ? 1u : 0u);
+          mma_commit(smem_addr(&pv_bar[c][g & 1]));
+          if (tile_end) mma_commit(smem_addr(&vempty[rv.stage]));
+        }
+        __syncwarp();
+        if (tile_end) rv.advance();
       }
-      // Every product issued completes before TMEM is released.
-      __syncwarp();
-      if (elect_one()) mma_commit(smem_addr(&done_bar[c]));
-      __syncwarp();
-      drain_wait(smem_addr(&done_bar[c]), 0, a.status);
+      for (int j = (n + 1) / 2; ok && j < w.j1 - w.j0; ++j) {
+        if (!wait(&vfull[rv.stage], rv.phase)) break;
+        if (!CODED && !wait(&vfix[rv.stage], rv.phase)) break;
+        if (lane == 0) mbar_arrive(smem_addr(&vempty[rv.stage]));
+        rv.advance();
+      }
     }
+    __syncwarp();
+    if (elect_one()) mma_commit(smem_addr(&done_bar[2 + c]));
+    __syncwarp();
+    drain_wait(smem_addr(&done_bar[2 + c]), 0, a.status);
   } else if (warp == 3) {
     // ------------------------------------------ values of V that a mask hides
     if constexpr (!CODED) {
@@ -460,32 +444,46 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           const int key0 = j * BN;
           if (key0 + BN > seen_min) {
             uint8_t* v = mem + Cfg::OFF_V + rv.stage * Cfg::TILE;
+            // Rows that some row of the item does not see, up to the last one
+            // that the products read (16 at a time).
             const int from = max(0, seen_min - key0);
-            bool hit = false;
-            for (int i = lane; i < (BN - from) * 8; i += 32) {
-              const int r = from + (i >> 3), u = i & 7;
+            const int seen_max = max(seq_row_seen(a, w.s, w.row0 + w.rows - 1), 1);
+            const int last = min(BN, ((seen_max + 15) & ~15) - key0);
+            const int units = max(0, last - from) * 8;  // per chunk
+            const int gone = w.s.L - key0;  // rows from here on are not the sequence's
+            bool found = false;
+            for (int i0 = lane; i0 < units; i0 += 128) {
 #pragma unroll
-              for (int ch = 0; ch < Cfg::CHUNKS; ++ch) {
-                uint4* p = reinterpret_cast<uint4*>(v + ch * Cfg::CHUNK + sw128(r, u));
-                if (key0 + r >= w.s.L) {
-                  *p = make_uint4(0, 0, 0, 0);
-                  continue;
-                }
-                uint4 x = *p;
-                if (!any_not_finite<TQ>(x)) continue;
-                EQ* e = reinterpret_cast<EQ*>(&x);
+              for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * 32, r = from + (i >> 3), u = i & 7;
+                if (i >= units) continue;
 #pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                  const float f = to_float(e[b]);
-                  if (fabsf(f) <= 3.402823466e38f) continue;
-                  const int kind = f != f ? 0 : (f > 0.f ? 1 : 2);
-                  atomicMin(&ps[kind * DHP + ch * 64 + u * 8 + b], key0 + r);
-                  from_float(0.f, e[b]);
+                for (int ch = 0; ch < Cfg::CHUNKS; ++ch) {
+                  uint4* p = reinterpret_cast<uint4*>(v + ch * Cfg::CHUNK + sw128(r, u));
+                  if (r >= gone) *p = make_uint4(0, 0, 0, 0);
+                  else found |= any_not_finite<TQ>(*p);
                 }
-                *p = x;
-                hit = true;
               }
             }
+            const bool hit = __any_sync(0xffffffffu, found);
+            if (hit)
+              for (int i = lane; i < units; i += 32) {
+                const int r = from + (i >> 3), u = i & 7;
+                for (int ch = 0; ch < Cfg::CHUNKS; ++ch) {
+                  uint4* p = reinterpret_cast<uint4*>(v + ch * Cfg::CHUNK + sw128(r, u));
+                  uint4 x = *p;
+                  EQ* e = reinterpret_cast<EQ*>(&x);
+#pragma unroll
+                  for (int b = 0; b < 8; ++b) {
+                    const float f = to_float(e[b]);
+                    if (fabsf(f) <= 3.402823466e38f) continue;
+                    const int kind = f != f ? 0 : (f > 0.f ? 1 : 2);
+                    atomicMin(&ps[kind * DHP + ch * 64 + u * 8 + b], key0 + r);
+                    from_float(0.f, e[b]);
+                  }
+                  *p = x;
+                }
+              }
             if (hit) poison_set[at] = 1;
             fence_proxy_async_smem();  // the products read V through the async proxy
           }
@@ -548,7 +546,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               } else {
                 mul = vmul[hf];
               }
-              const uint64_t mul2 = pack_f32x2(mul, mul);
+              // The factor as the sum of two f16: its own rounding would be one
+              // error of all the key's values.
+              const __half2 hi = __float2half2_rn(mul);
+              const __half2 lo = __float2half2_rn(mul - __low2float(hi));
 #pragma unroll
               for (int i = 0; i < DHP / 32; ++i) {
                 const int u = part * (DHP / 32) + i;  // 16 codes
@@ -559,10 +560,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                   const uint32_t h = codes_to_f16<TK>((xs[k >> 1] >> (16 * (k & 1))) & 0xffffu);
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                  float lo, hi;
-                  unpack_f32x2(mul_f32x2(pack_f32x2(f.x, f.y), mul2), lo, hi);
-                  y[k] = pack_f16(lo, hi);
+                  const __half2 code = *reinterpret_cast<const __half2*>(&h);
+                  const __half2 v = __hfma2(code, lo, __hmul2(code, hi));
+                  y[k] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 uint8_t* ch = to + (u >> 2) * Cfg::CHUNK;
                 *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2)) =
@@ -699,13 +699,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           const uint64_t x = fma_f32x2(
               pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), mul2, off2);
           float p0, p1;
-          if (k % 16 < kPolyPairs * 2 && !masked) {
-            exp2_poly<BF16 ? 3 : 4>(x, p0, p1);
-          } else {
-            unpack_f32x2(x, p0, p1);
-            p0 = fast_exp2(p0);
-            p1 = fast_exp2(p1);
-          }
+          unpack_f32x2(x, p0, p1);
+          p0 = fast_exp2(p0);
+          p1 = fast_exp2(p1);
           ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
           s[k >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
         }
