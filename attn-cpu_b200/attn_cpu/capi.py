@@ -6,6 +6,7 @@ for device memory and streams) and enqueue on the current torch stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -457,40 +458,65 @@ class KVCacheDev:
 
 
 # ------------------------------------------------- ragged sequences, paged KV cache
-_TYPES = None  # torch dtype -> ATTNB_TYPE_*
+# These calls are made once per layer and step, where a few microseconds of the
+# host count: the checks below read each property of a tensor once.
+_torch = _raw_stream = None
+_TYPES: dict = {}  # torch dtype -> ATTNB_TYPE_*
+_workspace_bytes: dict = {}
 
 
-def _type_of(t, name: str) -> int:
-    global _TYPES
-    if _TYPES is None:
-        import torch
+def _setup() -> None:
+    global _torch, _TYPES, _raw_stream
+    import torch
 
-        _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
-                  torch.int8: 4}
-    try:
-        return _TYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"{name}: {t.dtype} is not supported") from None
+    _torch = torch
+    # torch's current stream as an address, without an object around it.
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
+              torch.int8: 4}
+    lib()
+
+
+def _on(device, stream):
+    """None when `device` is current and no stream is given (the usual case),
+    else a context that makes both current: what is allocated inside belongs to
+    that stream."""
+    if _torch is None:
+        _setup()
+    if device.type != "cuda":
+        raise ValueError("CUDA tensors expected")
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, not on {device}")
+        return _torch.cuda.stream(stream)
+    if device.index != _torch.cuda.current_device():
+        return _torch.cuda.device(device)
+    return None
 
 
 def _rows(t, name: str, device) -> Rows:
     """attnb_rows view of a CUDA tensor [tokens, heads, Dh]."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, Dh]")
+    try:
+        n, h, d = t.shape
+    except ValueError:
+        raise ValueError(f"{name} must be [tokens, heads, Dh]") from None
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     sT, sH, sD = t.stride()
-    if sD != 1 and t.shape[2] > 1:
+    if sD != 1 and d > 1:
         raise ValueError(f"{name} needs a unit stride of the head size")
-    n, h, d = t.shape
-    return Rows(t.data_ptr(), _type_of(t, name), n, h, d, sT, sH)
+    ty = _TYPES.get(t.dtype)
+    if ty is None:
+        raise ValueError(f"{name}: {t.dtype} is not supported")
+    return Rows(t.data_ptr(), ty, n, h, d, sT, sH)
 
 
 def _offsets(t, name: str, device, n=None) -> int:
     """Device address of a contiguous int32 vector (of n entries)."""
-    if t.dim() != 1 or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+    if t.dtype != _torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector")
-    if n is not None and t.shape[0] != n:
+    if n is not None and len(t) != n:
         raise ValueError(f"{name} must have {n} entries, one more than sequences for offsets")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -498,81 +524,57 @@ def _offsets(t, name: str, device, n=None) -> int:
 
 
 def _pages(k_pages, v_pages, k_scale, v_scale, device) -> KvPages:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError("k_pages and v_pages must be [pages, H, page_size, Dh] of one type")
-    n, H, page, Dh = k_pages.shape
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale),
-                    ("v_scale", v_scale)):
+    n, H, page, Dh = shape
+    ty = _TYPES.get(k_pages.dtype)
+    if ty is None:
+        raise ValueError(f"k_pages: {k_pages.dtype} is not supported")
+    at = []
+    for t in (k_pages, v_pages, k_scale, v_scale):
         if t is None:
+            at.append(None)
             continue
         if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+            raise ValueError(f"pages and scales must be on {device}, not on {t.device}")
         if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        if name.endswith("scale") and (tuple(t.shape) != (n, H, page)
-                                       or str(t.dtype) != "torch.float32"):
-            raise ValueError(f"{name} must be float32 [pages, H, page_size]")
-    return KvPages(k_pages.data_ptr(), v_pages.data_ptr(),
-                   None if k_scale is None else k_scale.data_ptr(),
-                   None if v_scale is None else v_scale.data_ptr(), _type_of(k_pages, "k_pages"),
-                   n, H, page, Dh)
+            raise ValueError("pages and scales must be contiguous")
+        if len(at) >= 2 and (t.dtype != _torch.float32 or t.shape != shape[:3]):
+            raise ValueError("k_scale and v_scale must be float32 [pages, H, page_size]")
+        at.append(t.data_ptr())
+    return KvPages(*at, ty, n, H, page, Dh)
 
 
 def _seqs(cu, table, lens, device) -> Seqs:
-    if table.dim() != 2 or str(table.dtype) != "torch.int32" or table.device != device or \
+    if table.dtype != _torch.int32 or table.dim() != 2 or table.device != device or \
             (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"table must be int32 [sequences, pages] on {device}, rows contiguous")
-    batch = table.shape[0]
+    batch, width = table.shape
     return Seqs(_offsets(cu, "cu", device, batch + 1), batch, table.data_ptr(), table.stride(0),
-                table.shape[1], _offsets(lens, "lens", device, batch))
-
-
-class _On:
-    """Makes `device` the current one, and `stream` torch's current stream, for
-    the length of a call; .stream is the raw stream to enqueue on.  A workspace
-    that is allocated inside belongs to that stream."""
-
-    def __init__(self, device, stream):
-        import torch
-
-        if device.type != "cuda":
-            raise ValueError("CUDA tensors expected")
-        self._ctx = None
-        if stream is not None:
-            if stream.device != device:
-                raise ValueError(f"stream is on {stream.device}, not on {device}")
-            self._ctx = torch.cuda.stream(stream)
-        elif device.index != torch.cuda.current_device():
-            self._ctx = torch.cuda.device(device)
-
-    def __enter__(self):
-        import torch
-
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        self.stream = torch.cuda.current_stream().cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-
-
-_workspace_bytes: dict = {}
+                width, _offsets(lens, "lens", device, batch))
 
 
 def _workspace(device, q_heads: int, kv_heads: int, Dh: int):
     """A fresh workspace from torch's allocator: calls in flight at the same
     time, and captured graphs, each have their own."""
-    import torch
-
+    if kv_heads == 0 or q_heads % kv_heads:
+        raise ValueError("Q heads must be a multiple of the KV heads")
     key = (device.index, q_heads, kv_heads, Dh)
     n = _workspace_bytes.get(key)
     if n is None:
         size = ctypes.c_size_t()
         check(lib().attnb_seq_workspace(q_heads, kv_heads, Dh, ctypes.byref(size)))
         n = _workspace_bytes[key] = size.value
-    return torch.empty(n, dtype=torch.uint8, device=device), n
+    return _torch.empty(n, dtype=_torch.uint8, device=device), n
+
+
+def _scale(scale) -> float:
+    if scale is None:
+        return 0.0  # the library's 1 / sqrt(Dh)
+    if not scale > 0:
+        raise ValueError("scale must be positive")
+    return float(scale)
 
 
 def attn_packed_dev(Q, K, V, O, cu_q, cu_k=None, causal=False, scale=None, stream=None) -> None:
@@ -583,25 +585,19 @@ def attn_packed_dev(Q, K, V, O, cu_q, cu_k=None, causal=False, scale=None, strea
     sequence sees all its keys, each row before it one less.  heads is a
     multiple of kv_heads.  Rows of O behind cu_q[-1] stay as they are."""
     dev = Q.device
-    with _On(dev, stream) as on:
-        q, k, v, o = (_rows(t, n, dev) for t, n in ((Q, "Q"), (K, "K"), (V, "V"), (O, "O")))
-        if cu_q.dim() != 1 or cu_q.shape[0] < 1:
-            raise ValueError("cu_q must have one entry more than there are sequences")
-        batch = cu_q.shape[0] - 1
-        cq = _offsets(cu_q, "cu_q", dev)
-        ck = cq if cu_k is None else _offsets(cu_k, "cu_k", dev, batch + 1)
-        if k.heads == 0 or q.heads % k.heads:
-            raise ValueError("Q heads must be a multiple of the KV heads")
-        ws, n = _workspace(dev, q.heads, k.heads, q.Dh)
-        check(lib().attnb_attn_packed_dev(q, k, v, o, cq, ck, batch, int(causal),
-                                          0.0 if scale is None else _scale(scale), ws.data_ptr(),
-                                          n, on.stream))
-
-
-def _scale(scale) -> float:
-    if not scale > 0:
-        raise ValueError("scale must be positive")
-    return float(scale)
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return attn_packed_dev(Q, K, V, O, cu_q, cu_k, causal, scale)
+    q, k, v, o = _rows(Q, "Q", dev), _rows(K, "K", dev), _rows(V, "V", dev), _rows(O, "O", dev)
+    cq = _offsets(cu_q, "cu_q", dev)
+    batch = len(cu_q) - 1
+    if batch < 0:
+        raise ValueError("cu_q must have one entry more than there are sequences")
+    ck = cq if cu_k is None else _offsets(cu_k, "cu_k", dev, batch + 1)
+    ws, n = _workspace(dev, q.heads, k.heads, q.Dh)
+    check(_lib.attnb_attn_packed_dev(q, k, v, o, cq, ck, batch, int(causal), _scale(scale),
+                                     ws.data_ptr(), n, _raw_stream(dev.index)))
 
 
 def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=True, scale=None,
@@ -613,16 +609,17 @@ def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=Tr
     lens[b] tokens in pages table[b] (all int32).  max_new: the most rows of one
     sequence, where the caller knows it; it only steers the choice of kernel."""
     dev = Q.device
-    with _On(dev, stream) as on:
-        q, o = _rows(Q, "Q", dev), _rows(O, "O", dev)
-        pg = _pages(k_pages, v_pages, k_scale, v_scale, dev)
-        sq = _seqs(cu, table, lens, dev)
-        if pg.H == 0 or q.heads % pg.H:
-            raise ValueError("Q heads must be a multiple of the KV heads")
-        ws, n = _workspace(dev, q.heads, pg.H, q.Dh)
-        check(lib().attnb_attn_paged_dev(q, pg, o, sq, max_new, int(causal),
-                                         0.0 if scale is None else _scale(scale), ws.data_ptr(),
-                                         n, on.stream))
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new, causal, scale,
+                                  k_scale, v_scale)
+    q, o = _rows(Q, "Q", dev), _rows(O, "O", dev)
+    pg = _pages(k_pages, v_pages, k_scale, v_scale, dev)
+    sq = _seqs(cu, table, lens, dev)
+    ws, n = _workspace(dev, q.heads, pg.H, q.Dh)
+    check(_lib.attnb_attn_paged_dev(q, pg, o, sq, max_new, int(causal), _scale(scale),
+                                    ws.data_ptr(), n, _raw_stream(dev.index)))
 
 
 def kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale=None, v_scale=None,
@@ -631,10 +628,13 @@ def kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale=None, v
     them for float8_e4m3fn and int8 pages (attnb_kv_pages_append_dev); lens
     counts them already.  Other arguments as in attn_paged_dev."""
     dev = K.device
-    with _On(dev, stream) as on:
-        check(lib().attnb_kv_pages_append_dev(
-            _rows(K, "K", dev), _rows(V, "V", dev), _pages(k_pages, v_pages, k_scale, v_scale, dev),
-            _seqs(cu, table, lens, dev), on.stream))
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale, v_scale)
+    check(_lib.attnb_kv_pages_append_dev(
+        _rows(K, "K", dev), _rows(V, "V", dev), _pages(k_pages, v_pages, k_scale, v_scale, dev),
+        _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
 
 
 def kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale=None, v_scale=None,
@@ -642,10 +642,13 @@ def kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale=None, v_s
     """Read the last cu[b+1] - cu[b] tokens of each sequence out of the pages
     into K, V [tokens, kv_heads, Dh] (attnb_kv_pages_read_dev)."""
     dev = K.device
-    with _On(dev, stream) as on:
-        check(lib().attnb_kv_pages_read_dev(
-            _pages(k_pages, v_pages, k_scale, v_scale, dev), _rows(K, "K", dev),
-            _rows(V, "V", dev), _seqs(cu, table, lens, dev), on.stream))
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale, v_scale)
+    check(_lib.attnb_kv_pages_read_dev(
+        _pages(k_pages, v_pages, k_scale, v_scale, dev), _rows(K, "K", dev), _rows(V, "V", dev),
+        _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
 
 
 class PagedKVCacheDev:
@@ -698,7 +701,8 @@ class PagedKVCacheDev:
             raise ValueError("a sequence would outgrow max_tokens")
         if sum(want) - sum(len(h) for h in self._held) > len(self._free):
             raise ValueError("the pool has too few free pages")
-        with _On(self.table.device, stream):
+        on = _on(self.table.device, stream)
+        with on or contextlib.nullcontext():
             grew = False
             for held, w in zip(self._held, want):
                 while len(held) < w:
@@ -735,7 +739,8 @@ class PagedKVCacheDev:
 
         if k.shape[0] != self.lengths[b] or v.shape[0] != self.lengths[b]:
             raise ValueError("k and v must hold the sequence's tokens")
-        with _On(self.table.device, stream):
+        on = _on(self.table.device, stream)
+        with on or contextlib.nullcontext():
             cu = torch.tensor([0, self.lengths[b]], dtype=torch.int32, device=self.table.device)
             kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1],
                               self.lens[b:b + 1], self.k_scale, self.v_scale)

@@ -12,10 +12,13 @@
 // of zeros has scale 0; one with an Inf or NaN has scale NaN and codes 0, so
 // that it cannot be read back as something finite.
 //
-// Bound by memory: a token is read once and its codes written once.  A group of
-// 8 to 32 lanes takes one vector of K or V with 4 elements a lane and step, so
-// that the maximum is a few shuffles and no vector is read twice; rows that are
-// not aligned for that are read element by element.
+// Bound by memory: a token is read once and its codes written once.  A CTA takes
+// some tokens that follow one another, all heads of K and V.  Where a token
+// lives takes a search and three dependent reads, as long as hundreds of
+// streamed bytes, so one thread per token finds the places of all of them first.
+// Then a group of 8 to 32 lanes takes one vector, 8 elements a lane (one 16-byte
+// read of a 16-bit row), so that the maximum is a few shuffles and no vector is
+// read twice; rows that are not aligned for that are read element by element.
 #include <algorithm>
 #include <cmath>
 
@@ -89,161 +92,199 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&q)[4], elem_t<kI8>*
   return r;
 }
 
-// One vector per group of LANES lanes; NC groups of 4 elements per lane.
-template <int TX, int TC, int LANES, int NC>
+constexpr int kMaxTokens = 32;  // per CTA
+
+// Where the CTA's tokens [t0, t0 + n) live: the place of head 0, -1 for a place
+// out of range and -2 for a row of no sequence.
+__device__ __forceinline__ void find_places(const SeqTable& sq, const KvPages& pg, int t0, int n,
+                                            int64_t* at, int* index_status) {
+  if ((int)threadIdx.x < n) {
+    int first, count;
+    const int t = t0 + threadIdx.x;
+    at[threadIdx.x] = seq_of(sq, t, first, count) < 0 ? -2 : place_of(sq, pg, t, index_status);
+  }
+  __syncthreads();
+}
+
+// 8 elements from d on, those past Dh as zeros.
+template <class E>
+__device__ __forceinline__ void load8(const E* p, int d, int Dh, bool vec, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (vec) {  // Dh is a multiple of 8
+    if (d >= Dh) return;
+    struct alignas(sizeof(E) * 8 >= 16 ? 16 : 8) Eight {
+      E e[8];
+    };
+    const Eight f = *reinterpret_cast<const Eight*>(p + d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(f.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d + i < Dh) x[i] = to_float(p[d + i]);
+  }
+}
+template <class E>
+__device__ __forceinline__ void store8(E* p, int d, int Dh, bool vec, const float (&x)[8]) {
+  if (vec) {
+    if (d >= Dh) return;
+    struct alignas(sizeof(E) * 8 >= 16 ? 16 : 8) Eight {
+      E e[8];
+    };
+    Eight f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) from_float(x[i], f.e[i]);
+    *reinterpret_cast<Eight*>(p + d) = f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d + i < Dh) from_float(x[i], p[d + i]);
+  }
+}
+
+// One vector per group of LANES lanes.
+template <int TX, int TC, int LANES>
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const RowsView K, const RowsView V, const KvPages pg, const SeqTable sq,
-                  const bool vec, int* index_status) {
+                  const int tokens, const bool vec, int* index_status) {
   using EX = elem_t<TX>;
   using EC = elem_t<TC>;
   constexpr bool CODED = TC == kE4M3 || TC == kI8;
-  const int per_block = kThreads / LANES;
-  const int e = threadIdx.x % LANES;
-  const int Dh = pg.Dh;
-  const int64_t vectors = (int64_t)sq.total * 2 * pg.H;
+  __shared__ int64_t places[kMaxTokens];
+  const int e = threadIdx.x % LANES, d = e * 8;
+  const int Dh = pg.Dh, H2 = 2 * pg.H;
   grid_dep_wait();
-  for (int64_t i = (int64_t)blockIdx.x * per_block + threadIdx.x / LANES; i < vectors;
-       i += (int64_t)gridDim.x * per_block) {
-    // A group's lanes share i; the other groups of the warp may have left.
-    const unsigned mask =
-        LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
-    const int h = (int)(i % pg.H);
-    const int64_t tv = i / pg.H;
-    const bool is_v = tv >= sq.total;
-    const int t = (int)(is_v ? tv - sq.total : tv);
+  const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
+  find_places(sq, pg, t0, n, places, index_status);
+  // A group's lanes share their vector; the other groups of the warp may have left.
+  const unsigned mask =
+      LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+#pragma unroll 2
+  for (int i = threadIdx.x / LANES; i < n * H2; i += kThreads / LANES) {
+    const int tl = i / H2, kvh = i - tl * H2;
+    const bool is_v = kvh >= pg.H;
+    const int h = is_v ? kvh - pg.H : kvh;
     const RowsView& src = is_v ? V : K;
-    const EX* p = static_cast<const EX*>(src.data) + (int64_t)t * src.sT + (int64_t)h * src.sH;
-    float x[NC][4];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = (c * LANES + e) * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[c][j] = 0.f;
-      if (vec) {
-        if (d < Dh) load4(p + d, x[c]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d + j < Dh) x[c][j] = to_float(p[d + j]);
-      }
-    }
-    const int64_t at0 = place_of(sq, pg, t, index_status);
+    const EX* p = static_cast<const EX*>(src.data) + (int64_t)(t0 + tl) * src.sT + (int64_t)h * src.sH;
+    float x[8];
+    load8(p, d, Dh, vec, x);
+    const int64_t at0 = places[tl];
     if (at0 < 0) continue;
     const int64_t at = at0 + ((int64_t)h << pg.page_shift);
-    float top = 0.f;
+    EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + at * Dh;
     if constexpr (CODED) {
       constexpr float C = TC == kE4M3 ? 448.f : 127.f;
+      float top = 0.f;
       bool bad = false;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          top = fmaxf(top, fabsf(x[c][j]));
-          bad |= !(fabsf(x[c][j]) <= 3.402823466e38f);
-        }
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-        bad |= __shfl_xor_sync(mask, (int)bad, o) != 0;
+      for (int j = 0; j < 8; ++j) {
+        top = fmaxf(top, fabsf(x[j]));
+        bad |= !(fabsf(x[j]) <= 3.402823466e38f);
       }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+      bad = (__ballot_sync(mask, bad) & mask) != 0;
       if (e == 0)
         (is_v ? pg.v_scale : pg.k_scale)[at] = bad ? __int_as_float(0x7fffffff) : top / C;
       if (bad) top = 0.f;
-      EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + at * Dh;
+      // x * (C / a) is off by less than 2^-22 of it: where 2^-22 up and down give
+      // the same codes, those are the ones; else (next to a tie) the quotient
+      // decides.  C / a overflows for tiny a, and is not used for large ones.
+      const float inv = top > 0x1p-100f && top < 0x1p100f ? C / top : 0.f;
+      uint32_t r2[2];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = (c * LANES + e) * 4;
-        if (d >= Dh) continue;
-        float q[4];
+      for (int k = 0; k < 2; ++k) {
+        float up[4], down[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = top > 0.f ? quotient<TX>(x[c][j], top, C) : 0.f;
-        const uint32_t r = pack_codes(q, out);
-        if (vec) {
-          *reinterpret_cast<uint32_t*>(out + d) = r;
-        } else {
+        for (int j = 0; j < 4; ++j) {
+          const float q = x[4 * k + j] * inv;
+          up[j] = q * (1.f + 0x1p-22f);
+          down[j] = q * (1.f - 0x1p-22f);
+        }
+        r2[k] = pack_codes(up, out);
+        if (r2[k] != pack_codes(down, out) || inv == 0.f) {
+          float q[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (d + j < Dh) reinterpret_cast<uint8_t*>(out)[d + j] = (uint8_t)(r >> (8 * j));
+            q[j] = top > 0.f ? quotient<TX>(x[4 * k + j], top, C) : 0.f;
+          r2[k] = pack_codes(q, out);
         }
       }
-    } else {
-      EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + at * Dh;
+      const uint2 r = make_uint2(r2[0], r2[1]);
+      if (vec) {
+        if (d < Dh) *reinterpret_cast<uint2*>(out + d) = r;
+      } else {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = (c * LANES + e) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d + j < Dh) from_float(x[c][j], out[d + j]);
+        for (int j = 0; j < 8; ++j)
+          if (d + j < Dh)
+            reinterpret_cast<uint8_t*>(out)[d + j] = (uint8_t)((j < 4 ? r.x : r.y) >> (8 * (j & 3)));
       }
+    } else {
+      store8(out, d, Dh, vec, x);
     }
   }
 }
 
-template <int TX, int TC, int LANES, int NC>
+template <int TX, int TC, int LANES>
 __global__ void __launch_bounds__(kThreads)
     read_kernel(const KvPages pg, const RowsView K, const RowsView V, const SeqTable sq,
-                const bool vec, int* index_status) {
+                const int tokens, const bool vec, int* index_status) {
   using EX = elem_t<TX>;
   using EC = elem_t<TC>;
   constexpr bool CODED = TC == kE4M3 || TC == kI8;
-  const int per_block = kThreads / LANES;
-  const int e = threadIdx.x % LANES;
-  const int Dh = pg.Dh;
-  const int64_t vectors = (int64_t)sq.total * 2 * pg.H;
+  __shared__ int64_t places[kMaxTokens];
+  const int d = threadIdx.x % LANES * 8;
+  const int Dh = pg.Dh, H2 = 2 * pg.H;
   grid_dep_wait();
-  for (int64_t i = (int64_t)blockIdx.x * per_block + threadIdx.x / LANES; i < vectors;
-       i += (int64_t)gridDim.x * per_block) {
-    const int h = (int)(i % pg.H);
-    const int64_t tv = i / pg.H;
-    const bool is_v = tv >= sq.total;
-    const int t = (int)(is_v ? tv - sq.total : tv);
-    int first, count;
-    if (seq_of(sq, t, first, count) < 0) continue;  // a row of no sequence stays as it is
-    const int64_t at0 = place_of(sq, pg, t, index_status);
+  const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
+  find_places(sq, pg, t0, n, places, index_status);
+#pragma unroll 2
+  for (int i = threadIdx.x / LANES; i < n * H2; i += kThreads / LANES) {
+    const int tl = i / H2, kvh = i - tl * H2;
+    const bool is_v = kvh >= pg.H;
+    const int h = is_v ? kvh - pg.H : kvh;
+    const int64_t at0 = places[tl];
+    if (at0 == -2) continue;  // a row of no sequence stays as it is
     const int64_t at = at0 + ((int64_t)h << pg.page_shift);
-    const float scale = CODED && at0 >= 0 ? __ldg((is_v ? pg.v_scale : pg.k_scale) + at) : 1.f;
-    const EC* p = static_cast<const EC*>(is_v ? pg.v : pg.k) + at * Dh;
-    const RowsView& dst = is_v ? V : K;
-    EX* out = static_cast<EX*>(dst.data) + (int64_t)t * dst.sT + (int64_t)h * dst.sH;
+    float x[8];
+    if (at0 >= 0) {
+      load8(static_cast<const EC*>(is_v ? pg.v : pg.k) + at * Dh, d, Dh, vec, x);
+      if constexpr (CODED) {
+        const float scale = (is_v ? pg.v_scale : pg.k_scale)[at];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = (c * LANES + e) * 4;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (at0 >= 0) {
-        if (vec) {
-          if (d < Dh) load4(p + d, x);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (d + j < Dh) x[j] = to_float(p[d + j]);
-        }
+        for (int j = 0; j < 8; ++j) x[j] *= scale;
       }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (d + j < Dh) from_float(CODED ? x[j] * scale : x[j], out[d + j]);
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
     }
+    const RowsView& dst = is_v ? V : K;
+    store8(static_cast<EX*>(dst.data) + (int64_t)(t0 + tl) * dst.sT + (int64_t)h * dst.sH, d, Dh,
+           vec, x);
   }
 }
 
 bool vec_rows(const RowsView& r) {
-  const int b = 4 * elem_bytes(r.type);
-  return reinterpret_cast<uintptr_t>(r.data) % b == 0 && r.sT % 4 == 0 && r.sH % 4 == 0 &&
-         r.Dh % 4 == 0;
+  // 8 elements are read as 16 bytes (32-bit ones as two times 16).
+  const int unit = 16 / elem_bytes(r.type);
+  return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.sT % unit == 0 && r.sH % unit == 0 &&
+         r.Dh % 8 == 0;
 }
 bool vec_pages(const KvPages& p) {
-  const int b = 4 * elem_bytes(p.type);
+  const int b = std::min(16, 8 * elem_bytes(p.type));
   return reinterpret_cast<uintptr_t>(p.k) % b == 0 && reinterpret_cast<uintptr_t>(p.v) % b == 0 &&
-         p.Dh % 4 == 0;
+         p.Dh % 8 == 0;
 }
 
-// f(type of the rows, type of the pages, lanes per vector, 4-element groups per lane).
+// f(type of the rows, type of the pages, lanes per vector).
 template <class F>
 void dispatch(const RowsView& K, const KvPages& pg, F&& f) {
   auto sizes = [&](auto tx, auto tc) {
     using std::integral_constant;
-    if (pg.Dh <= 64) f(tx, tc, integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    else if (pg.Dh <= 128) f(tx, tc, integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    else f(tx, tc, integral_constant<int, 32>{}, integral_constant<int, 2>{});
+    if (pg.Dh <= 64) f(tx, tc, integral_constant<int, 8>{});
+    else if (pg.Dh <= 128) f(tx, tc, integral_constant<int, 16>{});
+    else f(tx, tc, integral_constant<int, 32>{});
   };
   with_value_type(K.type, [&](auto tx) {
     if (pg.type == kE4M3) sizes(tx, std::integral_constant<int, kE4M3>{});
@@ -252,10 +293,10 @@ void dispatch(const RowsView& K, const KvPages& pg, F&& f) {
   });
 }
 
-int grid_of(const SeqTable& sq, const KvPages& pg, int lanes, int num_sms) {
-  const int64_t vectors = (int64_t)sq.total * 2 * pg.H;
-  const int per_block = kThreads / lanes;
-  return (int)std::min<int64_t>((vectors + per_block - 1) / per_block, (int64_t)num_sms * 8);
+// Tokens per CTA: as many as leave six CTAs to an SM, so that few tokens spread
+// over the machine and many share the search.
+int tokens_per_cta(const SeqTable& sq, int num_sms) {
+  return std::max(1, std::min(kMaxTokens, sq.total / (6 * num_sms)));
 }
 
 }  // namespace
@@ -263,22 +304,22 @@ int grid_of(const SeqTable& sq, const KvPages& pg, int lanes, int num_sms) {
 void kv_pages_append_launch(const RowsView& K, const RowsView& V, const KvPages& pg,
                             const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s) {
   const bool vec = vec_rows(K) && vec_rows(V) && vec_pages(pg);
-  dispatch(K, pg, [&](auto tx, auto tc, auto lanes, auto nc) {
-    constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value;
-    constexpr int LN = decltype(lanes)::value, NC = decltype(nc)::value;
-    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, NC>, dim3(grid_of(sq, pg, LN, num_sms)),
-                          dim3(kThreads), 0, s, K, V, pg, sq, vec, index_status));
+  const int tokens = tokens_per_cta(sq, num_sms);
+  dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
+    constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
+    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN>, dim3((sq.total + tokens - 1) / tokens),
+                          dim3(kThreads), 0, s, K, V, pg, sq, tokens, vec, index_status));
   });
 }
 
 void kv_pages_read_launch(const KvPages& pg, const RowsView& K, const RowsView& V,
                           const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s) {
   const bool vec = vec_rows(K) && vec_rows(V) && vec_pages(pg);
-  dispatch(K, pg, [&](auto tx, auto tc, auto lanes, auto nc) {
-    constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value;
-    constexpr int LN = decltype(lanes)::value, NC = decltype(nc)::value;
-    ATTNB_CUDA(launch_pdl(read_kernel<TX, TC, LN, NC>, dim3(grid_of(sq, pg, LN, num_sms)),
-                          dim3(kThreads), 0, s, pg, K, V, sq, vec, index_status));
+  const int tokens = tokens_per_cta(sq, num_sms);
+  dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
+    constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
+    ATTNB_CUDA(launch_pdl(read_kernel<TX, TC, LN>, dim3((sq.total + tokens - 1) / tokens),
+                          dim3(kThreads), 0, s, pg, K, V, sq, tokens, vec, index_status));
   });
 }
 
