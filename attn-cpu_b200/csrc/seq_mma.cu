@@ -287,11 +287,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             uint32_t b[4];
             ldsm4(st + sw128(kr, k + ((lane >> 3) & 1)), b);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                mma16816<false>(s[t], q[k + e], codes_to_f16<TK>(b[2 * t + e] & 0xffffu),
-                                codes_to_f16<TK>(b[2 * t + e] >> 16));
+              for (int t = 0; t < 2; ++t) {
+                uint32_t b0, b1;
+                codes_to_f16<TK>(b[2 * t + e], b0, b1);
+                mma16816<false>(s[t], q[k + e], b0, b1);
+              }
           }
         } else {
 #pragma unroll
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               k0 *= ks;
               k1 *= ks;
               add = __log2f(use);
-              vinv[t][e] = 1.f / use;
+              vinv[t][e] = fast_exp2(-add);
             }
             s[t][e] = fmaf(s[t][e], k0, add);
             s[t][e + 2] = fmaf(s[t][e + 2], k1, add);
@@ -406,13 +408,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             ldsm4_t(st + Cfg::TILE + sw128(vr, u + (lane >> 4)), b);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t lo = b[2 * e], hi = b[2 * e + 1];
-              // bytes: (key, d), (key, d+1), (key+1, d), (key+1, d+1)
-              mma16816<false>(acc[2 * (u + e)], p, codes_to_f16<TK>(__byte_perm(lo, 0, 0x4420) & 0xffffu),
-                              codes_to_f16<TK>(__byte_perm(hi, 0, 0x4420) & 0xffffu));
-              mma16816<false>(acc[2 * (u + e) + 1], p,
-                              codes_to_f16<TK>(__byte_perm(lo, 0, 0x4431) & 0xffffu),
-                              codes_to_f16<TK>(__byte_perm(hi, 0, 0x4431) & 0xffffu));
+              // bytes: (key, d), (key, d+1), (key+1, d), (key+1, d+1), brought to
+              // pairs of keys: d, then d + 1
+              uint32_t lo0, lo1, hi0, hi1;
+              codes_to_f16<TK>(__byte_perm(b[2 * e], 0, 0x3120), lo0, lo1);
+              codes_to_f16<TK>(__byte_perm(b[2 * e + 1], 0, 0x3120), hi0, hi1);
+              mma16816<false>(acc[2 * (u + e)], p, lo0, hi0);
+              mma16816<false>(acc[2 * (u + e) + 1], p, lo1, hi1);
             }
           }
         } else {

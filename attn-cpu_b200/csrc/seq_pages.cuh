@@ -39,22 +39,24 @@ __device__ __forceinline__ uint32_t sw128(int r, int u) {
   return (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
 }
 
-// Two codes (low 16 bits) to two f16, exactly.
+// Four codes to two pairs of f16, exactly.
 template <int T>
-__device__ __forceinline__ uint32_t codes_to_f16(uint32_t two) {
-  uint32_t r;
+__device__ __forceinline__ void codes_to_f16(uint32_t four, uint32_t& lo, uint32_t& hi) {
   if constexpr (T == kE4M3) {
-    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}\n"
-        : "=r"(r)
-        : "r"(two));
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
   } else {
     // 1024 + (code + 128) has the shifted code as its last mantissa bits.
-    const uint32_t shifted = __byte_perm(two ^ 0x8080u, 0x64646464u, 0x4140);
+    const uint32_t x = four ^ 0x80808080u;
     const __half2 base = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&shifted), base);
-    r = *reinterpret_cast<const uint32_t*>(&x);
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 l = __hsub2(*reinterpret_cast<const __half2*>(&a), base);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), base);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
   }
-  return r;
 }
 
 // The power of two that brings a row whose largest magnitude is `top` to

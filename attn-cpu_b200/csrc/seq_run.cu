@@ -10,35 +10,69 @@
 namespace attnb {
 namespace {
 
+constexpr int kMergeThreads = 256;
+
 // Joins the pieces of each item that a cut fell into: block c the item that
-// goes on in CTA c, if it began in CTA c - 1.
+// goes on in CTA c, if it began in CTA c - 1.  An item of a long context has
+// hundreds of pieces: their weights are found by as many threads, and groups of
+// 128 threads (one per dimension) sum every second one.
 template <int T>
-__global__ void __launch_bounds__(128) seq_merge_kernel(const SeqAttnArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnArgs a) {
   using E = elem_t<T>;
+  constexpr int kChunk = 256;  // pieces whose weights are held at a time
+  __shared__ float weight[kChunk];
+  __shared__ float red[kMergeThreads];
   grid_dep_wait();
   const int c = blockIdx.x + 1;
   const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];
   if (!d.continues || d.item0 < (c - 1) * d.quota) return;
-  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1;
+  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1, pieces = last - c + 2;
   // The first piece of CTA c - 1, or a later one.
   const int slot0 = 2 * (c - 1) + (d.item0 - d.extra <= (c - 1) * d.quota ? 0 : 1);
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
-  const int Dh = a.q.Dh;
+  const int Dh = a.q.Dh, tid = threadIdx.x;
+  const int wide = Dh <= 128 ? 128 : 256;  // threads per group
+  const int group = tid / wide, groups = kMergeThreads / wide, x = tid % wide;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? slot0 : 2 * (c - 1 + i)) * a.rows; };
   for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
-    float top = ml[(int64_t)slot0 * a.rows + r].x;
-    for (int i = c; i <= last; ++i) top = fmaxf(top, ml[(int64_t)2 * i * a.rows + r].x);
-    const int row = d.first_row + r;
-    E* o = static_cast<E*>(a.o.data) + (int64_t)(d.row_token + row / a.G) * a.o.sT +
-           (int64_t)(d.kv_head * a.G + row % a.G) * a.o.sH;
-    for (int x = threadIdx.x; x < Dh; x += blockDim.x) {
-      float sum = 0.f, acc = 0.f;
-      for (int i = c - 1; i <= last; ++i) {
-        const int64_t at = (int64_t)(i < c ? slot0 : 2 * i) * a.rows + r;
-        const float2 p = ml[at];
+    float top = -INFINITY;
+    for (int i = tid; i < pieces; i += kMergeThreads) top = fmaxf(top, ml[slot(i) + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    __syncthreads();  // the row before is done with the shared arrays
+    if ((tid & 31) == 0) red[tid >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < kMergeThreads / 32; ++i) top = fmaxf(top, red[i]);
+    float acc = 0.f, sum = 0.f;
+    for (int i0 = 0; i0 < pieces; i0 += kChunk) {
+      const int n = min(kChunk, pieces - i0);
+      __syncthreads();
+      if (tid < n) {
+        const float2 p = ml[slot(i0 + tid) + r];
         const float f = p.x == -INFINITY ? 0.f : fast_exp2(p.x - top);
+        weight[tid] = f;
         sum = fmaf(f, p.y, sum);
-        acc = fmaf(f, a.ws_o[at * Dh + x], acc);
       }
+      __syncthreads();
+      if (x < Dh) {
+#pragma unroll 8
+        for (int i = group; i < n; i += groups)
+          acc = fmaf(weight[i], a.ws_o[(slot(i0 + i) + r) * Dh + x], acc);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (group > 0) red[x] = acc;  // two groups at most
+    if ((tid & 31) == 0) weight[tid >> 5] = sum;
+    __syncthreads();
+    if (group == 0 && x < Dh) {
+      if (groups > 1) acc += red[x];
+      sum = 0.f;
+      for (int i = 0; i < kMergeThreads / 32; ++i) sum += weight[i];
+      const int row = d.first_row + r;
+      E* o = static_cast<E*>(a.o.data) + (int64_t)(d.row_token + row / a.G) * a.o.sT +
+             (int64_t)(d.kv_head * a.G + row % a.G) * a.o.sH;
       from_float(sum == 0.f ? 0.f : acc / sum, o[x]);
     }
   }
@@ -95,7 +129,8 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {
     ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
-                          dim3(sp.ctas - 1, std::min(a.rows, 16)), dim3(128), 0, s, a));
+                          dim3(sp.ctas - 1, kind == kTc ? 16 : 4), dim3(kMergeThreads), 0, s,
+                          a));
   });
 }
 

@@ -558,11 +558,15 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
                 uint32_t y[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const uint32_t h = codes_to_f16<TK>((xs[k >> 1] >> (16 * (k & 1))) & 0xffffu);
-                  const __half2 code = *reinterpret_cast<const __half2*>(&h);
-                  const __half2 v = __hfma2(code, lo, __hmul2(code, hi));
-                  y[k] = *reinterpret_cast<const uint32_t*>(&v);
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t h[2];
+                  codes_to_f16<TK>(xs[k], h[0], h[1]);
+#pragma unroll
+                  for (int b = 0; b < 2; ++b) {
+                    const __half2 code = *reinterpret_cast<const __half2*>(&h[b]);
+                    const __half2 v = __hfma2(code, lo, __hmul2(code, hi));
+                    y[2 * k + b] = *reinterpret_cast<const uint32_t*>(&v);
+                  }
                 }
                 uint8_t* ch = to + (u >> 2) * Cfg::CHUNK;
                 *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2)) =
