@@ -237,7 +237,7 @@ void kv_pages_read_launch(const KvPages& pg, const RowsView& K, const RowsView& 
                           const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s);
 
 // Attention of packed query rows over packed keys (pages.k == nullptr) or over
-// pages.  One launch of a K6-K8 kernel works through the items of the schedule
+// pages.  One launch of a K6-K9 kernel works through the items of the schedule
 // in seq.cuh, a second one joins the items that several CTAs shared.
 struct SeqAttnArgs {
   RowsView q, o, k, v;  // k, v: packed keys only
@@ -275,6 +275,9 @@ void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 bool seq_tc_supported(const SeqAttnArgs& a);
 int seq_tc_rows(int G);
 void seq_tc_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+// K9: fp32 products on tensor cores, any type and stride, head size up to 128,
+// 128 rows per item.
+void seq_tf32_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // Whether TMA can read the pages, and the map of one of the two pools with
 // copies of up to `rows` rows of one page.
 bool seq_pages_tma(const SeqAttnArgs& a);

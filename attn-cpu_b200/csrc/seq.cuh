@@ -1,4 +1,4 @@
-// seq.cuh -- the schedule of the attention kernels over ragged sequences (K6-K8)
+// seq.cuh -- the schedule of the attention kernels over ragged sequences (K6-K9)
 // and what they share: bounds of a sequence, the split of all work over the
 // CTAs, and the places of partial results.
 //
@@ -12,7 +12,7 @@
 // contexts all load the CTAs evenly, and nothing about the lengths has to be
 // known on the host.  An item counts `extra` tiles more than it has, ahead of
 // its first, for what it costs besides (its queries, its output).  An item that a cut falls into is joined afterwards
-// (seq_merge.cu) from the pieces' running maximum, sum and accumulator; a CTA
+// (seq_run.cu) from the pieces' running maximum, sum and accumulator; a CTA
 // has at most two such pieces, its first and its last, so the workspace does
 // not grow with the batch.
 //

@@ -34,6 +34,24 @@ __global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnA
   const int wide = Dh <= 128 ? 128 : 256;  // threads per group
   const int group = tid / wide, groups = kMergeThreads / wide, x = tid % wide;
   auto slot = [&](int i) { return (int64_t)(i == 0 ? slot0 : 2 * (c - 1 + i)) * a.rows; };
+  if (pieces <= 8) {  // the usual case: a row per group, nothing shared
+      for (int r = blockIdx.y * groups + group; r < d.rows; r += gridDim.y * groups) {
+        if (x >= Dh) continue;
+        float top = -INFINITY, acc = 0.f, sum = 0.f;
+        for (int i = 0; i < pieces; ++i) top = fmaxf(top, ml[slot(i) + r].x);
+        for (int i = 0; i < pieces; ++i) {
+          const float2 p = ml[slot(i) + r];
+          const float f = p.x == -INFINITY ? 0.f : fast_exp2(p.x - top);
+          sum = fmaf(f, p.y, sum);
+          acc = fmaf(f, a.ws_o[(slot(i) + r) * Dh + x], acc);
+        }
+        const int row = d.first_row + r;
+        E* o = static_cast<E*>(a.o.data) + (int64_t)(d.row_token + row / a.G) * a.o.sT +
+               (int64_t)(d.kv_head * a.G + row % a.G) * a.o.sH;
+        from_float(sum == 0.f ? 0.f : acc / sum, o[x]);
+      }
+    return;
+  }
   for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
     float top = -INFINITY;
     for (int i = tid; i < pieces; i += kMergeThreads) top = fmaxf(top, ml[slot(i) + r].x);
@@ -89,11 +107,13 @@ struct Space {
 Space simt_space(int Dh, int num_sms) { return {Dh <= 128 ? 4 : 2, 2 * num_sms}; }
 Space mma_space(int num_sms) { return {16, 2 * num_sms}; }
 Space tc_space(int G, int num_sms) { return {seq_tc_rows(G), num_sms}; }
+Space tf32_space(int num_sms) { return {128, num_sms}; }
 
 }  // namespace
 
 size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
   size_t n = std::max(simt_space(Dh, num_sms).bytes(Dh), mma_space(num_sms).bytes(Dh));
+  if (Dh <= 128) n = std::max(n, tf32_space(num_sms).bytes(Dh));
   if (G <= 128 && Dh <= 128) n = std::max(n, tc_space(G, num_sms).bytes(Dh));
   return n + 256;
 }
@@ -104,17 +124,19 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // New tokens of one sequence: the caller's bound, or the mean.
   const int64_t rows =
       (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
-  enum { kSimt, kMma, kTc } kind = kSimt;
+  enum { kSimt, kMma, kTc, kTf32 } kind = kSimt;
   if (seq_mma_supported(a) && rows <= 32) kind = kMma;
   else if (seq_tc_supported(a)) kind = kTc;
   else if (seq_mma_supported(a)) kind = kMma;
-  const Space sp = kind == kTc    ? tc_space(a.G, num_sms)
-                   : kind == kMma ? mma_space(num_sms)
-                                  : simt_space(a.q.Dh, num_sms);
+  else if (a.q.Dh <= 128 && rows > 8) kind = kTf32;
+  const Space sp = kind == kTc     ? tc_space(a.G, num_sms)
+                   : kind == kMma  ? mma_space(num_sms)
+                   : kind == kTf32 ? tf32_space(num_sms)
+                                   : simt_space(a.q.Dh, num_sms);
   a.rows = sp.rows;
-  a.kt_shift = kind == kTc ? 7 : 6;
+  a.kt_shift = kind == kTc ? 7 : kind == kTf32 ? 5 : 6;
   a.min_tiles = 2;
-  a.extra = kind == kTc ? 2 : 1;
+  a.extra = kind == kTc || kind == kTf32 ? 2 : 1;
   uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
   if (p + sp.bytes(a.q.Dh) > reinterpret_cast<uintptr_t>(ws) + ws_bytes)
     fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
@@ -125,11 +147,12 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   a.ws_o = reinterpret_cast<float*>(p);
   if (kind == kTc) seq_tc_launch(a, sp.ctas, s);
   else if (kind == kMma) seq_mma_launch(a, sp.ctas, s);
+  else if (kind == kTf32) seq_tf32_launch(a, sp.ctas, s);
   else seq_simt_launch(a, sp.ctas, s);
   // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {
     ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
-                          dim3(sp.ctas - 1, kind == kTc ? 16 : 4), dim3(kMergeThreads), 0, s,
+                          dim3(sp.ctas - 1, kind == kTc || kind == kTf32 ? 16 : 4), dim3(kMergeThreads), 0, s,
                           a));
   });
 }

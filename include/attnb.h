@@ -388,7 +388,9 @@ ATTNB_API int attnb_seq_workspace(int q_heads, int kv_heads, int Dh, size_t* byt
  * sequence's keys, rows [cu_k[b], cu_k[b+1]) of K and V.  With causal != 0 its
  * last row sees every key and each row before it one key less.  Query head h
  * reads KV head h / (Q.heads / K.heads); a row that sees no key gives zeros.
- * Q, K, V and O have one type; scale <= 0 means 1 / sqrt(Dh). */
+ * Q, K, V and O have one type; scale <= 0 means 1 / sqrt(Dh).  What a row does
+ * not see does not reach it, NaN and infinities included; F32 keys that it does
+ * see have to be finite (their products are split in two), or it is NaN. */
 ATTNB_API int attnb_attn_packed_dev(const attnb_rows* Q, const attnb_rows* K, const attnb_rows* V,
                                     const attnb_rows* O, const int32_t* cu_q,
                                     const int32_t* cu_k, int batch, int causal, float scale,
