@@ -267,7 +267,7 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
 
 // The kernels (K6: any type, stride and head size up to 256).
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
-// K7: 16-bit queries over 16-bit or coded pages, 16 rows per item.
+// K7: 16-bit queries over 16-bit or coded pages, 8 or 16 rows per item.
 bool seq_mma_supported(const SeqAttnArgs& a);
 void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // K8: 16-bit queries over packed keys or pages, two tiles of up to 128 rows per

@@ -1,20 +1,23 @@
-// seq_mma.cu -- K7: attention of few query rows (16 of a KV head at a time, as in
-// generation steps) over pages, 16-bit queries, 16-bit or coded keys.
+// seq_mma.cu -- K7: attention of few query rows (8 or 16 of a KV head at a time, as
+// in generation steps) over pages, 16-bit queries, 16-bit or coded keys.
 //
 // Bound by memory: every key is read once from HBM for all the query heads of
 // its KV head.  With 8 query heads a key of 512 bytes costs 4096 operations, 51
 // TFLOP/s at HBM rate and twice that over codes, more than CUDA cores have next
 // to the rest of the work: the products go to the tensor cores, in the
 // warp-wide form (mma.sync m16n8k16).  A 128-row tile of tcgen05 would hold 8
-// useful rows in 128; the 16-row form needs no accumulator outside registers
-// and its rate is far above what the memory asks for.
+// useful rows in 128; here the 16 rows of the instruction are keys (S^T = K Q^T)
+// and dimensions (O^T = V^T P^T), and the 8 columns are query rows, so that a
+// step of 4 or 8 query heads wastes little of either product, and a thread holds
+// half the weights and accumulators that rows of queries would take.
 //
 // A CTA is four warps and a loader.  The loader streams tiles of 64 keys (K and
 // V, and the scales of codes) by TMA into a ring, page by page, across the ends
-// of pieces, so that the memory pipe does not drain between items; two CTAs
-// share an SM.  Each warp takes 16 of the 64 keys with all rows: Q stays in
-// registers, S = Q K^T goes straight into the weights' A fragment, and the
-// running maximum, sum and accumulator are the warp's own until the piece ends.
+// of pieces, so that the memory pipe does not drain between items; two or three
+// CTAs share an SM.  Each warp takes 16 of the 64 keys with all rows: Q stays in
+// registers, S^T becomes the weights' B fragment by one transposition of 8 x 8
+// values, and the running maximum, sum and accumulator are the warp's own until
+// the piece ends.
 //
 // Codes: both products run in f16, where e4m3 and int8 codes are exact.  Q is
 // brought to [1, 2) by a power of two per row (bf16 has more range than f16).
@@ -35,25 +38,29 @@
 namespace attnb {
 namespace {
 
-constexpr int kRows = 16;
 constexpr int kKeys = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 
-template <int TK, int DHP>
+// NR: query rows / 8.
+template <int TK, int DHP, int NR>
 struct MmaCfg {
   static constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  static constexpr int ROWS = 8 * NR;
+  static constexpr int CTAS = NR == 1 ? 3 : 2;         // per SM
   static constexpr int CHUNKS = CODED ? 1 : DHP / 64;  // 128-byte pieces of a row
   static constexpr int CHUNK = kKeys * 128;
   static constexpr int TILE = CHUNKS * CHUNK;          // K or V
   static constexpr int STAGE = 2 * TILE + (CODED ? 1024 : 0);
-  static constexpr int STAGES = CODED ? 5 : (DHP == 128 ? 3 : 6);
-  // Exchange at the end of a piece: 32 dimensions of 4 warps x 16 rows.
+  // Together the CTAs of an SM have about 190 KB of copies in flight.
+  static constexpr int STAGES = CODED ? (NR == 1 ? 3 : 5)
+                                      : (DHP == 128 ? (NR == 1 ? 2 : 3) : (NR == 1 ? 4 : 6));
+  // Exchange at the end of a piece: 32 dimensions of 4 warps' rows.
   static constexpr int XROW = 36;
   static constexpr int OFF_X = STAGES * STAGE;
-  static constexpr int OFF_POISON = OFF_X + kWarps * kRows * XROW * 4;
+  static constexpr int OFF_POISON = OFF_X + kWarps * ROWS * XROW * 4;
   static constexpr int SMEM = OFF_POISON + 3 * DHP * 4 + 1024;
-  static_assert(SMEM <= 112 * 1024, "two CTAs per SM");
+  static_assert(SMEM + 2048 <= 227 * 1024 / CTAS, "CTAs per SM");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -69,39 +76,46 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "memory");
 }
 template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (BF16)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 tile of 16-bit values, transposed across the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
 // TQ: type of Q and O; TK: TQ or codes; DHP: head size padded to 64 or 128.
-template <int TQ, int TK, int DHP>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int TQ, int TK, int DHP, int NR>
+__global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     seq_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ SeqAttnArgs a) {
-  using Cfg = MmaCfg<TK, DHP>;
+  using Cfg = MmaCfg<TK, DHP, NR>;
   using EQ = elem_t<TQ>;
   constexpr bool CODED = Cfg::CODED;
   constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
   constexpr int ST = Cfg::STAGES;
-  constexpr int KS = DHP / 16;  // steps of the product over the head dimension
-  constexpr int NT = DHP / 8;   // 8-wide column tiles of the output
+  constexpr int ROWS = Cfg::ROWS;
+  constexpr int KS = DHP / 16;  // 16 dimensions each
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[ST], empty[ST];
   __shared__ SeqShared sh;
-  __shared__ float2 sm_ml[kWarps][kRows];
+  __shared__ float2 sm_ml[kWarps][ROWS];
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -202,174 +216,166 @@ __global__ void __launch_bounds__(kThreads, 2)
   Ring<ST> ring;
   bool ok = true;
   for (bool first = true; it.next(a, w); first = false) {
-    // Q as A fragments: rows g and g + 8, by step of 16 dimensions.  16-bit keys:
+    // Q^T as B fragments: row 8 r + g, by step of 16 dimensions.  16-bit keys:
     // dimensions 2c, 2c+1 and 2c+8, 2c+9 of the step; codes: 4c .. 4c+3, as a
     // 4-byte unit of ldmatrix holds them.
-    uint32_t q[KS][4];
-    int seen[2];
-    float qs[2];
+    uint32_t q[NR][KS][2];
+    float mulq[NR][2];  // score to exponent, of this thread's rows 8 r + 2c, + 1
+    int seen[NR][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i, row = w.row0 + r;
-      seen[i] = 0;
-      qs[i] = a.scale_log2;
-      float x[KS][4];
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[k][e] = 0.f;
-      if (r < w.rows) {
-        seen[i] = seq_row_seen(a, w.s, row);
-        const EQ* p = static_cast<const EQ*>(a.q.data) + (int64_t)(w.s.q0 + row / a.G) * a.q.sT +
-                      (int64_t)(w.h * a.G + row % a.G) * a.q.sH;
+    for (int r = 0; r < NR; ++r) {
+      const int row = w.row0 + 8 * r + g;
+      const bool there = 8 * r + g < w.rows;
+      const EQ* p = static_cast<const EQ*>(a.q.data) + (int64_t)(w.s.q0 + row / a.G) * a.q.sT +
+                    (int64_t)(w.h * a.G + row % a.G) * a.q.sH;
+      if constexpr (CODED) {
+        float x[KS][4], top = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          if constexpr (CODED) {
-            if (k * 16 + 4 * c < a.q.Dh) load4(p + k * 16 + 4 * c, x[k]);
-          } else {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = k * 16 + 2 * c + 8 * e;
-              if (d < a.q.Dh) {  // Dh is even here
-                const uint32_t two = __ldg(reinterpret_cast<const uint32_t*>(p + d));
-                q[k][i + 2 * e] = two;
-              } else {
-                q[k][i + 2 * e] = 0;
-              }
-            }
-          }
-        }
-      } else if constexpr (!CODED) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) q[k][i] = q[k][i + 2] = 0;
-      }
-      if constexpr (CODED) {
-        float top = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
+          for (int e = 0; e < 4; ++e) x[k][e] = 0.f;
+          if (there && k * 16 + 4 * c < a.q.Dh) load4(p + k * 16 + 4 * c, x[k]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[k][e]));
+        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float f = row_scale(top);
-        qs[i] = a.scale_log2 / f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          q[k][i] = pack_f16(x[k][0] * f, x[k][1] * f);
-          q[k][i + 2] = pack_f16(x[k][2] * f, x[k][3] * f);
+          q[r][k][0] = pack_f16(x[k][0] * f, x[k][1] * f);
+          q[r][k][1] = pack_f16(x[k][2] * f, x[k][3] * f);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          mulq[r][i] = a.scale_log2 / __shfl_sync(0xffffffffu, f, (2 * c + i) * 4);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = k * 16 + 2 * c + 8 * e;  // Dh is even here
+            q[r][k][e] =
+                there && d < a.q.Dh ? __ldg(reinterpret_cast<const uint32_t*>(p + d)) : 0u;
+          }
+        mulq[r][0] = mulq[r][1] = a.scale_log2;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = 8 * r + 2 * c + i;
+        seen[r][i] = rr < w.rows ? seq_row_seen(a, w.s, w.row0 + rr) : 0;
       }
     }
     const int seen_min = seq_row_seen(a, w.s, w.row0);  // of the piece's first row
-    float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float acc[KS][NR][4], m[NR][2], l[NR][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int r = 0; r < NR; ++r) {
+      m[r][0] = m[r][1] = -INFINITY;
+      l[r][0] = l[r][1] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+      for (int u = 0; u < KS; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[u][r][e] = 0.f;
+    }
 
     for (int j = w.j0; j < w.j1; ++j) {
-      if (ok) ok = mbar_wait(smem_addr(&full[ring.stage]), ring.phase, abort_p, a.status);
+      if (ok) ok = mbar_wait_quick(smem_addr(&full[ring.stage]), ring.phase, abort_p, a.status);
       ok = __all_sync(0xffffffffu, ok);
       const uint32_t st = base + ring.stage * Cfg::STAGE;
       const int key0 = j * kKeys + warp * 16;
       const bool masked = key0 + 16 > seen_min;  // warp-uniform
       if (ok && key0 < w.s.L) {
-        // ---- S = Q K^T for 16 keys: two column tiles of 8
-        float s[2][4];
+        // ---- S^T = K Q^T: keys g, g + 8 by rows 2c, 2c + 1
+        float s[NR][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
-        const int kr = warp * 16 + (lane & 7) + ((lane >> 4) << 3);  // this lane's matrix row
+          for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
+        const int kr = warp * 16 + (lane & 15);  // this lane's matrix row
         if constexpr (CODED) {
 #pragma unroll
           for (int k = 0; k < KS; k += 2) {
             uint32_t b[4];
-            ldsm4(st + sw128(kr, k + ((lane >> 3) & 1)), b);
+            ldsm4(st + sw128(kr, k + (lane >> 4)), b);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+              uint32_t a0, a1, a2, a3;
+              codes_to_f16<TK>(b[2 * e], a0, a2);
+              codes_to_f16<TK>(b[2 * e + 1], a1, a3);
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                uint32_t b0, b1;
-                codes_to_f16<TK>(b[2 * t + e], b0, b1);
-                mma16816<false>(s[t], q[k + e], b0, b1);
-              }
+              for (int r = 0; r < NR; ++r)
+                mma16816<false>(s[r], a0, a1, a2, a3, q[r][k + e][0], q[r][k + e][1]);
+            }
           }
         } else {
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             uint32_t b[4];
-            ldsm4(st + (k >> 2) * Cfg::CHUNK + sw128(kr, (k & 3) * 2 + ((lane >> 3) & 1)), b);
-            mma16816<BF16>(s[0], q[k], b[0], b[1]);
-            mma16816<BF16>(s[1], q[k], b[2], b[3]);
+            ldsm4(st + (k >> 2) * Cfg::CHUNK + sw128(kr, (k & 3) * 2 + (lane >> 4)), b);
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              mma16816<BF16>(s[r], b[0], b[1], b[2], b[3], q[r][k][0], q[r][k][1]);
           }
         }
         // ---- weights
-        float vinv[2][2];  // codes: 1 / vscale
+        float mulk[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, vinv[2] = {1.f, 1.f};  // of keys g, g + 8
+        if constexpr (CODED) {
+          const float* sc =
+              reinterpret_cast<const float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = key0 + t * 8 + 2 * c + e;
-            float k0 = qs[0], k1 = qs[1], add = 0.f;
-            if constexpr (CODED) {
-              const float* sc = reinterpret_cast<const float*>(
-                  mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
-              const int at = warp * 16 + t * 8 + 2 * c + e;
-              const float ks = sc[at];
-              // A vector of zeros has scale 0; any small one does for it.
-              const float vs = sc[kKeys + at];
-              const float use = vs < 0x1p-60f ? 0x1p-60f : vs;
-              k0 *= ks;
-              k1 *= ks;
-              add = __log2f(use);
-              vinv[t][e] = fast_exp2(-add);
-            }
-            s[t][e] = fmaf(s[t][e], k0, add);
-            s[t][e + 2] = fmaf(s[t][e + 2], k1, add);
-            if (masked) {
-              if (key >= seen[0]) s[t][e] = -INFINITY;
-              if (key >= seen[1]) s[t][e + 2] = -INFINITY;
-            }
+          for (int i = 0; i < 2; ++i) {
+            const int at = warp * 16 + g + 8 * i;
+            mulk[i] = sc[at];
+            // A vector of zeros has scale 0; any small one does for it.
+            const float vs = sc[kKeys + at];
+            add[i] = __log2f(vs < 0x1p-60f ? 0x1p-60f : vs);
+            vinv[i] = fast_exp2(-add[i]);
           }
-        float alpha[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float top = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          top = fmaxf(top, m[i]);
-          const float use = top == -INFINITY ? 0.f : top;
-          alpha[i] = fast_exp2(m[i] - use);
-          m[i] = top;
-          float sum = 0.f;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float p = fast_exp2(s[t][2 * i + e] - use);
-              s[t][2 * i + e] = p;
-              // The scale of a masked key may be anything.
-              if constexpr (CODED) sum += p != 0.f ? p * vinv[t][e] : 0.f;
-              else sum += p;
-            }
-          l[i] = fmaf(l[i], alpha[i], sum);
         }
-        uint32_t p[4];
+        uint32_t p[NR][2];
+        bool moved = false;
+        float alpha[NR][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int r = 0; r < NR; ++r) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            p[2 * t + i] = BF16 ? pack_bf16(s[t][2 * i], s[t][2 * i + 1])
-                                : pack_f16(s[t][2 * i], s[t][2 * i + 1]);
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            acc[t][0] *= alpha[0];
-            acc[t][1] *= alpha[0];
-            acc[t][2] *= alpha[1];
-            acc[t][3] *= alpha[1];
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (CODED) s[r][e] = fmaf(s[r][e], mulq[r][e & 1] * mulk[e >> 1], add[e >> 1]);
+            else s[r][e] *= mulq[r][e & 1];
+            if (masked && key0 + g + 8 * (e >> 1) >= seen[r][e & 1]) s[r][e] = -INFINITY;
           }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(s[r][i], s[r][i + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[r][i]);
+            const float use = top == -INFINITY ? 0.f : top;
+            alpha[r][i] = fast_exp2(m[r][i] - use);
+            moved |= alpha[r][i] != 1.f;
+            m[r][i] = top;
+            l[r][i] *= alpha[r][i];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float x = fast_exp2(s[r][i + 2 * k] - use);
+              s[r][i + 2 * k] = x;
+              // The scale of a masked key may be anything.
+              if constexpr (CODED) l[r][i] += x != 0.f ? x * vinv[k] : 0.f;
+              else l[r][i] += x;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            p[r][k] = transposed(BF16 ? pack_bf16(s[r][2 * k], s[r][2 * k + 1])
+                                      : pack_f16(s[r][2 * k], s[r][2 * k + 1]));
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int u = 0; u < KS; ++u)
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[u][r][e] *= alpha[r][e & 1];
         }
         // ---- values that a mask hides (written codes are finite)
         if (CODED ? key0 + 16 > w.s.L : masked) {
@@ -399,31 +405,34 @@ __global__ void __launch_bounds__(kThreads, 2)
           fence_proxy_async_smem();  // the next copy into the stage comes after these writes
           __syncwarp();
         }
-        // ---- O += P V
-        const int vr = warp * 16 + (lane & 15);  // this lane's matrix row
+        // ---- O^T += V^T P^T, 16 dimensions at a time
         if constexpr (CODED) {
 #pragma unroll
-          for (int u = 0; u < KS; u += 2) {  // 16 dimensions each
+          for (int u = 0; u < KS; u += 2) {
             uint32_t b[4];
-            ldsm4_t(st + Cfg::TILE + sw128(vr, u + (lane >> 4)), b);
+            ldsm4_t(st + Cfg::TILE + sw128(kr, u + (lane >> 4)), b);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               // bytes: (key, d), (key, d+1), (key+1, d), (key+1, d+1), brought to
-              // pairs of keys: d, then d + 1
-              uint32_t lo0, lo1, hi0, hi1;
-              codes_to_f16<TK>(__byte_perm(b[2 * e], 0, 0x3120), lo0, lo1);
-              codes_to_f16<TK>(__byte_perm(b[2 * e + 1], 0, 0x3120), hi0, hi1);
-              mma16816<false>(acc[2 * (u + e)], p, lo0, hi0);
-              mma16816<false>(acc[2 * (u + e) + 1], p, lo1, hi1);
+              // pairs of keys: d = 2g, then 2g + 1
+              uint32_t a0, a1, a2, a3;
+              codes_to_f16<TK>(__byte_perm(b[2 * e], 0, 0x3120), a0, a1);
+              codes_to_f16<TK>(__byte_perm(b[2 * e + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+                mma16816<false>(acc[u + e][r], a0, a1, a2, a3, p[r][0], p[r][1]);
             }
           }
         } else {
+          const int vr = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
 #pragma unroll
-          for (int t = 0; t < NT; t += 2) {
+          for (int u = 0; u < KS; ++u) {
             uint32_t b[4];
-            ldsm4_t(st + Cfg::TILE + (t >> 3) * Cfg::CHUNK + sw128(vr, (t & 7) + (lane >> 4)), b);
-            mma16816<BF16>(acc[t], p, b[0], b[1]);
-            mma16816<BF16>(acc[t + 1], p, b[2], b[3]);
+            ldsm4_t(st + Cfg::TILE + (u >> 2) * Cfg::CHUNK +
+                        sw128(vr, (u & 3) * 2 + ((lane >> 3) & 1)), b);
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              mma16816<BF16>(acc[u][r], b[0], b[1], b[2], b[3], p[r][0], p[r][1]);
           }
         }
       }
@@ -434,60 +443,58 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     // ---- the warps' sums meet, 32 dimensions at a time
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = l[i];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (c == 0) sm_ml[warp][g + 8 * i] = make_float2(m[i], sum);
-    }
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum = l[r][i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) sm_ml[warp][8 * r + 2 * c + i] = make_float2(m[r][i], sum);
+      }
     named_bar_sync(1, kWarps * 32);
     const int slot = seq_slot(w, first);
-    float f[2], total[2], top[2];
+    float f[NR][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i;
-      top[i] = -INFINITY;
-      for (int k = 0; k < kWarps; ++k) top[i] = fmaxf(top[i], sm_ml[k][r].x);
-      const float use = top[i] == -INFINITY ? 0.f : top[i];
-      total[i] = 0.f;
-      for (int k = 0; k < kWarps; ++k)
-        total[i] += fast_exp2(sm_ml[k][r].x - use) * sm_ml[k][r].y;
-      f[i] = fast_exp2(m[i] - use);
-      if (slot < 0) f[i] = total[i] == 0.f ? 0.f : f[i] / total[i];
-      else if (warp == 0 && c == 0 && r < w.rows)
-        reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * kRows + r] =
-            make_float2(top[i], total[i]);
-    }
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = 8 * r + 2 * c + i;
+        float top = -INFINITY, total = 0.f;
+        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, sm_ml[k][rr].x);
+        const float use = top == -INFINITY ? 0.f : top;
+        for (int k = 0; k < kWarps; ++k)
+          total += fast_exp2(sm_ml[k][rr].x - use) * sm_ml[k][rr].y;
+        f[r][i] = fast_exp2(m[r][i] - use);
+        if (slot < 0) f[r][i] = total == 0.f ? 0.f : f[r][i] / total;
+        else if (warp == 0 && g == 0 && rr < w.rows)
+          reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * ROWS + rr] = make_float2(top, total);
+      }
     float* x = reinterpret_cast<float*>(mem + Cfg::OFF_X);
 #pragma unroll
     for (int q4 = 0; q4 < DHP / 32; ++q4) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int nt = q4 * 4 + t;
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float* row = x + (warp * kRows + g + 8 * i) * Cfg::XROW;
-          const float v0 = acc[nt][2 * i] * f[i], v1 = acc[nt][2 * i + 1] * f[i];
-          if constexpr (CODED) {  // tile nt: dimensions 16 (nt/2) + 4c + (nt & 1), + 2
-            row[(t >> 1) * 16 + 4 * c + (t & 1)] = v0;
-            row[(t >> 1) * 16 + 4 * c + (t & 1) + 2] = v1;
-          } else {
-            *reinterpret_cast<float2*>(row + t * 8 + 2 * c) = make_float2(v0, v1);
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = t * 16 + (CODED ? 2 * g + (e >> 1) : g + 8 * (e >> 1));
+            x[(warp * ROWS + 8 * r + 2 * c + (e & 1)) * Cfg::XROW + d] =
+                acc[q4 * 2 + t][r][e] * f[r][e & 1];
           }
-        }
-      }
       named_bar_sync(1, kWarps * 32);
-      for (int i = threadIdx.x; i < kRows * 32; i += kWarps * 32) {
+      for (int i = threadIdx.x; i < ROWS * 32; i += kWarps * 32) {
         const int r = i >> 5, d = q4 * 32 + (i & 31);
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) v += x[(k * kRows + r) * Cfg::XROW + (i & 31)];
+        for (int k = 0; k < kWarps; ++k) v += x[(k * ROWS + r) * Cfg::XROW + (i & 31)];
         if (r < w.rows && d < a.q.Dh) {
           const int row = w.row0 + r;
           if constexpr (!CODED)
             v = poisoned(v, poison, poison + DHP, poison + 2 * DHP, d, seq_row_seen(a, w.s, row));
           if (slot >= 0)
-            a.ws_o[((int64_t)slot * kRows + r) * a.q.Dh + d] = v;
+            a.ws_o[((int64_t)slot * ROWS + r) * a.q.Dh + d] = v;
           else
             from_float(v, *(static_cast<EQ*>(a.o.data) +
                             (int64_t)(w.s.q0 + row / a.G) * a.o.sT +
@@ -503,21 +510,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-template <int TQ, int TK, int DHP>
+template <int TQ, int TK, int DHP, int NR>
 void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensorMap& v,
             cudaStream_t s) {
-  using Cfg = MmaCfg<TK, DHP>;
+  using Cfg = MmaCfg<TK, DHP, NR>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   ATTNB_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load() & bit)) {
-    ATTNB_CUDA(cudaFuncSetAttribute(seq_mma_kernel<TQ, TK, DHP>,
+    ATTNB_CUDA(cudaFuncSetAttribute(seq_mma_kernel<TQ, TK, DHP, NR>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     configured.fetch_or(bit);
   }
-  ATTNB_CUDA(launch_pdl(seq_mma_kernel<TQ, TK, DHP>, dim3(ctas), dim3(kThreads), Cfg::SMEM, s, k,
-                        v, a));
+  ATTNB_CUDA(launch_pdl(seq_mma_kernel<TQ, TK, DHP, NR>, dim3(ctas), dim3(kThreads), Cfg::SMEM, s,
+                        k, v, a));
 }
 
 }  // namespace
@@ -552,8 +559,13 @@ void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   auto go = [&](auto tq, auto tk) {
     constexpr int TQ = decltype(tq)::value, TK = decltype(tk)::value;
     if constexpr (TQ != kF32) {
-      if (a.q.Dh <= 64) launch<TQ, TK, 64>(a, ctas, k, v, s);
-      else launch<TQ, TK, 128>(a, ctas, k, v, s);
+      if (a.rows == 8) {
+        if (a.q.Dh <= 64) launch<TQ, TK, 64, 1>(a, ctas, k, v, s);
+        else launch<TQ, TK, 128, 1>(a, ctas, k, v, s);
+      } else {
+        if (a.q.Dh <= 64) launch<TQ, TK, 64, 2>(a, ctas, k, v, s);
+        else launch<TQ, TK, 128, 2>(a, ctas, k, v, s);
+      }
     }
   };
   with_value_type(a.q.type, [&](auto tq) {
