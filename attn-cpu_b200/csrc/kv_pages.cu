@@ -361,10 +361,10 @@ void dispatch(const RowsView& K, const KvPages& pg, F&& f) {
   });
 }
 
-// Tokens per CTA: as many as leave six CTAs to an SM, so that few tokens spread
-// over the machine and many share the search.
+// Tokens per CTA: as many as leave four CTAs to an SM (all of them fit at once),
+// so that few tokens spread over the machine and many share the search.
 int tokens_per_cta(const SeqTable& sq, int num_sms) {
-  return std::max(1, std::min(kMaxTokens, sq.total / (6 * num_sms)));
+  return std::max(1, std::min(kMaxTokens, (sq.total + 4 * num_sms - 1) / (4 * num_sms)));
 }
 
 }  // namespace

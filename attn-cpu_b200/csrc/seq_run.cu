@@ -12,10 +12,12 @@ namespace {
 
 constexpr int kMergeThreads = 256;
 
-// Joins the pieces of each item that a cut fell into: block c the item that
-// goes on in CTA c, if it began in CTA c - 1.  An item of a long context has
-// hundreds of pieces: their weights are found by as many threads, and groups of
-// 128 threads (one per dimension) sum every second one.
+// Joins the pieces of each item that a cut fell into.  The blocks of all the CTAs
+// that go on with an item share its rows (an item of a long context has hundreds
+// of pieces, and as many blocks).  Few pieces, the usual case: groups of 128
+// threads (one per dimension) take a row each.  Many: the block takes a row, its
+// threads find the pieces' weights side by side, and each group sums every
+// second piece.
 template <int T>
 __global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnArgs a) {
   using E = elem_t<T>;
@@ -25,17 +27,19 @@ __global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnA
   grid_dep_wait();
   const int c = blockIdx.x + 1;
   const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];
-  if (!d.continues || d.item0 < (c - 1) * d.quota) return;
-  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1, pieces = last - c + 2;
-  // The first piece of CTA c - 1, or a later one.
-  const int slot0 = 2 * (c - 1) + (d.item0 - d.extra <= (c - 1) * d.quota ? 0 : 1);
+  if (!d.continues) return;
+  const int own = (int)udiv(d.item0, d.quota);  // the CTA with the first piece
+  const int last = (int)udiv(d.item1 + d.quota - 1, d.quota) - 1, pieces = last - own + 1;
+  // It is that CTA's first piece, or a later one.
+  const int slot0 = 2 * own + (d.item0 - d.extra <= own * d.quota ? 0 : 1);
+  const int worker = (c - own - 1) * gridDim.y + blockIdx.y, workers = (pieces - 1) * gridDim.y;
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
   const int Dh = a.q.Dh, tid = threadIdx.x;
   const int wide = Dh <= 128 ? 128 : 256;  // threads per group
   const int group = tid / wide, groups = kMergeThreads / wide, x = tid % wide;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? slot0 : 2 * (c - 1 + i)) * a.rows; };
-  if (pieces <= 8) {  // the usual case: a row per group, nothing shared
-      for (int r = blockIdx.y * groups + group; r < d.rows; r += gridDim.y * groups) {
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? slot0 : 2 * (own + i)) * a.rows; };
+  if (pieces <= 8) {
+      for (int r = worker * groups + group; r < d.rows; r += workers * groups) {
         if (x >= Dh) continue;
         float top = -INFINITY, acc = 0.f, sum = 0.f;
         for (int i = 0; i < pieces; ++i) top = fmaxf(top, ml[slot(i) + r].x);
@@ -52,7 +56,7 @@ __global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnA
       }
     return;
   }
-  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
+  for (int r = worker; r < d.rows; r += workers) {
     float top = -INFINITY;
     for (int i = tid; i < pieces; i += kMergeThreads) top = fmaxf(top, ml[slot(i) + r].x);
 #pragma unroll
@@ -155,7 +159,7 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {
     ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
-                          dim3(sp.ctas - 1, kind == kTc || kind == kTf32 ? 16 : 4), dim3(kMergeThreads), 0, s,
+                          dim3(sp.ctas - 1, kind == kTc || kind == kTf32 ? 16 : 2), dim3(kMergeThreads), 0, s,
                           a));
   });
 }
