@@ -701,27 +701,30 @@ class PagedKVCacheDev:
             raise ValueError("a sequence would outgrow max_tokens")
         if sum(want) - sum(len(h) for h in self._held) > len(self._free):
             raise ValueError("the pool has too few free pages")
-        on = _on(self.table.device, stream)
-        with on or contextlib.nullcontext():
-            grew = False
-            for held, w in zip(self._held, want):
-                while len(held) < w:
-                    held.append(self._free.pop())
-                    grew = True
-            self.lengths = [n + m for n, m in zip(self.lengths, new)]
-            dev = self.table.device
-            if grew:
-                width = self.table.shape[1]
-                self.table.copy_(torch.tensor([h + [0] * (width - len(h)) for h in self._held],
-                                              dtype=torch.int32))
-            self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
-            cu = [0]
-            for n in new:
-                cu.append(cu[-1] + n)
-            self._new, self.cu = new, torch.tensor(cu, dtype=torch.int32, device=dev)
-            if cu[-1]:
+        held, free, lengths = [list(h) for h in self._held], list(self._free), list(self.lengths)
+        self._new = None
+        try:
+            with _on(self.table.device, stream) or contextlib.nullcontext():
+                for h, w in zip(self._held, want):
+                    while len(h) < w:
+                        h.append(self._free.pop())
+                self.lengths = [n + m for n, m in zip(self.lengths, new)]
+                if self._held != held:
+                    width = self.table.shape[1]
+                    self.table.copy_(torch.tensor([h + [0] * (width - len(h)) for h in self._held],
+                                                  dtype=torch.int32))
+                self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+                cu = [0]
+                for n in new:
+                    cu.append(cu[-1] + n)
+                self.cu = torch.tensor(cu, dtype=torch.int32, device=self.table.device)
                 kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
                                     self.lens, self.k_scale, self.v_scale)
+        except Exception:  # a rejected append changes nothing
+            self._held, self._free, self.lengths = held, free, lengths
+            self.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+            raise
+        self._new = new
 
     def attend(self, q, o, causal=True, scale=None, stream=None) -> None:
         """o = attention of q [sum(new), heads, Dh], the queries of the tokens
@@ -739,11 +742,11 @@ class PagedKVCacheDev:
 
         if k.shape[0] != self.lengths[b] or v.shape[0] != self.lengths[b]:
             raise ValueError("k and v must hold the sequence's tokens")
-        on = _on(self.table.device, stream)
-        with on or contextlib.nullcontext():
+        with _on(self.table.device, stream) or contextlib.nullcontext():
+            # The length on the device is that of the last append.
             cu = torch.tensor([0, self.lengths[b]], dtype=torch.int32, device=self.table.device)
-            kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1],
-                              self.lens[b:b + 1], self.k_scale, self.v_scale)
+            kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1], cu[1:],
+                              self.k_scale, self.v_scale)
 
     def truncate(self, b: int, length: int) -> None:
         """Keep the first `length` tokens of sequence b (0 gives all its pages

@@ -65,7 +65,7 @@ __device__ __forceinline__ void codes_to_f16(uint32_t four, uint32_t& lo, uint32
 __device__ __forceinline__ float row_scale(float top) {
   const int e = (int)(__float_as_uint(top) >> 23);  // top >= 0
   if (e == 0 || e == 255) return 1.f;
-  return __uint_as_float((uint32_t)min(254 - e, 253) << 23);
+  return __uint_as_float((uint32_t)max(254 - e, 1) << 23);  // [2, 4) next to overflow
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {

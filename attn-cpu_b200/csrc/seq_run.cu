@@ -108,7 +108,10 @@ struct Space {
     return (size_t)ctas * (2 * rows * ((size_t)Dh * 4 + 8) + sizeof(SeqSplit)) + 64;
   }
 };
-Space simt_space(int Dh, int num_sms) { return {Dh <= 128 ? 4 : 2, 2 * num_sms}; }
+Space simt_space(int Dh, int64_t rows, int num_sms) {
+  if (Dh > 128) return {2, 2 * num_sms};
+  return rows == 1 ? Space{1, 3 * num_sms} : Space{4, 2 * num_sms};
+}
 // Rows of a KV head in one item: 8 for a step of up to 8 query heads, else 16.
 Space mma_space(int64_t rows, int num_sms) {
   return rows <= 8 ? Space{8, 3 * num_sms} : Space{16, 2 * num_sms};
@@ -119,7 +122,7 @@ Space tf32_space(int num_sms) { return {128, num_sms}; }
 }  // namespace
 
 size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
-  size_t n = std::max(simt_space(Dh, num_sms).bytes(Dh), mma_space(16, num_sms).bytes(Dh));
+  size_t n = std::max(simt_space(Dh, 4, num_sms).bytes(Dh), mma_space(16, num_sms).bytes(Dh));
   if (Dh <= 128) n = std::max(n, tf32_space(num_sms).bytes(Dh));
   if (G <= 128 && Dh <= 128) n = std::max(n, tc_space(G, num_sms).bytes(Dh));
   return n + 256;
@@ -139,7 +142,7 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   const Space sp = kind == kTc     ? tc_space(a.G, num_sms)
                    : kind == kMma  ? mma_space(rows, num_sms)
                    : kind == kTf32 ? tf32_space(num_sms)
-                                   : simt_space(a.q.Dh, num_sms);
+                                   : simt_space(a.q.Dh, rows, num_sms);
   a.rows = sp.rows;
   a.kt_shift = kind == kTc ? 7 : kind == kTf32 ? 5 : 6;
   a.min_tiles = 2;

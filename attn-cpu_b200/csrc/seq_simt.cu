@@ -12,7 +12,8 @@
 // Each group keeps its own maximum, sum and accumulator in registers; they meet
 // in shared memory once per piece.  Four rows are what the registers hold (64
 // for q, 64 for the accumulator, 64 for K or V in flight); more rows read the
-// keys again, from L2.
+// keys again, from L2.  For a single row (a step without grouped heads) the
+// registers hold V next to K, so that both are in flight at once.
 #include <cmath>
 
 #include "seq.cuh"
@@ -49,7 +50,7 @@ __device__ __forceinline__ void load_row(const E* p, int e, int Dh, bool vec, fl
 }
 
 template <int TQ, int TK, int R, int NC>
-__global__ void __launch_bounds__(kThreads) seq_simt_kernel(const SeqAttnArgs a, const bool qvec,
+__global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(const SeqAttnArgs a, const bool qvec,
                                                             const bool kvec) {
   using EQ = elem_t<TQ>;
   using EK = elem_t<TK>;
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(kThreads) seq_simt_kernel(const SeqAttnArgs a,
         }
       }
       float s[R][kKeys];
+      float v[R == 1 ? kKeys : 1][NC * 4];
       {
         float x[kKeys][NC * 4];
 #pragma unroll
@@ -132,6 +134,11 @@ __global__ void __launch_bounds__(kThreads) seq_simt_kernel(const SeqAttnArgs a,
 #pragma unroll
           for (int i = 0; i < NC * 4; ++i) x[u][i] = 0.f;
           if (kp[u]) load_row<EK, NC>(kp[u], e, Dh, kvec, x[u]);
+        }
+        if constexpr (R == 1) {
+#pragma unroll
+          for (int u = 0; u < kKeys; ++u)
+            if (vp[u]) load_row<EK, NC>(vp[u], e, Dh, kvec, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < kKeys; ++u)
@@ -167,15 +174,15 @@ __global__ void __launch_bounds__(kThreads) seq_simt_kernel(const SeqAttnArgs a,
 #pragma unroll
       for (int u = 0; u < kKeys; ++u) {
         if (!vp[u]) continue;
-        float x[NC * 4];
-        load_row<EK, NC>(vp[u], e, Dh, kvec, x);
+        const int at = R == 1 ? u : 0;
+        if constexpr (R > 1) load_row<EK, NC>(vp[u], e, Dh, kvec, v[0]);
         const int key = key0 + u * kGroups;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           // A masked value may be anything: it is left out, not multiplied by 0.
           if (key >= seen[r]) continue;
 #pragma unroll
-          for (int i = 0; i < NC * 4; ++i) acc[r][i] = fmaf(s[r][u], x[i], acc[r][i]);
+          for (int i = 0; i < NC * 4; ++i) acc[r][i] = fmaf(s[r][u], v[at][i], acc[r][i]);
         }
       }
     }
@@ -244,15 +251,17 @@ void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
                   rows_aligned(a.v.data, a.v.sT, a.v.sH, a.q.Dh, tk);
   auto go = [&](auto tq, auto tkc) {
     constexpr int TQ = decltype(tq)::value, TK = decltype(tkc)::value;
-    if (a.q.Dh <= 64)
-      ATTNB_CUDA(launch_pdl(seq_simt_kernel<TQ, TK, 4, 2>, dim3(ctas), dim3(kThreads), 0, s, a,
+    auto run = [&](auto rows, auto nc) {
+      constexpr int R = decltype(rows)::value, NC = decltype(nc)::value;
+      ATTNB_CUDA(launch_pdl(seq_simt_kernel<TQ, TK, R, NC>, dim3(ctas), dim3(kThreads), 0, s, a,
                             qvec, kvec));
-    else if (a.q.Dh <= 128)
-      ATTNB_CUDA(launch_pdl(seq_simt_kernel<TQ, TK, 4, 4>, dim3(ctas), dim3(kThreads), 0, s, a,
-                            qvec, kvec));
-    else
-      ATTNB_CUDA(launch_pdl(seq_simt_kernel<TQ, TK, 2, 8>, dim3(ctas), dim3(kThreads), 0, s, a,
-                            qvec, kvec));
+    };
+    using std::integral_constant;
+    if (a.q.Dh > 128) run(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+    else if (a.rows == 1 && a.q.Dh <= 64) run(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    else if (a.rows == 1) run(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else if (a.q.Dh <= 64) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
   };
   with_value_type(a.q.type, [&](auto tq) {
     if (tk == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});

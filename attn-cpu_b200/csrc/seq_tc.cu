@@ -533,9 +533,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                   km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
                   vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
                 }
-                // The largest scales' powers of two (as in row_scale, kept to
+                // The largest scales' powers of two (as in row_scale; V's kept to
                 // 2^-60 .. 2^60: sums carry their inverses).
-                const float ke = fminf(fmaxf(1.f / row_scale(km), 0x1p-60f), 0x1p60f);
+                const float ke = 1.f / row_scale(km);
                 const float ve = fminf(fmaxf(1.f / row_scale(vm), 0x1p-60f), 0x1p60f);
                 if (!gone) mul = sc[row] / ke;
                 vmul[hf] = gone ? 0.f : sc[64 + row] / ve;
@@ -608,6 +608,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       const int64_t token = w.s.q0 + row / a.G;
       const int head = w.h * a.G + row % a.G;
       float m = -INFINITY, l = 0.f, scale = a.scale_log2;
+      float mraw = 0.f;  // m as a score of the current step, 0 while there is none
       if (ok && n > 0 && !qtma) {
         // ---- Q: this thread's row into its tile (the products that read the
         // row before are done: the last S of the piece before has been seen)
@@ -686,22 +687,28 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
-        const float top = fmaf(max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]), mul, add);
-        const bool need = top > m + kRescaleGap;
+        const float smax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        const float top = fmaf(smax, mul, add);
+        // (m + 8 would round, next to 2^27; beyond 2^26 a new maximum always moves m.)
+        const bool need = top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
         const bool rescale = __any_sync(0xffffffffu, need);
         float alpha = 1.f;
         if (need) {
           alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
           m = top;
+          mraw = smax;
+        } else if (CODED && m != -INFINITY) {
+          mraw = (m - add) / mul;
         }
-        const float use = m == -INFINITY ? 0.f : m;
-        const float off = add - use;
-        const uint64_t mul2 = pack_f32x2(mul, mul), off2 = pack_f32x2(off, off);
+        // Exponents from the difference to the maximum's score: the maximum's own
+        // is 0 whatever its magnitude, where s * mul - m would be off by the last
+        // place of m (32 for scores of 2^28).
+        const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-mraw, -mraw);
         uint64_t ls[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < BS; k += 2) {
-          const uint64_t x = fma_f32x2(
-              pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), mul2, off2);
+          const uint64_t x = mul_f32x2(
+              add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), ref2), mul2);
           float p0, p1;
           unpack_f32x2(x, p0, p1);
           p0 = fast_exp2(p0);

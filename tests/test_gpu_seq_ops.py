@@ -30,9 +30,9 @@ def _smax(q, k, scale=None):
     return float(q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max()) * s if q.numel() and k.numel() else 1.0
 
 
-def _check(o, ref, mag, dtype, smax, coded=False, L=1):
+def _check(o, ref, mag, dtype, smax, coded=False, L=1, floor=0.0):
     o = o.double().cpu()
-    bound = seq_ref.attention_bound(dtype, mag, ref, smax, coded, ref.shape[-1], L)
+    bound = seq_ref.attention_bound(dtype, mag, ref, smax, coded, ref.shape[-1], L) + floor
     bad = ~((o - ref).abs() <= bound)
     assert not bad.any(), (int(bad.sum()), float(((o - ref).abs() / bound).nan_to_num(1e9).max()))
 
@@ -565,3 +565,66 @@ def test_python_layer_refusals(cuda):
         capi.check(capi.lib().attnb_attn_packed_dev(
             *(capi._rows(t, "x", q.device) for t in (q, k, k, o)), cu.data_ptr(), cu.data_ptr(), 1,
             1, 0.0, o.data_ptr(), 64, capi._stream()))
+
+
+def test_cache_object_refused_append_and_truncated_read(cuda):
+    """A rejected append leaves the cache as it was; a truncated sequence reads back its prefix."""
+    H, D = 2, 64
+    cache = capi.PagedKVCacheDev(2, H, D, num_pages=12, page_size=16, dtype=BF16)
+    g = _gen(30)
+    k, v = (_randn(g, 70, H, D, dtype=BF16) for _ in range(2))
+    cache.append(k, v, [50, 20])
+    with pytest.raises(capi.AttnbError, match="matching the pages"):
+        cache.append(*(torch.zeros(60, H + 1, D, dtype=BF16, device="cuda") for _ in range(2)),
+                     [60, 0])
+    assert cache.lengths == [50, 20]
+    k2, v2 = (_randn(g, 3, H, D, dtype=BF16) for _ in range(2))
+    cache.append(k2, v2, [3, 0])
+    cache.truncate(0, 33)
+    back = [torch.empty(33, H, D, dtype=BF16, device="cuda") for _ in range(2)]
+    cache.read(0, *back)
+    assert torch.equal(back[0], k[:33]) and torch.equal(back[1], v[:33])
+    back = [torch.empty(20, H, D, dtype=BF16, device="cuda") for _ in range(2)]
+    cache.read(1, *back)
+    assert torch.equal(back[0], k[50:]) and torch.equal(back[1], v[50:])
+    with pytest.raises(ValueError, match="append first"):
+        cache.attend(k[:1].expand(1, H, D), torch.empty(1, H, D, dtype=BF16, device="cuda"))
+
+
+@pytest.mark.parametrize("cache_type", [E4M3, I8])
+@pytest.mark.parametrize("new", [1, 60])
+def test_queries_and_keys_of_any_magnitude(cuda, cache_type, new):
+    """Rows of queries next to overflow, tiny ones and zeros, and keys and values whose scales are
+    far apart: codes and rows are brought to f16 by powers of two."""
+    p = Pool([200], 1, 64, 16, BF16, cache_type, 31)
+    p.x[0][:] *= 2.0 ** -100
+    p.x[1][::3] *= 2.0 ** -20
+    p.x[1][1::3] *= 2.0 ** 30
+    p.append()
+    q = _randn(_gen(31), new, 4, 64, dtype=BF16)
+    q *= 2.0 ** 100
+    q[:, 2] = 0
+    q[:, 3] = (q[:, 3].sign() * 1.5) * 2.0 ** 127  # scores of 2^28: one key takes all
+    o = torch.empty_like(q)
+    capi.attn_paged_dev(q, p.kp, p.vp, o, seq_ref.starts([new]), p.table, p.lens, new, True, None,
+                        p.ks, p.vs)
+    ks, vs = p.held(0), p.held(1)
+    ref, mag = seq_ref.attention(q, ks, vs, [new])
+    assert torch.isfinite(o.float()).all() and (o[:, 3] != 0).any()
+    # Weights and values are f16 over codes.  Below 2^-14 f16 has steps of 2^-24, so a weight is off
+    # by up to 2^-25 of the row's largest one (which is at least 1 before it is rounded, and at most
+    # the sum it is divided by): 2^-25 sum |v_j| in all.  A value is off by up to 2^-25 of a unit that
+    # is at most the largest |v| of its 64 keys, twice (two roundings), and the weights sum to 1.
+    v = vs[0][:, 0].abs()
+    floor = 2.0 ** -25 * v.sum(0) + 2.0 ** -24 * v.max()
+    _check(o[:, :3], ref[:, :3], mag[:, :3], BF16, _smax(q[:, :3].cpu(), ks[0]), True, 200, floor)
+
+
+def test_no_keys_at_all(cuda):
+    for dtype in (F32, BF16):
+        q = _randn(_gen(32), 20, 4, 64, dtype=dtype)
+        k = q[:0, :2]
+        o = torch.full_like(q, float("nan"))
+        none = torch.zeros(3, dtype=torch.int32, device="cuda")
+        capi.attn_packed_dev(q, k, k, o, seq_ref.starts([5, 15]), none)
+        assert (o == 0).all()
