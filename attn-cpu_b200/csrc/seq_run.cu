@@ -112,7 +112,9 @@ Space simt_space(int Dh, int64_t rows, int num_sms) {
   if (Dh > 128) return {2, 2 * num_sms};
   return rows == 1 ? Space{1, 3 * num_sms} : Space{4, 2 * num_sms};
 }
-// Rows of a KV head in one item: 8 for a step of up to 8 query heads, else 16.
+// Rows of a KV head in one item: 8 for a step of up to 8 query heads, else 16 (32
+// sequences of 4096 bf16 keys: 4 rows 91 us against 94, e4m3 59 against 90; 16
+// rows 169 us against 103, e4m3 99 against 98).
 Space mma_space(int64_t rows, int num_sms) {
   return rows <= 8 ? Space{8, 3 * num_sms} : Space{16, 2 * num_sms};
 }
@@ -134,16 +136,17 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // New tokens of one sequence: the caller's bound, or the mean.
   const int64_t rows =
       (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
-  // K7 up to 32 rows (a step, or a few drafted tokens): 64 sequences over e4m3
-  // pages take it 122 us, where 256-row items would convert every key in four
-  // warps; past two of its 16-row items the keys would be read a third time.
-  // K9 over 8 rows: K6 reads the keys once for every 4 rows (440 us against 123
-  // on 3 fp32 prompts of 101-901 tokens).
+  // Rows of one KV head and sequence.  16-bit pages: K7 up to 32 rows, K8 beyond (32
+  // sequences of 4096 keys, 8 KV heads of 128: 16 rows 103 us against 192, 32 rows
+  // 183 against 187, 48 rows 257 against 191); codes, which K8 converts in four
+  // warps: up to 64 (64 rows 325 us against 343, 128 rows 620 against 320).  In
+  // fp32, K9 over 16 rows (8 sequences of 2000 keys, 4 KV heads of 64: 16 rows 53 us
+  // both, 64 rows 62 us against K6's 169).
   enum { kSimt, kMma, kTc, kTf32 } kind = kSimt;
-  if (seq_mma_supported(a) && rows <= 32) kind = kMma;
+  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 64 : 32)) kind = kMma;
   else if (seq_tc_supported(a)) kind = kTc;
   else if (seq_mma_supported(a)) kind = kMma;
-  else if (a.q.Dh <= 128 && rows > 8) kind = kTf32;
+  else if (a.q.Dh <= 128 && rows > 16) kind = kTf32;
   const Space sp = kind == kTc     ? tc_space(a.G, num_sms)
                    : kind == kMma  ? mma_space(rows, num_sms)
                    : kind == kTf32 ? tf32_space(num_sms)
