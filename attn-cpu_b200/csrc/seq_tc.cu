@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       while (ok && it.next(a, w)) {
         const int at = piece % kPoison;
         int* ps = reinterpret_cast<int*>(mem + Cfg::OFF_X) + at * 3 * DHP;
-        if (poison_set[at]) {  // set by piece - kPoison, whose outputs come first
+        // Piece - kPoison had the place before; its outputs come first.
+        auto settle = [&] {
           const uint64_t t0 = globaltimer();
           const int want = 4 * (piece - kPoison + 1);
           while (*(volatile int*)&outputs[0] < want || *(volatile int*)&outputs[1] < want) {
@@ -436,6 +437,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             }
           }
           __syncwarp();
+        };
+        if (*(volatile int*)&poison_set[at]) {
+          settle();
           for (int i = lane; i < 3 * DHP; i += 32) ps[i] = INT_MAX;
           if (lane == 0) poison_set[at] = 0;
           __syncwarp();
@@ -469,6 +473,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               }
             }
             const bool hit = __any_sync(0xffffffffu, found);
+            if (hit) settle();
             if (hit)
               for (int i = lane; i < units; i += 32) {
                 const int r = from + (i >> 3), u = i & 7;

@@ -628,3 +628,27 @@ def test_no_keys_at_all(cuda):
         none = torch.zeros(3, dtype=torch.int32, device="cuda")
         capi.attn_packed_dev(q, k, k, o, seq_ref.starts([5, 15]), none)
         assert (o == 0).all()
+
+
+def test_masked_infinities_in_many_short_sequences(cuda):
+    """Sequences of a tile or less, every second one with values that only its last row may see:
+    the notes about masked values of one item do not reach its neighbours."""
+    new = [3, 70, 1, 40, 129, 5] * 120
+    D, g = 64, _gen(33)
+    q = _randn(g, sum(new), 4, D, dtype=BF16)
+    k, v = (_randn(g, sum(new), 2, D, dtype=BF16) for _ in range(2))
+    ref, mag = seq_ref.attention(q, _split(k, new), _split(v, new), new)
+    smax = _smax(q, k)
+    first, last = [], 0
+    for i, n in enumerate(new):
+        last += n
+        if i % 2 and n > 1:
+            v[last - 1] = float("inf") if i % 4 == 1 else float("nan")
+            first.append(last - 1)
+    o = torch.full_like(q, 3.0)
+    capi.attn_packed_dev(q, k, v, o, seq_ref.starts(new), causal=True)
+    poisoned = torch.zeros(len(q), dtype=torch.bool)
+    poisoned[first] = True
+    assert not torch.isfinite(o[poisoned.cuda()].float()).any()
+    _check(o[~poisoned.cuda()], ref[~poisoned], mag[~poisoned], BF16, smax, L=130)
+    capi.stream_status()
