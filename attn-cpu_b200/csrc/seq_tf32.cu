@@ -50,6 +50,14 @@ __device__ __forceinline__ float2 split_tf32(float x) {
   return make_float2(big, tf32_round(x - big));
 }
 
+// tf32_round adds to the bits, which takes a NaN with a full payload (what CUDA's
+// arithmetic returns) to -0 and one with a small payload to infinity.  Operands
+// therefore hold a NaN as this one, which is rounded to itself; its small part
+// becomes -0.
+__device__ __forceinline__ float plain_nan(float x) {
+  return x != x ? __int_as_float(0x7fc00000) : x;
+}
+
 __device__ __forceinline__ void mma_tf32_sync(float (&d)[4], const float (&a)[4], float b0,
                                               float b1) {
   asm volatile(
@@ -97,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                       (int64_t)(w.h * a.G + row % a.G) * a.q.sH + d]) *
             a.scale_log2;
       }
-      qs[r * Cfg::QROW + d] = x;
+      qs[r * Cfg::QROW + d] = plain_nan(x);
     }
     // K and V of a tile as they come, times their scales.
     float kr[QUADS][4], vr[QUADS][4];
@@ -174,8 +182,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           finite = finite && fabsf(vr[u][e]) <= 3.402823466e38f;
-          kp[r * Cfg::KROW + d + e] = split_tf32(kr[u][e]);
-          vp[r * Cfg::VROW + d + e] = split_tf32(vr[u][e]);
+          kp[r * Cfg::KROW + d + e] = split_tf32(plain_nan(kr[u][e]));
+          vp[r * Cfg::VROW + d + e] = split_tf32(plain_nan(vr[u][e]));
         }
       }
       // A V that is not finite cannot be split, and must not reach the rows that
