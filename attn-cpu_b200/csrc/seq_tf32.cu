@@ -49,6 +49,14 @@ __device__ __forceinline__ float2 split_tf32(float x) {
   const float big = tf32_round(x);
   return make_float2(big, tf32_round(x - big));
 }
+// The same where x may be next to the largest fp32 number.  That rounds to
+// infinity; there both parts are cut off, so that their sum stays below it.
+__device__ __forceinline__ float2 split_tf32_any(float x) {
+  const float2 s = split_tf32(x);
+  if (fabsf(s.x) != INFINITY) return s;
+  const float big = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+  return make_float2(big, __uint_as_float(__float_as_uint(x - big) & 0xFFFFE000u));
+}
 
 // tf32_round adds to the bits, which takes a NaN with a full payload (what CUDA's
 // arithmetic returns) to -0 and one with a small payload to infinity.  Operands
@@ -182,8 +190,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           finite = finite && fabsf(vr[u][e]) <= 3.402823466e38f;
-          kp[r * Cfg::KROW + d + e] = split_tf32(plain_nan(kr[u][e]));
-          vp[r * Cfg::VROW + d + e] = split_tf32(plain_nan(vr[u][e]));
+          kp[r * Cfg::KROW + d + e] = split_tf32_any(plain_nan(kr[u][e]));
+          vp[r * Cfg::VROW + d + e] = split_tf32_any(plain_nan(vr[u][e]));
         }
       }
       // A V that is not finite cannot be split, and must not reach the rows that

@@ -121,6 +121,21 @@ def test_nan_in_fp32(cuda, bits, paged, n):
     _check(torch.where(want, 0.0, o.cpu()), torch.where(want, 0.0, ref[0]), bound)
 
 
+@pytest.mark.parametrize("n", [3, 300])
+def test_largest_fp32_values(cuda, n):
+    """The largest and the lowest fp32 number among the values stay finite numbers."""
+    D, L = 64, 300
+    g = _gen(42)
+    q, k, v = _randn(g, n, 4, D), _randn(g, L, 2, D), _randn(g, L, 2, D)
+    v[0, :, 3] = torch.finfo(F32).max
+    v[0, :, 4] = torch.finfo(F32).min
+    ref = _reference(q, k, v)
+    o = torch.empty_like(q)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    capi.attn_packed_dev(q, k, v, o, cu, seq_ref.starts([L]), causal=True)
+    _check(o, ref[0], _bound(F32, False, ref, L))
+
+
 @pytest.mark.parametrize("rows,cache", [(F32, E4M3), (F32, I8)])
 @pytest.mark.parametrize("n", [3, 300])
 @pytest.mark.parametrize("bad", ["k", "v"])
