@@ -21,11 +21,13 @@
 //
 // Codes: both products run in f16, where e4m3 and int8 codes are exact.  Q is
 // brought to [1, 2) by a power of two per row (bf16 has more range than f16).
-// The V scale enters the exponent: with s' = s + log2(vscale) and m the maximum
-// of s', the weights 2^(s' - m) lie in [0, 1] whatever the scales are, and the
-// sum takes 2^(s' - m) / vscale.  Weights are rounded to the products' type
-// once (half a step of 2^-11 in f16, 2^-8 in bf16, of weights at most 1); sums,
-// maxima and accumulators are fp32.
+// The V scale enters the exponent of a weight, which keeps a reference of its
+// own: with m the running maximum of the scores, the sum takes 2^(s - m) and the
+// product 2^(s - m + log2(vscale) - rho), rho a running bound of that exponent
+// (which may pass it by 8: f16 holds 2^8).  So neither overflows or vanishes whatever
+// the scales are, and a vector of zeros (scale 0) weighs nothing; 2^rho goes
+// into the output.  Weights are rounded to the products' type once (half a step
+// of 2^-11 in f16, 2^-8 in bf16); sums, maxima and accumulators are fp32.
 //
 // Measured: 32 sequences of 500-4096 bf16 keys, 32/8 heads (296 MB) 59 us, 64 of
 // 1000-8192 keys in e4m3 (622 MB) 122 us, both 5 TB/s with the join; one context
@@ -46,6 +48,8 @@ namespace {
 constexpr int kKeys = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
+constexpr float kRhoGap = 8.f;
+constexpr float kNoRho = -1e30f;  // no weight so far: any exponent is above it
 
 // NR: query rows / 8.
 template <int TK, int DHP, int NR>
@@ -176,9 +180,9 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           if constexpr (CODED) {
             if (page[i] < a.pages.num_pages) {
               bytes += 2 * box * 4;
-            } else if (lane < 2) {  // no such page: codes 0 with a scale of 1
+            } else if (lane < 2) {  // no such page: codes 0 with a scale of 0
               float* sc = reinterpret_cast<float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
-              for (int k = 0; k < box; ++k) sc[lane * kKeys + i * box + k] = 1.f;
+              for (int k = 0; k < box; ++k) sc[lane * kKeys + i * box + k] = 0.f;
               fence_proxy_async_smem();
             }
           }
@@ -273,10 +277,12 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     }
     const int seen_min = seq_row_seen(a, w.s, w.row0);  // of the piece's first row
     float acc[KS][NR][4], m[NR][2], l[NR][2];
+    float rho[NR][2];  // codes: the product's reference, relative to m
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       m[r][0] = m[r][1] = -INFINITY;
       l[r][0] = l[r][1] = 0.f;
+      rho[r][0] = rho[r][1] = kNoRho;
 #pragma unroll
       for (int u = 0; u < KS; ++u)
 #pragma unroll
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           }
         }
         // ---- weights
-        float mulk[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, vinv[2] = {1.f, 1.f};  // of keys g, g + 8
+        float mulk[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};  // of keys g, g + 8
         if constexpr (CODED) {
           const float* sc =
               reinterpret_cast<const float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
@@ -331,20 +337,17 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           for (int i = 0; i < 2; ++i) {
             const int at = warp * 16 + g + 8 * i;
             mulk[i] = sc[at];
-            // A vector of zeros has scale 0; any small one does for it.
-            const float vs = sc[kKeys + at];
-            add[i] = __log2f(vs < 0x1p-60f ? 0x1p-60f : vs);
-            vinv[i] = fast_exp2(-add[i]);
+            lv[i] = __log2f(sc[kKeys + at]);  // -inf for a vector of zeros
           }
         }
         uint32_t p[NR][2];
         bool moved = false;
-        float alpha[NR][2];
+        float alpha[NR][2];  // what acc is multiplied by
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if constexpr (CODED) s[r][e] = fmaf(s[r][e], mulq[r][e & 1] * mulk[e >> 1], add[e >> 1]);
+            if constexpr (CODED) s[r][e] *= mulq[r][e & 1] * mulk[e >> 1];
             else s[r][e] *= mulq[r][e & 1];
             if (masked && key0 + g + 8 * (e >> 1) >= seen[r][e & 1]) s[r][e] = -INFINITY;
           }
@@ -356,25 +359,58 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             top = fmaxf(top, m[r][i]);
             const float use = top == -INFINITY ? 0.f : top;
-            alpha[r][i] = fast_exp2(m[r][i] - use);
-            moved |= alpha[r][i] != 1.f;
+            const float beta = fast_exp2(m[r][i] - use);
+            if constexpr (CODED) {
+              if (m[r][i] != -INFINITY) rho[r][i] -= top - m[r][i];
+            } else {
+              alpha[r][i] = beta;
+              moved |= beta != 1.f;
+            }
             m[r][i] = top;
-            l[r][i] *= alpha[r][i];
+            l[r][i] *= beta;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const float x = fast_exp2(s[r][i + 2 * k] - use);
-              s[r][i + 2 * k] = x;
-              // The scale of a masked key may be anything.
-              if constexpr (CODED) l[r][i] += x != 0.f ? x * vinv[k] : 0.f;
-              else l[r][i] += x;
+              const float x = s[r][i + 2 * k] - use;
+              const float weight = fast_exp2(x);
+              l[r][i] += weight;
+              if constexpr (CODED) {
+                // The scale of a masked key may be anything.
+                s[r][i + 2 * k] = x == -INFINITY ? x : x + lv[k];
+                moved |= s[r][i + 2 * k] - rho[r][i] > kRhoGap;
+              } else {
+                s[r][i + 2 * k] = weight;
+              }
             }
           }
+        }
+        moved = __any_sync(0xffffffffu, moved);
+        if constexpr (CODED) {
+          if (moved) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float top = fmaxf(s[r][i], s[r][i + 2]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                top = fmaxf(top, rho[r][i]);
+                alpha[r][i] = fast_exp2(rho[r][i] - top);
+                rho[r][i] = top;
+              }
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][e] = fast_exp2(s[r][e] - rho[r][e & 1]);
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
             p[r][k] = transposed(BF16 ? pack_bf16(s[r][2 * k], s[r][2 * k + 1])
                                       : pack_f16(s[r][2 * k], s[r][2 * k + 1]));
-        }
-        if (__any_sync(0xffffffffu, moved)) {
+        if (moved) {
 #pragma unroll
           for (int u = 0; u < KS; ++u)
 #pragma unroll
@@ -459,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
       }
     named_bar_sync(1, kWarps * 32);
     const int slot = seq_slot(w, first);
-    float f[NR][2];
+    float f[NR][2], fr[NR][2];  // two factors: 2^rho may lie below the smallest fp32 number
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -470,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         const float use = top == -INFINITY ? 0.f : top;
         for (int k = 0; k < kWarps; ++k)
           total += fast_exp2(sm_ml[k][rr].x - use) * sm_ml[k][rr].y;
-        f[r][i] = fast_exp2(m[r][i] - use);
+        fr[r][i] = CODED ? fast_exp2(0.5f * (m[r][i] - use + rho[r][i])) : 1.f;
+        f[r][i] = CODED ? fr[r][i] : fast_exp2(m[r][i] - use);
         if (slot < 0) f[r][i] = total == 0.f ? 0.f : f[r][i] / total;
         else if (warp == 0 && g == 0 && rr < w.rows)
           reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * ROWS + rr] = make_float2(top, total);
@@ -486,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           for (int e = 0; e < 4; ++e) {
             const int d = t * 16 + (CODED ? 2 * g + (e >> 1) : g + 8 * (e >> 1));
             x[(warp * ROWS + 8 * r + 2 * c + (e & 1)) * Cfg::XROW + d] =
-                acc[q4 * 2 + t][r][e] * f[r][e & 1];
+                (CODED ? acc[q4 * 2 + t][r][e] * fr[r][e & 1] : acc[q4 * 2 + t][r][e]) * f[r][e & 1];
           }
       named_bar_sync(1, kWarps * 32);
       for (int i = threadIdx.x; i < ROWS * 32; i += kWarps * 32) {

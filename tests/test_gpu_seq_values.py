@@ -9,7 +9,7 @@ import torch
 
 import seq_ref
 from attn_cpu import capi
-from test_gpu_seq_ops import E4M3, F16, F32, I8, Pool, _gen, _randn
+from test_gpu_seq_ops import BF16, E4M3, F16, F32, I8, Pool, _gen, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +157,14 @@ def test_vectors_that_are_not_finite_in_pages(cuda, rows, cache, n, bad):
     assert torch.equal(torch.isnan(o).cpu(), want)
     o = torch.where(want, 0.0, o.double().cpu())
     _check(o, torch.where(want, 0.0, ref[0]), _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, E4M3), (F32, I8)])
+@pytest.mark.parametrize("n", [1, 12])
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -70, 1e-20, 1e-5, 1e25, 2.0 ** 80])
+def test_values_of_any_size(cuda, rows, cache, n, size):
+    D, L = 64, 400
+    q = _randn(_gen(48), n, 4, D, dtype=rows)
+    p = _pool(L, 2, D, rows, cache, 49, v=lambda x: x.float() * size)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
