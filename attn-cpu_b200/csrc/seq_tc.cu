@@ -33,8 +33,12 @@
 // scale's power of two, rounded to f16 twice (2^-11 of a value each, where the
 // codes themselves are 2^-4 or 2^-8 off); keys whose scale is 2^14 below the largest
 // lose bits that are 2^-25 of the largest.  2^E goes into the rows' scale, and
-// V's 2^F into the exponent, s' = s + F, with 2^-F on the sum: nothing is left
-// to do for single keys in the softmax.
+// V's 2^F into the weights' exponent: nothing is left to do for single keys in
+// the softmax.  As in seq_mma.cu the weights of the product have a reference rho
+// of their own beside the sum's maximum m, 2^(s - m + F - rho), so that V may have
+// any size and change it from block to block; 2^rho goes into the output.  The
+// sum is theirs times 2^(rho - F), and takes exponentials of its own where that
+// factor is far from 1.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -51,6 +55,8 @@ constexpr int BM = 128;
 constexpr int BN = 128;  // keys of a tile in shared memory
 constexpr int BS = 64;   // keys of a step
 constexpr float kRescaleGap = 8.f;
+constexpr float kNoRho = -1e30f;  // no weight so far: any exponent is above it
+constexpr float kSumGap = 40.f;
 constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
 
 template <bool CODED, int DHP>
@@ -218,10 +224,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           }
           const int my_key = key0 + lane * box;
           const bool there = page < a.pages.num_pages;
-          if (lane < copies && !is_v && !there) {  // no such page: codes 0 with scales of 1
+          if (lane < copies && !is_v && !there) {  // no such page: codes 0 with scales of 0
             float* sc = reinterpret_cast<float*>(mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW +
                                                  64 * 128);
-            for (int k = 0; k < box; ++k) sc[lane * box + k] = sc[64 + lane * box + k] = 1.f;
+            for (int k = 0; k < box; ++k) sc[lane * box + k] = sc[64 + lane * box + k] = 0.f;
             fence_proxy_async_smem();
           }
           __syncwarp();
@@ -541,15 +547,15 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                   km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
                   vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
                 }
-                // The largest scales' powers of two (as in row_scale; V's kept to
-                // 2^-60 .. 2^60: sums carry their inverses).
-                const float ke = 1.f / row_scale(km);
-                const float ve = fminf(fmaxf(1.f / row_scale(vm), 0x1p-60f), 0x1p60f);
+                // The largest scales' powers of two (as in row_scale).
+                const float ke = 1.f / row_scale(km), ve = 1.f / row_scale(vm);
                 if (!gone) mul = sc[row] / ke;
                 vmul[hf] = gone ? 0.f : sc[64 + row] / ve;
                 if (t == 0) {
                   xt[hf] = ke;
-                  xt[2 + hf] = (float)((int)(__float_as_uint(ve) >> 23) - 127);
+                  // Values that are all zero weigh nothing.
+                  xt[2 + hf] =
+                      vm == 0.f ? -INFINITY : (float)((int)(__float_as_uint(ve) >> 23) - 127);
                 }
               } else {
                 mul = vmul[hf];
@@ -616,7 +622,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       const int64_t token = w.s.q0 + row / a.G;
       const int head = w.h * a.G + row % a.G;
       float m = -INFINITY, l = 0.f, scale = a.scale_log2;
-      float mraw = 0.f;  // m as a score of the current step, 0 while there is none
+      float mraw = 0.f;    // 16-bit keys: m as a score, 0 while there is none
+      float rho = kNoRho;  // codes: the product's reference, relative to m
       if (ok && n > 0 && !qtma) {
         // ---- Q: this thread's row into its tile (the products that read the
         // row before are done: the last S of the piece before has been seen)
@@ -673,15 +680,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         const int kb0 = w.j0 * BN + i * BS;
         // Masks only occur in some steps; a warp applies them only there.
         const bool masked = __any_sync(0xffffffffu, kb0 + BS > seen);
-        // Score to exponent: times mul, plus add.
-        float mul = scale, add = 0.f, linv = 1.f;
-        if constexpr (CODED) {
-          const float* x = reinterpret_cast<const float*>(
-              mem + Cfg::OFF_X + ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE) + (i & 1);
-          mul = scale * x[0];
-          add = x[2];
-          linv = fast_exp2(-add);
-        }
         uint32_t s[BS];
         tmem_ld64(sb, s);
         if (masked) {
@@ -696,27 +694,64 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           for (int u = 0; u < 4; ++u)
             mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
         const float smax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        const float top = fmaf(smax, mul, add);
-        // (m + 8 would round, next to 2^27; beyond 2^26 a new maximum always moves m.)
-        const bool need = top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
-        const bool rescale = __any_sync(0xffffffffu, need);
-        float alpha = 1.f;
-        if (need) {
-          alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
-          m = top;
-          mraw = smax;
-        } else if (CODED && m != -INFINITY) {
-          mraw = (m - add) / mul;
+        // Score to exponent: (s - sref) * mul + shift.  The maximum's own is exact
+        // whatever its magnitude, where s * mul - m would be off by the last place
+        // of m (32 for scores of 2^28).
+        float mul = scale, sref, shift = 0.f, top;
+        bool need;
+        float alpha = 1.f;  // what O is multiplied by
+        float lmul = 1.f;   // weight to term of the sum
+        if constexpr (CODED) {
+          const float* x = reinterpret_cast<const float*>(
+              mem + Cfg::OFF_X + ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE) + (i & 1);
+          mul = fmaxf(scale * x[0], 0x1p-126f);  // a masked -inf stays one
+          const float f = x[2];
+          top = smax * mul;
+          sref = smax == -INFINITY ? 0.f : smax;
+          if (top - m > kRescaleGap) {
+            if (m != -INFINITY) rho -= top - m;
+            l *= fast_exp2(m - top);
+            m = top;
+          }
+          const float lift = top == -INFINITY ? top : top - m;
+          need = lift + f - rho > kRescaleGap;
+          if (need) {
+            alpha = fast_exp2(rho - (lift + f));
+            rho = lift + f;
+          }
+          shift = lift + f - rho;
+          if (fabsf(rho - f) <= kSumGap) {
+            lmul = fast_exp2(rho - f);
+          } else {
+            // Weights of the product that are far from the sum's tell nothing of it.
+            lmul = 0.f;
+            if (top != -INFINITY) {
+#pragma unroll
+              for (int k = 0; k < BS; ++k)
+                l += fast_exp2(fmaf(__uint_as_float(s[k]) - sref, mul, lift));
+            }
+          }
+        } else {
+          top = smax * mul;
+          // (m + 8 would round, next to 2^27; beyond 2^26 a new maximum always moves m.)
+          need = top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
+          if (need) {
+            alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
+            l *= alpha;
+            m = top;
+            mraw = smax;
+          }
+          sref = mraw;
         }
-        // Exponents from the difference to the maximum's score: the maximum's own
-        // is 0 whatever its magnitude, where s * mul - m would be off by the last
-        // place of m (32 for scores of 2^28).
-        const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-mraw, -mraw);
+        const bool rescale = __any_sync(0xffffffffu, need);
+        const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-sref, -sref);
+        const uint64_t shift2 = pack_f32x2(shift, shift);
         uint64_t ls[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < BS; k += 2) {
-          const uint64_t x = mul_f32x2(
-              add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), ref2), mul2);
+          const uint64_t d =
+              add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), ref2);
+          const uint64_t x = CODED ? fma_f32x2(d, mul2, shift2) : mul_f32x2(d, mul2);
           float p0, p1;
           unpack_f32x2(x, p0, p1);
           p0 = fast_exp2(p0);
@@ -727,7 +762,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         tmem_st32(sb, *reinterpret_cast<const uint32_t(*)[32]>(s));
         float l0, l1;
         unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
-        l = fmaf(l0 + l1, linv, l * alpha);
+        l = fmaf(l0 + l1, lmul, l);
         // A score that is NaN or +inf makes the whole row NaN.
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         if (rescale && i > 0) {
@@ -754,7 +789,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       const int slot = seq_slot(w, first);
       if (ok && rows > 0) {
         tc_fence_after();
-        const float mulo = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        float mulo = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        // Two factors: 2^rho may lie below the smallest fp32 number.
+        const float half_rho = CODED ? fast_exp2(0.5f * rho) : 1.f;
+        mulo *= half_rho;
         const int* ps = reinterpret_cast<const int*>(mem + Cfg::OFF_X) + (piece % kPoison) * 3 * DHP;
         const bool hit = !CODED && *(volatile int*)&poison_set[piece % kPoison] != 0;
         const int64_t prow = (int64_t)slot * a.rows + c * half + r;
@@ -776,7 +814,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mulo);
+          for (int i = 0; i < 32; ++i) {
+            const float x = __uint_as_float(o[i]);
+            o[i] = __float_as_uint((CODED ? x * half_rho : x) * mulo);
+          }
           if (hit) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)

@@ -48,7 +48,8 @@ def _bound(rows, coded, ref, L, exact_k=False):
     since the sum of the weights is off as well: 5 * 2^-11 * s2 of sum p |v| (nothing where the
     factors are powers of two).  Weights below 2^-14 of the row's largest p_j v_j have f16's steps
     of 2^-24 and are off by 2^-25 of it each; where keys share one power of two, their scales may
-    differ by 2^6 and the reference is up to 2^7 above the largest p_j v_j."""
+    differ by 2^6 and the reference is up to 2^7 above the largest p_j v_j.  Outputs in f16 have
+    steps of 2^-24 below 2^-14 as well: their rounding is off by up to 2^-25."""
     out, mag, most, smax, s2 = ref
     rel = seq_ref.HALF[F32] * (40 * smax + 4 * out.shape[-1] ** 0.5 + 2 * L ** 0.5 + 16)
     floor = 0.0
@@ -57,7 +58,7 @@ def _bound(rows, coded, ref, L, exact_k=False):
         floor = 2.0 ** -25 * 2.0 ** 7 * L * most
     elif rows != F32:
         rel += seq_ref.HALF[rows]
-    return mag * rel + out.abs() * 1.01 * seq_ref.HALF[rows] + floor
+    return mag * rel + out.abs() * 1.01 * seq_ref.HALF[rows] + floor + (2.0 ** -25 if rows == F16 else 0.0)
 
 
 def _check(o, ref, bound):
@@ -136,6 +137,9 @@ def test_largest_fp32_values(cuda, n):
     _check(o, ref[0], _bound(F32, False, ref, L))
 
 
+CODED = [(BF16, E4M3), (F16, E4M3), (F32, E4M3), (BF16, I8), (F16, I8), (F32, I8)]
+
+
 @pytest.mark.parametrize("rows,cache", [(F32, E4M3), (F32, I8)])
 @pytest.mark.parametrize("n", [3, 300])
 @pytest.mark.parametrize("bad", ["k", "v"])
@@ -160,7 +164,7 @@ def test_vectors_that_are_not_finite_in_pages(cuda, rows, cache, n, bad):
 
 
 @pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, E4M3), (F32, I8)])
-@pytest.mark.parametrize("n", [1, 12])
+@pytest.mark.parametrize("n", [1, 12, 60, 300])
 @pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -70, 1e-20, 1e-5, 1e25, 2.0 ** 80])
 def test_values_of_any_size(cuda, rows, cache, n, size):
     D, L = 64, 400
@@ -168,3 +172,85 @@ def test_values_of_any_size(cuda, rows, cache, n, size):
     p = _pool(L, 2, D, rows, cache, 49, v=lambda x: x.float() * size)
     ref = _reference(q, p.held(0)[0], p.held(1)[0])
     _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+def _blocks(L, sizes):
+    """A factor for each token: 64 of one size, then 64 of the next."""
+    s = torch.tensor(sizes, device="cuda").repeat(-(-L // (64 * len(sizes))))
+    return s.repeat_interleave(64)[:L, None, None]
+
+
+@pytest.mark.parametrize("rows,cache", CODED)
+@pytest.mark.parametrize("n", [1, 60, 300])
+@pytest.mark.parametrize("sizes", [(0.0, 1e-4), (1e-4, 0.0, 1.0), (0.0, 2e-5), (2e-5, 1.0, 300.0)])
+def test_value_sizes_that_change_between_blocks(cuda, rows, cache, n, sizes):
+    """Whole blocks of zeros or of other sizes beside small values.  Each block's share of an output
+    is held to its own size: where one block's values are large they set the bound's floor."""
+    D, L = 64, 400
+    q = _randn(_gen(50), n, 4, D, dtype=rows)
+    p = _pool(L, 2, D, rows, cache, 51, v=lambda x: x.float() * _blocks(L, sizes))
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, E4M3)])
+@pytest.mark.parametrize("n", [3, 300])
+@pytest.mark.parametrize("qsize,ksize", [(1e-18, 1e-18), (2.0 ** -100, 2.0 ** -40), (2.0 ** -126, 2.0 ** -100),
+                                         (2.0 ** 100, 2.0 ** -100)])
+def test_tiny_queries_and_keys(cuda, rows, cache, n, qsize, ksize):
+    """Scores next to 0 over values whose size changes from block to block."""
+    D, L = 64, 400
+    q = (_randn(_gen(56), n, 4, D) * qsize).to(rows)
+    p = _pool(L, 2, D, rows, cache, 57, lambda x: x.float() * ksize,
+              lambda x: x.float() * _blocks(L, (1.0, 2.0 ** -12)))
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
+@pytest.mark.parametrize("n", [1, 60])
+def test_one_key_takes_all(cuda, cache, n):
+    """Scores of 2^28: the output is the value of the key with the largest score."""
+    D, L = 64, 200
+    q = (_randn(_gen(60), n, 4, D).sign() * 1.5 * 2.0 ** 127).to(BF16)
+    p = _pool(L, 1, D, BF16, cache, 61, lambda x: x.float() * 2.0 ** -100)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    k = p.held(0)[0][:, 0]
+    s = torch.einsum("nhd,ld->nhl", q.double().cpu(), k) * D ** -0.5
+    s = torch.where(torch.arange(L) <= (L - n + torch.arange(n))[:, None, None], s, -torch.inf)
+    two = s.topk(2, -1).values
+    # Rows whose two best scores are nearer than the roundings of K (5 * 2^-11 * s2, as in _bound) and
+    # of fp32 sums allow are left out; there are few.
+    clear = two[..., 0] - two[..., 1] > 5 * HALF_F16 * ref[4] + 2.0 ** -19 * ref[3]
+    assert clear.float().mean() > 0.8
+    out = ref[0] * clear[..., None]
+    o = _attend(p, q).double().cpu() * clear[..., None]
+    # V as code * factor in f16 (two roundings) and the output in bf16.
+    _check(o, out, out.abs() * (2 * HALF_F16 + 1.01 * seq_ref.HALF[BF16]) + 2.0 ** -24 * ref[1].max())
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_short_chunks_over_codes(cuda, cache, D):
+    """Chunks of one and a few steps, with fewer keys than rows or more, whose tiles have scales of
+    their own: each tile's belong to it for as long as both row tiles of an item need them."""
+    keys = [(b * 37) % 260 + 1 for b in range(70)]
+    new = [(b * 53) % 200 + 40 for b in range(70)]
+    new = [min(n, 2 * k + 30) for n, k in zip(new, keys)]
+    p = Pool(keys, 2, D, 32, BF16, cache, 63)
+    size = torch.tensor([2.0 ** ((b * 7) % 11 - 5) for b in range(70)], device="cuda")
+    p.x[1] = (p.x[1] * size.repeat_interleave(torch.tensor(keys, device="cuda"))[:, None, None]).to(BF16)
+    p.append()
+    q = _randn(_gen(64), sum(new), 4, D, dtype=BF16)
+    o = torch.full_like(q, 7.0)
+    capi.attn_paged_dev(q, p.kp, p.vp, o, seq_ref.starts(new), p.table, p.lens, max(new), True, None,
+                        p.ks, p.vs)
+    first = 0
+    for n, k, v in zip(new, *(p.held(i) for i in (0, 1))):
+        there = min(n, len(k))  # the rows before see no key
+        rows = slice(first + n - there, first + n)
+        ref = _reference(q[rows], k, v)
+        _check(o[rows], ref[0], _bound(BF16, True, ref, len(k)))
+        assert (o[first:first + n - there] == 0).all()
+        first += n
+    capi.stream_status()
