@@ -18,11 +18,12 @@
 //   Warp 0 loads; warps 1 and 2 issue the chains' scores and two others their
 //   P V (a thread that waits for the one would hold up the other); warps 4-7 and
 //   8-11 own one row of A or B per thread; one warp clears masked V values.
-//   With codes, warps 12-15 turn them into f16 tiles.
+//   With codes, warps 12-15 turn them into f16 tiles, by factors that warp 17 has
+//   made of their scales.
 //   CTAs are persistent and walk the pieces of the schedule in seq.cuh.
 //   Measured: prompts of 5000 and 8000 tokens, 32/8 heads, bf16, 750 us (970
 //   TFLOP/s of visible work); chunks of 1024-2048 tokens over 6000-16000 int8 keys
-//   1.15 ms (519 TFLOP/s: the conversion of codes shares the SM's issue slots).
+//   983 us (607 TFLOP/s: the conversion of codes shares the SM's issue slots).
 //
 // The running maximum moves only when it grows by more than 8 (weights stay
 // below 2^8, which f16 and bf16 hold); O and the sum are rescaled then.  Weights
@@ -31,14 +32,18 @@
 // Codes: both products run in f16.  Q is brought to [1, 2) by a power of two per
 // row, and 64 keys at a time K becomes code * scale / 2^E with 2^E the largest
 // scale's power of two, rounded to f16 twice (2^-11 of a value each, where the
-// codes themselves are 2^-4 or 2^-8 off); keys whose scale is 2^14 below the largest
-// lose bits that are 2^-25 of the largest.  2^E goes into the rows' scale, and
+// codes themselves are 2^-4 or 2^-8 off).  2^E goes into the rows' scale, and
 // V's 2^F into the weights' exponent: nothing is left to do for single keys in
-// the softmax.  As in seq_mma.cu the weights of the product have a reference rho
-// of their own beside the sum's maximum m, 2^(s - m + F - rho), so that V may have
-// any size and change it from block to block; 2^rho goes into the output.  The
-// sum is theirs times 2^(rho - F), and takes exponentials of its own where that
-// factor is far from 1.
+// the softmax.  Where the scales of 64 keys are more than 2^6 apart, or one is not
+// finite, zero (V) or next to the ends of fp32, the tiles hold the codes as they
+// are and the softmax takes each key's scales, as in seq_mma.cu: so a key that a
+// row does not see changes nothing for it, whatever its scales are.
+// As there, the weights of the product have a reference rho of their own beside
+// the sum's maximum m, 2^(s - m + F - rho), so that V may have any size and change
+// it from block to block; 2^rho goes into the output.  The sum is theirs times
+// 2^(rho - F); where that factor could be far from 1, since F has changed much in
+// the piece, the keys go by their own scales too and the sum by exponentials of
+// its own.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -56,13 +61,18 @@ constexpr int BN = 128;  // keys of a tile in shared memory
 constexpr int BS = 64;   // keys of a step
 constexpr float kRescaleGap = 8.f;
 constexpr float kNoRho = -1e30f;  // no weight so far: any exponent is above it
-constexpr float kSumGap = 40.f;
+// V's powers of two in steps that take their sum from the product's weights: with
+// lo and hi the least and the greatest F so far, lo - 8 <= rho <= hi + 8 (the row's
+// best key was in one of them, and none is more than 8 above m), so the factor
+// 2^(rho - F) stays within 2^40 and no term that counts is lost.
+constexpr int kSpread = 24;
 constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
 
 template <bool CODED, int DHP>
 struct TcCfg {
-  static constexpr int THREADS = CODED ? 544 : 448;
+  static constexpr int THREADS = CODED ? 576 : 448;
   static constexpr int PV_A = CODED ? 3 : 12, PV_B = CODED ? 16 : 13;  // warps that issue P V
+  static constexpr int SCALER = 17;              // codes: warp that looks at the scales
   static constexpr int CHUNKS = DHP / 64;        // 128-byte pieces of a 16-bit row
   static constexpr int CHUNK = BN * 128;         // 16 KB: 128 rows x 64 columns
   static constexpr int TILE = CHUNKS * CHUNK;    // Q, K or V
@@ -74,10 +84,14 @@ struct TcCfg {
   static constexpr int OFF_V = OFF_K + K_ST * TILE;
   static constexpr int OFF_RAW = OFF_V + V_ST * TILE;
   static constexpr int OFF_X = OFF_RAW + (CODED ? RAW_ST * RAW : 0);
-  // Codes: four powers of two, of as many tiles as K tiles may
-  // be ahead of the softmax that reads them; else poison.
-  static constexpr int SCALES = K_ST + 2;
-  static constexpr int XTILE = 16;
+  // Codes: what the softmax needs of a tile, by half: E's and F's powers of two,
+  // both NaN where the keys go by their own scales, and then K scales and
+  // logarithms of V scales; else poison.  When a tile's raw half is there, V of the
+  // tile before the last has been converted, so the softmax is at most V_ST tiles
+  // behind that one.
+  static constexpr int SCALES = V_ST + 2;
+  static constexpr int XHEAD = 4;  // floats
+  static constexpr int XTILE = XHEAD * 4 + 2 * 128 * 4;
   // 2 KB per softmax warp to write outputs through; with codes Q's place serves.
   static constexpr int OFF_OUT = OFF_X + (CODED ? SCALES * XTILE : kPoison * 3 * DHP * 4);
   static constexpr int SMEM = OFF_OUT + (CODED ? 0 : 8 * 2048) + 1024;
@@ -93,10 +107,75 @@ __device__ __forceinline__ bool any_not_finite(const uint4& x) {
           0x80008000u) != 0;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// A step of the softmax over codes whose keys go by scales of their own (`keys`:
+// K scales, logarithms of V scales): largest exponent of the step.  Rare, so
+// that it may take three passes over the scores in TMEM; a call keeps it from
+// costing the other steps registers.
+struct RowState {
+  float m, l, rho, alpha;
+  bool need;
+};
+__device__ __noinline__ float step_by_key(RowState& st, uint32_t sb, int kb0, int seen,
+                                          float scale, const float* keys) {
+  float m = st.m, l = st.l, rho = st.rho, top = -INFINITY, best = -INFINITY;
+  uint32_t s[32];
+  auto exponent = [&](int k, uint32_t x) {
+    return kb0 + k >= seen ? -INFINITY : __uint_as_float(x) * (scale * keys[k]);
+  };
+#pragma unroll 1
+  for (int k0 = 0; k0 < BS; k0 += 32) {
+    tmem_ld32(sb + k0, s);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) top = max_nan(top, exponent(k0 + k, s[k]));
+  }
+  if (top - m > kRescaleGap) {
+    if (m != -INFINITY) rho -= top - m;
+    l *= fast_exp2(m - top);
+    m = top;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  // The scale of a masked key may be anything.
+  auto product = [&](int k, float e) { return e == -INFINITY ? e : e - ref + keys[64 + k]; };
+#pragma unroll 1
+  for (int k0 = 0; k0 < BS; k0 += 32) {
+    tmem_ld32(sb + k0, s);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const float e = exponent(k0 + k, s[k]);
+      l += fast_exp2(e - ref);
+      best = fmaxf(best, product(k0 + k, e));
+    }
+  }
+  st.need = best - rho > kRescaleGap;
+  if (st.need) {
+    st.alpha = fast_exp2(rho - best);
+    rho = best;
+  }
+#pragma unroll 1
+  for (int k0 = 0; k0 < BS; k0 += 32) {
+    tmem_ld32(sb + k0, s);
+    uint32_t p[16];
+#pragma unroll
+    for (int k = 0; k < 32; k += 2)
+      p[k >> 1] = pack_f16(fast_exp2(product(k0 + k, exponent(k0 + k, s[k])) - rho),
+                           fast_exp2(product(k0 + k + 1, exponent(k0 + k + 1, s[k + 1])) - rho));
+    tmem_st16(sb + (k0 >> 1), p);  // over scores that have been read
+  }
+  st.m = m;
+  st.l = l;
+  st.rho = rho;
+  return top;
 }
 
 template <int TQ, int TK, int DHP>
@@ -114,7 +193,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
-  __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
+  __shared__ __align__(8) uint64_t rfull[RST], rempty[RST], sfull[4];
   __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2][2], p_bar[2][2], pv_bar[2][2],
       done_bar[4];
   __shared__ SeqShared sh;
@@ -142,8 +221,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     }
     for (int i = 0; i < RST; ++i) {
       mbar_init(smem_addr(&rfull[i]), 1);
-      mbar_init(smem_addr(&rempty[i]), 4);
+      mbar_init(smem_addr(&rempty[i]), 5);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(smem_addr(&sfull[i]), 1);
     for (int c = 0; c < 2; ++c) {
       mbar_init(smem_addr(&q_bar[c]), qtma ? 1 : 4);
       mbar_init(smem_addr(&q_free[c]), 1);
@@ -508,6 +588,84 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         ++piece;
       }
     }
+  } else if (warp == Cfg::SCALER) {
+    // ------------------------------------ scales of 64 keys: what they share
+    if constexpr (CODED) {
+      Ring<RST> ring;
+      bool ok = true;
+      uint32_t tile = 0;
+      while (ok && it.next(a, w)) {
+        int lo = INT_MAX, hi = INT_MIN;  // V's powers of two in the piece so far
+        for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
+#pragma unroll 1
+          for (int part = 0; part < 4; ++part) {  // as the loader: K, K, V, V
+            ok = warp_wait(&rfull[ring.stage], ring.phase);
+            if (!ok) break;
+            if (part < 2) {
+              float* sc = reinterpret_cast<float*>(mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW + 64 * 128);
+              float* xt = reinterpret_cast<float*>(mem + Cfg::OFF_X +
+                                                   (tile % Cfg::SCALES) * Cfg::XTILE);
+              const int left = w.s.L - j * BN - part * 64;
+              const bool in0 = lane < left, in1 = lane + 32 < left;
+              // Scales past the sequence may be anything, and do not count.
+              const float k0 = in0 ? sc[lane] : 0.f, k1 = in1 ? sc[lane + 32] : 0.f;
+              const float v0 = in0 ? sc[lane + 64] : 0.f, v1 = in1 ? sc[lane + 96] : 0.f;
+              // Largest and smallest by their bits: those of an infinity or a NaN (and
+              // of a negative number) are above all others.  K scales of 0 take no part.
+              auto bits = [](float x) { return __float_as_uint(x); };
+              const uint32_t kmax = __reduce_max_sync(0xffffffffu, max(bits(k0), bits(k1)));
+              const uint32_t vmax = __reduce_max_sync(0xffffffffu, max(bits(v0), bits(v1)));
+              const uint32_t kmin = __reduce_min_sync(0xffffffffu, min(bits(k0) - 1u, bits(k1) - 1u));
+              const uint32_t vmin =
+                  __reduce_min_sync(0xffffffffu, min(in0 ? bits(v0) : ~0u, in1 ? bits(v1) : ~0u));
+              constexpr uint32_t kLow = 0x0d800000u, kHigh = 0x71800000u;  // 2^-100, 2^100
+              bool wide = false;
+              if (left > 0) {
+                // (A value of 0 may be the row's best key without a part in the
+                // product, whose weights then may lie anywhere.)
+                lo = min(lo, vmin < kLow || vmax > kHigh ? INT_MIN / 2 : (int)(vmin >> 23));
+                hi = max(hi, (int)(vmax >> 23));
+                wide = kmax > kHigh || kmin < kLow || (kmax != 0u && kmax - kmin > (6u << 23)) ||
+                       vmax > kHigh || vmin < kLow || vmax - vmin > (6u << 23) || hi - lo > kSpread;
+              }
+              // The largest scales' powers of two (as in row_scale), inverted.
+              const float ke = row_scale(__uint_as_float(kmax)), ve = row_scale(__uint_as_float(vmax));
+              if (lane == 0) {
+                const float own = __int_as_float(0x7fffffff);
+                xt[part] = wide ? own : 1.f / ke;
+                xt[2 + part] = wide ? own : (float)(127 - (int)(bits(ve) >> 23));
+              }
+              if (wide) {
+                float* keys = xt + Cfg::XHEAD + part * 128;
+                keys[lane] = k0;
+                keys[lane + 32] = k1;
+                keys[lane + 64] = __log2f(v0);
+                keys[lane + 96] = __log2f(v1);
+              }
+              // In the scales' place their factors as sums of two f16: one rounding
+              // would be an error that all the key's values share.
+              auto split = [&](float scale, float by) {
+                const float f = wide ? 1.f : scale * by;
+                const __half hi16 = __float2half_rn(f);
+                const __half2 both = __halves2half2(hi16, __float2half_rn(f - __half2float(hi16)));
+                return *reinterpret_cast<const float*>(&both);
+              };
+              sc[lane] = split(k0, ke);
+              sc[lane + 32] = split(k1, ke);
+              sc[lane + 64] = split(v0, ve);
+              sc[lane + 96] = split(v1, ve);
+              fence_proxy_async_smem();  // the next copy into the stage comes after these writes
+            }
+            __syncwarp();
+            if (lane == 0) {
+              if (part < 2) mbar_arrive(smem_addr(&sfull[(2 * tile + part) & 3]));
+              mbar_arrive(smem_addr(&rempty[ring.stage]));
+            }
+            ring.advance();
+          }
+        }
+      }
+    }
   } else if (warp >= 12) {
     // ------------------------------------------------------ codes to f16 tiles
     if constexpr (CODED) {
@@ -519,52 +677,35 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       uint32_t tile = 0;
       while (ok && it.next(a, w)) {
         for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
-          float vmul[2];  // of this thread's two keys
+          uint32_t vmul0 = 0, vmul1 = 0;  // factors of this thread's two keys, as two f16 each
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             ok = ok && (kv ? warp_wait(&vempty[rv.stage], rv.phase ^ 1u)
                            : warp_wait(&kempty[rk.stage], rk.phase ^ 1u));
             uint8_t* to = mem + (kv ? Cfg::OFF_V + rv.stage * Cfg::TILE
                                     : Cfg::OFF_K + rk.stage * Cfg::TILE);
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
               ok = ok && warp_wait(&rfull[ring.stage], ring.phase);
               if (!ok) break;
               const uint8_t* from = mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
-              float* xt = reinterpret_cast<float*>(mem + Cfg::OFF_X +
-                                                   (tile % Cfg::SCALES) * Cfg::XTILE);
-              const int r = hf * 64 + row, left = w.s.L - j * BN - hf * 64;
-              const bool gone = row >= left;  // stale: K is masked later, V is zeroed here
-              float mul = 0.f;
+              const int r = hf * 64 + row;
+              const bool gone = row >= w.s.L - j * BN - hf * 64;  // stale
+              uint32_t mul;
               if (kv == 0) {
-                // Scales of a key past the sequence may be anything.
-                const float* sc = reinterpret_cast<const float*>(from + 64 * 128);
-                float km = fmaxf(lane < left ? sc[lane] : 0.f, lane + 32 < left ? sc[lane + 32] : 0.f);
-                float vm = fmaxf(lane < left ? sc[64 + lane] : 0.f,
-                                 lane + 32 < left ? sc[96 + lane] : 0.f);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                  km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
-                  vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
-                }
-                // The largest scales' powers of two (as in row_scale).
-                const float ke = 1.f / row_scale(km), ve = 1.f / row_scale(vm);
-                if (!gone) mul = sc[row] / ke;
-                vmul[hf] = gone ? 0.f : sc[64 + row] / ve;
-                if (t == 0) {
-                  xt[hf] = ke;
-                  // Values that are all zero weigh nothing.
-                  xt[2 + hf] =
-                      vm == 0.f ? -INFINITY : (float)((int)(__float_as_uint(ve) >> 23) - 127);
-                }
+                const uint32_t n = 2 * tile + hf;
+                ok = warp_wait(&sfull[n & 3], (n >> 2) & 1);
+                if (!ok) break;
+                const uint32_t* sc = reinterpret_cast<const uint32_t*>(from + 64 * 128);
+                mul = sc[row];
+                if (hf) vmul1 = sc[64 + row];
+                else vmul0 = sc[64 + row];
               } else {
-                mul = vmul[hf];
+                mul = hf ? vmul1 : vmul0;
               }
-              // The factor as the sum of two f16: its own rounding would be one
-              // error of all the key's values.
-              const __half2 hi = __float2half2_rn(mul);
-              const __half2 lo = __float2half2_rn(mul - __low2float(hi));
-#pragma unroll
+              const __half2 both = *reinterpret_cast<const __half2*>(&mul);
+              const __half2 hi = __low2half2(both), lo = __high2half2(both);
+#pragma unroll 1  // (the instruction cache, see the softmax: 983 us, 1062 with two)
               for (int i = 0; i < DHP / 32; ++i) {
                 const int u = part * (DHP / 32) + i;  // 16 codes
                 uint4 x = *reinterpret_cast<const uint4*>(from + sw128(row, u));
@@ -680,59 +821,108 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         const int kb0 = w.j0 * BN + i * BS;
         // Masks only occur in some steps; a warp applies them only there.
         const bool masked = __any_sync(0xffffffffu, kb0 + BS > seen);
-        uint32_t s[BS];
-        tmem_ld64(sb, s);
-        if (masked) {
-#pragma unroll
-          for (int k = 0; k < BS; ++k)
-            if (kb0 + k >= seen) s[k] = __float_as_uint(-INFINITY);
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int k = 0; k < BS; k += 8)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
-        const float smax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        // Score to exponent: (s - sref) * mul + shift.  The maximum's own is exact
-        // whatever its magnitude, where s * mul - m would be off by the last place
-        // of m (32 for scores of 2^28).
-        float mul = scale, sref, shift = 0.f, top;
+        const float* xt = reinterpret_cast<const float*>(
+            mem + Cfg::OFF_X + (CODED ? ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE : 0));
+        float top, alpha = 1.f;  // largest exponent of the step; what O is multiplied by
         bool need;
-        float alpha = 1.f;  // what O is multiplied by
-        float lmul = 1.f;   // weight to term of the sum
         if constexpr (CODED) {
-          const float* x = reinterpret_cast<const float*>(
-              mem + Cfg::OFF_X + ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE) + (i & 1);
-          mul = fmaxf(scale * x[0], 0x1p-126f);  // a masked -inf stays one
-          const float f = x[2];
-          top = smax * mul;
-          sref = smax == -INFINITY ? 0.f : smax;
-          if (top - m > kRescaleGap) {
-            if (m != -INFINITY) rho -= top - m;
-            l *= fast_exp2(m - top);
-            m = top;
-          }
-          const float lift = top == -INFINITY ? top : top - m;
-          need = lift + f - rho > kRescaleGap;
-          if (need) {
-            alpha = fast_exp2(rho - (lift + f));
-            rho = lift + f;
-          }
-          shift = lift + f - rho;
-          if (fabsf(rho - f) <= kSumGap) {
-            lmul = fast_exp2(rho - f);
-          } else {
-            // Weights of the product that are far from the sum's tell nothing of it.
-            lmul = 0.f;
-            if (top != -INFINITY) {
+          // The code of this loop and of the conversion share the schedulers'
+          // instruction caches and are bound by them (unrolled, 4.4 of the 13 cycles a warp
+          // took for an instruction were waits for the instruction): so 32 scores at a
+          // time in loops, read from TMEM twice, and masks in a pass of their own.
+          uint32_t s[32];
+          const float f = xt[2 + (i & 1)];
+          if (f == f) {
+            if (masked) {
+#pragma unroll 1
+              for (int k0 = 0; k0 < BS; k0 += 32) {
+                tmem_ld32(sb + k0, s);
 #pragma unroll
-              for (int k = 0; k < BS; ++k)
-                l += fast_exp2(fmaf(__uint_as_float(s[k]) - sref, mul, lift));
+                for (int k = 0; k < 32; ++k)
+                  if (kb0 + k0 + k >= seen) s[k] = __float_as_uint(-INFINITY);
+                tmem_st32(sb + k0, s);
+              }
+              tmem_wait_st();
             }
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int k0 = 0; k0 < BS; k0 += 32) {
+              tmem_ld32(sb + k0, s);
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]),
+                                   __uint_as_float(s[k + 2 * u + 1]));
+            }
+            const float smax = max_nan(mx[0], mx[1]);
+            // (No factor below the smallest normal number: a masked -inf stays one.)
+            const float mul = fmaxf(scale * xt[i & 1], 0x1p-126f);
+            top = smax * mul;
+            if (top - m > kRescaleGap) {
+              if (m != -INFINITY) rho -= top - m;
+              l *= fast_exp2(m - top);
+              m = top;
+            }
+            const float best = top == -INFINITY ? top : top - m + f;
+            need = best - rho > kRescaleGap;
+            if (need) {
+              alpha = fast_exp2(rho - best);
+              rho = best;
+            }
+            // Score to exponent: (s - smax) * mul + shift; the maximum's own is exact
+            // whatever its magnitude.
+            const float sref = smax == -INFINITY ? 0.f : smax, shift = best - rho;
+            const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-sref, -sref);
+            const uint64_t shift2 = pack_f32x2(shift, shift);
+            uint64_t ls[2] = {0, 0};
+#pragma unroll 1
+            for (int k0 = 0; k0 < BS; k0 += 32) {
+              tmem_ld32(sb + k0, s);
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const uint64_t x =
+                    fma_f32x2(add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                        ref2),
+                              mul2, shift2);
+                float p0, p1;
+                unpack_f32x2(x, p0, p1);
+                p0 = fast_exp2(p0);
+                p1 = fast_exp2(p1);
+                ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
+                s[k >> 1] = pack_f16(p0, p1);
+              }
+              // Over scores that have been read.
+              tmem_st16(sb + (k0 >> 1), *reinterpret_cast<const uint32_t(*)[16]>(s));
+            }
+            float l0, l1;
+            unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
+            l = fmaf(l0 + l1, fast_exp2(rho - f), l);
+          } else {
+            RowState st{m, l, rho, alpha, false};
+            top = step_by_key(st, sb, kb0, seen, scale, xt + Cfg::XHEAD + (i & 1) * 128);
+            m = st.m;
+            l = st.l;
+            rho = st.rho;
+            alpha = st.alpha;
+            need = st.need;
           }
         } else {
-          top = smax * mul;
+          uint32_t s[BS];
+          tmem_ld64(sb, s);
+          if (masked) {
+#pragma unroll
+            for (int k = 0; k < BS; ++k)
+              if (kb0 + k >= seen) s[k] = __float_as_uint(-INFINITY);
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < BS; k += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
+          const float smax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+          top = smax * scale;
           // (m + 8 would round, next to 2^27; beyond 2^26 a new maximum always moves m.)
           need = top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
           if (need) {
@@ -741,28 +931,28 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             m = top;
             mraw = smax;
           }
-          sref = mraw;
+          // Exponents from the difference to the maximum's score: the maximum's own
+          // is 0 whatever its magnitude, where s * scale - m would be off by the last
+          // place of m (32 for scores of 2^28).
+          const uint64_t mul2 = pack_f32x2(scale, scale), ref2 = pack_f32x2(-mraw, -mraw);
+          uint64_t ls[2] = {0, 0};
+#pragma unroll
+          for (int k = 0; k < BS; k += 2) {
+            const uint64_t x = mul_f32x2(
+                add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), ref2), mul2);
+            float p0, p1;
+            unpack_f32x2(x, p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
+            s[k >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
+          }
+          tmem_st32(sb, *reinterpret_cast<const uint32_t(*)[32]>(s));
+          float l0, l1;
+          unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
+          l += l0 + l1;
         }
         const bool rescale = __any_sync(0xffffffffu, need);
-        const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-sref, -sref);
-        const uint64_t shift2 = pack_f32x2(shift, shift);
-        uint64_t ls[2] = {0, 0};
-#pragma unroll
-        for (int k = 0; k < BS; k += 2) {
-          const uint64_t d =
-              add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), ref2);
-          const uint64_t x = CODED ? fma_f32x2(d, mul2, shift2) : mul_f32x2(d, mul2);
-          float p0, p1;
-          unpack_f32x2(x, p0, p1);
-          p0 = fast_exp2(p0);
-          p1 = fast_exp2(p1);
-          ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
-          s[k >> 1] = BF16 ? pack_bf16(p0, p1) : pack_f16(p0, p1);
-        }
-        tmem_st32(sb, *reinterpret_cast<const uint32_t(*)[32]>(s));
-        float l0, l1;
-        unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
-        l = fmaf(l0 + l1, lmul, l);
         // A score that is NaN or +inf makes the whole row NaN.
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         if (rescale && i > 0) {

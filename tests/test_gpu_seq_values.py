@@ -140,7 +140,7 @@ def test_largest_fp32_values(cuda, n):
 CODED = [(BF16, E4M3), (F16, E4M3), (F32, E4M3), (BF16, I8), (F16, I8), (F32, I8)]
 
 
-@pytest.mark.parametrize("rows,cache", [(F32, E4M3), (F32, I8)])
+@pytest.mark.parametrize("rows,cache", CODED)
 @pytest.mark.parametrize("n", [3, 300])
 @pytest.mark.parametrize("bad", ["k", "v"])
 def test_vectors_that_are_not_finite_in_pages(cuda, rows, cache, n, bad):
@@ -161,6 +161,23 @@ def test_vectors_that_are_not_finite_in_pages(cuda, rows, cache, n, bad):
     assert torch.equal(torch.isnan(o).cpu(), want)
     o = torch.where(want, 0.0, o.double().cpu())
     _check(o, torch.where(want, 0.0, ref[0]), _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("rows,cache", CODED)
+@pytest.mark.parametrize("n", [3, 300])
+@pytest.mark.parametrize("big", ["k", "v"])
+def test_huge_vectors_behind_the_mask(cuda, rows, cache, n, big):
+    """A large finite vector at the end changes nothing for the rows that do not see it."""
+    D, L = 64, 400
+    q = _randn(_gen(45), n, 4, D, dtype=rows)
+    p = _pool(L, 2, D, rows, cache, 46)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    p.x["kv".index(big)][L - 1] = _randn(_gen(47), 2, D) * (3e4 if rows == F16 else 1e30)
+    p.x["kv".index(big)][L - 1].clamp_(*((-6e4, 6e4) if rows == F16 else (-1e31, 1e31)))
+    p.append()
+    o = _attend(p, q)[:n - 1]
+    ref = tuple(x[:n - 1] if torch.is_tensor(x) else x for x in ref)
+    _check(o, ref[0], _bound(rows, True, ref, L))
 
 
 @pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, E4M3), (F32, I8)])
@@ -193,6 +210,55 @@ def test_value_sizes_that_change_between_blocks(cuda, rows, cache, n, sizes):
     _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
 
 
+@pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, I8)])
+@pytest.mark.parametrize("n", [1, 60, 300])
+def test_value_sizes_that_no_f16_holds_together(cuda, rows, cache, n):
+    """Rows whose weight lies on small values alone: the keys of the large ones score low."""
+    D, L = 64, 400
+    q = _randn(_gen(52), n, 4, D, dtype=rows)
+    q[..., 0] = 8.0
+
+    def keys(x):
+        x = x.clone()
+        x[..., 0] = 4.0
+        x[::3, :, 0] = -60.0  # with q_0 = 8 a score of -64 less than the others: 2^-92
+        return x
+
+    def values(x):
+        x = x.float() * 1e-6
+        x[::3] *= 1e20
+        return x
+
+    p = _pool(L, 2, D, rows, cache, 53, keys, values)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    assert float(ref[1].max()) < 1e-4
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("rows,cache", CODED)
+@pytest.mark.parametrize("n", [3, 300])
+def test_key_sizes_that_differ_in_a_block(cuda, rows, cache, n):
+    """Some keys 2^15 times the others, all with very low scores: the others' scores keep their
+    bits."""
+    D, L = 64, 400
+    q = _randn(_gen(54), n, 4, D, dtype=rows)
+    q[..., 0] = 1.0
+
+    def keys(x):
+        x = x.clone()
+        x[::5] = 0
+        x[::5, :, 0] = -30000.0  # a score of -3750
+        return x
+
+    p = _pool(L, 2, D, rows, cache, 55, keys)
+    k, v = p.held(0)[0], p.held(1)[0]
+    out, mag, most, _, _ = _reference(q, k, v)
+    rest = torch.arange(L) % 5 != 0  # the weights of the large keys are 0 in 64 bits too
+    _, _, _, smax, s2 = _reference(q, k[rest], v[rest], causal=False)
+    ref = out, mag, most, smax, s2
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
 @pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (BF16, I8), (F32, E4M3)])
 @pytest.mark.parametrize("n", [3, 300])
 @pytest.mark.parametrize("qsize,ksize", [(1e-18, 1e-18), (2.0 ** -100, 2.0 ** -40), (2.0 ** -126, 2.0 ** -100),
@@ -205,6 +271,28 @@ def test_tiny_queries_and_keys(cuda, rows, cache, n, qsize, ksize):
               lambda x: x.float() * _blocks(L, (1.0, 2.0 ** -12)))
     ref = _reference(q, p.held(0)[0], p.held(1)[0])
     _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("rows,cache", CODED)
+@pytest.mark.parametrize("n", [1, 3, 30, 300])
+@pytest.mark.parametrize("L", [3, 65, 300])
+def test_weights_over_codes_have_the_bits_of_f16(cuda, rows, cache, n, L):
+    """Key scales that are powers of two, so that what is left is the rounding of weights and
+    values: bf16 weights, 2^-8, would not pass for rows in f16."""
+    if n > L:
+        pytest.skip("more new tokens than tokens")
+    D = 64
+    q = _randn(_gen(58), n, 4, D, dtype=rows)
+
+    def keys(x):
+        x = x.float().clamp(-1.7, 1.7)
+        x[..., 0] = seq_ref.TOP[cache] * 2.0 ** -8 * (4 if cache == I8 else 1)
+        return x
+
+    p = _pool(L, 2, D, rows, cache, 59, keys)
+    assert torch.equal(torch.frexp(p.ks[p.table[0, :1].long(), :, 0])[0].cpu(), torch.full((1, 2), 0.5))
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L, exact_k=True))
 
 
 @pytest.mark.parametrize("cache", [E4M3, I8])
