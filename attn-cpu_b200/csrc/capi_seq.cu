@@ -15,6 +15,8 @@ constexpr int kMaxDh = 256;
 
 void invalid(const std::string& msg) { fail(ATTNB_ERR_INVALID_ARGUMENT, msg); }
 
+bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 void check_rows(const attnb_rows* r, const char* name, bool output) {
   const std::string n(name);
   if (!r) invalid("Null " + n + " descriptor");
@@ -57,6 +59,8 @@ KvPages pages_of(const attnb_kv_pages* p, int row_type) {
     invalid("pages are not aligned to their elements");
   if (elem_coded(p->type) && (!p->k_scale || !p->v_scale))
     invalid("E4M3 and I8 pages need scales");
+  if (!aligned4(p->k_scale) || !aligned4(p->v_scale))
+    invalid("scales are not aligned to their elements");
   if (!elem_coded(p->type) && (p->k_scale || p->v_scale))
     invalid("only E4M3 and I8 pages have scales");
   return KvPages{p->k, p->v, p->k_scale, p->v_scale, p->type, p->num_pages, p->H, shift, p->Dh};
@@ -68,6 +72,8 @@ SeqTable seqs_of(const attnb_seqs* q, int total) {
   if (q->max_pages < 0) invalid("max_pages must be non-negative");
   if (q->batch > 0 && (!q->cu || !q->lens || (q->max_pages > 0 && !q->table)))
     invalid("Null cu, lens or table");
+  if (!aligned4(q->cu) || !aligned4(q->lens) || !aligned4(q->table))
+    invalid("cu, lens or table is not aligned to its elements");
   if (q->batch > 1 && q->table_stride < 0) invalid("table_stride must be non-negative");
   return SeqTable{q->cu, q->batch, total, q->table, q->table_stride, q->max_pages, q->lens};
 }
@@ -128,6 +134,8 @@ int attnb_attn_packed_dev(const attnb_rows* Q, const attnb_rows* K, const attnb_
       invalid("tokens times query heads per KV head must be below 2^30");
     if (batch < 0) invalid("batch must be non-negative");
     if (batch > 0 && (!cu_q || !cu_k)) invalid("Null cu_q or cu_k");
+    if (!aligned4(cu_q)) invalid("cu_q is not aligned to its elements");
+    if (!aligned4(cu_k)) invalid("cu_k is not aligned to its elements");
     if (!std::isfinite(scale)) invalid("scale must be finite");
     if (batch == 0 || Q->tokens == 0) return;
     if (!workspace) invalid("Null workspace");
