@@ -657,7 +657,9 @@ class PagedKVCacheDev:
     and writes its new tokens (quantising them for dtype torch.float8_e4m3fn or
     torch.int8), ``attend`` runs the new tokens' queries over everything held.
     Page numbers and lengths are kept on the host and copied to the device when
-    they change; work is enqueued on ``stream`` (default: torch's current one)."""
+    they change, to the same addresses (a captured ``attend`` can be replayed after
+    later appends of as many tokens); work is enqueued on ``stream`` (default:
+    torch's current one)."""
 
     def __init__(self, batch: int, H: int, Dh: int, num_pages: int, page_size: int = 64,
                  dtype=None, max_tokens: int | None = None, device=None):
@@ -684,6 +686,8 @@ class PagedKVCacheDev:
         self.lengths = [0] * batch
         self.table = torch.zeros(batch, width, dtype=torch.int32, device=device)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._cu = [0] * (batch + 1)  # as in cu
+        self.cu = torch.zeros(batch + 1, dtype=torch.int32, device=device)
         self._new = None
 
     def append(self, k, v, new, stream=None) -> None:
@@ -701,30 +705,37 @@ class PagedKVCacheDev:
             raise ValueError("a sequence would outgrow max_tokens")
         if sum(want) - sum(len(h) for h in self._held) > len(self._free):
             raise ValueError("the pool has too few free pages")
-        held, free, lengths = [list(h) for h in self._held], list(self._free), list(self.lengths)
-        self._new = None
-        try:
-            with _on(self.table.device, stream) or contextlib.nullcontext():
-                for h, w in zip(self._held, want):
-                    while len(h) < w:
-                        h.append(self._free.pop())
-                self.lengths = [n + m for n, m in zip(self.lengths, new)]
-                if self._held != held:
-                    width = self.table.shape[1]
-                    self.table.copy_(torch.tensor([h + [0] * (width - len(h)) for h in self._held],
-                                                  dtype=torch.int32))
-                self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
-                cu = [0]
-                for n in new:
-                    cu.append(cu[-1] + n)
-                self.cu = torch.tensor(cu, dtype=torch.int32, device=self.table.device)
+        on = _on(self.table.device, stream) or contextlib.nullcontext()
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        before = [list(h) for h in self._held], list(self._free), self.lengths, self._cu
+        for h, w in zip(self._held, want):
+            while len(h) < w:
+                h.append(self._free.pop())
+        self.lengths = [n + m for n, m in zip(self.lengths, new)]
+        self._cu = cu
+        with on:
+            try:
+                self._send(self._held != before[0])
                 kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
                                     self.lens, self.k_scale, self.v_scale)
-        except Exception:  # a rejected append changes nothing
-            self._held, self._free, self.lengths = held, free, lengths
-            self.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
-            raise
+            except Exception:  # a refused append changes nothing
+                self._held, self._free, self.lengths, self._cu = before
+                self._send(True)
+                raise
         self._new = new
+
+    def _send(self, table: bool) -> None:
+        """Lengths, offsets and (where it changed) the table to the device."""
+        import torch
+
+        if table:
+            width = self.table.shape[1]
+            self.table.copy_(torch.tensor([h + [0] * (width - len(h)) for h in self._held],
+                                          dtype=torch.int32))
+        self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+        self.cu.copy_(torch.tensor(self._cu, dtype=torch.int32))
 
     def attend(self, q, o, causal=True, scale=None, stream=None) -> None:
         """o = attention of q [sum(new), heads, Dh], the queries of the tokens
