@@ -659,7 +659,7 @@ class PagedKVCacheDev:
     Page numbers and lengths are kept on the host and copied to the device when
     they change, to the same addresses (a captured ``attend`` can be replayed after
     later appends of as many tokens); work is enqueued on ``stream`` (default:
-    torch's current one)."""
+    torch's current one), and calls on different streams are ordered by the caller."""
 
     def __init__(self, batch: int, H: int, Dh: int, num_pages: int, page_size: int = 64,
                  dtype=None, max_tokens: int | None = None, device=None):
@@ -689,6 +689,11 @@ class PagedKVCacheDev:
         self._cu = [0] * (batch + 1)  # as in cu
         self.cu = torch.zeros(batch + 1, dtype=torch.int32, device=device)
         self._new = None
+        # The calls may name any stream: none runs before these fills, nor before what
+        # had the memory until now.
+        home = torch.cuda.current_stream(self.table.device)
+        home.synchronize()
+        self._home = home.cuda_stream
 
     def append(self, k, v, new, stream=None) -> None:
         """k, v: the new tokens of all sequences, packed [sum(new), H, Dh]; new:
@@ -716,6 +721,7 @@ class PagedKVCacheDev:
         self.lengths = [n + m for n, m in zip(self.lengths, new)]
         self._cu = cu
         with on:
+            self._use()
             try:
                 self._send(self._held != before[0])
                 kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
@@ -725,6 +731,17 @@ class PagedKVCacheDev:
                 self._send(True)
                 raise
         self._new = new
+
+    def _use(self) -> None:
+        """On a stream other than the constructor's: the memory is in use there
+        too, and stays taken until that stream is past it."""
+        stream = _torch.cuda.current_stream(self.table.device)
+        if stream.cuda_stream == self._home or _torch.cuda.is_current_stream_capturing():
+            return
+        for t in (self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.table, self.lens,
+                  self.cu):
+            if t is not None:
+                t.record_stream(stream)
 
     def _send(self, table: bool) -> None:
         """Lengths, offsets and (where it changed) the table to the device."""
@@ -744,8 +761,10 @@ class PagedKVCacheDev:
             raise ValueError("append first: the queries belong to the tokens appended last")
         if q.shape[0] != sum(self._new):
             raise ValueError("q must hold one row for each token appended last")
-        attn_paged_dev(q, self.k_pages, self.v_pages, o, self.cu, self.table, self.lens,
-                       max(self._new), causal, scale, self.k_scale, self.v_scale, stream)
+        with _on(self.table.device, stream) or contextlib.nullcontext():
+            self._use()
+            attn_paged_dev(q, self.k_pages, self.v_pages, o, self.cu, self.table, self.lens,
+                           max(self._new), causal, scale, self.k_scale, self.v_scale)
 
     def read(self, b: int, k, v, stream=None) -> None:
         """The tokens of sequence b into k, v [lengths[b], H, Dh]."""
@@ -754,6 +773,7 @@ class PagedKVCacheDev:
         if k.shape[0] != self.lengths[b] or v.shape[0] != self.lengths[b]:
             raise ValueError("k and v must hold the sequence's tokens")
         with _on(self.table.device, stream) or contextlib.nullcontext():
+            self._use()
             # The length on the device is that of the last append.
             cu = torch.tensor([0, self.lengths[b]], dtype=torch.int32, device=self.table.device)
             kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1], cu[1:],
