@@ -572,7 +572,7 @@ def _workspace(device, q_heads: int, kv_heads: int, Dh: int):
 def _scale(scale) -> float:
     if scale is None:
         return 0.0  # the library's 1 / sqrt(Dh)
-    if not scale > 0:
+    if not ctypes.c_float(float(scale)).value > 0:  # as the library sees it: 0 is the default there
         raise ValueError("scale must be positive")
     return float(scale)
 

@@ -12,6 +12,7 @@ using namespace attnb;
 namespace {
 
 constexpr int kMaxDh = 256;
+constexpr float kLog2e = 1.44269504f;
 
 void invalid(const std::string& msg) { fail(ATTNB_ERR_INVALID_ARGUMENT, msg); }
 
@@ -88,6 +89,11 @@ void check_heads(const attnb_rows* Q, const attnb_rows* O, int kv_heads, int kv_
     invalid("tokens times query heads per KV head must be below 2^30");
 }
 
+void check_scale(float scale) {
+  if (!std::isfinite(scale) || (scale > 0.f && !std::isfinite(scale * kLog2e)))
+    invalid("scale must be finite, times log2(e) too");
+}
+
 SeqAttnArgs attn_args(const attnb_rows* Q, const attnb_rows* O, int kv_heads, int causal,
                       float scale, DeviceCtx& c) {
   SeqAttnArgs a{};
@@ -136,7 +142,7 @@ int attnb_attn_packed_dev(const attnb_rows* Q, const attnb_rows* K, const attnb_
     if (batch > 0 && (!cu_q || !cu_k)) invalid("Null cu_q or cu_k");
     if (!aligned4(cu_q)) invalid("cu_q is not aligned to its elements");
     if (!aligned4(cu_k)) invalid("cu_k is not aligned to its elements");
-    if (!std::isfinite(scale)) invalid("scale must be finite");
+    check_scale(scale);
     if (batch == 0 || Q->tokens == 0) return;
     if (!workspace) invalid("Null workspace");
     DeviceCtx& c = current_ctx();
@@ -163,7 +169,7 @@ int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pages, const
     if (max_new < 0) invalid("max_new must be non-negative");
     if (((int64_t)sq.max_pages << pg.page_shift) * (Q->heads / pg.H) >= (1 << 30))
       invalid("the table's tokens times query heads per KV head must be below 2^30");
-    if (!std::isfinite(scale)) invalid("scale must be finite");
+    check_scale(scale);
     if (sq.batch == 0 || sq.total == 0) return;
     if (!workspace) invalid("Null workspace");
     DeviceCtx& c = current_ctx();
