@@ -4,11 +4,13 @@
 // A vector x of Dh values (one token, one KV head) is stored in e4m3 or int8 as
 //     a = max |x|,   code = round(x * C / a),   scale = a / C    (C = 448 or 127)
 // with ties to even, so the largest value is the largest code and the value
-// read back is code * scale.  x * C / a is decided exactly: for 16-bit x the
-// product has at most 20 bits and the fp32 quotient cannot land on a tie that
-// the exact one is not on (the two differ by 2^-18 of it at least, half a unit
-// in the last place of fp32 is 2^-24); for fp32 x the quotient is taken in 64
-// bits, by the same argument (product 33 bits, distance 2^-42).  A vector
+// read back is code * scale.  The code is that of the exact x * C / a, found
+// without a division: for 16-bit x from x * (C / a), which is off by 2^-23 at
+// most, rounded to 21 bits: x * C has at most 18 bits and a tie times a at most 19, so
+// a quotient that is not on a tie is 2^-19 away from it and stays on its side, and
+// one on a tie is put back on it.  For fp32 x the product's bounds up and down
+// decide where they agree, elsewhere the quotient in 64 bits (product 33 bits,
+// distance 2^-42).  Where C / a leaves fp32's range all take the quotient.  A vector
 // of zeros has scale 0; one with an Inf or NaN has scale NaN and codes 0, so
 // that it cannot be read back as something finite.
 //
@@ -166,11 +168,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// One vector per group of LANES lanes, kFlight of them in flight: the CTAs of an
-// SM keep enough reads going, and more registers would cost some of those (prompts
-// of 11.7k tokens to e4m3 and back: 61 us; 79 with 2 in flight, 80 with 4).
-constexpr int kFlight = 1;
-
+// One vector per group of LANES lanes at a time: the CTAs of an SM keep enough
+// reads going, and more registers would cost some of those (prompts of 11.7k tokens
+// to e4m3 and back: 61 us; 79 with two vectors in flight, 80 with four).
 template <int TX, int TC, int LANES>
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const RowsView K, const RowsView V, const KvPages pg, const SeqTable sq,
@@ -187,84 +187,69 @@ __global__ void __launch_bounds__(kThreads)
   // A group's lanes share their vector; the other groups of the warp may have left.
   const unsigned mask =
       LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
-  Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H);
-  while (at.tl < n) {
-    Eight<EX> raw[kFlight];
-    int64_t place[kFlight];
-    bool is_v[kFlight];
+  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H); at.tl < n; at.next()) {
+    const bool is_v = at.kvh >= pg.H;
+    const int h = is_v ? at.kvh - pg.H : at.kvh;
+    const int64_t first = places[at.tl];
+    if (first < 0) continue;
+    const int64_t place = first + ((int64_t)h << pg.page_shift);
+    const RowsView& src = is_v ? V : K;
+    const Eight<EX> raw = load8(static_cast<const EX*>(src.data) + (int64_t)(t0 + at.tl) * src.sT +
+                                    (int64_t)h * src.sH,
+                                d, Dh, vec);
+    EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + place * Dh;
+    if constexpr (CODED) {
+      constexpr float C = TC == kE4M3 ? 448.f : 127.f;
+      float x[8], top = 0.f;
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u, at.next()) {
-      place[u] = -1;
-      if (at.tl >= n) continue;
-      is_v[u] = at.kvh >= pg.H;
-      const int h = is_v[u] ? at.kvh - pg.H : at.kvh;
-      const int64_t first = places[at.tl];
-      if (first < 0) continue;
-      place[u] = first + ((int64_t)h << pg.page_shift);
-      const RowsView& src = is_v[u] ? V : K;
-      raw[u] = load8(static_cast<const EX*>(src.data) + (int64_t)(t0 + at.tl) * src.sT +
-                         (int64_t)h * src.sH,
-                     d, Dh, vec);
-    }
-#pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      if (place[u] < 0) continue;
-      EC* out = static_cast<EC*>(is_v[u] ? pg.v : pg.k) + place[u] * Dh;
-      if constexpr (CODED) {
-        constexpr float C = TC == kE4M3 ? 448.f : 127.f;
-        float x[8], top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = to_float(raw[u].e[j]);
-          top = max_nan(top, fabsf(x[j]));
-        }
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
-        const bool bad = !(top <= 3.402823466e38f);  // a NaN stays one through the maximum
-        if (e == 0)
-          (is_v[u] ? pg.v_scale : pg.k_scale)[place[u]] =
-              bad ? __int_as_float(0x7fffffff) : top / C;
-        if (bad) top = 0.f;
-        // C / a overflows for tiny a, and is not used for large ones.
-        const float inv = top > 0x1p-100f && top < 0x1p100f ? C / top : 0.f;
-        uint32_t r[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float q[4];
-          bool exact = inv == 0.f;
-          if constexpr (TX == kF32) {
-            // x * (C / a) is off by less than 2^-22 of it: where 2^-22 up and down
-            // give the same codes, those are the ones; else the quotient decides.
-            float down[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float x0 = x[4 * k + j] * inv;
-              q[j] = x0 * (1.f + 0x1p-22f);
-              down[j] = x0 * (1.f - 0x1p-22f);
-            }
-            r[k] = pack_codes(q, out);
-            exact = exact || r[k] != pack_codes(down, out);
-          } else {
-            // Off by 2^-23 at most.  To 21 bits, what should be a tie is one again,
-            // and what should not stays on its side (it is 2^-19 away).
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              q[j] = __uint_as_float((__float_as_uint(x[4 * k + j] * inv) + 4u) & ~7u);
-            r[k] = pack_codes(q, out);
-          }
-          if (exact) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              q[j] = top > 0.f ? quotient<TX>(x[4 * k + j], top, C) : 0.f;
-            r[k] = pack_codes(q, out);
-          }
-        }
-        Eight<EC> codes;
-        memcpy(&codes, r, 8);
-        store8(out, d, Dh, vec, codes);
-      } else {
-        store8(out, d, Dh, vec, raw[u]);
+      for (int j = 0; j < 8; ++j) {
+        x[j] = to_float(raw.e[j]);
+        top = max_nan(top, fabsf(x[j]));
       }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+      const bool bad = !(top <= 3.402823466e38f);  // a NaN stays one through the maximum
+      if (e == 0)
+        (is_v ? pg.v_scale : pg.k_scale)[place] = bad ? __int_as_float(0x7fffffff) : top / C;
+      if (bad) top = 0.f;
+      // C / a overflows for tiny a, and is not used for large ones.
+      const float inv = top > 0x1p-100f && top < 0x1p100f ? C / top : 0.f;
+      uint32_t r[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float q[4];
+        bool exact = inv == 0.f;
+        if constexpr (TX == kF32) {
+          // x * (C / a) is off by less than 2^-22 of it: where 2^-22 up and down
+          // give the same codes, those are the ones; else the quotient decides.
+          float down[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x0 = x[4 * k + j] * inv;
+            q[j] = x0 * (1.f + 0x1p-22f);
+            down[j] = x0 * (1.f - 0x1p-22f);
+          }
+          r[k] = pack_codes(q, out);
+          exact = exact || r[k] != pack_codes(down, out);
+        } else {
+          // Off by 2^-23 at most.  To 21 bits, what should be a tie is one again,
+          // and what should not stays on its side (it is 2^-19 away).
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            q[j] = __uint_as_float((__float_as_uint(x[4 * k + j] * inv) + 4u) & ~7u);
+          r[k] = pack_codes(q, out);
+        }
+        if (exact) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) q[j] = top > 0.f ? quotient<TX>(x[4 * k + j], top, C) : 0.f;
+          r[k] = pack_codes(q, out);
+        }
+      }
+      Eight<EC> codes;
+      memcpy(&codes, r, 8);
+      store8(out, d, Dh, vec, codes);
+    } else {
+      store8(out, d, Dh, vec, raw);
     }
   }
 }
@@ -312,37 +297,23 @@ __global__ void __launch_bounds__(kThreads)
   grid_dep_wait();
   const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
   find_places(sq, pg, t0, n, places, index_status);
-  Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H);
-  while (at.tl < n) {
-    Eight<EC> raw[kFlight];
-    float scale[kFlight];
-    EX* out[kFlight];
-#pragma unroll
-    for (int u = 0; u < kFlight; ++u, at.next()) {
-      out[u] = nullptr;
-      if (at.tl >= n) continue;
-      const bool is_v = at.kvh >= pg.H;
-      const int h = is_v ? at.kvh - pg.H : at.kvh;
-      const int64_t first = places[at.tl];
-      if (first == -2) continue;  // a row of no sequence stays as it is
-      const RowsView& dst = is_v ? V : K;
-      out[u] = static_cast<EX*>(dst.data) + (int64_t)(t0 + at.tl) * dst.sT + (int64_t)h * dst.sH;
-      memset(&raw[u], 0, sizeof(raw[u]));
-      scale[u] = 1.f;
-      if (first < 0) continue;  // a bad place reads as zeros
+  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H); at.tl < n; at.next()) {
+    const bool is_v = at.kvh >= pg.H;
+    const int h = is_v ? at.kvh - pg.H : at.kvh;
+    const int64_t first = places[at.tl];
+    if (first == -2) continue;  // a row of no sequence stays as it is
+    const RowsView& dst = is_v ? V : K;
+    EX* out = static_cast<EX*>(dst.data) + (int64_t)(t0 + at.tl) * dst.sT + (int64_t)h * dst.sH;
+    Eight<EC> raw;
+    memset(&raw, 0, sizeof(raw));
+    float scale = 1.f;
+    if (first >= 0) {  // a bad place reads as zeros
       const int64_t place = first + ((int64_t)h << pg.page_shift);
-      raw[u] = load8(static_cast<const EC*>(is_v ? pg.v : pg.k) + place * Dh, d, Dh, vec);
-      if constexpr (CODED) scale[u] = (is_v ? pg.v_scale : pg.k_scale)[place];
+      raw = load8(static_cast<const EC*>(is_v ? pg.v : pg.k) + place * Dh, d, Dh, vec);
+      if constexpr (CODED) scale = (is_v ? pg.v_scale : pg.k_scale)[place];
     }
-#pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      if (!out[u]) continue;
-      if constexpr (CODED) {
-        store8(out[u], d, Dh, vec, decode8<TX, TC>(raw[u], scale[u]));
-      } else {
-        store8(out[u], d, Dh, vec, raw[u]);
-      }
-    }
+    if constexpr (CODED) store8(out, d, Dh, vec, decode8<TX, TC>(raw, scale));
+    else store8(out, d, Dh, vec, raw);
   }
 }
 
