@@ -342,3 +342,23 @@ def test_many_short_chunks_over_codes(cuda, cache, D):
         assert (o[first:first + n - there] == 0).all()
         first += n
     capi.stream_status()
+
+
+@pytest.mark.parametrize("rows,cache", [(BF16, E4M3), (F16, I8), (F32, E4M3)])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("n", [1, 200])
+def test_long_context_of_changing_sizes(cuda, rows, cache, D, n):
+    """A context that many CTAs share: their pieces have references of their own, some of them over
+    values of one size, some over several, zeros among them, and keys of several sizes too."""
+    L = 20011
+    q = _randn(_gen(66), n, 8, D, dtype=rows)
+    sizes = (1.0, 1.0, 1.0, 2.0 ** -10, 0.0, 2.0 ** -10, 30.0) if rows == F16 else \
+        (1.0, 1.0, 1.0, 1e-9, 0.0, 1e-9, 1e-9, 1e5)
+
+    def keys(x):
+        return x.float() * torch.where(torch.arange(L, device="cuda") % 97 == 0, 2.0 ** -9, 1.0)[:, None, None]
+
+    p = _pool(L, 2, D, rows, cache, 67, keys, lambda x: x.float() * _blocks(L, sizes))
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+    capi.stream_status()
