@@ -34,14 +34,17 @@
 // scale's power of two, rounded to f16 twice (2^-11 of a value each, where the
 // codes themselves are 2^-4 or 2^-8 off).  2^E goes into the rows' scale, and
 // V's 2^F into the weights' exponent: nothing is left to do for single keys in
-// the softmax.  Where the scales of 64 keys are more than 2^6 apart, or one is not
+// the softmax.  Where V's scales of 64 keys are more than 2^6 apart (then weights
+// would lose bits to the larger ones), or K's more than 2^10 (then f16's steps
+// would pass 2^-22 of the smaller keys' largest value), or one is not
 // finite, zero (V) or next to the ends of fp32, the tiles hold the codes as they
 // are and the softmax takes each key's scales, as in seq_mma.cu: so a key that a
-// row does not see changes nothing for it, whatever its scales are.
+// row does not see changes nothing for it, whatever its scales are.  (Where all
+// steps go so, the int8 chunks below take 1.4 to 1.9 ms.)
 // As there, the weights of the product have a reference rho of their own beside
 // the sum's maximum m, 2^(s - m + F - rho), so that V may have any size and change
 // it from block to block; 2^rho goes into the output.  The sum is theirs times
-// 2^(rho - F); where that factor could be far from 1, since F has changed much in
+// 2^(rho - F); where that factor could be large, since V was much larger earlier in
 // the piece, the keys go by their own scales too and the sum by exponentials of
 // its own.
 #include <algorithm>
@@ -61,10 +64,11 @@ constexpr int BN = 128;  // keys of a tile in shared memory
 constexpr int BS = 64;   // keys of a step
 constexpr float kRescaleGap = 8.f;
 constexpr float kNoRho = -1e30f;  // no weight so far: any exponent is above it
-// V's powers of two in steps that take their sum from the product's weights: with
-// lo and hi the least and the greatest F so far, lo - 8 <= rho <= hi + 8 (the row's
-// best key was in one of them, and none is more than 8 above m), so the factor
-// 2^(rho - F) stays within 2^40 and no term that counts is lost.
+// How much larger V of an earlier step may be (in powers of two) where a step takes
+// its sum from the product's weights.  With hi the greatest F so far rho <= hi + 8
+// (no score is more than 8 above m), so the factor 2^(rho - F) stays below 2^40
+// and no weight that counts has vanished.  (A small factor is harmless: the sum holds
+// the 1 of the row's best key.)
 constexpr int kSpread = 24;
 constexpr int kPoison = 6;  // pieces that warp 3 may be ahead of the outputs, and more
 
@@ -127,34 +131,60 @@ struct RowState {
   bool need;
 };
 __device__ __noinline__ float step_by_key(RowState& st, uint32_t sb, int kb0, int seen,
-                                          float scale, const float* keys) {
+                                          float scale, const float4* keys) {
   float m = st.m, l = st.l, rho = st.rho, top = -INFINITY, best = -INFINITY;
   uint32_t s[32];
-  auto exponent = [&](int k, uint32_t x) {
-    return kb0 + k >= seen ? -INFINITY : __uint_as_float(x) * (scale * keys[k]);
+  // Exponents of 32 keys in place of their scores.
+  auto load = [&](int k0) {
+    tmem_ld32(sb + k0, s);
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) {
+      const float4 x = keys[(k0 + k) >> 2];
+      const float ks[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s[k + e] = kb0 + k0 + k + e >= seen
+                       ? __float_as_uint(-INFINITY)
+                       : __float_as_uint(__uint_as_float(s[k + e]) * (scale * ks[e]));
+    }
   };
 #pragma unroll 1
   for (int k0 = 0; k0 < BS; k0 += 32) {
-    tmem_ld32(sb + k0, s);
+    load(k0);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) top = max_nan(top, exponent(k0 + k, s[k]));
+    for (int k = 0; k < 32; k += 2)
+      top = max3_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+    tmem_st32(sb + k0, s);
   }
+  tmem_wait_st();
   if (top - m > kRescaleGap) {
     if (m != -INFINITY) rho -= top - m;
     l *= fast_exp2(m - top);
     m = top;
   }
   const float ref = m == -INFINITY ? 0.f : m;
-  // The scale of a masked key may be anything.
-  auto product = [&](int k, float e) { return e == -INFINITY ? e : e - ref + keys[64 + k]; };
+  // The product's exponents but for rho; the scale of a masked key may be anything.
+  auto product = [&](int k0, int k, float (&u)[4]) {
+    const float4 x = keys[(BS + k0 + k) >> 2];
+    const float lv[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float t = __uint_as_float(s[k + e]);
+      u[e] = t == -INFINITY ? t : t - ref + lv[e];
+    }
+  };
 #pragma unroll 1
   for (int k0 = 0; k0 < BS; k0 += 32) {
     tmem_ld32(sb + k0, s);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const float e = exponent(k0 + k, s[k]);
-      l += fast_exp2(e - ref);
-      best = fmaxf(best, product(k0 + k, e));
+    for (int k = 0; k < 32; k += 4) {
+      float u[4];
+      product(k0, k, u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l += fast_exp2(__uint_as_float(s[k + e]) - ref);
+        best = fmaxf(best, u[e]);
+      }
     }
   }
   st.need = best - rho > kRescaleGap;
@@ -167,9 +197,12 @@ __device__ __noinline__ float step_by_key(RowState& st, uint32_t sb, int kb0, in
     tmem_ld32(sb + k0, s);
     uint32_t p[16];
 #pragma unroll
-    for (int k = 0; k < 32; k += 2)
-      p[k >> 1] = pack_f16(fast_exp2(product(k0 + k, exponent(k0 + k, s[k])) - rho),
-                           fast_exp2(product(k0 + k + 1, exponent(k0 + k + 1, s[k + 1])) - rho));
+    for (int k = 0; k < 32; k += 4) {
+      float u[4];
+      product(k0, k, u);
+      p[k >> 1] = pack_f16(fast_exp2(u[0] - rho), fast_exp2(u[1] - rho));
+      p[(k >> 1) + 1] = pack_f16(fast_exp2(u[2] - rho), fast_exp2(u[3] - rho));
+    }
     tmem_st16(sb + (k0 >> 1), p);  // over scores that have been read
   }
   st.m = m;
@@ -595,7 +628,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       bool ok = true;
       uint32_t tile = 0;
       while (ok && it.next(a, w)) {
-        int lo = INT_MAX, hi = INT_MIN;  // V's powers of two in the piece so far
+        int hi = INT_MIN;  // V's greatest power of two in the piece so far
         for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
 #pragma unroll 1
           for (int part = 0; part < 4; ++part) {  // as the loader: K, K, V, V
@@ -621,12 +654,10 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               constexpr uint32_t kLow = 0x0d800000u, kHigh = 0x71800000u;  // 2^-100, 2^100
               bool wide = false;
               if (left > 0) {
-                // (A value of 0 may be the row's best key without a part in the
-                // product, whose weights then may lie anywhere.)
-                lo = min(lo, vmin < kLow || vmax > kHigh ? INT_MIN / 2 : (int)(vmin >> 23));
-                hi = max(hi, (int)(vmax >> 23));
-                wide = kmax > kHigh || kmin < kLow || (kmax != 0u && kmax - kmin > (6u << 23)) ||
-                       vmax > kHigh || vmin < kLow || vmax - vmin > (6u << 23) || hi - lo > kSpread;
+                const int e = (int)(vmax >> 23);
+                hi = max(hi, e);
+                wide = kmax > kHigh || kmin < kLow || (kmax != 0u && kmax - kmin > (10u << 23)) ||
+                       vmax > kHigh || vmin < kLow || vmax - vmin > (6u << 23) || hi - e > kSpread;
               }
               // The largest scales' powers of two (as in row_scale), inverted.
               const float ke = row_scale(__uint_as_float(kmax)), ve = row_scale(__uint_as_float(vmax));
@@ -900,7 +931,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             l = fmaf(l0 + l1, fast_exp2(rho - f), l);
           } else {
             RowState st{m, l, rho, alpha, false};
-            top = step_by_key(st, sb, kb0, seen, scale, xt + Cfg::XHEAD + (i & 1) * 128);
+            top = step_by_key(st, sb, kb0, seen, scale,
+                              reinterpret_cast<const float4*>(xt + Cfg::XHEAD + (i & 1) * 128));
             m = st.m;
             l = st.l;
             rho = st.rho;

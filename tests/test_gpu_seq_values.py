@@ -274,13 +274,11 @@ def test_tiny_queries_and_keys(cuda, rows, cache, n, qsize, ksize):
 
 
 @pytest.mark.parametrize("rows,cache", CODED)
-@pytest.mark.parametrize("n", [1, 3, 30, 300])
-@pytest.mark.parametrize("L", [3, 65, 300])
+@pytest.mark.parametrize("n,L", [(1, 3), (3, 3), (1, 65), (3, 65), (30, 65), (1, 300), (3, 300),
+                                 (30, 300), (300, 300)])
 def test_weights_over_codes_have_the_bits_of_f16(cuda, rows, cache, n, L):
     """Key scales that are powers of two, so that what is left is the rounding of weights and
     values: bf16 weights, 2^-8, would not pass for rows in f16."""
-    if n > L:
-        pytest.skip("more new tokens than tokens")
     D = 64
     q = _randn(_gen(58), n, 4, D, dtype=rows)
 
@@ -362,3 +360,29 @@ def test_long_context_of_changing_sizes(cuda, rows, cache, D, n):
     ref = _reference(q, p.held(0)[0], p.held(1)[0])
     _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
     capi.stream_status()
+
+
+@pytest.mark.parametrize("rows,cache", CODED)
+@pytest.mark.parametrize("n", [1, 12, 300])
+def test_first_key_takes_the_weight_and_has_no_value(cuda, rows, cache, n):
+    """The first key's weight is 1 but for 2^-20 or so and its value is 0: what is left of the
+    others comes out with its bits."""
+    D, L = 64, 400
+    q = _randn(_gen(68), n, 4, D, dtype=rows)
+    q[..., 0] = 4.0
+
+    def keys(x):
+        x = x.clone()
+        x[..., 0] = 0
+        x[0] = 0
+        x[0, :, 0] = 40.0
+        return x
+
+    def values(x):
+        x = x.clone()
+        x[0] = 0
+        return x
+
+    p = _pool(L, 2, D, rows, cache, 69, keys, values)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])
+    _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
