@@ -3,10 +3,15 @@
 //
 // Every product is three tf32 products of split operands, big.big + big.small +
 // small.big, as in the 3xTF32 kernels of this library: an fp32 value is the sum
-// of two tf32 values but for 2^-22 of it, and sums are fp32.  Bound by the
-// warp-wide tensor instruction (mma.sync m16n8k8): tcgen05 has tf32 products too,
-// but its operands would have to be split and packed by another launch, for
-// lengths that only the device knows.
+// of two tf32 values but for 2^-22 of it.  The instruction cuts its fp32 sums off
+// instead of rounding them, so long sums through it come out short: scores of 64
+// dimensions and outputs of 450 keys were off by 2.2e-6.  So the cross terms of a
+// score have a sum of their own, its large terms go in sums of 32 dimensions, and a
+// tile's P V starts at 0 and meets O in a rounded fma: 4.0e-7 (fp32 products and sums
+// of torch: 5.4e-7), in the same time.
+// Bound by the warp-wide tensor instruction (mma.sync m16n8k8) and the plain loads
+// that feed it.  tcgen05, over tiles that are split in shared memory as K3's are,
+// has more room; that form is not built for ragged sequences.
 //
 // A CTA of eight warps takes 128 rows of one KV head, 16 a warp, and walks 32
 // keys at a time.  K and V are read by all threads while the tile before is
@@ -17,7 +22,7 @@
 // so column 2c of the scores serves as column c of A, 2c + 1 as c + 4, and V's
 // rows are picked accordingly.
 //
-// Measured: three sequences of 101-901 fp32 tokens, 16/4 heads of 64, 123 us where
+// Measured: three sequences of 101-901 fp32 tokens, 16/4 heads of 64, 127 us where
 // K6 takes 440.
 #include <algorithm>
 #include <atomic>
@@ -200,30 +205,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (j + 1 < w.j1) fetch(j + 1);
       if (!rows_here) continue;
       // ---- scores: four column tiles of 8 keys
-      float s[4][4];
+      float s[4][4], cross[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[t][e] = cross[t][e] = 0.f;
       const float* qr = qs + (warp * 16 + g) * Cfg::QROW + c;
 #pragma unroll
-      for (int k = 0; k < DH / 8; ++k) {
-        float big[4], small[4];
+      for (int k0 = 0; k0 < DH / 8; k0 += 4) {
+        float part[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 x = split_tf32(qr[(e & 1) * 8 * Cfg::QROW + k * 8 + (e >> 1) * 4]);
-          big[e] = x.x;
-          small[e] = x.y;
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[t][e] = 0.f;
+#pragma unroll
+        for (int k = k0; k < k0 + 4; ++k) {
+          float big[4], small[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = split_tf32(qr[(e & 1) * 8 * Cfg::QROW + k * 8 + (e >> 1) * 4]);
+            big[e] = x.x;
+            small[e] = x.y;
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float2 b0 = kp[(t * 8 + g) * Cfg::KROW + k * 8 + c];
+            const float2 b1 = kp[(t * 8 + g) * Cfg::KROW + k * 8 + c + 4];
+            mma_tf32_sync(cross[t], small, b0.x, b1.x);
+            mma_tf32_sync(cross[t], big, b0.y, b1.y);
+            mma_tf32_sync(part[t], big, b0.x, b1.x);
+          }
         }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float2 b0 = kp[(t * 8 + g) * Cfg::KROW + k * 8 + c];
-          const float2 b1 = kp[(t * 8 + g) * Cfg::KROW + k * 8 + c + 4];
-          mma_tf32_sync(s[t], small, b0.x, b1.x);
-          mma_tf32_sync(s[t], big, b0.y, b1.y);
-          mma_tf32_sync(s[t], big, b0.x, b1.x);
-        }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] += part[t][e];
       }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] += cross[t][e];
       // ---- weights
       if (masked) {
 #pragma unroll
@@ -252,14 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             l[i] += s[t][2 * i + e];
           }
       }
-#pragma unroll
-      for (int t = 0; t < DH / 8; ++t) {
-        acc[t][0] *= alpha[0];
-        acc[t][1] *= alpha[0];
-        acc[t][2] *= alpha[1];
-        acc[t][3] *= alpha[1];
-      }
       if (!plain) {
+#pragma unroll
+        for (int t = 0; t < DH / 8; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][e] *= alpha[e >> 1];
         // Every key's row by itself: p of key k lies with lane (g, k / 2 % 4).
         for (int k = 0; k < kKeys; ++k) {
           const int src = (lane & ~3) | ((k >> 1) & 3);
@@ -286,25 +304,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         continue;
       }
-      // ---- O += P V, 8 keys at a time
+      // ---- O = alpha O + P V
+      float big[4][4], small[4][4];
 #pragma unroll
-      for (int t8 = 0; t8 < 4; ++t8) {
-        float big[4], small[4];
+      for (int t8 = 0; t8 < 4; ++t8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           // A's column c is key 2c, its column c + 4 key 2c + 1.
           const float2 x = split_tf32(s[t8][(e & 1) * 2 + (e >> 1)]);
-          big[e] = x.x;
-          small[e] = x.y;
+          big[t8][e] = x.x;
+          small[t8][e] = x.y;
         }
 #pragma unroll
-        for (int t = 0; t < DH / 8; ++t) {
+      for (int t = 0; t < DH / 8; ++t) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t8 = 0; t8 < 4; ++t8) {
           const float2 b0 = vp[(t8 * 8 + 2 * c) * Cfg::VROW + t * 8 + g];
           const float2 b1 = vp[(t8 * 8 + 2 * c + 1) * Cfg::VROW + t * 8 + g];
-          mma_tf32_sync(acc[t], small, b0.x, b1.x);
-          mma_tf32_sync(acc[t], big, b0.y, b1.y);
-          mma_tf32_sync(acc[t], big, b0.x, b1.x);
+          mma_tf32_sync(part, small[t8], b0.x, b1.x);
+          mma_tf32_sync(part, big[t8], b0.y, b1.y);
+          mma_tf32_sync(part, big[t8], b0.x, b1.x);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(acc[t][e], alpha[e >> 1], part[e]);
       }
     }
     // ---- output

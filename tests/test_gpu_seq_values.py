@@ -386,3 +386,26 @@ def test_first_key_takes_the_weight_and_has_no_value(cuda, rows, cache, n):
     p = _pool(L, 2, D, rows, cache, 69, keys, values)
     ref = _reference(q, p.held(0)[0], p.held(1)[0])
     _check(_attend(p, q), ref[0], _bound(rows, True, ref, L))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("paged", [False, True])
+def test_fp32_sums_are_rounded(cuda, D, paged):
+    """Root mean square of the error relative to the outputs'.  A product of split operands is off by
+    2^-22 of its largest terms; sums that are rounded are off at random, by 2^-24 a step: for scores
+    of up to 4 or so in units of log2 some 20 steps make 2^-24 * 4 * sqrt(20), and the outputs' own
+    sums as much again, 1.2e-6 at worst and half of it in the mean square.  Sums that are cut off are
+    off by half of 2^-23 at every one of 3 D / 8 steps, all to one side: 2e-6 and more."""
+    n = 900
+    g = _gen(70)
+    q, k, v = _randn(g, n, 4, D) * 1.5, _randn(g, n, 2, D), _randn(g, n, 2, D)
+    k *= _randn(g, 1, 2, D).abs() + 0.5
+    ref = _reference(q, k, v)[0]
+    if paged:
+        p = _pool(n, 2, D, F32, F32, 71, lambda x: k, lambda x: v)
+        o = _attend(p, q)
+    else:
+        o = torch.empty_like(q)
+        capi.attn_packed_dev(q, k, v, o, seq_ref.starts([n]), causal=True)
+    err = float((o.double().cpu() - ref).norm() / ref.norm())
+    assert err <= 1e-6, err
