@@ -18,35 +18,32 @@
 //   Warp 0 loads; warps 1 and 2 issue the chains' scores and two others their
 //   P V (a thread that waits for the one would hold up the other); warps 4-7 and
 //   8-11 own one row of A or B per thread; one warp clears masked V values.
-//   With codes, warps 12-15 turn them into f16 tiles, by factors that warp 17 has
-//   made of their scales.
+//   With codes, warps 12-15 turn them into f16 tiles and warp 17 looks at their
+//   scales.
 //   CTAs are persistent and walk the pieces of the schedule in seq.cuh.
 //   Measured: prompts of 5000 and 8000 tokens, 32/8 heads, bf16, 750 us (970
 //   TFLOP/s of visible work); chunks of 1024-2048 tokens over 6000-16000 int8 keys
-//   983 us (607 TFLOP/s: the conversion of codes shares the SM's issue slots).
+//   1.03 ms (578 TFLOP/s: the conversion of codes shares the SM's issue slots; with
+//   the scales in the f16 tiles 0.98 ms, and two roundings of every K and V more).
 //
 // The running maximum moves only when it grows by more than 8 (weights stay
 // below 2^8, which f16 and bf16 hold); O and the sum are rescaled then.  Weights
 // are rounded to 16 bits once, to nearest; maxima, sums and O are fp32.
 //
-// Codes: both products run in f16.  Q is brought to [1, 2) by a power of two per
-// row, and 64 keys at a time K becomes code * scale / 2^E with 2^E the largest
-// scale's power of two, rounded to f16 twice (2^-11 of a value each, where the
-// codes themselves are 2^-4 or 2^-8 off).  2^E goes into the rows' scale, and
-// V's 2^F into the weights' exponent: nothing is left to do for single keys in
-// the softmax.  Where V's scales of 64 keys are more than 2^6 apart (then weights
-// would lose bits to the larger ones), or K's more than 2^10 (then f16's steps
-// would pass 2^-22 of the smaller keys' largest value), or one is not
-// finite, zero (V) or next to the ends of fp32, the tiles hold the codes as they
-// are and the softmax takes each key's scales, as in seq_mma.cu: so a key that a
-// row does not see changes nothing for it, whatever its scales are.  (Where all
-// steps go so, the int8 chunks below take 1.4 to 1.9 ms.)
-// As there, the weights of the product have a reference rho of their own beside
-// the sum's maximum m, 2^(s - m + F - rho), so that V may have any size and change
-// it from block to block; 2^rho goes into the output.  The sum is theirs times
-// 2^(rho - F); where that factor could be large, since V was much larger earlier in
-// the piece, the keys go by their own scales too and the sum by exponentials of
-// its own.
+// Codes: both products run in f16, over the codes as they are (exact).  Q is
+// brought to [1, 2) by a power of two per row; a score is multiplied in fp32 by its
+// key's K scale, and a weight by its V scale before it is rounded to f16.
+// 64 keys share a power of two 2^E of their K scales, which goes into the row's
+// scale, and 2^F of their V scales, which goes into the weights' exponent.
+// The weights of the product have a reference rho of their own beside the sum's
+// maximum m, 2^(s - m + F - rho), so that V may have any size and change it from
+// block to block; 2^rho goes into the output.  The sum is theirs times 2^(rho - F).
+// Some steps go key by key, scales of V in the exponent as in seq_mma.cu and a sum
+// with exponentials of its own: where V scales are more than 2^6 apart (weights
+// would lose bits to the larger ones) or V was much larger earlier in the piece, and
+// where one is zero, not finite or next to the ends of fp32.  So a key that a row
+// does not see changes nothing for it, whatever its scales are.  (Where all steps go
+// so, chunks of 1024-2048 tokens over 6000-16000 keys take 1.6 to 1.8 ms.)
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -88,11 +85,11 @@ struct TcCfg {
   static constexpr int OFF_V = OFF_K + K_ST * TILE;
   static constexpr int OFF_RAW = OFF_V + V_ST * TILE;
   static constexpr int OFF_X = OFF_RAW + (CODED ? RAW_ST * RAW : 0);
-  // Codes: what the softmax needs of a tile, by half: E's and F's powers of two,
-  // both NaN where the keys go by their own scales, and then K scales and
-  // logarithms of V scales; else poison.  When a tile's raw half is there, V of the
-  // tile before the last has been converted, so the softmax is at most V_ST tiles
-  // behind that one.
+  // Codes: what the softmax needs of a tile, by half: E's and F's powers of two and
+  // the keys' scales over them; where the keys go one by one both are NaN and K
+  // scales and logarithms of V scales follow.  Else poison.  When a tile's raw half is
+  // there, V of the tile before the last has been converted, so the softmax is at
+  // most V_ST tiles behind that one.
   static constexpr int SCALES = V_ST + 2;
   static constexpr int XHEAD = 4;  // floats
   static constexpr int XTILE = XHEAD * 4 + 2 * 128 * 4;
@@ -226,7 +223,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t kfull[KST], kempty[KST], vfull[VST], vempty[VST], vfix[VST];
-  __shared__ __align__(8) uint64_t rfull[RST], rempty[RST], sfull[4];
+  __shared__ __align__(8) uint64_t rfull[RST], rempty[RST];
   __shared__ __align__(8) uint64_t q_bar[2], q_free[2], s_bar[2][2], p_bar[2][2], pv_bar[2][2],
       done_bar[4];
   __shared__ SeqShared sh;
@@ -244,7 +241,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     abort_flag = 0;
     outputs[0] = outputs[1] = 0;
     for (int i = 0; i < KST; ++i) {
-      mbar_init(smem_addr(&kfull[i]), CODED ? 4 : 1);
+      mbar_init(smem_addr(&kfull[i]), CODED ? 5 : 1);
       mbar_init(smem_addr(&kempty[i]), 2);
     }
     for (int i = 0; i < VST; ++i) {
@@ -256,7 +253,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       mbar_init(smem_addr(&rfull[i]), 1);
       mbar_init(smem_addr(&rempty[i]), 5);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_addr(&sfull[i]), 1);
     for (int c = 0; c < 2; ++c) {
       mbar_init(smem_addr(&q_bar[c]), qtma ? 1 : 4);
       mbar_init(smem_addr(&q_free[c]), 1);
@@ -625,6 +621,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     // ------------------------------------ scales of 64 keys: what they share
     if constexpr (CODED) {
       Ring<RST> ring;
+      Ring<KST> rk;
       bool ok = true;
       uint32_t tile = 0;
       while (ok && it.next(a, w)) {
@@ -635,7 +632,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             ok = warp_wait(&rfull[ring.stage], ring.phase);
             if (!ok) break;
             if (part < 2) {
-              float* sc = reinterpret_cast<float*>(mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW + 64 * 128);
+              const float* sc = reinterpret_cast<const float*>(mem + Cfg::OFF_RAW +
+                                                               ring.stage * Cfg::RAW + 64 * 128);
               float* xt = reinterpret_cast<float*>(mem + Cfg::OFF_X +
                                                    (tile % Cfg::SCALES) * Cfg::XTILE);
               const int left = w.s.L - j * BN - part * 64;
@@ -656,8 +654,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               if (left > 0) {
                 const int e = (int)(vmax >> 23);
                 hi = max(hi, e);
-                wide = kmax > kHigh || kmin < kLow || (kmax != 0u && kmax - kmin > (10u << 23)) ||
-                       vmax > kHigh || vmin < kLow || vmax - vmin > (6u << 23) || hi - e > kSpread;
+                wide = kmax > kHigh || kmin < kLow || vmax > kHigh || vmin < kLow ||
+                       vmax - vmin > (6u << 23) || hi - e > kSpread;
               }
               // The largest scales' powers of two (as in row_scale), inverted.
               const float ke = row_scale(__uint_as_float(kmax)), ve = row_scale(__uint_as_float(vmax));
@@ -666,34 +664,23 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                 xt[part] = wide ? own : 1.f / ke;
                 xt[2 + part] = wide ? own : (float)(127 - (int)(bits(ve) >> 23));
               }
-              if (wide) {
-                float* keys = xt + Cfg::XHEAD + part * 128;
-                keys[lane] = k0;
-                keys[lane + 32] = k1;
-                keys[lane + 64] = __log2f(v0);
-                keys[lane + 96] = __log2f(v1);
-              }
-              // In the scales' place their factors as sums of two f16: one rounding
-              // would be an error that all the key's values share.
-              auto split = [&](float scale, float by) {
-                const float f = wide ? 1.f : scale * by;
-                const __half hi16 = __float2half_rn(f);
-                const __half2 both = __halves2half2(hi16, __float2half_rn(f - __half2float(hi16)));
-                return *reinterpret_cast<const float*>(&both);
-              };
-              sc[lane] = split(k0, ke);
-              sc[lane + 32] = split(k1, ke);
-              sc[lane + 64] = split(v0, ve);
-              sc[lane + 96] = split(v1, ve);
-              fence_proxy_async_smem();  // the next copy into the stage comes after these writes
+              float* keys = xt + Cfg::XHEAD + part * 128;
+              // (No factor of 0: a masked -inf stays one.)
+              auto kscale = [&](float x) { return wide ? x : fmaxf(x * ke, 0x1p-126f); };
+              auto vscale = [&](float x) { return wide ? __log2f(x) : x * ve; };
+              keys[lane] = kscale(k0);
+              keys[lane + 32] = kscale(k1);
+              keys[lane + 64] = vscale(v0);
+              keys[lane + 96] = vscale(v1);
             }
             __syncwarp();
             if (lane == 0) {
-              if (part < 2) mbar_arrive(smem_addr(&sfull[(2 * tile + part) & 3]));
+              if (part == 1) mbar_arrive(smem_addr(&kfull[rk.stage]));
               mbar_arrive(smem_addr(&rempty[ring.stage]));
             }
             ring.advance();
           }
+          rk.advance();
         }
       }
     }
@@ -708,7 +695,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       uint32_t tile = 0;
       while (ok && it.next(a, w)) {
         for (int j = w.j0; ok && j < w.j1; ++j, ++tile) {
-          uint32_t vmul0 = 0, vmul1 = 0;  // factors of this thread's two keys, as two f16 each
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             ok = ok && (kv ? warp_wait(&vempty[rv.stage], rv.phase ^ 1u)
@@ -722,21 +708,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               const uint8_t* from = mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
               const int r = hf * 64 + row;
               const bool gone = row >= w.s.L - j * BN - hf * 64;  // stale
-              uint32_t mul;
-              if (kv == 0) {
-                const uint32_t n = 2 * tile + hf;
-                ok = warp_wait(&sfull[n & 3], (n >> 2) & 1);
-                if (!ok) break;
-                const uint32_t* sc = reinterpret_cast<const uint32_t*>(from + 64 * 128);
-                mul = sc[row];
-                if (hf) vmul1 = sc[64 + row];
-                else vmul0 = sc[64 + row];
-              } else {
-                mul = hf ? vmul1 : vmul0;
-              }
-              const __half2 both = *reinterpret_cast<const __half2*>(&mul);
-              const __half2 hi = __low2half2(both), lo = __high2half2(both);
-#pragma unroll 1  // (the instruction cache, see the softmax: 983 us, 1062 with two)
+#pragma unroll 1  // (the instruction cache, see the softmax)
               for (int i = 0; i < DHP / 32; ++i) {
                 const int u = part * (DHP / 32) + i;  // 16 codes
                 uint4 x = *reinterpret_cast<const uint4*>(from + sw128(row, u));
@@ -744,16 +716,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
                 uint32_t y[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  uint32_t h[2];
-                  codes_to_f16<TK>(xs[k], h[0], h[1]);
-#pragma unroll
-                  for (int b = 0; b < 2; ++b) {
-                    const __half2 code = *reinterpret_cast<const __half2*>(&h[b]);
-                    const __half2 v = __hfma2(code, lo, __hmul2(code, hi));
-                    y[2 * k + b] = *reinterpret_cast<const uint32_t*>(&v);
-                  }
-                }
+                for (int k = 0; k < 4; ++k) codes_to_f16<TK>(xs[k], y[2 * k], y[2 * k + 1]);
                 uint8_t* ch = to + (u >> 2) * Cfg::CHUNK;
                 *reinterpret_cast<uint4*>(ch + sw128(r, (u & 3) * 2)) =
                     make_uint4(y[0], y[1], y[2], y[3]);
@@ -863,6 +826,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           // time in loops, read from TMEM twice, and masks in a pass of their own.
           uint32_t s[32];
           const float f = xt[2 + (i & 1)];
+          const float4* keys = reinterpret_cast<const float4*>(xt + Cfg::XHEAD + (i & 1) * 128);
           if (f == f) {
             if (masked) {
 #pragma unroll 1
@@ -875,17 +839,29 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               }
               tmem_wait_st();
             }
+            auto two = [&](int k) {
+              return pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+            };
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
             for (int k0 = 0; k0 < BS; k0 += 32) {
               tmem_ld32(sb + k0, s);
 #pragma unroll
-              for (int k = 0; k < 32; k += 4)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                  mx[u] = max3_nan(mx[u], __uint_as_float(s[k + 2 * u]),
-                                   __uint_as_float(s[k + 2 * u + 1]));
+              for (int k = 0; k < 32; k += 4) {
+                const float4 ks = keys[(k0 + k) >> 2];
+                float s0, s1, s2, s3;
+                unpack_f32x2(mul_f32x2(two(k), pack_f32x2(ks.x, ks.y)), s0, s1);
+                unpack_f32x2(mul_f32x2(two(k + 2), pack_f32x2(ks.z, ks.w)), s2, s3);
+                mx[0] = max3_nan(mx[0], s0, s1);
+                mx[1] = max3_nan(mx[1], s2, s3);
+                s[k] = __float_as_uint(s0);
+                s[k + 1] = __float_as_uint(s1);
+                s[k + 2] = __float_as_uint(s2);
+                s[k + 3] = __float_as_uint(s3);
+              }
+              tmem_st32(sb + k0, s);
             }
+            tmem_wait_st();
             const float smax = max_nan(mx[0], mx[1]);
             // (No factor below the smallest normal number: a masked -inf stays one.)
             const float mul = fmaxf(scale * xt[i & 1], 0x1p-126f);
@@ -911,17 +887,19 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             for (int k0 = 0; k0 < BS; k0 += 32) {
               tmem_ld32(sb + k0, s);
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const uint64_t x =
-                    fma_f32x2(add_f32x2(pack_f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                                        ref2),
-                              mul2, shift2);
-                float p0, p1;
-                unpack_f32x2(x, p0, p1);
-                p0 = fast_exp2(p0);
-                p1 = fast_exp2(p1);
-                ls[(k >> 1) & 1] = add_f32x2(ls[(k >> 1) & 1], pack_f32x2(p0, p1));
-                s[k >> 1] = pack_f16(p0, p1);
+              for (int k = 0; k < 32; k += 4) {
+                const float4 vs = keys[(BS + k0 + k) >> 2];
+                auto weights = [&](uint64_t t, float x, float y, uint64_t& sum) {
+                  float p0, p1;
+                  unpack_f32x2(fma_f32x2(add_f32x2(t, ref2), mul2, shift2), p0, p1);
+                  const uint64_t p = pack_f32x2(fast_exp2(p0), fast_exp2(p1));
+                  sum = add_f32x2(sum, p);
+                  unpack_f32x2(mul_f32x2(p, pack_f32x2(x, y)), p0, p1);
+                  return pack_f16(p0, p1);
+                };
+                const uint64_t t0 = two(k), t1 = two(k + 2);  // (the first is written over)
+                s[k >> 1] = weights(t0, vs.x, vs.y, ls[0]);
+                s[(k >> 1) + 1] = weights(t1, vs.z, vs.w, ls[1]);
               }
               // Over scores that have been read.
               tmem_st16(sb + (k0 >> 1), *reinterpret_cast<const uint32_t(*)[16]>(s));
@@ -931,8 +909,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             l = fmaf(l0 + l1, fast_exp2(rho - f), l);
           } else {
             RowState st{m, l, rho, alpha, false};
-            top = step_by_key(st, sb, kb0, seen, scale,
-                              reinterpret_cast<const float4*>(xt + Cfg::XHEAD + (i & 1) * 128));
+            top = step_by_key(st, sb, kb0, seen, scale, keys);
             m = st.m;
             l = st.l;
             rho = st.rho;

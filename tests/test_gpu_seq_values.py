@@ -409,3 +409,19 @@ def test_fp32_sums_are_rounded(cuda, D, paged):
         capi.attn_packed_dev(q, k, v, o, seq_ref.starts([n]), causal=True)
     err = float((o.double().cpu() - ref).norm() / ref.norm())
     assert err <= 1e-6, err
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
+@pytest.mark.parametrize("n,L", [(1, 1500), (10, 1500), (200, 300), (300, 3000)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_f16_over_codes_rounds_weights_and_outputs_only(cuda, cache, n, L, D):
+    """Root mean square of the error relative to the outputs'.  A rounding to f16 is off by 2^-11 at
+    most and evenly spread, 2^-11 / sqrt(3) * 0.75 in the mean square over a binade (values spread
+    over it), 2.1e-4: one of the outputs, one of the weights, together 3.0e-4.  A third and fourth of
+    keys or values, or any of scores, would pass 3.3e-4 by far: scores are several units large."""
+    q = _randn(_gen(72), n, 8, D, dtype=F16) * 1.5
+    p = _pool(L, 2, D, F16, cache, 73, lambda x: x.float() * 1.5)
+    ref = _reference(q, p.held(0)[0], p.held(1)[0])[0]
+    o = _attend(p, q).double().cpu()
+    err = float((o - ref).norm() / ref.norm())
+    assert err <= 3.3e-4, err
