@@ -29,10 +29,10 @@
 // into the output.  Weights are rounded to the products' type once (half a step
 // of 2^-11 in f16, 2^-8 in bf16); sums, maxima and accumulators are fp32.
 //
-// Measured: 32 sequences of 500-4096 bf16 keys, 32/8 heads (296 MB) 59 us, 64 of
-// 1000-8192 keys in e4m3 (622 MB) 122 us, both 5 TB/s with the join; one context
-// of 100001 keys (205 MB) 52 us.  With query rows as the instruction's 16 rows and
-// two CTAs an SM the e4m3 case took 165 us.
+// Measured: 32 sequences of 500-4096 bf16 keys, 32/8 heads (296 MB) 58 us, 64 of
+// 1000-8192 keys in e4m3 (622 MB) 126 us, 5 TB/s with the join; one context of
+// 100001 keys (205 MB) 52 us.  With query rows as the instruction's 16 rows and two
+// CTAs an SM the e4m3 case took 165 us.
 #include <algorithm>
 #include <atomic>
 #include <climits>

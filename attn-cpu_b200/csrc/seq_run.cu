@@ -137,13 +137,13 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   const int64_t rows =
       (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
   // Rows of one KV head and sequence.  16-bit pages: K7 up to 32 rows, K8 beyond (32
-  // sequences of 4096 keys, 8 KV heads of 128: 16 rows 103 us against 192, 32 rows
-  // 183 against 187, 48 rows 257 against 191); codes, which K8 converts in four
-  // warps: up to 64 (64 rows 325 us against 343, 128 rows 620 against 320).  In
+  // sequences of 4096 keys, 8 KV heads of 128: 16 rows 102 us against 193, 32 rows
+  // 186 against 184, 48 rows 271 against 189); codes, which K8 converts in four
+  // warps: up to 48 (e4m3: 48 rows 267 us against 282, 64 rows 347 against 284).  In
   // fp32, K9 over 16 rows (8 sequences of 2000 keys, 4 KV heads of 64: 16 rows 53 us
   // both, 64 rows 62 us against K6's 169).
   enum { kSimt, kMma, kTc, kTf32 } kind = kSimt;
-  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 64 : 32)) kind = kMma;
+  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 48 : 32)) kind = kMma;
   else if (seq_tc_supported(a)) kind = kTc;
   else if (seq_mma_supported(a)) kind = kMma;
   else if (a.q.Dh <= 128 && rows > 16) kind = kTf32;

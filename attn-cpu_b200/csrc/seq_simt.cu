@@ -15,8 +15,10 @@
 // keys again, from L2.  For a single row (a step without grouped heads) the
 // registers hold V next to K, so that both are in flight at once.
 //
-// Bound by the loads that the registers leave in flight: 8 sequences x 32 heads x
-// 4096 fp32 keys in pages of 16 (1.07 GB) take 290 us, 3.7 TB/s.
+// Bound by the loads in flight: 8 sequences x 32 heads x 4096 fp32 keys in pages of
+// 16 (1.07 GB) take 295 us, 3.6 TB/s.  The form for a single row of a head size over
+// 64 spills (772 bytes stored a thread at 168 registers), a ring of tiles in shared
+// memory, as K7 has, would keep more of them going.
 #include <cmath>
 
 #include "seq.cuh"

@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         const float* xt = reinterpret_cast<const float*>(
             mem + Cfg::OFF_X + (CODED ? ((tile0 + (i >> 1)) % Cfg::SCALES) * Cfg::XTILE : 0));
         float top, alpha = 1.f;  // largest exponent of the step; what O is multiplied by
-        bool need;
+        bool rescale;            // in some row of the warp
         if constexpr (CODED) {
           // The code of this loop and of the conversion share the schedulers'
           // instruction caches and are bound by them (unrolled, 4.4 of the 13 cycles a warp
@@ -872,7 +872,8 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               m = top;
             }
             const float best = top == -INFINITY ? top : top - m + f;
-            need = best - rho > kRescaleGap;
+            const bool need = best - rho > kRescaleGap;
+            rescale = __any_sync(0xffffffffu, need);
             if (need) {
               alpha = fast_exp2(rho - best);
               rho = best;
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             l = st.l;
             rho = st.rho;
             alpha = st.alpha;
-            need = st.need;
+            rescale = __any_sync(0xffffffffu, st.need);
           }
         } else {
           uint32_t s[BS];
@@ -933,7 +934,9 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           const float smax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
           top = smax * scale;
           // (m + 8 would round, next to 2^27; beyond 2^26 a new maximum always moves m.)
-          need = top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
+          const bool need =
+              top - m > kRescaleGap || (top >= m && fabsf(top) > 0x1p26f && top != -INFINITY);
+          rescale = __any_sync(0xffffffffu, need);
           if (need) {
             alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
             l *= alpha;
@@ -961,7 +964,6 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           unpack_f32x2(add_f32x2(ls[0], ls[1]), l0, l1);
           l += l0 + l1;
         }
-        const bool rescale = __any_sync(0xffffffffu, need);
         // A score that is NaN or +inf makes the whole row NaN.
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         if (rescale && i > 0) {

@@ -356,7 +356,10 @@ typedef struct attnb_rows {
 
 /* The pages of a KV cache: k and v are [num_pages, H, page_size, Dh], dense,
  * page_size 16, 32, 64 or 128.  E4M3 and I8 pages hold codes; their scales are
- * [num_pages, H, page_size], NULL for the other types. */
+ * [num_pages, H, page_size], NULL for the other types.  Tokens in coded pages are
+ * as attnb_kv_pages_append_dev writes them: codes are finite (E4M3's NaN codes do
+ * not occur), scales are not negative, and a vector that is not finite has scale
+ * NaN.  Pointers are aligned to their elements. */
 typedef struct attnb_kv_pages {
   void* k;
   void* v;
