@@ -162,12 +162,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // One vector per group of LANES lanes at a time: the CTAs of an SM keep enough
 // reads going, and more registers would cost some of those (prompts of 11.7k tokens
 // to e4m3 and back: 61 us; 79 with two vectors in flight, 80 with four).

@@ -1,5 +1,5 @@
 // seq_pages.cuh -- how the kernels that read pages by TMA (K7, K8) bring a tile
-// of keys into shared memory, and what both do with codes and masked values.
+// of keys into shared memory, and what they (and K5) do with codes and masked values.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -66,6 +66,13 @@ __device__ __forceinline__ float row_scale(float top) {
   const int e = (int)(__float_as_uint(top) >> 23);  // top >= 0
   if (e == 0 || e == 255) return 1.f;
   return __uint_as_float((uint32_t)max(254 - e, 1) << 23);  // [2, 4) next to overflow
+}
+
+// The larger one, or NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
