@@ -39,7 +39,9 @@ EXPORTED = [
     "attnb_kv_cache_truncate", "attnb_kv_cache_append", "attnb_kv_cache_step",
     "attnb_kv_cache_step_dev",
     "attnb_seq_workspace", "attnb_attn_packed_dev", "attnb_attn_paged_dev",
-    "attnb_kv_pages_append_dev", "attnb_kv_pages_read_dev",
+    "attnb_kv_pages_append_dev", "attnb_kv_pages_read_dev", "attnb_kv_pages_append_rope_dev",
+    "attnb_kv_blocks_bounds_dev", "attnb_blocks_workspace", "attnb_kv_blocks_select_dev",
+    "attnb_attn_blocks_dev",
 ]
 
 
@@ -58,10 +60,22 @@ class Rows(ctypes.Structure):
 
 
 class KvPages(ctypes.Structure):
-    """attnb_kv_pages: k, v, k_scale, v_scale, type, num_pages, H, page_size, Dh."""
+    """attnb_kv_pages: k, v, k_scale, v_scale, type, num_pages, H, page_size, Dh, k_group, v_group."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
                 ("v_scale", ctypes.c_void_p), ("type", ctypes.c_int), ("num_pages", ctypes.c_int),
-                ("H", ctypes.c_int), ("page_size", ctypes.c_int), ("Dh", ctypes.c_int)]
+                ("H", ctypes.c_int), ("page_size", ctypes.c_int), ("Dh", ctypes.c_int),
+                ("k_group", ctypes.c_void_p), ("v_group", ctypes.c_void_p)]
+
+
+class Rope(ctypes.Structure):
+    """attnb_rope: inv_freq, pairs, interleaved."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("pairs", ctypes.c_int),
+                ("interleaved", ctypes.c_int)]
+
+
+class Bounds(ctypes.Structure):
+    """attnb_bounds: data, type."""
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int)]
 
 
 class Seqs(ctypes.Structure):
@@ -141,6 +155,13 @@ def lib() -> ctypes.CDLL:
         L.attnb_attn_paged_dev.argtypes = [R, P, R, S, i, i, f, vp, ctypes.c_size_t, vp]
         L.attnb_kv_pages_append_dev.argtypes = [R, R, P, S, vp]
         L.attnb_kv_pages_read_dev.argtypes = [P, R, R, S, vp]
+        B = ctypes.POINTER(Bounds)
+        L.attnb_kv_pages_append_rope_dev.argtypes = [R, R, R, R, P, S, ctypes.POINTER(Rope), vp]
+        L.attnb_kv_blocks_bounds_dev.argtypes = [P, B, S, vp]
+        L.attnb_blocks_workspace.argtypes = [i, i, i, i, i, i, ctypes.POINTER(ctypes.c_size_t)]
+        L.attnb_kv_blocks_select_dev.argtypes = [R, B, i, i, i, S, i, i, vp, i, vp, ctypes.c_size_t,
+                                                 vp]
+        L.attnb_attn_blocks_dev.argtypes = [R, P, R, S, vp, i, f, vp, ctypes.c_size_t, vp]
         for name in EXPORTED:
             if name not in ("attnb_last_error", "attnb_version"):
                 getattr(L, name).restype = ctypes.c_int
@@ -461,6 +482,7 @@ class KVCacheDev:
 # These calls are made once per layer and step, where a few microseconds of the
 # host count: the checks below read each property of a tensor once.
 _torch = _raw_stream = None
+_I4 = 6  # torch.uint8 pages: two 4-bit codes a byte
 _TYPES: dict = {}  # torch dtype -> ATTNB_TYPE_*
 _workspace_bytes: dict = {}
 
@@ -474,7 +496,7 @@ def _setup() -> None:
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda index: torch.cuda.current_stream(index).cuda_stream)
     _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
-              torch.int8: 4}
+              torch.int8: 4, torch.uint8: _I4}
     lib()
 
 
@@ -523,7 +545,7 @@ def _offsets(t, name: str, device, n=None) -> int:
     return t.data_ptr()
 
 
-def _pages(k_pages, v_pages, k_scale, v_scale, device) -> KvPages:
+def _pages(k_pages, v_pages, k_scale, v_scale, device, k_group=None, v_group=None) -> KvPages:
     shape = k_pages.shape
     if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError("k_pages and v_pages must be [pages, H, page_size, Dh] of one type")
@@ -543,7 +565,24 @@ def _pages(k_pages, v_pages, k_scale, v_scale, device) -> KvPages:
         if len(at) >= 2 and (t.dtype != _torch.float32 or t.shape != shape[:3]):
             raise ValueError("k_scale and v_scale must be float32 [pages, H, page_size]")
         at.append(t.data_ptr())
-    return KvPages(*at, ty, n, H, page, Dh)
+    if ty != _I4:
+        if k_group is not None or v_group is not None:
+            raise ValueError("only uint8 pages have k_group and v_group")
+        return KvPages(*at, ty, n, H, page, Dh)
+    Dh *= 2
+    want = (n, H, page, i4_group_bytes(Dh))
+    for t in (k_group, v_group):
+        if t is None or t.dtype != _torch.uint8 or t.shape != want or not t.is_contiguous():
+            raise ValueError(f"uint8 pages need k_group and v_group, contiguous uint8 {want}")
+        if t.device != device:
+            raise ValueError(f"pages and factors must be on {device}, not on {t.device}")
+        at.append(t.data_ptr())
+    return KvPages(*at[:4], ty, n, H, page, Dh, *at[4:])
+
+
+def i4_group_bytes(Dh: int) -> int:
+    """Length of the last dimension of a 4-bit cache's k_group and v_group."""
+    return 4 * -(-Dh // 128)
 
 
 def _seqs(cu, table, lens, device) -> Seqs:
@@ -601,11 +640,13 @@ def attn_packed_dev(Q, K, V, O, cu_q, cu_k=None, causal=False, scale=None, strea
 
 
 def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=True, scale=None,
-                   k_scale=None, v_scale=None, stream=None) -> None:
+                   k_scale=None, v_scale=None, stream=None, k_group=None, v_group=None) -> None:
     """O = attention of new tokens over a paged cache (attnb_attn_paged_dev): Q,
     O [tokens, heads, Dh]; k_pages, v_pages [pages, kv_heads, page_size, Dh] of
     Q's type, or float8_e4m3fn or int8 codes with k_scale, v_scale [pages,
-    kv_heads, page_size]; sequence b is rows cu[b]:cu[b+1] of Q, the last of the
+    kv_heads, page_size], or uint8 [pages, kv_heads, page_size, Dh / 2], two 4-bit
+    codes a byte, with scales and k_group, v_group, uint8 [pages, kv_heads,
+    page_size, i4_group_bytes(Dh)]; sequence b is rows cu[b]:cu[b+1] of Q, the last of the
     lens[b] tokens in pages table[b] (all int32).  max_new: the most rows of one
     sequence, where the caller knows it; it only steers the choice of kernel."""
     dev = Q.device
@@ -613,9 +654,9 @@ def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=Tr
     if on is not None:
         with on:
             return attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new, causal, scale,
-                                  k_scale, v_scale)
+                                  k_scale, v_scale, None, k_group, v_group)
     q, o = _rows(Q, "Q", dev), _rows(O, "O", dev)
-    pg = _pages(k_pages, v_pages, k_scale, v_scale, dev)
+    pg = _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group)
     sq = _seqs(cu, table, lens, dev)
     ws, n = _workspace(dev, q.heads, pg.H, q.Dh)
     check(_lib.attnb_attn_paged_dev(q, pg, o, sq, max_new, int(causal), _scale(scale),
@@ -623,46 +664,167 @@ def attn_paged_dev(Q, k_pages, v_pages, O, cu, table, lens, max_new=0, causal=Tr
 
 
 def kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale=None, v_scale=None,
-                        stream=None) -> None:
+                        stream=None, k_group=None, v_group=None) -> None:
     """Write new tokens K, V [tokens, kv_heads, Dh] into the pages, quantising
-    them for float8_e4m3fn and int8 pages (attnb_kv_pages_append_dev); lens
+    them for float8_e4m3fn, int8 and uint8 pages (attnb_kv_pages_append_dev); lens
     counts them already.  Other arguments as in attn_paged_dev."""
     dev = K.device
     on = _on(dev, stream)
     if on is not None:
         with on:
-            return kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale, v_scale)
+            return kv_pages_append_dev(K, V, k_pages, v_pages, cu, table, lens, k_scale, v_scale,
+                                       None, k_group, v_group)
     check(_lib.attnb_kv_pages_append_dev(
-        _rows(K, "K", dev), _rows(V, "V", dev), _pages(k_pages, v_pages, k_scale, v_scale, dev),
+        _rows(K, "K", dev), _rows(V, "V", dev),
+        _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group),
         _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
 
 
+def kv_pages_append_rope_dev(K, V, k_pages, v_pages, cu, table, lens, inv_freq, interleaved=False,
+                             Q=None, Q_out=None, k_scale=None, v_scale=None, stream=None,
+                             k_group=None, v_group=None) -> None:
+    """kv_pages_append_dev with K rotated by its tokens' positions on the way, and
+    the queries Q [tokens, heads, Dh] rotated into Q_out, which may be Q
+    (attnb_kv_pages_append_rope_dev).  inv_freq: float32 [pairs], the angle of
+    each pair of dimensions from one position to the next; the pairs are (i, i + pairs)
+    or, interleaved, (2i, 2i + 1), and dimensions from 2 * pairs on stay."""
+    dev = K.device
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return kv_pages_append_rope_dev(K, V, k_pages, v_pages, cu, table, lens, inv_freq,
+                                            interleaved, Q, Q_out, k_scale, v_scale, None, k_group,
+                                            v_group)
+    if inv_freq.dtype != _torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or \
+            inv_freq.device != dev:
+        raise ValueError(f"inv_freq must be a contiguous float32 vector on {dev}")
+    if (Q is None) != (Q_out is None):
+        raise ValueError("Q and Q_out belong together")
+    check(_lib.attnb_kv_pages_append_rope_dev(
+        None if Q is None else _rows(Q, "Q", dev),
+        None if Q is None else _rows(Q_out, "Q_out", dev), _rows(K, "K", dev), _rows(V, "V", dev),
+        _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group),
+        _seqs(cu, table, lens, dev), Rope(inv_freq.data_ptr(), len(inv_freq), int(interleaved)),
+        _raw_stream(dev.index)))
+
+
 def kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale=None, v_scale=None,
-                      stream=None) -> None:
+                      stream=None, k_group=None, v_group=None) -> None:
     """Read the last cu[b+1] - cu[b] tokens of each sequence out of the pages
     into K, V [tokens, kv_heads, Dh] (attnb_kv_pages_read_dev)."""
     dev = K.device
     on = _on(dev, stream)
     if on is not None:
         with on:
-            return kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale, v_scale)
+            return kv_pages_read_dev(k_pages, v_pages, K, V, cu, table, lens, k_scale, v_scale,
+                                     None, k_group, v_group)
     check(_lib.attnb_kv_pages_read_dev(
-        _pages(k_pages, v_pages, k_scale, v_scale, dev), _rows(K, "K", dev), _rows(V, "V", dev),
-        _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
+        _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group), _rows(K, "K", dev),
+        _rows(V, "V", dev), _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
+
+
+def _bounds(bounds, pages: int, heads: int, Dh: int, device) -> Bounds:
+    if bounds.shape != (pages, heads, 2, Dh) or not bounds.is_contiguous() or \
+            bounds.device != device:
+        raise ValueError(f"bounds must be [pages, H, 2, Dh] = {(pages, heads, 2, Dh)}, contiguous, "
+                         f"on {device}")
+    ty = _TYPES.get(bounds.dtype)
+    if ty is None:
+        raise ValueError(f"bounds: {bounds.dtype} is not supported")
+    return Bounds(bounds.data_ptr(), ty)
+
+
+def _lists(blocks, tokens: int, heads: int, device) -> int:
+    if blocks.dtype != _torch.int32 or blocks.dim() != 3 or \
+            tuple(blocks.shape[:2]) != (tokens, heads) or not blocks.is_contiguous():
+        raise ValueError(f"blocks must be contiguous int32 [{tokens}, {heads}, take]")
+    if blocks.device != device:
+        raise ValueError(f"blocks is on {blocks.device}, not on {device}")
+    return blocks.data_ptr()
+
+
+def _blocks_workspace(device, tokens, q_heads, kv_heads, Dh, take, max_pages):
+    size = ctypes.c_size_t()
+    check(_lib.attnb_blocks_workspace(tokens, q_heads, kv_heads, Dh, take, max_pages,
+                                      ctypes.byref(size)))
+    return _torch.empty(size.value, dtype=_torch.uint8, device=device), size.value
+
+
+def kv_blocks_bounds_dev(k_pages, bounds, cu, table, lens, k_scale=None, k_group=None,
+                         stream=None) -> None:
+    """Least and greatest value of the keys of each block (one page of a sequence)
+    that the new tokens complete, into bounds [pages, kv_heads, 2, Dh]
+    (attnb_kv_blocks_bounds_dev): float32, bfloat16 or float16, for uncoded pages
+    their type.  Call it after each append; other arguments as there."""
+    dev = k_pages.device
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return kv_blocks_bounds_dev(k_pages, bounds, cu, table, lens, k_scale, k_group)
+    pg = _pages(k_pages, k_pages, k_scale, k_scale, dev, k_group, k_group)
+    check(_lib.attnb_kv_blocks_bounds_dev(pg, _bounds(bounds, pg.num_pages, pg.H, pg.Dh, dev),
+                                          _seqs(cu, table, lens, dev), _raw_stream(dev.index)))
+
+
+def kv_blocks_select_dev(Q, bounds, blocks, cu, table, lens, page_size, keep_first=1, keep_last=1,
+                         stream=None) -> None:
+    """The blocks that each of Q's tokens [tokens, heads, Dh] attends to, by their
+    bounds, into blocks, int32 [tokens, kv_heads, take], ascending, -1 behind the
+    last one (attnb_kv_blocks_select_dev): the first keep_first, the last keep_last
+    (the token's own is the last), and those that may hold the greatest scores."""
+    dev = Q.device
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return kv_blocks_select_dev(Q, bounds, blocks, cu, table, lens, page_size, keep_first,
+                                        keep_last)
+    q = _rows(Q, "Q", dev)
+    if bounds.dim() != 4:
+        raise ValueError("bounds must be [pages, H, 2, Dh]")
+    n, H = bounds.shape[:2]
+    b = _bounds(bounds, n, H, q.Dh, dev)
+    at, take = _lists(blocks, q.tokens, H, dev), blocks.shape[2]
+    sq = _seqs(cu, table, lens, dev)
+    ws, size = _blocks_workspace(dev, q.tokens, q.heads, H, q.Dh, take, sq.max_pages)
+    check(_lib.attnb_kv_blocks_select_dev(q, b, n, H, page_size, sq, keep_first, keep_last, at,
+                                          take, ws.data_ptr(), size, _raw_stream(dev.index)))
+
+
+def attn_blocks_dev(Q, k_pages, v_pages, O, blocks, cu, table, lens, scale=None, k_scale=None,
+                    v_scale=None, stream=None, k_group=None, v_group=None) -> None:
+    """attn_paged_dev, causal, over the listed blocks alone (attnb_attn_blocks_dev):
+    blocks int32 [tokens, kv_heads, take] as kv_blocks_select_dev writes it, or
+    ascending lists of the caller's own, -1 behind the last entry."""
+    dev = Q.device
+    on = _on(dev, stream)
+    if on is not None:
+        with on:
+            return attn_blocks_dev(Q, k_pages, v_pages, O, blocks, cu, table, lens, scale, k_scale,
+                                   v_scale, None, k_group, v_group)
+    q, o = _rows(Q, "Q", dev), _rows(O, "O", dev)
+    pg = _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group)
+    sq = _seqs(cu, table, lens, dev)
+    at, take = _lists(blocks, q.tokens, pg.H, dev), blocks.shape[2]
+    ws, size = _blocks_workspace(dev, q.tokens, q.heads, pg.H, q.Dh, take, sq.max_pages)
+    check(_lib.attnb_attn_blocks_dev(q, pg, o, sq, at, take, _scale(scale), ws.data_ptr(), size,
+                                     _raw_stream(dev.index)))
 
 
 class PagedKVCacheDev:
     """A K/V cache for `batch` sequences in one pool of pages, the ragged
     counterpart of KVCacheDev: ``append`` gives each sequence the pages it needs
-    and writes its new tokens (quantising them for dtype torch.float8_e4m3fn or
-    torch.int8), ``attend`` runs the new tokens' queries over everything held.
+    and writes its new tokens (quantising them for dtype torch.float8_e4m3fn,
+    torch.int8 or torch.uint8, which is 4 bits, and rotating the keys where it is
+    given inv_freq), ``attend`` runs the new tokens' queries over everything held.
+    With bounds (True, or their dtype for coded pages; bfloat16 there by default)
+    ``attend_blocks`` runs them over a few pages of each sequence that it selects.
     Page numbers and lengths are kept on the host and copied to the device when
     they change, to the same addresses (a captured ``attend`` can be replayed after
     later appends of as many tokens); work is enqueued on ``stream`` (default:
     torch's current one), and calls on different streams are ordered by the caller."""
 
     def __init__(self, batch: int, H: int, Dh: int, num_pages: int, page_size: int = 64,
-                 dtype=None, max_tokens: int | None = None, device=None):
+                 dtype=None, max_tokens: int | None = None, device=None, bounds=False):
         import torch
 
         if batch <= 0 or num_pages <= 0:
@@ -673,12 +835,25 @@ class PagedKVCacheDev:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None \
             else torch.device(device)
         self.batch, self.H, self.Dh, self.page_size = batch, H, Dh, page_size
-        self.k_pages, self.v_pages = (torch.empty(num_pages, H, page_size, Dh, dtype=dtype,
+        if dtype == torch.uint8 and Dh % 32:
+            raise ValueError("pages of 4 bits need a head size that is a multiple of 32")
+        coded = dtype in (torch.float8_e4m3fn, torch.int8, torch.uint8)
+        if not isinstance(bounds, bool) and bounds is not None and not coded and bounds != dtype:
+            raise ValueError("bounds of uncoded pages have their type")
+        wide = Dh // 2 if dtype == torch.uint8 else Dh
+        self.k_pages, self.v_pages = (torch.empty(num_pages, H, page_size, wide, dtype=dtype,
                                                   device=device) for _ in range(2))
-        self.k_scale = self.v_scale = None
-        if dtype in (torch.float8_e4m3fn, torch.int8):
+        self.k_scale = self.v_scale = self.k_group = self.v_group = self.bounds = None
+        if coded:
             self.k_scale, self.v_scale = (torch.empty(num_pages, H, page_size, device=device)
                                           for _ in range(2))
+        if dtype == torch.uint8:
+            self.k_group, self.v_group = (torch.empty(num_pages, H, page_size, i4_group_bytes(Dh),
+                                                      dtype=torch.uint8, device=device)
+                                          for _ in range(2))
+        if bounds:
+            kind = (torch.bfloat16 if coded else dtype) if bounds is True else bounds
+            self.bounds = torch.empty(num_pages, H, 2, Dh, dtype=kind, device=device)
         most = num_pages * page_size if max_tokens is None else max_tokens
         width = max(1, -(-most // page_size))
         self._free = list(range(num_pages - 1, -1, -1))
@@ -695,9 +870,11 @@ class PagedKVCacheDev:
         home.synchronize()
         self._home = home.cuda_stream
 
-    def append(self, k, v, new, stream=None) -> None:
+    def append(self, k, v, new, stream=None, inv_freq=None, interleaved=False, q=None,
+               q_out=None) -> None:
         """k, v: the new tokens of all sequences, packed [sum(new), H, Dh]; new:
-        how many each sequence brings (a list of ints)."""
+        how many each sequence brings (a list of ints).  inv_freq: k is rotated by
+        its tokens' positions on the way, and q into q_out (kv_pages_append_rope_dev)."""
         import torch
 
         new = [int(n) for n in new]
@@ -710,6 +887,8 @@ class PagedKVCacheDev:
             raise ValueError("a sequence would outgrow max_tokens")
         if sum(want) - sum(len(h) for h in self._held) > len(self._free):
             raise ValueError("the pool has too few free pages")
+        if inv_freq is None and (q is not None or q_out is not None):
+            raise ValueError("q is rotated with inv_freq only")
         on = _on(self.table.device, stream) or contextlib.nullcontext()
         cu = [0]
         for n in new:
@@ -724,8 +903,18 @@ class PagedKVCacheDev:
             self._use()
             try:
                 self._send(self._held != before[0])
-                kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
-                                    self.lens, self.k_scale, self.v_scale)
+                if inv_freq is None:
+                    kv_pages_append_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
+                                        self.lens, self.k_scale, self.v_scale,
+                                        k_group=self.k_group, v_group=self.v_group)
+                else:
+                    kv_pages_append_rope_dev(k, v, self.k_pages, self.v_pages, self.cu, self.table,
+                                             self.lens, inv_freq, interleaved, q, q_out,
+                                             self.k_scale, self.v_scale, k_group=self.k_group,
+                                             v_group=self.v_group)
+                if self.bounds is not None:
+                    kv_blocks_bounds_dev(self.k_pages, self.bounds, self.cu, self.table, self.lens,
+                                         self.k_scale, self.k_group)
             except Exception:  # a refused append changes nothing
                 self._held, self._free, self.lengths, self._cu = before
                 self._send(True)
@@ -738,8 +927,8 @@ class PagedKVCacheDev:
         stream = _torch.cuda.current_stream(self.table.device)
         if stream.cuda_stream == self._home or _torch.cuda.is_current_stream_capturing():
             return
-        for t in (self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.table, self.lens,
-                  self.cu):
+        for t in (self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.k_group,
+                  self.v_group, self.bounds, self.table, self.lens, self.cu):
             if t is not None:
                 t.record_stream(stream)
 
@@ -757,14 +946,40 @@ class PagedKVCacheDev:
     def attend(self, q, o, causal=True, scale=None, stream=None) -> None:
         """o = attention of q [sum(new), heads, Dh], the queries of the tokens
         appended last, over their sequences."""
+        self._check_queries(q)
+        with _on(self.table.device, stream) or contextlib.nullcontext():
+            self._use()
+            attn_paged_dev(q, self.k_pages, self.v_pages, o, self.cu, self.table, self.lens,
+                           max(self._new), causal, scale, self.k_scale, self.v_scale,
+                           k_group=self.k_group, v_group=self.v_group)
+
+    def _check_queries(self, q) -> None:
         if self._new is None:
             raise ValueError("append first: the queries belong to the tokens appended last")
         if q.shape[0] != sum(self._new):
             raise ValueError("q must hold one row for each token appended last")
+
+    def attend_blocks(self, q, o, take: int, keep_first: int = 1, keep_last: int = 1, scale=None,
+                      stream=None):
+        """As a causal ``attend``, each token and KV head over `take` pages of its
+        sequence: the first keep_first, the last keep_last and those that may hold
+        the greatest scores (kv_blocks_select_dev).  Returns the page numbers within the
+        sequences, int32 [sum(new), H, take]."""
+        if self.bounds is None:
+            raise ValueError("attend_blocks needs a cache with bounds")
+        self._check_queries(q)
+        if take < 1:
+            raise ValueError("take must be positive")
         with _on(self.table.device, stream) or contextlib.nullcontext():
             self._use()
-            attn_paged_dev(q, self.k_pages, self.v_pages, o, self.cu, self.table, self.lens,
-                           max(self._new), causal, scale, self.k_scale, self.v_scale)
+            blocks = _torch.empty(q.shape[0], self.H, take, dtype=_torch.int32,
+                                  device=self.table.device)
+            where = self.cu, self.table, self.lens
+            kv_blocks_select_dev(q, self.bounds, blocks, *where, self.page_size, keep_first,
+                                 keep_last)
+            attn_blocks_dev(q, self.k_pages, self.v_pages, o, blocks, *where, scale, self.k_scale,
+                            self.v_scale, k_group=self.k_group, v_group=self.v_group)
+        return blocks
 
     def read(self, b: int, k, v, stream=None) -> None:
         """The tokens of sequence b into k, v [lengths[b], H, Dh]."""
@@ -777,7 +992,8 @@ class PagedKVCacheDev:
             # The length on the device is that of the last append.
             cu = torch.tensor([0, self.lengths[b]], dtype=torch.int32, device=self.table.device)
             kv_pages_read_dev(self.k_pages, self.v_pages, k, v, cu, self.table[b:b + 1], cu[1:],
-                              self.k_scale, self.v_scale)
+                              self.k_scale, self.v_scale, k_group=self.k_group,
+                              v_group=self.v_group)
 
     def truncate(self, b: int, length: int) -> None:
         """Keep the first `length` tokens of sequence b (0 gives all its pages

@@ -199,16 +199,25 @@ void gemm_pack_b(const float* B, int64_t ldb, bool b_kmajor, int N, int K, bool 
 
 // ------------------------------- ragged sequences and the paged KV cache
 // Element types (the values of ATTNB_TYPE_* in attnb.h).
-enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2, kE4M3 = 3, kI8 = 4 };
+enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2, kE4M3 = 3, kI8 = 4, kI4 = 6 };
+// Of one element; of the smallest unit, a byte of two, for I4.
 inline int elem_bytes(int t) { return t == kF32 ? 4 : (t == kBF16 || t == kF16) ? 2 : 1; }
-inline bool elem_coded(int t) { return t == kE4M3 || t == kI8; }  // codes with a scale per vector
+// Codes with a scale per vector.
+constexpr bool elem_coded(int t) { return t == kE4M3 || t == kI8 || t == kI4; }
+inline int vector_bytes(int t, int Dh) { return t == kI4 ? Dh / 2 : Dh * elem_bytes(t); }
+constexpr int kI4Group = 32;  // dimensions that share a factor
+// Bytes of a vector's factors, a multiple of four.
+__host__ __device__ constexpr int i4_group_bytes(int Dh) { return (Dh + 127) / 128 * 4; }
 
 // Pages [num_pages, H, 1 << page_shift, Dh] of K and of V; for coded types the
-// scales are [num_pages, H, 1 << page_shift].
+// scales are [num_pages, H, 1 << page_shift].  I4 holds two codes a byte and, for each
+// vector, a factor of 0 to 255 per 32 dimensions (k_group, v_group, i4_group_bytes a
+// vector): x_d = scale * factor * (nibble - 8).
 struct KvPages {
   void *k, *v;
   float *k_scale, *v_scale;
   int type, num_pages, H, page_shift, Dh;
+  uint8_t *k_group, *v_group;
 };
 // Sequence b owns rows [cu[b], cu[b+1]) of the packed tokens, its tokens'
 // pages are table[b * table_stride + i], i < max_pages, and it holds lens[b]
@@ -233,6 +242,16 @@ struct RowsView {
 // for coded types; read the packed tokens' places back into K, V.
 void kv_pages_append_launch(const RowsView& K, const RowsView& V, const KvPages& pg,
                             const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s);
+// The same with K rotated by its tokens' positions on the way, and the rows Q too, into
+// QO (Q.data null: no such rows).  Pair i of a vector at position p turns by
+// p * inv_freq[i], i < pairs: dimensions i and i + pairs, or 2i and 2i + 1.
+struct Rope {
+  const float* inv_freq;
+  int pairs, interleaved;
+};
+void kv_pages_append_rope_launch(const RowsView& Q, const RowsView& QO, const RowsView& K,
+                                 const RowsView& V, const KvPages& pg, const SeqTable& sq,
+                                 const Rope& rope, int* index_status, int num_sms, cudaStream_t s);
 void kv_pages_read_launch(const KvPages& pg, const RowsView& K, const RowsView& V,
                           const SeqTable& sq, int* index_status, int num_sms, cudaStream_t s);
 
@@ -247,6 +266,11 @@ struct SeqAttnArgs {
   int G;                // query heads per KV head
   int causal;
   float scale_log2;     // softmax scale times log2(e)
+  // Attention to selected blocks (sel_heads > 0, else 0): "sequence" v of the schedule is
+  // one token's query heads of one KV head, v = token * sel_heads + KV head.  Row v of
+  // seqs.table holds its pages, seqs.lens[v] how many keys they have for it (-1: no such
+  // row), and each counts for sel_tiles tiles on the line whatever it has.
+  int sel_heads, sel_tiles;
   // Schedule: rows per item, log2 of the keys per tile, fewest tiles per CTA,
   // tiles that an item counts for besides its own.
   int rows, kt_shift, min_tiles, extra;
@@ -264,6 +288,28 @@ size_t seq_workspace_bytes(int G, int Dh, int num_sms);
 // it only steers the choice of kernel.
 void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
                   cudaStream_t s);
+
+// The same over blocks of its own for each token and KV head: blocks [tokens][H][take],
+// ascending, -1 behind the last one.  a.pages and a.seqs as for seq_attn_run.
+size_t seq_blocks_workspace_bytes(int tokens, int H, int G, int Dh, int take, int num_sms);
+void seq_attn_blocks_run(SeqAttnArgs a, const int32_t* blocks, int take, void* ws, size_t ws_bytes,
+                         int num_sms, cudaStream_t s);
+
+// K10 (kv_blocks.cu).  bounds: [num_pages][H][2][Dh], least and greatest value of a page's
+// keys, for the pages that the sequences' new tokens complete.
+void kv_blocks_bounds_launch(const KvPages& pg, void* bounds, int bounds_type, const SeqTable& sq,
+                             int* index_status, int num_sms, cudaStream_t s);
+// The `take` blocks of each of q's tokens and KV heads: the first keep_first, the last
+// keep_last (its own last), and the others with the greatest scores.
+size_t kv_blocks_workspace_bytes(int tokens, int H, int max_pages);
+void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, int H,
+                          int page_shift, const SeqTable& sq, int keep_first, int keep_last,
+                          int32_t* blocks, int take, void* ws, size_t ws_bytes, int* index_status,
+                          cudaStream_t s);
+// Lists as page numbers [tokens * H][take] and keys that they hold for their token
+// [tokens * H] (-1: a row of no sequence).
+void kv_blocks_lists_launch(const SeqTable& sq, const KvPages& pg, const int32_t* blocks, int take,
+                            int32_t* pages, int32_t* lens, int* index_status, cudaStream_t s);
 
 // The kernels (K6: any type, stride and head size up to 256).
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);

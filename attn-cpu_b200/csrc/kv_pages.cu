@@ -1,5 +1,6 @@
 // kv_pages.cu -- K5: writing packed tokens into the pages of a KV cache, as they
-// are or as 8-bit codes, and reading them back.
+// are or as codes of 8 or 4 bits, rotated by their positions on the way where asked,
+// and reading them back.
 //
 // A vector x of Dh values (one token, one KV head) is stored in e4m3 or int8 as
 //     a = max |x|,   code = round(x * C / a),   scale = a / C    (C = 448 or 127)
@@ -13,6 +14,24 @@
 // distance 2^-42).  Where C / a leaves fp32's range all take the quotient.  A vector
 // of zeros has scale 0; one with an Inf or NaN has scale NaN and codes 0, so
 // that it cannot be read back as something finite.
+//
+// In 4 bits a vector is stored as
+//     a = max |x|,   a_g = max |x| over 32 dimensions,   r_g = ceil(255 a_g / a),
+//     code = round(x * 1785 / (a r_g)),   scale = a / 1785
+// (1785 = 7 * 255), codes from -7 to 7 held as 1 to 15: a strong channel costs the other
+// groups nothing, code * r_g stays below 2048, so that it is a whole number which f16 holds
+// exactly, and one scale per vector is left for the attention to apply.  Factors and
+// codes are those of the exact quotients: a candidate from the fp32 quotient is
+// settled by comparing products, 255 a_g with r a, and 3570 |x| with (2m + 1) a r.
+// For 16-bit x these have at most 23 bits and are exact in fp32, once tiny and huge vectors are
+// brought near 1; for fp32 x they are taken in 64 bits.
+//
+// Rotation: x' = x cos t -+ y sin t with y the other one of the pair and t = position *
+// inv_freq.  The angle is reduced to a fraction of a turn in 64 bits (at
+// position 100000 an fp32 product is off by 0.004), once per token and
+// pair of a CTA for all heads; then everything is fp32.  The result is rounded to the rows'
+// type once and stored as that: the same numbers as rotating first and
+// appending then.
 //
 // Bound by memory: a token is read once and its codes written once.  A CTA takes
 // some tokens that follow one another, all heads of K and V.  Where a token
@@ -36,26 +55,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The sequence that packed token t belongs to: the last b with cu[b] <= t
-// (clamped as in seq_rows), or -1 when its range does not hold t.
-__device__ __forceinline__ int seq_of(const SeqTable& sq, int t, int& first, int& count) {
-  int lo = 0, hi = sq.batch;  // cu[lo] <= t is kept true for lo > 0
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(sq.cu + mid) <= t) lo = mid;
-    else hi = mid;
-  }
-  seq_rows(sq.cu, lo, sq.total, first, count);
-  return t >= first && t < first + count ? lo : -1;
-}
-
-// Place of packed token t in a [.., H, page, ..] pool for head 0, or -1.
-__device__ __forceinline__ int64_t place_of(const SeqTable& sq, const KvPages& pg, int t,
-                                            int* index_status) {
-  int first, count;
-  const int b = seq_of(sq, t, first, count);
-  if (b < 0) return -1;
-  const int64_t pos = (int64_t)__ldg(sq.lens + b) - count + (t - first);
+// Place of position `pos` of sequence b in a [.., H, page, ..] pool for head 0, or -1.
+__device__ __forceinline__ int64_t place_of(const SeqTable& sq, const KvPages& pg, int b,
+                                            int64_t pos, int* index_status) {
   if (pos < 0 || pos >= ((int64_t)sq.max_pages << pg.page_shift)) {
     raise_index(index_status);
     return -1;
@@ -100,13 +102,17 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&q)[4], elem_t<kI8>*
 constexpr int kMaxTokens = 32;  // per CTA
 
 // Where the CTA's tokens [t0, t0 + n) live: the place of head 0, -1 for a place
-// out of range and -2 for a row of no sequence.
+// out of range and -2 for a row of no sequence.  Their positions go to `position`
+// where that is given.
 __device__ __forceinline__ void find_places(const SeqTable& sq, const KvPages& pg, int t0, int n,
-                                            int64_t* at, int* index_status) {
+                                            int64_t* at, int* index_status,
+                                            int64_t* position = nullptr) {
   if ((int)threadIdx.x < n) {
     int first, count;
-    const int t = t0 + threadIdx.x;
-    at[threadIdx.x] = seq_of(sq, t, first, count) < 0 ? -2 : place_of(sq, pg, t, index_status);
+    const int t = t0 + threadIdx.x, b = seq_of(sq, t, first, count);
+    const int64_t pos = b < 0 ? 0 : (int64_t)__ldg(sq.lens + b) - count + (t - first);
+    at[threadIdx.x] = b < 0 ? -2 : place_of(sq, pg, b, pos, index_status);
+    if (position) position[threadIdx.x] = pos;
   }
   __syncthreads();
 }
@@ -143,7 +149,7 @@ __device__ __forceinline__ void store8(E* p, int d, int Dh, bool vec, const Eigh
 }
 
 // Steps through the CTA's vectors, a group's share of them: token by token, all
-// heads of K, then of V.  No division but at the start.
+// heads of K, then of V (and of Q).  No division but at the start.
 struct Walk {
   int tl, kvh, dt, dr, H2;
   __device__ __forceinline__ Walk(int first, int step, int heads2) : H2(heads2) {
@@ -162,37 +168,186 @@ struct Walk {
   }
 };
 
+// The share of one lane (dimensions d to d + 7) in 4 bits: its eight codes and its
+// group's factor.  top: the vector's largest magnitude, finite.  All lanes of
+// `mask` call.
+template <int TX>
+__device__ __forceinline__ uint32_t i4_codes(const float (&x)[8], float top, unsigned mask,
+                                             int& factor) {
+  // 16-bit values: products exact in fp32, once the vector is brought near 1.
+  using Wide = std::conditional_t<TX == kF32, double, float>;
+  float near = 1.f;
+  if (TX != kF16) near = top > 0x1p60f ? 0x1p-64f : top < 0x1p-60f ? 0x1p64f : 1.f;
+  float y[8], own = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    y[j] = fabsf(x[j]) * near;
+    own = fmaxf(own, y[j]);
+  }
+  own = fmaxf(own, __shfl_xor_sync(mask, own, 1));  // 32 dimensions are four lanes
+  own = fmaxf(own, __shfl_xor_sync(mask, own, 2));
+  factor = 0;
+  if (!(own > 0.f)) return 0x88888888u;
+  const float a = top * near;
+  int r = min(max((int)ceilf(own / a * 255.f), 1), 255);
+  const Wide want = (Wide)own * (Wide)255;
+  if ((Wide)(r - 1) * (Wide)a >= want) --r;
+  if ((Wide)r * (Wide)a < want) ++r;
+  factor = r;
+  const Wide ar = (Wide)a * (Wide)r;
+  const float inv = 1785.f / (float)ar;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // A whole number next below the quotient (or, where that is next to a whole number,
+    // that one: both round the same way), and which side of the tie above it
+    // the quotient is on.
+    const float m = floorf(y[j] * inv);
+    const Wide p = (Wide)y[j] * (Wide)3570, tie = (Wide)(2.f * m + 1.f) * ar;
+    int c = (int)m;
+    if (p > tie || (p == tie && (c & 1))) ++c;
+    codes |= (uint32_t)(x[j] < 0.f ? 8 - c : 8 + c) << (4 * j);
+  }
+  return codes;
+}
+
+// cos and sin of every token and pair of the CTA, [n][pairs].
+__device__ __forceinline__ void turn_angles(const Rope& rope, const int64_t* position, int n,
+                                            float2* turns) {
+  for (int i = threadIdx.x; i < n * rope.pairs; i += kThreads) {
+    const int t = i / rope.pairs, p = i - t * rope.pairs;
+    const double turn = (double)position[t] * (double)__ldg(rope.inv_freq + p) * 0.15915494309189535;
+    const float part = (float)(turn - rint(turn));  // of a turn, at most a half
+    float2 cs;
+    sincospif(2.f * part, &cs.y, &cs.x);
+    turns[i] = cs;
+  }
+}
+
+// The lane's cos and sin for one token, the sign of the sine with the element's side of its
+// pair.  Elements that stay have 1 and 0.
+__device__ __forceinline__ void lane_turns(const Rope& rope, const float2* turns, int d,
+                                           float (&co)[8], float (&si)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int x = d + j;
+    const bool second = rope.interleaved ? (x & 1) : x >= rope.pairs;
+    const int p = rope.interleaved ? x >> 1 : second ? x - rope.pairs : x;
+    const bool turned = x < 2 * rope.pairs;
+    const float2 cs = turned ? turns[p] : make_float2(1.f, 0.f);
+    co[j] = cs.x;
+    si[j] = second ? cs.y : -cs.y;
+  }
+}
+
+// The lane's eight elements of the row at p, turned.  All lanes of the row call, and
+// none has stored before all have read (rows may be turned in place).
+template <class E>
+__device__ __forceinline__ Eight<E> turned8(const E* p, const Eight<E>& raw, const Rope& rope, int d,
+                                            int Dh, bool vec, const float (&co)[8],
+                                            const float (&si)[8]) {
+  Eight<E> other = raw;
+  const int half = rope.pairs;
+  if (!rope.interleaved && d < 2 * half) {
+    if (vec && half % 8 == 0) {
+      other = load8(p, d < half ? d + half : d - half, Dh, true);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int x = d + j;
+        if (x < 2 * half) other.e[j] = p[x < half ? x + half : x - half];
+      }
+    }
+  }
+  Eight<E> out = raw;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (d + j >= 2 * half) continue;
+    const float y = to_float(rope.interleaved ? raw.e[j ^ 1] : other.e[j]);
+    from_float(fmaf(to_float(raw.e[j]), co[j], y * si[j]), out.e[j]);
+  }
+  return out;
+}
+
 // One vector per group of LANES lanes at a time: the CTAs of an SM keep enough
 // reads going, and more registers would cost some of those (prompts of 11.7k tokens
 // to e4m3 and back: 61 us; 79 with two vectors in flight, 80 with four).
-template <int TX, int TC, int LANES>
+template <int TX, int TC, int LANES, bool ROPE>
 __global__ void __launch_bounds__(kThreads)
-    append_kernel(const RowsView K, const RowsView V, const KvPages pg, const SeqTable sq,
-                  const int tokens, const bool vec, int* index_status) {
+    append_kernel(const RowsView K, const RowsView V, const RowsView Q, const RowsView QO,
+                  const KvPages pg, const SeqTable sq, const Rope rope, const int tokens,
+                  const bool vec, int* index_status) {
   using EX = elem_t<TX>;
   using EC = elem_t<TC>;
-  constexpr bool CODED = TC == kE4M3 || TC == kI8;
-  __shared__ int64_t places[kMaxTokens];
+  constexpr bool CODED = elem_coded(TC);
+  __shared__ int64_t places[kMaxTokens], position[ROPE ? kMaxTokens : 1];
+  extern __shared__ float2 turns[];
   const int e = threadIdx.x % LANES, d = e * 8;
   const int Dh = pg.Dh;
   grid_dep_wait();
   const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
-  find_places(sq, pg, t0, n, places, index_status);
+  find_places(sq, pg, t0, n, places, index_status, ROPE ? position : nullptr);
+  if constexpr (ROPE) {
+    turn_angles(rope, position, n, turns);
+    __syncthreads();
+  }
   // A group's lanes share their vector; the other groups of the warp may have left.
   const unsigned mask =
       LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
-  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H); at.tl < n; at.next()) {
-    const bool is_v = at.kvh >= pg.H;
-    const int h = is_v ? at.kvh - pg.H : at.kvh;
+  float co[8], si[8];
+  int turned = -1;  // the token that they are of
+  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H + (ROPE ? Q.heads : 0)); at.tl < n;
+       at.next()) {
     const int64_t first = places[at.tl];
-    if (first < 0) continue;
+    const int64_t t = t0 + at.tl;
+    const bool is_q = ROPE && at.kvh >= 2 * pg.H;
+    if (first < (is_q ? -1 : 0)) continue;  // Q's rows are turned wherever K may go
+    const bool is_v = at.kvh >= pg.H;
+    const int h = is_q ? at.kvh - 2 * pg.H : is_v ? at.kvh - pg.H : at.kvh;
+    const RowsView& src = is_q ? Q : is_v ? V : K;
+    const EX* row = static_cast<const EX*>(src.data) + t * src.sT + (int64_t)h * src.sH;
+    Eight<EX> raw = load8(row, d, Dh, vec);
+    if constexpr (ROPE) {
+      if (is_q || !is_v) {
+        if (turned != at.tl) {
+          turned = at.tl;
+          lane_turns(rope, turns + at.tl * rope.pairs, d, co, si);
+        }
+        raw = turned8(row, raw, rope, d, Dh, vec, co, si);
+      }
+      if (is_q) {
+        __syncwarp(mask);
+        store8(static_cast<EX*>(QO.data) + t * QO.sT + (int64_t)h * QO.sH, d, Dh, vec, raw);
+        continue;
+      }
+    }
     const int64_t place = first + ((int64_t)h << pg.page_shift);
-    const RowsView& src = is_v ? V : K;
-    const Eight<EX> raw = load8(static_cast<const EX*>(src.data) + (int64_t)(t0 + at.tl) * src.sT +
-                                    (int64_t)h * src.sH,
-                                d, Dh, vec);
-    EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + place * Dh;
-    if constexpr (CODED) {
+    if constexpr (TC == kI4) {
+      float x[8], top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = to_float(raw.e[j]);
+        top = max_nan(top, fabsf(x[j]));
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+      const bool bad = !(top <= 3.402823466e38f);
+      if (e == 0)
+        (is_v ? pg.v_scale : pg.k_scale)[place] = bad ? __int_as_float(0x7fffffff) : top / 1785.f;
+      if (bad) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      }
+      int factor;
+      const uint32_t codes = i4_codes<TX>(x, top, mask, factor);
+      if (d < Dh)
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(is_v ? pg.v : pg.k) +
+                                     place * (Dh / 2) + d / 2) = codes;
+      const int bytes = i4_group_bytes(Dh);
+      if (e % 4 == 0 && e / 4 < bytes)
+        (is_v ? pg.v_group : pg.k_group)[place * bytes + e / 4] = (uint8_t)factor;
+    } else if constexpr (CODED) {
+      EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + place * Dh;
       constexpr float C = TC == kE4M3 ? 448.f : 127.f;
       float x[8], top = 0.f;
 #pragma unroll
@@ -243,7 +398,7 @@ __global__ void __launch_bounds__(kThreads)
       memcpy(&codes, r, 8);
       store8(out, d, Dh, vec, codes);
     } else {
-      store8(out, d, Dh, vec, raw);
+      store8(static_cast<EC*>(is_v ? pg.v : pg.k) + place * Dh, d, Dh, vec, raw);
     }
   }
 }
@@ -284,7 +439,7 @@ __global__ void __launch_bounds__(kThreads)
                 const int tokens, const bool vec, int* index_status) {
   using EX = elem_t<TX>;
   using EC = elem_t<TC>;
-  constexpr bool CODED = TC == kE4M3 || TC == kI8;
+  constexpr bool CODED = elem_coded(TC);
   __shared__ int64_t places[kMaxTokens];
   const int d = threadIdx.x % LANES * 8;
   const int Dh = pg.Dh;
@@ -298,16 +453,33 @@ __global__ void __launch_bounds__(kThreads)
     if (first == -2) continue;  // a row of no sequence stays as it is
     const RowsView& dst = is_v ? V : K;
     EX* out = static_cast<EX*>(dst.data) + (int64_t)(t0 + at.tl) * dst.sT + (int64_t)h * dst.sH;
-    Eight<EC> raw;
-    memset(&raw, 0, sizeof(raw));
-    float scale = 1.f;
-    if (first >= 0) {  // a bad place reads as zeros
-      const int64_t place = first + ((int64_t)h << pg.page_shift);
-      raw = load8(static_cast<const EC*>(is_v ? pg.v : pg.k) + place * Dh, d, Dh, vec);
-      if constexpr (CODED) scale = (is_v ? pg.v_scale : pg.k_scale)[place];
+    if constexpr (TC == kI4) {
+      Eight<EX> back;
+      memset(&back, 0, sizeof(back));
+      if (first >= 0 && d < Dh) {
+        const int64_t place = first + ((int64_t)h << pg.page_shift);
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(
+            static_cast<const uint8_t*>(is_v ? pg.v : pg.k) + place * (Dh / 2) + d / 2);
+        const float scale = (is_v ? pg.v_scale : pg.k_scale)[place];
+        float x[8];
+        i4_values(codes, (is_v ? pg.v_group : pg.k_group)[place * i4_group_bytes(Dh) + d / kI4Group],
+                  x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) from_float(x[j] * scale, back.e[j]);
+      }
+      store8(out, d, Dh, vec, back);
+    } else {
+      Eight<EC> raw;
+      memset(&raw, 0, sizeof(raw));
+      float scale = 1.f;
+      if (first >= 0) {  // a bad place reads as zeros
+        const int64_t place = first + ((int64_t)h << pg.page_shift);
+        raw = load8(static_cast<const EC*>(is_v ? pg.v : pg.k) + place * Dh, d, Dh, vec);
+        if constexpr (CODED) scale = (is_v ? pg.v_scale : pg.k_scale)[place];
+      }
+      if constexpr (CODED) store8(out, d, Dh, vec, decode8<TX, TC>(raw, scale));
+      else store8(out, d, Dh, vec, raw);
     }
-    if constexpr (CODED) store8(out, d, Dh, vec, decode8<TX, TC>(raw, scale));
-    else store8(out, d, Dh, vec, raw);
   }
 }
 
@@ -318,6 +490,7 @@ bool vec_rows(const RowsView& r) {
          r.Dh % 8 == 0;
 }
 bool vec_pages(const KvPages& p) {
+  if (p.type == kI4) return true;  // their own reads and writes, of 4 bytes
   const int b = std::min(16, 8 * elem_bytes(p.type));
   return reinterpret_cast<uintptr_t>(p.k) % b == 0 && reinterpret_cast<uintptr_t>(p.v) % b == 0 &&
          p.Dh % 8 == 0;
@@ -335,6 +508,7 @@ void dispatch(const RowsView& K, const KvPages& pg, F&& f) {
   with_value_type(K.type, [&](auto tx) {
     if (pg.type == kE4M3) sizes(tx, std::integral_constant<int, kE4M3>{});
     else if (pg.type == kI8) sizes(tx, std::integral_constant<int, kI8>{});
+    else if (pg.type == kI4) sizes(tx, std::integral_constant<int, kI4>{});
     else sizes(tx, tx);
   });
 }
@@ -354,8 +528,26 @@ void kv_pages_append_launch(const RowsView& K, const RowsView& V, const KvPages&
   ProfScope prof("kv_pages", s);
   dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
     constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
-    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN>, dim3((sq.total + tokens - 1) / tokens),
-                          dim3(kThreads), 0, s, K, V, pg, sq, tokens, vec, index_status));
+    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, false>,
+                          dim3((sq.total + tokens - 1) / tokens), dim3(kThreads), 0, s, K, V,
+                          RowsView{}, RowsView{}, pg, sq, Rope{}, tokens, vec, index_status));
+  });
+}
+
+void kv_pages_append_rope_launch(const RowsView& Q, const RowsView& QO, const RowsView& K,
+                                 const RowsView& V, const KvPages& pg, const SeqTable& sq,
+                                 const Rope& rope, int* index_status, int num_sms,
+                                 cudaStream_t s) {
+  const bool vec = vec_rows(K) && vec_rows(V) && vec_pages(pg) &&
+                   (Q.heads == 0 || (vec_rows(Q) && vec_rows(QO)));
+  const int tokens = tokens_per_cta(sq, num_sms);
+  ProfScope prof("kv_pages", s);
+  dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
+    constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
+    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, true>,
+                          dim3((sq.total + tokens - 1) / tokens), dim3(kThreads),
+                          tokens * rope.pairs * sizeof(float2), s, K, V, Q, QO, pg, sq, rope,
+                          tokens, vec, index_status));
   });
 }
 

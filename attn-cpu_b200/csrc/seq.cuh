@@ -16,6 +16,12 @@
 // has at most two such pieces, its first and its last, so the workspace does
 // not grow with the batch.
 //
+// Attention to selected blocks runs on the same line, with a "sequence" for each
+// token and KV head that has pages of its own.  These are many and much the same,
+// so that each counts for as many tiles as the longest may have: a CTA finds its
+// place by one division, where the sum over their own lengths would cost more than
+// it evens out.
+//
 // Lengths and page numbers come from device memory and are clamped here, so
 // that wrong ones lead to no access out of range.
 #pragma once
@@ -56,8 +62,29 @@ __device__ __forceinline__ void seq_rows(const int32_t* cu, int b, int total, in
   count = clampi(__ldg(cu + b + 1), first, total) - first;
 }
 
+// The sequence that packed token t belongs to: the last b with cu[b] <= t
+// (clamped as in seq_rows), or -1 when its range does not hold t.
+__device__ __forceinline__ int seq_of(const SeqTable& sq, int t, int& first, int& count) {
+  int lo = 0, hi = sq.batch;  // cu[lo] <= t is kept true for lo > 0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(sq.cu + mid) <= t) lo = mid;
+    else hi = mid;
+  }
+  seq_rows(sq.cu, lo, sq.total, first, count);
+  return t >= first && t < first + count ? lo : -1;
+}
+
 __device__ __forceinline__ SeqInfo seq_info(const SeqAttnArgs& a, int b) {
   SeqInfo i;
+  if (a.sel_heads) {
+    const int len = __ldg(a.seqs.lens + b);
+    i.q0 = b / a.sel_heads;
+    i.n = len >= 0 ? 1 : 0;
+    i.k0 = 0;
+    i.L = max(len, 0);
+    return i;
+  }
   seq_rows(a.seqs.cu, b, a.seqs.total, i.q0, i.n);
   if (a.pages.k) {
     const int len = __ldg(a.seqs.lens + b);
@@ -186,8 +213,30 @@ struct SeqShared {
   int b, m;
 };
 
+// Items of a KV head, and tiles that one of them counts for, with selected blocks.
+__device__ __forceinline__ int sel_items(const SeqAttnArgs& a) {
+  return (a.G + a.rows - 1) / a.rows;
+}
+__device__ __forceinline__ int sel_span(const SeqAttnArgs& a) { return a.sel_tiles + a.extra; }
+
 // All threads of the block; false when the CTA has nothing to do.
 __device__ inline bool seq_locate(const SeqAttnArgs& a, SeqShared& sh, SeqPlace& p) {
+  if (a.sel_heads) {
+    const int M = sel_items(a), span = sel_span(a);
+    const long long total = (long long)a.seqs.batch * M * span;
+    p.quota = max((long long)a.min_tiles, (long long)udiv(total + gridDim.x - 1, gridDim.x));
+    p.t0 = p.quota * blockIdx.x;
+    p.t1 = min(total, p.t0 + p.quota);
+    __syncthreads();  // as below: what was set up is seen
+    if (p.t0 >= total) return false;
+    const long long item = (long long)udiv(p.t0, span);
+    p.b = (int)udiv(item, M);
+    p.m = (int)(item - (long long)p.b * M);
+    p.h = p.b % a.sel_heads;
+    p.item0 = item * span;
+    p.j = (int)(p.t0 - p.item0);
+    return true;
+  }
   const int tid = threadIdx.x, nt = blockDim.x, batch = a.seqs.batch;
   auto weight = [&](int b) -> long long {
     if (b >= batch) return 0;
@@ -258,13 +307,16 @@ struct SeqPiece {
   SeqInfo s;
   int b, h, m, j0, j1, nt;
   int row0, rows;  // its rows [row0, row0 + rows) of the sequence's n * G
+  bool head;       // of the item that the CTA's first tile lies in
 };
 
 // Steps through a CTA's pieces; every role of a kernel runs one of its own.
-struct SeqIter {
+// SEL: in a kernel that selected blocks may come to.
+template <bool SEL>
+struct SeqIterOf {
   long long t, t1;
   int b, h, m, j;
-  bool fresh;
+  bool fresh, head;
   SeqInfo s;
   int items;
   __device__ __forceinline__ void start(const SeqPlace& p) {
@@ -274,9 +326,10 @@ struct SeqIter {
     h = p.h;
     m = p.m;
     j = p.j;
-    fresh = true;
+    fresh = head = true;
   }
   __device__ __forceinline__ bool next(const SeqAttnArgs& a, SeqPiece& w) {
+    if (SEL && a.sel_heads) return next_selected(a, w);
     while (t < t1) {
       if (fresh) {
         s = seq_info(a, b);
@@ -293,6 +346,8 @@ struct SeqIter {
       w.j1 = max(0, end - a.extra);
       w.row0 = m * a.rows;
       w.rows = min(a.rows, s.n * a.G - w.row0);
+      w.head = head;
+      head = false;
       t += end - j;
       j = 0;
       if (++m == items) {
@@ -311,17 +366,45 @@ struct SeqIter {
     }
     return false;
   }
+  __device__ __forceinline__ bool next_selected(const SeqAttnArgs& a, SeqPiece& w) {
+    const int span = sel_span(a), M = sel_items(a);
+    while (t < t1) {
+      w.s = seq_info(a, b);
+      w.b = b;
+      w.h = h;
+      w.m = m;
+      w.nt = seq_tiles(a, w.s, m);
+      const int end = (int)min((long long)span, j + (t1 - t));
+      w.j0 = max(0, j - a.extra);
+      w.j1 = w.s.n ? min(w.nt, end - a.extra) : 0;
+      w.row0 = m * a.rows;
+      w.rows = min(a.rows, a.G - w.row0);
+      w.head = head;
+      head = false;
+      t += end - j;
+      j = 0;
+      if (++m == M) {
+        m = 0;
+        ++b;
+        if (++h == a.sel_heads) h = 0;
+      }
+      if (w.j1 > w.j0) return true;
+    }
+    return false;
+  }
 };
+
+using SeqIter = SeqIterOf<false>;
 
 // Number of keys that row r (of the sequence's n * G) sees.
 __device__ __forceinline__ int seq_row_seen(const SeqAttnArgs& a, const SeqInfo& s, int r) {
   return a.causal ? s.L - s.n + r / a.G + 1 : s.L;
 }
 
-// Which partial a piece writes (-1: none, it is a whole item): the CTA's first
-// piece goes to its slot 0, a later one to slot 1.
-__device__ __forceinline__ int seq_slot(const SeqPiece& w, bool first) {
-  return w.j0 == 0 && w.j1 == w.nt ? -1 : 2 * (int)blockIdx.x + (first ? 0 : 1);
+// Which partial a piece writes (-1: none, it is a whole item): one of the item that
+// the CTA's first tile lies in goes to its slot 0, a later one to slot 1.
+__device__ __forceinline__ int seq_slot(const SeqPiece& w) {
+  return w.j0 == 0 && w.j1 == w.nt ? -1 : 2 * (int)blockIdx.x + (w.head ? 0 : 1);
 }
 
 // One thread of every CTA, those without work included.
@@ -331,9 +414,9 @@ __device__ __forceinline__ void seq_write_split(const SeqAttnArgs& a, bool any,
   d.extra = a.extra;
   if (any && p.j > a.extra) {
     const SeqInfo s = seq_info(a, p.b);
-    d.continues = 1;
     d.item0 = p.item0 + a.extra;
     d.item1 = d.item0 + seq_tiles(a, s, p.m);
+    d.continues = s.n > 0 && p.t0 < d.item1;
     d.quota = p.quota;
     d.first_row = p.m * a.rows;
     d.rows = min(a.rows, s.n * a.G - d.first_row);

@@ -31,6 +31,10 @@ template <>
 struct Elem<kI8> {
   using type = int8_t;
 };
+template <>
+struct Elem<kI4> {
+  using type = uint8_t;  // two codes
+};
 template <int T>
 using elem_t = typename Elem<T>::type;
 
@@ -64,6 +68,21 @@ __device__ __forceinline__ void load4(const E* p, float (&x)[4]) {
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = to_float(f.e[i]);
+}
+
+// Eight 4-bit codes (of dimensions d to d + 7, lowest bits first) times their factor,
+// whole numbers up to 2040.
+__device__ __forceinline__ void i4_values(uint32_t codes, int factor, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    x[i] = (float)(((int)((codes >> (4 * i)) & 15u) - 8) * factor);
+}
+
+// Four codes at an even address, of dimensions of one group.
+__device__ __forceinline__ void load4_i4(const uint8_t* p, int factor, float (&x)[4]) {
+  const uint32_t codes = __ldg(reinterpret_cast<const uint16_t*>(p));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (float)(((int)((codes >> (4 * i)) & 15u) - 8) * factor);
 }
 
 // Calls f with the type as a compile-time constant.

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
   if (!any) return;
   __syncthreads();
 
-  SeqIter it;
+  SeqIterOf<true> it;
   it.start(place);
   SeqPiece w;
   if (warp == kWarps) {
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
   const int g = lane >> 2, c = lane & 3;  // fragment row and column group
   Ring<ST> ring;
   bool ok = true;
-  for (bool first = true; it.next(a, w); first = false) {
+  while (it.next(a, w)) {
     // Q^T as B fragments: row 8 r + g, by step of 16 dimensions.  16-bit keys:
     // dimensions 2c, 2c+1 and 2c+8, 2c+9 of the step; codes: 4c .. 4c+3, as a
     // 4-byte unit of ldmatrix holds them.
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         if (g == 0) sm_ml[warp][8 * r + 2 * c + i] = make_float2(m[r][i], sum);
       }
     named_bar_sync(1, kWarps * 32);
-    const int slot = seq_slot(w, first);
+    const int slot = seq_slot(w);
     float f[NR][2], fr[NR][2];  // two factors: 2^rho may lie below the smallest fp32 number
 #pragma unroll
     for (int r = 0; r < NR; ++r)
@@ -573,6 +573,7 @@ void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensor
 
 bool seq_pages_tma(const SeqAttnArgs& a) {
   const KvPages& p = a.pages;
+  if (p.type == kI4) return false;
   if (!p.k || p.num_pages == 0 || a.q.type == kF32 || p.Dh > 128) return false;
   if ((p.Dh * elem_bytes(p.type)) % 16 != 0) return false;
   auto at16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };

@@ -130,23 +130,12 @@ size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
   return n + 256;
 }
 
-void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
-                  cudaStream_t s) {
-  if (a.seqs.batch == 0 || a.seqs.total == 0) return;
-  // New tokens of one sequence: the caller's bound, or the mean.
-  const int64_t rows =
-      (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
-  // Rows of one KV head and sequence.  16-bit pages: K7 up to 32 rows, K8 beyond (32
-  // sequences of 4096 keys, 8 KV heads of 128: 16 rows 102 us against 193, 32 rows
-  // 186 against 184, 48 rows 271 against 189); codes, which K8 converts in four
-  // warps: up to 48 (e4m3: 48 rows 267 us against 282, 64 rows 347 against 284).  In
-  // fp32, K9 over 16 rows (8 sequences of 2000 keys, 4 KV heads of 64: 16 rows 53 us
-  // both, 64 rows 62 us against K6's 169).
-  enum { kSimt, kMma, kTc, kTf32 } kind = kSimt;
-  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 48 : 32)) kind = kMma;
-  else if (seq_tc_supported(a)) kind = kTc;
-  else if (seq_mma_supported(a)) kind = kMma;
-  else if (a.q.Dh <= 128 && rows > 16) kind = kTf32;
+enum Kind { kSimt, kMma, kTc, kTf32 };
+
+// Kernel, then join of what the cuts between CTAs split.  rows: query rows of a KV head and
+// sequence, as far as known.
+static void run(SeqAttnArgs a, Kind kind, int64_t rows, uintptr_t ws, uintptr_t ws_end, int num_sms,
+                cudaStream_t s) {
   const Space sp = kind == kTc     ? tc_space(a.G, num_sms)
                    : kind == kMma  ? mma_space(rows, num_sms)
                    : kind == kTf32 ? tf32_space(num_sms)
@@ -155,9 +144,8 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   a.kt_shift = kind == kTc ? 7 : kind == kTf32 ? 5 : 6;
   a.min_tiles = 2;
   a.extra = kind == kTc || kind == kTf32 ? 2 : 1;
-  uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
-  if (p + sp.bytes(a.q.Dh) > reinterpret_cast<uintptr_t>(ws) + ws_bytes)
-    fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
+  uintptr_t p = (ws + 255) & ~(uintptr_t)255;
+  if (p + sp.bytes(a.q.Dh) > ws_end) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
   a.ws_split = reinterpret_cast<void*>(p);
   p += sp.ctas * sizeof(SeqSplit);
   a.ws_ml = reinterpret_cast<float*>(p);
@@ -170,12 +158,56 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
     else if (kind == kTf32) seq_tf32_launch(a, sp.ctas, s);
     else seq_simt_launch(a, sp.ctas, s);
   }
-  // Joins what the cuts between CTAs split.
   with_value_type(a.o.type, [&](auto t) {
     ATTNB_CUDA(launch_pdl(seq_merge_kernel<decltype(t)::value>,
                           dim3(sp.ctas - 1, kind == kTc || kind == kTf32 ? 16 : 2), dim3(kMergeThreads), 0, s,
                           a));
   });
+}
+
+void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num_sms,
+                  cudaStream_t s) {
+  if (a.seqs.batch == 0 || a.seqs.total == 0) return;
+  // New tokens of one sequence: the caller's bound, or the mean.
+  const int64_t rows =
+      (int64_t)(max_new > 0 ? max_new : (a.seqs.total + a.seqs.batch - 1) / a.seqs.batch) * a.G;
+  // Rows of one KV head and sequence.  16-bit pages: K7 up to 32 rows, K8 beyond (32
+  // sequences of 4096 keys, 8 KV heads of 128: 16 rows 102 us against 193, 32 rows
+  // 186 against 184, 48 rows 271 against 189); codes, which K8 converts in four
+  // warps: up to 48 (e4m3: 48 rows 267 us against 282, 64 rows 347 against 284).  In
+  // fp32, K9 over 16 rows (8 sequences of 2000 keys, 4 KV heads of 64: 16 rows 53 us
+  // both, 64 rows 62 us against K6's 169).
+  Kind kind = kSimt;
+  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 48 : 32)) kind = kMma;
+  else if (seq_tc_supported(a)) kind = kTc;
+  else if (seq_mma_supported(a)) kind = kMma;
+  else if (a.q.Dh <= 128 && rows > 16) kind = kTf32;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(ws);
+  run(a, kind, rows, at, at + ws_bytes, num_sms, s);
+}
+
+size_t seq_blocks_workspace_bytes(int tokens, int H, int G, int Dh, int take, int num_sms) {
+  return (size_t)tokens * H * ((size_t)take + 1) * 4 + 256 + seq_workspace_bytes(G, Dh, num_sms);
+}
+
+void seq_attn_blocks_run(SeqAttnArgs a, const int32_t* blocks, int take, void* ws, size_t ws_bytes,
+                         int num_sms, cudaStream_t s) {
+  if (a.seqs.batch == 0 || a.seqs.total == 0) return;
+  const uintptr_t end = reinterpret_cast<uintptr_t>(ws) + ws_bytes;
+  const size_t rows = (size_t)a.seqs.total * a.pages.H;
+  uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
+  int32_t* const pages = reinterpret_cast<int32_t*>(p);
+  int32_t* const lens = pages + rows * take;
+  p += rows * (take + 1) * 4;
+  if (p > end) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
+  kv_blocks_lists_launch(a.seqs, a.pages, blocks, take, pages, lens, a.index_status, s);
+  // K6 or K7 take any number of rows; a token has few.
+  const Kind kind = seq_mma_supported(a) ? kMma : kSimt;
+  a.sel_heads = a.pages.H;
+  a.sel_tiles = (int)((((int64_t)take << a.pages.page_shift) + 63) >> 6);
+  a.causal = 0;  // the lengths are the token's own
+  a.seqs = SeqTable{nullptr, (int)rows, a.seqs.total, pages, take, take, lens};
+  run(a, kind, a.G, p, end, num_sms, s);
 }
 
 }  // namespace attnb

@@ -54,12 +54,25 @@ __device__ __forceinline__ void load_row(const E* p, int e, int Dh, bool vec, fl
   }
 }
 
+// The same of a row of 4-bit codes: 32 dimensions, and so one factor, for each c.
+template <int NC>
+__device__ __forceinline__ void load_row_i4(const uint8_t* p, const uint8_t* factors, int e, int Dh,
+                                            float (&x)[NC * 4]) {
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c * kI4Group < Dh) load4_i4(p + dim_of(e, c, 0) / 2, __ldg(factors + c), f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[c * 4 + i] = f[i];
+  }
+}
+
 template <int TQ, int TK, int R, int NC>
 __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(const SeqAttnArgs a, const bool qvec,
                                                             const bool kvec) {
   using EQ = elem_t<TQ>;
   using EK = elem_t<TK>;
-  constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  constexpr bool CODED = elem_coded(TK);
   constexpr int D = NC * 32;  // head size padded to the lanes' shares
   __shared__ SeqShared sh;
   __shared__ float sm_acc[kThreads / 32][R][D];
@@ -77,10 +90,10 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
   const bool paged = a.pages.k != nullptr;
   const int page_mask = (1 << a.pages.page_shift) - 1;
 
-  SeqIter it;
+  SeqIterOf<true> it;
   it.start(place);
   SeqPiece w;
-  for (bool first = true; it.next(a, w); first = false) {
+  while (it.next(a, w)) {
     float q[R][NC * 4], acc[R][NC * 4], m[R], l[R];
     int seen[R];
 #pragma unroll
@@ -102,6 +115,13 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
       const int key0 = (j << a.kt_shift) + group;
       const EK* kp[kKeys];
       const EK* vp[kKeys];
+      const uint8_t* kg[TK == kI4 ? kKeys : 1] = {};
+      const uint8_t* vg[TK == kI4 ? kKeys : 1] = {};
+      // One key's share of K or V.
+      auto load = [&](const EK* p, const uint8_t* factors, float (&x)[NC * 4]) {
+        if constexpr (TK == kI4) load_row_i4<NC>(p, factors, e, Dh, x);
+        else load_row<EK, NC>(p, e, Dh, kvec, x);
+      };
       float ks[kKeys], vs[kKeys];
 #pragma unroll
       for (int u = 0; u < kKeys; ++u) {
@@ -115,8 +135,13 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
             if (page >= 0) {  // a bad page reads as zeros
               const int64_t at =
                   (((int64_t)page * a.pages.H + w.h) << a.pages.page_shift) + (key & page_mask);
-              kp[u] = static_cast<const EK*>(a.pages.k) + at * Dh;
-              vp[u] = static_cast<const EK*>(a.pages.v) + at * Dh;
+              const int row = TK == kI4 ? Dh / 2 : Dh;
+              kp[u] = static_cast<const EK*>(a.pages.k) + at * row;
+              vp[u] = static_cast<const EK*>(a.pages.v) + at * row;
+              if constexpr (TK == kI4) {
+                kg[u] = a.pages.k_group + at * i4_group_bytes(Dh);
+                vg[u] = a.pages.v_group + at * i4_group_bytes(Dh);
+              }
               if (CODED) {
                 ks[u] = a.scale_log2 * __ldg(a.pages.k_scale + at);
                 vs[u] = __ldg(a.pages.v_scale + at);
@@ -138,12 +163,12 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
         for (int u = 0; u < kKeys; ++u) {
 #pragma unroll
           for (int i = 0; i < NC * 4; ++i) x[u][i] = 0.f;
-          if (kp[u]) load_row<EK, NC>(kp[u], e, Dh, kvec, x[u]);
+          if (kp[u]) load(kp[u], kg[TK == kI4 ? u : 0], x[u]);
         }
         if constexpr (R == 1) {
 #pragma unroll
           for (int u = 0; u < kKeys; ++u)
-            if (vp[u]) load_row<EK, NC>(vp[u], e, Dh, kvec, v[u]);
+            if (vp[u]) load(vp[u], vg[TK == kI4 ? u : 0], v[u]);
         }
 #pragma unroll
         for (int u = 0; u < kKeys; ++u)
@@ -180,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
       for (int u = 0; u < kKeys; ++u) {
         if (!vp[u]) continue;
         const int at = R == 1 ? u : 0;
-        if constexpr (R > 1) load_row<EK, NC>(vp[u], e, Dh, kvec, v[0]);
+        if constexpr (R > 1) load(vp[u], vg[TK == kI4 ? u : 0], v[0]);
         const int key = key0 + u * kGroups;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -211,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
       if (lane == 0) sm_ml[warp][r] = make_float2(top, sum);
     }
     __syncthreads();
-    const int slot = seq_slot(w, first);
+    const int slot = seq_slot(w);
     for (int r = 0; r < w.rows; ++r) {
       float top = -INFINITY;
       for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, sm_ml[i][r].x);
@@ -271,6 +296,7 @@ void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   with_value_type(a.q.type, [&](auto tq) {
     if (tk == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});
     else if (tk == kI8) go(tq, std::integral_constant<int, kI8>{});
+    else if (tk == kI4) go(tq, std::integral_constant<int, kI4>{});
     else go(tq, tq);
   });
 }

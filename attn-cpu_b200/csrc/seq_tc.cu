@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
     uint32_t g = 0, tile0 = 0;  // steps of this chain; tiles of the CTA
     bool ok = true;
     int piece = 0;
-    for (bool first = true; it.next(a, w); first = false, ++piece) {
+    for (; it.next(a, w); ++piece) {
       const int n = steps_of(c);
       const int rows = min(w.rows - c * half, half);  // of this chain, <= 0: none
       const bool mine = r < rows;
@@ -982,7 +982,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
       tile0 += w.j1 - w.j0;
       if (ok && n > 0) ok = warp_wait(&pv_bar[c][(g - 1) & 1], ((g - 1) >> 1) & 1);
       // ---- output: O / l, or the piece's partial result
-      const int slot = seq_slot(w, first);
+      const int slot = seq_slot(w);
       if (ok && rows > 0) {
         tc_fence_after();
         float mulo = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cfg = Tf32Cfg<DH>;
   using EQ = elem_t<TQ>;
   using EK = elem_t<TK>;
-  constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  constexpr bool CODED = elem_coded(TK);
   constexpr int QUADS = Cfg::EACH / 4;  // 4-element reads of K (and of V) per thread
   extern __shared__ uint8_t mem[];
   __shared__ SeqShared sh;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   SeqIter it;
   it.start(place);
   SeqPiece w;
-  for (bool first = true; it.next(a, w); first = false) {
+  while (it.next(a, w)) {
     // ---- Q, with the scale
     for (int i = tid; i < kRows * DH; i += kThreads) {
       const int r = i / DH, d = i % DH;
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int u = 0; u < QUADS; ++u) {
         const int i = tid + u * kThreads, key = j * kKeys + i / (DH / 4), d = i % (DH / 4) * 4;
         const EK *kx = nullptr, *vx = nullptr;
+        int kf = 0, vf = 0;  // 4-bit codes: the group's factors
         float ks = 1.f, vs = 1.f;
         if (key < w.s.L) {
           if (paged) {
@@ -134,8 +135,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (page >= 0) {  // a bad page reads as zeros
               const int64_t at = (((int64_t)page * a.pages.H + w.h) << a.pages.page_shift) +
                                  (key & ((1 << a.pages.page_shift) - 1));
-              kx = static_cast<const EK*>(a.pages.k) + at * Dh;
-              vx = static_cast<const EK*>(a.pages.v) + at * Dh;
+              const int row = TK == kI4 ? Dh / 2 : Dh;
+              kx = static_cast<const EK*>(a.pages.k) + at * row;
+              vx = static_cast<const EK*>(a.pages.v) + at * row;
+              if (TK == kI4 && d < Dh) {
+                kf = __ldg(a.pages.k_group + at * i4_group_bytes(Dh) + d / kI4Group);
+                vf = __ldg(a.pages.v_group + at * i4_group_bytes(Dh) + d / kI4Group);
+              }
               if (CODED) {
                 ks = __ldg(a.pages.k_scale + at);
                 vs = __ldg(a.pages.v_scale + at);
@@ -149,7 +155,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float k4[4] = {0.f, 0.f, 0.f, 0.f}, v4[4] = {0.f, 0.f, 0.f, 0.f};
         if (kx) {
-          if (kvec) {
+          if constexpr (TK == kI4) {
+            if (d < Dh) {
+              load4_i4(kx + d / 2, kf, k4);
+              load4_i4(vx + d / 2, vf, v4);
+            }
+          } else if (kvec) {
             if (d < Dh) {  // Dh is a multiple of 4
               load4(kx + d, k4);
               load4(vx + d, v4);
@@ -331,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // ---- output
-    const int slot = seq_slot(w, first);
+    const int slot = seq_slot(w);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float sum = l[i];
@@ -396,6 +407,7 @@ void seq_tf32_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   with_value_type(a.q.type, [&](auto tq) {
     if (tk == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});
     else if (tk == kI8) go(tq, std::integral_constant<int, kI8>{});
+    else if (tk == kI4) go(tq, std::integral_constant<int, kI4>{});
     else go(tq, tq);
   });
 }

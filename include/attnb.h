@@ -343,6 +343,8 @@ ATTNB_API int attnb_mha_block_dense_dev(const float* x, int batch, int T, int D,
 #define ATTNB_TYPE_F16 2
 #define ATTNB_TYPE_E4M3 3 /* pages only: 8-bit floating-point codes with a scale per vector */
 #define ATTNB_TYPE_I8 4   /* pages only: 8-bit integer codes with a scale per vector */
+#define ATTNB_TYPE_I4 6   /* pages only: 4-bit integer codes with a scale per vector and a
+                             factor per 32 dimensions */
 
 /* Packed rows [tokens, heads, Dh] of F32, BF16 or F16, Dh contiguous
  * (1 <= Dh <= 256); strides in elements.  Outputs need rows that do not
@@ -359,7 +361,14 @@ typedef struct attnb_rows {
  * [num_pages, H, page_size], NULL for the other types.  Tokens in coded pages are
  * as attnb_kv_pages_append_dev writes them: codes are finite (E4M3's NaN codes do
  * not occur), scales are not negative, and a vector that is not finite has scale
- * NaN.  Pointers are aligned to their elements. */
+ * NaN.  Pointers are aligned to their elements.
+ *
+ * I4 pages (Dh a multiple of 32) hold two codes a byte, dimension 2i in the low
+ * half: k and v are [num_pages, H, page_size, Dh / 2] bytes, and k_group and
+ * v_group [num_pages, H, page_size, 4 * ceil(Dh / 128)] bytes, one factor for each
+ * 32 dimensions (those past Dh are 0).  A value is scale * factor * (code - 8),
+ * codes 1 to 15.  These four start on 4-byte boundaries.  The last two
+ * fields are read for I4 pages only. */
 typedef struct attnb_kv_pages {
   void* k;
   void* v;
@@ -367,6 +376,8 @@ typedef struct attnb_kv_pages {
   float* v_scale;
   int type;
   int num_pages, H, page_size, Dh;
+  uint8_t* k_group;
+  uint8_t* v_group;
 } attnb_kv_pages;
 
 /* `batch` sequences: packed rows [cu[b], cu[b+1]) belong to sequence b (cu has
@@ -404,10 +415,32 @@ ATTNB_API int attnb_attn_packed_dev(const attnb_rows* Q, const attnb_rows* K, co
  * in the pages.  Pages of the rows' own type take them as they are.  E4M3 and
  * I8 pages take round(x * C / a) with a = max|x| over the vector and C = 448
  * or 127, ties to even, and the scale a / C; a vector of zeros has scale 0, and
- * one that holds an infinity or a NaN has scale NaN. */
+ * one that holds an infinity or a NaN has scale NaN.  I4 pages take, with a_g =
+ * max|x| over 32 dimensions, factors r = ceil(255 a_g / a), codes
+ * 8 + round(1785 x / (a r)), ties to even, and the scale a / 1785. */
 ATTNB_API int attnb_kv_pages_append_dev(const attnb_rows* K, const attnb_rows* V,
                                         const attnb_kv_pages* pages, const attnb_seqs* seqs,
                                         void* stream);
+/* Position rotation: pair i of a vector, i < pairs, at position p (0 for a
+ * sequence's first token) turns by the angle p * inv_freq[i] (device memory,
+ * [pairs]).  The pairs are dimensions i and i + pairs or, interleaved, 2i and
+ * 2i + 1; dimensions from 2 * pairs on stay as they are. */
+typedef struct attnb_rope {
+  const float* inv_freq;
+  int pairs;
+  int interleaved;
+} attnb_rope;
+
+/* attnb_kv_pages_append_dev with K rotated by its tokens' positions in their
+ * sequences on the way, and the rows Q (K's type, tokens and Dh, any number of
+ * heads) rotated into QO, which may be Q itself, with the same strides.  Q and QO
+ * may be NULL.  A rotated vector is rounded to the rows' type and stored as that.  Q's
+ * rows are written for every token of a sequence, also where a page number is out of
+ * range; rows of no sequence stay. */
+ATTNB_API int attnb_kv_pages_append_rope_dev(const attnb_rows* Q, const attnb_rows* QO,
+                                             const attnb_rows* K, const attnb_rows* V,
+                                             const attnb_kv_pages* pages, const attnb_seqs* seqs,
+                                             const attnb_rope* rope, void* stream);
 /* Reads the places of the packed rows (the last cu[b+1] - cu[b] tokens of each
  * sequence) out of the pages into K and V. */
 ATTNB_API int attnb_kv_pages_read_dev(const attnb_kv_pages* pages, const attnb_rows* K,
@@ -416,12 +449,59 @@ ATTNB_API int attnb_kv_pages_read_dev(const attnb_kv_pages* pages, const attnb_r
 /* Attention of the packed rows (new tokens, one and up per sequence) over the
  * lens[b] tokens that the pages hold, their own among them (append first);
  * otherwise as attnb_attn_packed_dev.  Q and O have one type; the pages have
- * that type or are E4M3 or I8.  max_new: the most rows of one sequence, as far
+ * that type or are E4M3, I8 or I4.  max_new: the most rows of one sequence, as far
  * as the caller knows (0: unknown); it steers the choice of kernel only. */
 ATTNB_API int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pages,
                                    const attnb_rows* O, const attnb_seqs* seqs, int max_new,
                                    int causal, float scale, void* workspace,
                                    size_t workspace_bytes, void* stream);
+
+/* Attention to selected blocks of a long context.  A block is one page of a
+ * sequence: block j holds tokens j * page_size to (j + 1) * page_size - 1.  Its
+ * bounds are the least and the greatest value of its keys in each dimension,
+ * rounded to `type` (F32, BF16 or F16): data is [num_pages, H, 2, Dh], dense. */
+typedef struct attnb_bounds {
+  void* data;
+  int type;
+} attnb_bounds;
+
+/* Writes the bounds of the blocks that the packed rows (the last cu[b+1] - cu[b]
+ * tokens of each sequence) complete; call it after each append.  Those of other
+ * pages stay.  Pages of F32, BF16 or F16 need bounds of their type.  Only k, its
+ * scales and factors are read. */
+ATTNB_API int attnb_kv_blocks_bounds_dev(const attnb_kv_pages* pages, const attnb_bounds* bounds,
+                                         const attnb_seqs* seqs, void* stream);
+
+/* Bytes of device workspace for the two calls below with these sizes on the current
+ * device (as with attnb_seq_workspace, one for each call in flight). */
+ATTNB_API int attnb_blocks_workspace(int tokens, int q_heads, int kv_heads, int Dh, int take,
+                                     int max_pages, size_t* bytes);
+
+/* The blocks that each packed row attends to, for each of the H KV heads: blocks
+ * is [Q.tokens, H, take] int32, ascending.  A row in block e of its sequence takes
+ * all of blocks 0 to e where these are no more than `take` (-1 fills the rest);
+ * else the first keep_first, the last keep_last (1 at least, its own among them)
+ * and, of the others, those with the greatest scores, the lower one of equal ones.
+ * The score is the sum over the query heads that read the KV head, and over the
+ * dimensions, of max(q least, q greatest): an upper bound of the sum of q . k for
+ * every key of the block.  Sums are in 64 bits; NaN is the greatest.  Q has the
+ * bounds' type.  The pages are [num_pages, H, page_size, Dh]; rows of no
+ * sequence stay as they are. */
+ATTNB_API int attnb_kv_blocks_select_dev(const attnb_rows* Q, const attnb_bounds* bounds,
+                                         int num_pages, int H, int page_size,
+                                         const attnb_seqs* seqs, int keep_first, int keep_last,
+                                         int32_t* blocks, int take, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
+/* attnb_attn_paged_dev, causal, over the listed blocks alone: blocks is [Q.tokens,
+ * pages' H, take].  A list is ascending and ends at its first entry that is -1;
+ * one that is not above the entry before it or lies behind the row's own block ends it
+ * too, and attnb_stream_status then reports ATTNB_ERR_INDEX.  A row whose list is
+ * empty gives zeros. */
+ATTNB_API int attnb_attn_blocks_dev(const attnb_rows* Q, const attnb_kv_pages* pages,
+                                    const attnb_rows* O, const attnb_seqs* seqs,
+                                    const int32_t* blocks, int take, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
