@@ -315,6 +315,8 @@ void kv_blocks_lists_launch(const SeqTable& sq, const KvPages& pg, const int32_t
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // K7: 16-bit queries over 16-bit or coded pages, 8 or 16 rows per item.
 bool seq_mma_supported(const SeqAttnArgs& a);
+// log2 of the keys of a tile.
+inline int seq_mma_key_shift(const SeqAttnArgs& a) { return a.pages.type == kI4 ? 7 : 6; }
 void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // K8: 16-bit queries over packed keys or pages, two tiles of up to 128 rows per
 // item (seq_tc_rows in all).

@@ -45,7 +45,6 @@
 namespace attnb {
 namespace {
 
-constexpr int kKeys = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr float kRhoGap = 8.f;
@@ -54,21 +53,30 @@ constexpr float kNoRho = -1e30f;  // no weight so far: any exponent is above it
 // NR: query rows / 8.
 template <int TK, int DHP, int NR>
 struct MmaCfg {
-  static constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  static constexpr bool CODED = elem_coded(TK), I4 = TK == kI4;
   static constexpr int ROWS = 8 * NR;
   static constexpr int CTAS = NR == 1 ? 3 : 2;         // per SM
-  static constexpr int CHUNKS = CODED ? 1 : DHP / 64;  // 128-byte pieces of a row
-  static constexpr int CHUNK = kKeys * 128;
+  static constexpr int KEYS = I4 ? 128 : 64;           // of a tile
+  static constexpr int HALVES = KEYS / (16 * kWarps);  // 16 keys each, of a warp
+  static constexpr int ROWB = I4 ? DHP / 2 : 128;      // bytes of a row in a tile
+  static constexpr int CHUNKS = CODED ? 1 : DHP / 64;  // such pieces of a row
+  static constexpr int CHUNK = KEYS * ROWB;
   static constexpr int TILE = CHUNKS * CHUNK;          // K or V
-  static constexpr int STAGE = 2 * TILE + (CODED ? 1024 : 0);
+  // Behind them the scales of K and V, and I4's factors.
+  static constexpr int STAGE = 2 * TILE + (I4 ? KEYS * 16 : CODED ? 1024 : 0);
   // Together the CTAs of an SM have about 190 KB of copies in flight.
-  static constexpr int STAGES = CODED ? (NR == 1 ? 3 : 5)
-                                      : (DHP == 128 ? (NR == 1 ? 2 : 3) : (NR == 1 ? 4 : 6));
+  static constexpr int STAGES = I4 ? (DHP == 128 ? 3 : 5) + (NR == 1 ? 0 : 2)
+                                : CODED ? (NR == 1 ? 3 : 5)
+                                : (DHP == 128 ? (NR == 1 ? 2 : 3) : (NR == 1 ? 4 : 6));
+  // I4, of a warp's 32 keys: factor times K scale by key and group, factors of V in f16 by
+  // group and pair of keys, logarithms of V scales.
+  static constexpr int PREP_V = 32 * 16, PREP_L = PREP_V + 4 * 16 * 16, PREP = PREP_L + 32 * 4;
   // Exchange at the end of a piece: 32 dimensions of 4 warps' rows.
   static constexpr int XROW = 36;
   static constexpr int OFF_X = STAGES * STAGE;
   static constexpr int OFF_POISON = OFF_X + kWarps * ROWS * XROW * 4;
-  static constexpr int SMEM = OFF_POISON + 3 * DHP * 4 + 1024;
+  static constexpr int OFF_PREP = OFF_POISON + 3 * DHP * 4;
+  static constexpr int SMEM = OFF_PREP + (I4 ? kWarps * PREP : 0) + 1024;
   static_assert(SMEM + 2048 <= 227 * 1024 / CTAS, "CTAs per SM");
 };
 
@@ -115,7 +123,8 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
                    const __grid_constant__ SeqAttnArgs a) {
   using Cfg = MmaCfg<TK, DHP, NR>;
   using EQ = elem_t<TQ>;
-  constexpr bool CODED = Cfg::CODED;
+  constexpr bool CODED = Cfg::CODED, I4 = Cfg::I4;
+  constexpr int kKeys = Cfg::KEYS, NH = Cfg::HALVES;
   constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
   constexpr int ST = Cfg::STAGES;
   constexpr int ROWS = Cfg::ROWS;
@@ -179,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           page[i] = win.get(a, w.b, at >> shift, used);
           if constexpr (CODED) {
             if (page[i] < a.pages.num_pages) {
-              bytes += 2 * box * 4;
+              bytes += (I4 ? 4 : 2) * box * 4;
             } else if (lane < 2) {  // no such page: codes 0 with a scale of 0
               float* sc = reinterpret_cast<float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
               for (int k = 0; k < box; ++k) sc[lane * kKeys + i * box + k] = 0.f;
@@ -190,7 +199,29 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
         __syncwarp();
-        if (lane < 2) {  // lane 0: K, lane 1: V
+        if constexpr (I4) {  // up to eight pages: K, V, both scales, both factors by lanes of their own
+          const int i = lane & 7, part = lane >> 3;
+          int mine = page[0];
+#pragma unroll
+          for (int k = 1; k < kKeys / 16; ++k)
+            if (k == i) mine = page[k];
+          if (i < copies) {
+            const int in_page = (j * kKeys + i * box) & ((1 << shift) - 1);
+            const int64_t at = (((int64_t)mine * a.pages.H + w.h) << shift) + in_page;
+            const uint32_t side = st + 2 * Cfg::TILE + i * box * 4;
+            if (part < 2) {
+              tma_load_4d(st + part * Cfg::TILE + i * box * Cfg::ROWB, part ? &tmV : &tmK, bar, 0,
+                          in_page, w.h, mine);
+            } else if (mine < a.pages.num_pages) {
+              const bool scales = part == 2;
+              const void* kp = scales ? (const void*)(a.pages.k_scale + at) : a.pages.k_group + at * 4;
+              const void* vp = scales ? (const void*)(a.pages.v_scale + at) : a.pages.v_group + at * 4;
+              const uint32_t to = side + (scales ? 0 : 8 * kKeys);
+              bulk_load(to, kp, box * 4, bar);
+              bulk_load(to + 4 * kKeys, vp, box * 4, bar);
+            }
+          }
+        } else if (lane < 2) {  // lane 0: K, lane 1: V
           const CUtensorMap* map = lane ? &tmV : &tmK;
           const float* sc = lane ? a.pages.v_scale : a.pages.k_scale;
 #pragma unroll
@@ -228,7 +259,11 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     // Q^T as B fragments: row 8 r + g, by step of 16 dimensions.  16-bit keys:
     // dimensions 2c, 2c+1 and 2c+8, 2c+9 of the step; codes: 4c .. 4c+3, as a
     // 4-byte unit of ldmatrix holds them.
+    // 4-bit codes: eight dimensions of every 32 as a 4-byte unit holds them, 8c + (0, 4),
+    // (1, 5), (2, 6), (3, 7), and every second of these pairs over 16, since its codes come
+    // out of the word times 16.
     uint32_t q[NR][KS][2];
+    float off[NR][I4 ? KS / 2 : 1][2];  // 4-bit codes: -8 sum of q over a group
     float mulq[NR][2];  // score to exponent, of this thread's rows 8 r + 2c, + 1
     int seen[NR][2];
 #pragma unroll
@@ -237,7 +272,43 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
       const bool there = 8 * r + g < w.rows;
       const EQ* p = static_cast<const EQ*>(a.q.data) + (int64_t)(w.s.q0 + row / a.G) * a.q.sT +
                     (int64_t)(w.h * a.G + row % a.G) * a.q.sH;
-      if constexpr (CODED) {
+      if constexpr (I4) {
+        float x[KS / 2][8], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS / 2; ++k) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+          if (there && k * 32 < a.q.Dh) {  // Dh is a multiple of 32
+            load4(p + k * 32 + 8 * c, *reinterpret_cast<float(*)[4]>(x[k]));
+            load4(p + k * 32 + 8 * c + 4, *reinterpret_cast<float(*)[4]>(x[k] + 4));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[k][e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float f = 256.f * row_scale(top);  // room below for the sixteenths
+#pragma unroll
+        for (int k = 0; k < KS / 2; ++k) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float over = i & 1 ? 0.0625f : 1.f;
+            const uint32_t two = pack_f16(x[k][i] * f * over, x[k][i + 4] * f * over);
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&two));
+            sum += (y.x + y.y) * (i & 1 ? 16.f : 1.f);
+            q[r][2 * k + (i >> 1)][i & 1] = two;
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            off[r][k][i] = -0x1p-21f * __shfl_sync(0xffffffffu, sum, (2 * c + i) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          mulq[r][i] = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, f, (2 * c + i) * 4);
+      } else if constexpr (CODED) {
         float x[KS][4], top = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
@@ -293,17 +364,75 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
       if (ok) ok = mbar_wait_quick(smem_addr(&full[ring.stage]), ring.phase, abort_p, a.status);
       ok = __all_sync(0xffffffffu, ok);
       const uint32_t st = base + ring.stage * Cfg::STAGE;
-      const int key0 = j * kKeys + warp * 16;
-      const bool masked = key0 + 16 > seen_min;  // warp-uniform
+      const int key0 = j * kKeys + warp * (16 * NH);
+      const bool masked = key0 + 16 * NH > seen_min;  // warp-uniform
       if (ok && key0 < w.s.L) {
-        // ---- S^T = K Q^T: keys g, g + 8 by rows 2c, 2c + 1
-        float s[NR][4];
+        // ---- S^T = K Q^T: keys g, g + 8 (of each 16) by rows 2c, 2c + 1
+        float s[NH][NR][4];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
-        const int kr = warp * 16 + (lane & 15);  // this lane's matrix row
-        if constexpr (CODED) {
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[hf][r][e] = 0.f;
+        const int kr = warp * (16 * NH) + (lane & 15);  // this lane's matrix row
+        uint8_t* const prep = mem + Cfg::OFF_PREP + warp * Cfg::PREP;
+        if constexpr (I4) {
+          // What the warp's 32 keys are multiplied by, a key a lane, once for all lanes.
+          const uint8_t* side = mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE;
+          const int key = warp * 32 + lane;
+          const float* scales = reinterpret_cast<const float*>(side);
+          const uint32_t* factors = reinterpret_cast<const uint32_t*>(side + 8 * kKeys);
+          const uint32_t kf = factors[key];
+          const float ks = scales[key];
+          // (2^23 + r has r as its last bits)
+          auto times = [&](int i) {
+            return (__uint_as_float(__byte_perm(kf, 0x4b000000u, 0x7540 + i)) - 8388608.f) * ks;
+          };
+          reinterpret_cast<float4*>(prep)[lane] =
+              make_float4(times(0), times(1), times(2), times(3));
+          reinterpret_cast<float*>(prep + Cfg::PREP_L)[lane] = __log2f(scales[kKeys + key]);
+          const uint2 vf = *reinterpret_cast<const uint2*>(factors + kKeys + (key & ~31) + (lane >> 1) * 2);
+          // groups 0 and 1, or 2 and 3, of both keys
+          const uint32_t two = __byte_perm(vf.x, vf.y, lane & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const I4Factors f = i4_factors(i ? two >> 8 : two);
+            reinterpret_cast<uint4*>(prep + Cfg::PREP_V)[((lane & 1) * 2 + i) * 16 + (lane >> 1)] =
+                make_uint4(f.low, f.high, f.add, 0u);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int hf = 0; hf < NH; ++hf) {
+            float fk[2][4];  // of keys g, g + 8, by group
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<float4*>(fk[i]) =
+                  reinterpret_cast<const float4*>(prep)[hf * 16 + g + 8 * i];
+#pragma unroll
+            for (int k = 0; k < KS / 2; k += 2) {
+              uint32_t b[4];
+              ldsm4(st + sw_rows<Cfg::ROWB>(kr + hf * 16, k + (lane >> 4)), b);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t x = b[2 * e], y = b[2 * e + 1], x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                  // The codes as they are, 1 to 15: their sum starts at that of -8 q.
+                  const float* o = off[r][k + e];
+                  float t[4] = {o[0], o[1], o[0], o[1]};
+                  mma16816<false>(t, x & kI4Low, y & kI4Low, x & kI4High, y & kI4High,
+                                  q[r][2 * (k + e)][0], q[r][2 * (k + e)][1]);
+                  mma16816<false>(t, x8 & kI4Low, y8 & kI4Low, x8 & kI4High, y8 & kI4High,
+                                  q[r][2 * (k + e) + 1][0], q[r][2 * (k + e) + 1][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    s[hf][r][i] = fmaf(t[i], fk[i >> 1][k + e], s[hf][r][i]);
+                }
+              }
+            }
+          }
+        } else if constexpr (CODED) {
 #pragma unroll
           for (int k = 0; k < KS; k += 2) {
             uint32_t b[4];
@@ -315,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
               codes_to_f16<TK>(b[2 * e + 1], a1, a3);
 #pragma unroll
               for (int r = 0; r < NR; ++r)
-                mma16816<false>(s[r], a0, a1, a2, a3, q[r][k + e][0], q[r][k + e][1]);
+                mma16816<false>(s[0][r], a0, a1, a2, a3, q[r][k + e][0], q[r][k + e][1]);
             }
           }
         } else {
@@ -325,12 +454,16 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
             ldsm4(st + (k >> 2) * Cfg::CHUNK + sw128(kr, (k & 3) * 2 + (lane >> 4)), b);
 #pragma unroll
             for (int r = 0; r < NR; ++r)
-              mma16816<BF16>(s[r], b[0], b[1], b[2], b[3], q[r][k][0], q[r][k][1]);
+              mma16816<BF16>(s[0][r], b[0], b[1], b[2], b[3], q[r][k][0], q[r][k][1]);
           }
         }
         // ---- weights
-        float mulk[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};  // of keys g, g + 8
-        if constexpr (CODED) {
+        float mulk[2] = {1.f, 1.f}, lv[2 * NH] = {};  // of keys g, g + 8 (of each 16)
+        if constexpr (I4) {
+#pragma unroll
+          for (int i = 0; i < 2 * NH; ++i)
+            lv[i] = reinterpret_cast<const float*>(prep + Cfg::PREP_L)[g + 8 * i];
+        } else if constexpr (CODED) {
           const float* sc =
               reinterpret_cast<const float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
 #pragma unroll
@@ -340,20 +473,26 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
             lv[i] = __log2f(sc[kKeys + at]);  // -inf for a vector of zeros
           }
         }
-        uint32_t p[NR][2];
+        uint32_t p[NH][NR][2];
         bool moved = false;
         float alpha[NR][2];  // what acc is multiplied by
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (CODED) s[r][e] *= mulq[r][e & 1] * mulk[e >> 1];
-            else s[r][e] *= mulq[r][e & 1];
-            if (masked && key0 + g + 8 * (e >> 1) >= seen[r][e & 1]) s[r][e] = -INFINITY;
-          }
+          for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (CODED && !I4) s[hf][r][e] *= mulq[r][e & 1] * mulk[e >> 1];
+              else s[hf][r][e] *= mulq[r][e & 1];
+              if (masked && key0 + hf * 16 + g + 8 * (e >> 1) >= seen[r][e & 1])
+                s[hf][r][e] = -INFINITY;
+            }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(s[r][i], s[r][i + 2]);
+            float top = fmaxf(s[0][r][i], s[0][r][i + 2]);
+#pragma unroll
+            for (int hf = 1; hf < NH; ++hf)
+              top = fmaxf(top, fmaxf(s[hf][r][i], s[hf][r][i + 2]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -369,16 +508,17 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
             m[r][i] = top;
             l[r][i] *= beta;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float x = s[r][i + 2 * k] - use;
+            for (int k = 0; k < 2 * NH; ++k) {
+              float& at = s[k >> 1][r][i + 2 * (k & 1)];
+              const float x = at - use;
               const float weight = fast_exp2(x);
               l[r][i] += weight;
               if constexpr (CODED) {
                 // The scale of a masked key may be anything.
-                s[r][i + 2 * k] = x == -INFINITY ? x : x + lv[k];
-                moved |= s[r][i + 2 * k] - rho[r][i] > kRhoGap;
+                at = x == -INFINITY ? x : x + lv[k];
+                moved |= at - rho[r][i] > kRhoGap;
               } else {
-                s[r][i + 2 * k] = weight;
+                at = weight;
               }
             }
           }
@@ -390,7 +530,10 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
             for (int r = 0; r < NR; ++r)
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                float top = fmaxf(s[r][i], s[r][i + 2]);
+                float top = fmaxf(s[0][r][i], s[0][r][i + 2]);
+#pragma unroll
+                for (int hf = 1; hf < NH; ++hf)
+                  top = fmaxf(top, fmaxf(s[hf][r][i], s[hf][r][i + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -400,16 +543,20 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
               }
           }
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
+          for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[r][e] = fast_exp2(s[r][e] - rho[r][e & 1]);
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[hf][r][e] = fast_exp2(s[hf][r][e] - rho[r][e & 1]);
         }
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            p[r][k] = transposed(BF16 ? pack_bf16(s[r][2 * k], s[r][2 * k + 1])
-                                      : pack_f16(s[r][2 * k], s[r][2 * k + 1]));
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              p[hf][r][k] = transposed(BF16 ? pack_bf16(s[hf][r][2 * k], s[hf][r][2 * k + 1])
+                                            : pack_f16(s[hf][r][2 * k], s[hf][r][2 * k + 1]));
         if (moved) {
 #pragma unroll
           for (int u = 0; u < KS; ++u)
@@ -418,8 +565,8 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[u][r][e] *= alpha[r][e & 1];
         }
-        // ---- values that a mask hides (written codes are finite)
-        if (CODED ? key0 + 16 > w.s.L : masked) {
+        // ---- values that a mask hides (written codes are finite, 4 bits always)
+        if (!I4 && (CODED ? key0 + 16 > w.s.L : masked)) {
           uint8_t* v = mem + ring.stage * Cfg::STAGE + Cfg::TILE;
           for (int i = lane; i < 16 * Cfg::CHUNKS * 8; i += 32) {
             const int r = i & 15, u = (i >> 4) & 7, ch = i >> 7;
@@ -447,7 +594,35 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           __syncwarp();
         }
         // ---- O^T += V^T P^T, 16 dimensions at a time
-        if constexpr (CODED) {
+        if constexpr (I4) {
+          const uint4* fv = reinterpret_cast<const uint4*>(prep + Cfg::PREP_V);
+#pragma unroll
+          for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+            for (int u = 0; u < KS / 2; u += 2) {
+              uint32_t b[4];
+              ldsm4_t(st + Cfg::TILE + sw_rows<Cfg::ROWB>(kr + hf * 16, u + (lane >> 4)), b);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                // keys 2c, 2c + 1 (and 8 more) in the halves, dimensions 4g .. 4g + 3 in a half
+                const uint32_t x = b[2 * e], y = b[2 * e + 1], x8 = x >> 8, y8 = y >> 8;
+                const uint4 fx = fv[(u + e) * 16 + hf * 8 + c], fy = fv[(u + e) * 16 + hf * 8 + c + 4];
+                const uint32_t x0 = fma_f16x2(x & kI4Low, fx.x, fx.z);
+                const uint32_t x1 = fma_f16x2(x & kI4High, fx.y, fx.z);
+                const uint32_t x2 = fma_f16x2(x8 & kI4Low, fx.x, fx.z);
+                const uint32_t x3 = fma_f16x2(x8 & kI4High, fx.y, fx.z);
+                const uint32_t y0 = fma_f16x2(y & kI4Low, fy.x, fy.z);
+                const uint32_t y1 = fma_f16x2(y & kI4High, fy.y, fy.z);
+                const uint32_t y2 = fma_f16x2(y8 & kI4Low, fy.x, fy.z);
+                const uint32_t y3 = fma_f16x2(y8 & kI4High, fy.y, fy.z);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                  mma16816<false>(acc[2 * (u + e)][r], x0, x1, y0, y1, p[hf][r][0], p[hf][r][1]);
+                  mma16816<false>(acc[2 * (u + e) + 1][r], x2, x3, y2, y3, p[hf][r][0], p[hf][r][1]);
+                }
+              }
+            }
+        } else if constexpr (CODED) {
 #pragma unroll
           for (int u = 0; u < KS; u += 2) {
             uint32_t b[4];
@@ -461,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
               codes_to_f16<TK>(__byte_perm(b[2 * e + 1], 0, 0x3120), a2, a3);
 #pragma unroll
               for (int r = 0; r < NR; ++r)
-                mma16816<false>(acc[u + e][r], a0, a1, a2, a3, p[r][0], p[r][1]);
+                mma16816<false>(acc[u + e][r], a0, a1, a2, a3, p[0][r][0], p[0][r][1]);
             }
           }
         } else {
@@ -473,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
                         sw128(vr, (u & 3) * 2 + ((lane >> 3) & 1)), b);
 #pragma unroll
             for (int r = 0; r < NR; ++r)
-              mma16816<BF16>(acc[u][r], b[0], b[1], b[2], b[3], p[r][0], p[r][1]);
+              mma16816<BF16>(acc[u][r], b[0], b[1], b[2], b[3], p[0][r][0], p[0][r][1]);
           }
         }
       }
@@ -507,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         for (int k = 0; k < kWarps; ++k)
           total += fast_exp2(sm_ml[k][rr].x - use) * sm_ml[k][rr].y;
         fr[r][i] = CODED ? fast_exp2(0.5f * (m[r][i] - use + rho[r][i])) : 1.f;
-        f[r][i] = CODED ? fr[r][i] : fast_exp2(m[r][i] - use);
+        f[r][i] = I4 ? fr[r][i] * kI4Unit : CODED ? fr[r][i] : fast_exp2(m[r][i] - use);
         if (slot < 0) f[r][i] = total == 0.f ? 0.f : f[r][i] / total;
         else if (warp == 0 && g == 0 && rr < w.rows)
           reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * ROWS + rr] = make_float2(top, total);
@@ -521,7 +696,8 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         for (int r = 0; r < NR; ++r)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int d = t * 16 + (CODED ? 2 * g + (e >> 1) : g + 8 * (e >> 1));
+            const int d = I4 ? 4 * g + 2 * t + (e >> 1)
+                             : t * 16 + (CODED ? 2 * g + (e >> 1) : g + 8 * (e >> 1));
             x[(warp * ROWS + 8 * r + 2 * c + (e & 1)) * Cfg::XROW + d] =
                 (CODED ? acc[q4 * 2 + t][r][e] * fr[r][e & 1] : acc[q4 * 2 + t][r][e]) * f[r][e & 1];
           }
@@ -573,19 +749,21 @@ void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensor
 
 bool seq_pages_tma(const SeqAttnArgs& a) {
   const KvPages& p = a.pages;
-  if (p.type == kI4) return false;
   if (!p.k || p.num_pages == 0 || a.q.type == kF32 || p.Dh > 128) return false;
-  if ((p.Dh * elem_bytes(p.type)) % 16 != 0) return false;
+  if (vector_bytes(p.type, p.Dh) % 16 != 0) return false;
   auto at16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   if (!at16(p.k) || !at16(p.v)) return false;
+  if (p.type == kI4 && !(at16(p.k_group) && at16(p.v_group))) return false;
   return !elem_coded(p.type) || (at16(p.k_scale) && at16(p.v_scale));
 }
 
 CUtensorMap seq_pages_map(const KvPages& p, const void* base, int rows) {
   const uint64_t eb = elem_bytes(p.type), page = 1u << p.page_shift;
-  const uint64_t dims[4] = {(uint64_t)p.Dh, page, (uint64_t)p.H, (uint64_t)p.num_pages};
-  const uint64_t strides[3] = {p.Dh * eb, p.Dh * page * eb, p.Dh * page * p.H * eb};
-  const uint32_t box[4] = {(uint32_t)(128 / eb), (uint32_t)std::min<uint64_t>(page, rows), 1, 1};
+  const uint64_t row = vector_bytes(p.type, p.Dh);
+  const uint64_t dims[4] = {row / eb, page, (uint64_t)p.H, (uint64_t)p.num_pages};
+  const uint64_t strides[3] = {row, row * page, row * page * p.H};
+  const uint32_t wide = p.type == kI4 ? (p.Dh <= 64 ? 32 : 64) : 128 / eb;
+  const uint32_t box[4] = {wide, (uint32_t)std::min<uint64_t>(page, rows), 1, 1};
   return make_tmap_nd(base, (int)eb, 4, dims, strides, box);
 }
 
@@ -597,8 +775,9 @@ bool seq_mma_supported(const SeqAttnArgs& a) {
 }
 
 void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
-  const CUtensorMap k = seq_pages_map(a.pages, a.pages.k, kKeys);
-  const CUtensorMap v = seq_pages_map(a.pages, a.pages.v, kKeys);
+  const int keys = 1 << a.kt_shift;
+  const CUtensorMap k = seq_pages_map(a.pages, a.pages.k, keys);
+  const CUtensorMap v = seq_pages_map(a.pages, a.pages.v, keys);
   auto go = [&](auto tq, auto tk) {
     constexpr int TQ = decltype(tq)::value, TK = decltype(tk)::value;
     if constexpr (TQ != kF32) {
@@ -614,6 +793,7 @@ void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   with_value_type(a.q.type, [&](auto tq) {
     if (a.pages.type == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});
     else if (a.pages.type == kI8) go(tq, std::integral_constant<int, kI8>{});
+    else if (a.pages.type == kI4) go(tq, std::integral_constant<int, kI4>{});
     else go(tq, tq);
   });
 }

@@ -39,6 +39,40 @@ __device__ __forceinline__ uint32_t sw128(int r, int u) {
   return (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
 }
 
+// The same for rows of 64 bytes with the 64-byte swizzle and of 32 bytes with the
+// 32-byte one (tile base 512-byte aligned): eight rows at one unit lie in
+// different banks.
+template <int ROW>
+__device__ __forceinline__ uint32_t sw_rows(int r, int u) {
+  if constexpr (ROW == 128) return sw128(r, u);
+  else if constexpr (ROW == 64) return (uint32_t)(r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+  else return (uint32_t)(r * 32 + ((u ^ ((r >> 2) & 1)) << 4));
+}
+
+// a * b + c of two pairs of f16.
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// 4-bit codes in f16.  Two codes masked out of a word are the subnormals
+// code * 2^-24 (mask 000f000f) or 16 code * 2^-24 (00f000f0); with their factors r,
+//     (code * 2^-24) * (r * 2^5) - r * 2^-16 = r * (code - 8) * 2^-19,
+// exact: a multiple of 2^-19 below 2^-8, in one FMA of two.
+constexpr uint32_t kI4Low = 0x000f000fu, kI4High = 0x00f000f0u;
+constexpr float kI4Unit = 0x1p19f;  // what such values are to be multiplied by
+struct I4Factors {
+  uint32_t low, high, add;  // pairs of f16: r 2^5, r 2^1, -r 2^-16
+};
+// From two factors in bits 0-7 and 16-23.
+__device__ __forceinline__ I4Factors i4_factors(uint32_t r) {
+  const uint32_t x = (r & 0x00ff00ffu) | 0x64006400u;  // 1024 + r
+  return {fma_f16x2(x, 0x50005000u, 0xf800f800u),       // 2^5, -2^15
+          fma_f16x2(x, 0x40004000u, 0xe800e800u),       // 2^1, -2^11
+          fma_f16x2(x, 0x81008100u, 0x24002400u)};      // -2^-16, 2^-6
+}
+
 // Four codes to two pairs of f16, exactly.
 template <int T>
 __device__ __forceinline__ void codes_to_f16(uint32_t four, uint32_t& lo, uint32_t& hi) {

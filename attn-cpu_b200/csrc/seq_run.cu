@@ -141,7 +141,7 @@ static void run(SeqAttnArgs a, Kind kind, int64_t rows, uintptr_t ws, uintptr_t 
                    : kind == kTf32 ? tf32_space(num_sms)
                                    : simt_space(a.q.Dh, rows, num_sms);
   a.rows = sp.rows;
-  a.kt_shift = kind == kTc ? 7 : kind == kTf32 ? 5 : 6;
+  a.kt_shift = kind == kTc ? 7 : kind == kTf32 ? 5 : kind == kMma ? seq_mma_key_shift(a) : 6;
   a.min_tiles = 2;
   a.extra = kind == kTc || kind == kTf32 ? 2 : 1;
   uintptr_t p = (ws + 255) & ~(uintptr_t)255;
@@ -204,7 +204,8 @@ void seq_attn_blocks_run(SeqAttnArgs a, const int32_t* blocks, int take, void* w
   // K6 or K7 take any number of rows; a token has few.
   const Kind kind = seq_mma_supported(a) ? kMma : kSimt;
   a.sel_heads = a.pages.H;
-  a.sel_tiles = (int)((((int64_t)take << a.pages.page_shift) + 63) >> 6);
+  const int kt = kind == kMma ? seq_mma_key_shift(a) : 6;
+  a.sel_tiles = (int)((((int64_t)take << a.pages.page_shift) + (1 << kt) - 1) >> kt);
   a.causal = 0;  // the lengths are the token's own
   a.seqs = SeqTable{nullptr, (int)rows, a.seqs.total, pages, take, take, lens};
   run(a, kind, a.G, p, end, num_sms, s);

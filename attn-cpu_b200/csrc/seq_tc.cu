@@ -1128,6 +1128,7 @@ CUtensorMap rows_map(const RowsView& r, int heads, int tokens) {
 }  // namespace
 
 bool seq_tc_supported(const SeqAttnArgs& a) {
+  if (a.pages.k && a.pages.type == kI4) return false;
   if (a.q.type == kF32 || a.G > BM || a.q.Dh > 128 || a.q.Dh % 8 != 0) return false;
   if (a.pages.k) return seq_pages_tma(a);
   return map_allowed(a.k) && map_allowed(a.v);

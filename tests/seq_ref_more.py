@@ -61,3 +61,25 @@ def select(score, take, first, last):
         return list(range(n))
     inner = torch.sort(score[first:n - last], descending=True, stable=True)[1] + first
     return sorted(list(range(first)) + inner[: take - first - last].tolist() + list(range(n - last, n)))
+
+
+def weight_floor(q, ks, vs, new, causal=True, scale=None):
+    """What subnormal weights add to attention_bound, [tokens, heads, 1].  Over codes the kernels round
+    a weight to f16 relative to 2^rho <= max_j p_j scale_j, which is absolute below 2^-14: by at most 2^-25.  The
+    codes (times their factors) are at most max |v_j| / scale_j, so that L keys are off by at most
+    2^-25 L max_j p_j max |v_j|."""
+    heads, D = q.shape[1:]
+    out = torch.zeros(q.shape[0], heads, 1, dtype=torch.float64)
+    first = 0
+    for n, k, v in zip(new, ks, vs):
+        L, H = k.shape[:2]
+        if n and L:
+            qq = q[first:first + n].double().cpu().permute(1, 0, 2)
+            kk, vv = (x.double().cpu().permute(1, 2, 0).repeat_interleave(heads // H, 0) for x in (k, v))
+            s = (qq @ kk) * (D ** -0.5 if scale is None else scale)
+            if causal:
+                s = s.masked_fill(~torch.ones(n, L, dtype=torch.bool).tril(L - n), -torch.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0)
+            out[first:first + n, :, 0] = (p * vv.abs().amax(1)[:, None]).amax(-1).T * (2.0 ** -25 * L)
+        first += n
+    return out

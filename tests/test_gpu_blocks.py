@@ -130,6 +130,7 @@ def _attended(p, q, blocks, new, keys, dtype, scale=None):
     capi.attn_blocks_dev(q, p.k, p.v, o, blocks, *p.where(new), scale, **p.kw)
     G, D = q.shape[1] // p.H, q.shape[2]
     ref, mag = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    floor = torch.zeros(*q.shape[:2], 1, dtype=torch.float64)
     ks, vs = ([_values(p, x, b, n) for b, n in enumerate(keys)] for x in ("k", "v"))
     t = 0
     for b, (n, L) in enumerate(zip(new, keys)):
@@ -138,11 +139,14 @@ def _attended(p, q, blocks, new, keys, dtype, scale=None):
             for h in range(p.H):
                 mine = [j for j in blocks[t, h].tolist() if j >= 0]
                 at = [x for j in mine for x in range(j * p.page, (j + 1) * p.page) if x <= pos]
-                r, m = seq_ref.attention(q[t:t + 1, h * G:(h + 1) * G], [ks[b][at][:, h:h + 1]], [vs[b][at][:, h:h + 1]], [1], scale=scale)
+                one = q[t:t + 1, h * G:(h + 1) * G], [ks[b][at][:, h:h + 1]], [vs[b][at][:, h:h + 1]], [1]
+                r, m = seq_ref.attention(*one, scale=scale)
                 ref[t, h * G:(h + 1) * G], mag[t, h * G:(h + 1) * G] = r[0], m[0]
+                if p.kind != dtype and dtype != F32:
+                    floor[t, h * G:(h + 1) * G] = more.weight_floor(*one, scale=scale)[0]
             t += 1
     smax = float(q.double().norm(dim=-1).max().cpu() * max(k.norm(dim=-1).max() for k in ks if len(k))) * (D ** -0.5 if scale is None else scale)
-    _check(o[:t], ref[:t], mag[:t], dtype, smax, p.kind != dtype, blocks.shape[2] * p.page)
+    _check(o[:t], ref[:t], mag[:t], dtype, smax, p.kind != dtype, blocks.shape[2] * p.page, floor[:t])
     return o
 
 

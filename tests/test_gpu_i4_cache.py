@@ -104,7 +104,8 @@ def _against(p, q, new, keys, dtype, most=0, causal=True, scale=None):
     D = q.shape[-1]
     smax = float(q.double().norm(dim=-1).max().cpu() * max(k.norm(dim=-1).max() for k in ks if len(k)))
     smax *= D ** -0.5 if scale is None else scale
-    _check(_attend(p, q, new, most, causal, scale), ref, mag, dtype, smax, True, max(keys))
+    floor = 0.0 if dtype == F32 else more.weight_floor(q, ks, vs, new, causal, scale)
+    _check(_attend(p, q, new, most, causal, scale), ref, mag, dtype, smax, True, max(keys), floor)
     capi.stream_status()
 
 
@@ -171,7 +172,8 @@ def test_stale_pages_stay_out(cuda, dtype, new):
     q = _randn(_gen(4), 2 * new, 4, 64, dtype=dtype)
     ref, mag = seq_ref.attention(q, ks, vs, count)
     smax = float(q.double().norm(dim=-1).max().cpu() * max(k.norm(dim=-1).max() for k in ks)) / 8
-    _check(_attend(p, q, count, new), ref, mag, dtype, smax, True, 333)
+    floor = 0.0 if dtype == F32 else more.weight_floor(q, ks, vs, count)
+    _check(_attend(p, q, count, new), ref, mag, dtype, smax, True, 333, floor)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -201,7 +203,8 @@ def test_bad_pages(cuda):
         q = _randn(_gen(4), 2 * new, 4, 64, dtype=BF16)
         ref, mag = seq_ref.attention(q, ks, vs, [new, new])
         smax = float(q.double().norm(dim=-1).max().cpu() * max(k.norm(dim=-1).max() for k in ks)) / 8
-        _check(_attend(p, q, [new, new], new), ref, mag, BF16, smax, True, 300)
+        _check(_attend(p, q, [new, new], new), ref, mag, BF16, smax, True, 300,
+               more.weight_floor(q, ks, vs, [new, new]))
         with pytest.raises(capi.AttnbError, match="out of range"):
             capi.stream_status()
 
@@ -230,7 +233,7 @@ def test_cache_object(cuda):
             vs.append(pair[1])
         ref, mag = seq_ref.attention(turned, ks, vs, new)
         smax = float(turned.double().norm(dim=-1).max() * max(k.double().norm(dim=-1).max() for k in ks)) * D ** -0.5
-        _check(o, ref, mag, BF16, smax, True, 200)
+        _check(o, ref, mag, BF16, smax, True, 200, more.weight_floor(turned, ks, vs, new))
         # what was appended is there, a code's step off at most
         for b, x in enumerate(_split(v, new)):
             held[2 + b] = torch.cat([held[2 + b], x])
