@@ -224,28 +224,10 @@ __device__ __forceinline__ void turn_angles(const Rope& rope, const int64_t* pos
   }
 }
 
-// The lane's cos and sin for one token, the sign of the sine with the element's side of its
-// pair.  Elements that stay have 1 and 0.
-__device__ __forceinline__ void lane_turns(const Rope& rope, const float2* turns, int d,
-                                           float (&co)[8], float (&si)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int x = d + j;
-    const bool second = rope.interleaved ? (x & 1) : x >= rope.pairs;
-    const int p = rope.interleaved ? x >> 1 : second ? x - rope.pairs : x;
-    const bool turned = x < 2 * rope.pairs;
-    const float2 cs = turned ? turns[p] : make_float2(1.f, 0.f);
-    co[j] = cs.x;
-    si[j] = second ? cs.y : -cs.y;
-  }
-}
-
-// The lane's eight elements of the row at p, turned.  All lanes of the row call, and
-// none has stored before all have read (rows may be turned in place).
+// The lane's eight elements of the row at p, turned; turns: its token's.
 template <class E>
 __device__ __forceinline__ Eight<E> turned8(const E* p, const Eight<E>& raw, const Rope& rope, int d,
-                                            int Dh, bool vec, const float (&co)[8],
-                                            const float (&si)[8]) {
+                                            int Dh, bool vec, const float2* turns) {
   Eight<E> other = raw;
   const int half = rope.pairs;
   if (!rope.interleaved && d < 2 * half) {
@@ -260,67 +242,227 @@ __device__ __forceinline__ Eight<E> turned8(const E* p, const Eight<E>& raw, con
     }
   }
   Eight<E> out = raw;
+  if (half % 8 == 0 && d < 2 * half) {  // all eight turn, and their angles lie together
+    const bool second = !rope.interleaved && d >= half;
+    float2 cs[8];
+    const float4* four = reinterpret_cast<const float4*>(
+        turns + (rope.interleaved ? d / 2 : second ? d - half : d));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!rope.interleaved || j < 2) {
+        const float4 c = four[j];
+        cs[2 * j] = make_float2(c.x, c.y);
+        cs[2 * j + 1] = make_float2(c.z, c.w);
+      }
+    }
+    if (rope.interleaved) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = to_float(raw.e[2 * j]), b = to_float(raw.e[2 * j + 1]);
+        from_float(fmaf(a, cs[j].x, -(b * cs[j].y)), out.e[2 * j]);
+        from_float(fmaf(b, cs[j].x, a * cs[j].y), out.e[2 * j + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = to_float(other.e[j]) * cs[j].y;
+        from_float(fmaf(to_float(raw.e[j]), cs[j].x, second ? y : -y), out.e[j]);
+      }
+    }
+    return out;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    if (d + j >= 2 * half) continue;
-    const float y = to_float(rope.interleaved ? raw.e[j ^ 1] : other.e[j]);
-    from_float(fmaf(to_float(raw.e[j]), co[j], y * si[j]), out.e[j]);
+    const int x = d + j;
+    if (x >= 2 * half) continue;
+    const bool second = rope.interleaved ? (j & 1) : x >= half;
+    const float2 cs = turns[rope.interleaved ? x >> 1 : second ? x - half : x];
+    const float near = to_float(raw.e[j ^ 1]), far = to_float(other.e[j]);
+    const float y = rope.interleaved ? near : far;
+    from_float(fmaf(to_float(raw.e[j]), cs.x, second ? y * cs.y : -(y * cs.y)), out.e[j]);
   }
   return out;
+}
+
+// Four elements as they lie in memory, and as floats; rounded once on the way back.
+template <int T>
+struct Four {
+  using Raw = std::conditional_t<T == kF32, float4, uint2>;
+  Raw raw;
+  __device__ __forceinline__ void load(const elem_t<T>* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void store(elem_t<T>* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void get(float (&x)[4]) const {
+    if constexpr (T == kF32) {
+      x[0] = raw.x, x[1] = raw.y, x[2] = raw.z, x[3] = raw.w;
+    } else if constexpr (T == kBF16) {
+      x[0] = __uint_as_float(raw.x << 16), x[1] = __uint_as_float(raw.x & 0xffff0000u);
+      x[2] = __uint_as_float(raw.y << 16), x[3] = __uint_as_float(raw.y & 0xffff0000u);
+    } else {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+  }
+  __device__ __forceinline__ void set(float a, float b, float c, float d) {
+    if constexpr (T == kF32) raw = make_float4(a, b, c, d);
+    else if constexpr (T == kBF16) raw = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
+    else raw = make_uint2(pack_f16(a, b), pack_f16(c, d));
+  }
+};
+
+// Vectors of the CTA's n tokens, `heads` each, from src to dst as they are, or turned (pairs > 0).
+// to(tl) is where token tl's first vector goes, null for one that is left out.  The layout has
+// to allow reads of four elements (vec) and pairs that are a multiple of four: a lane takes four
+// whole pairs, or eight dimensions that stay, and so reads nothing twice.  A group of lanes
+// takes several heads of one token in turn, four of them in flight.
+template <int TX, int LANES, class To>
+__device__ __forceinline__ void move_rows(const elem_t<TX>* src, int64_t src_t, int64_t src_h, To to,
+                                          int64_t dst_h, int heads, int Dh, int pairs,
+                                          bool interleaved, const float2* turns, int turns_t,
+                                          int n) {
+  using E = elem_t<TX>;
+  constexpr int U = 4, GROUPS = kThreads / LANES;
+  const int e = threadIdx.x % LANES;
+  const bool turned = e < pairs / 4;
+  const int d = turned && !interleaved ? 4 * e : 8 * e;
+  const int d2 = turned && !interleaved ? pairs + 4 * e : d + 4;
+  if (d2 >= Dh) return;
+  // Few tokens: several groups share one.
+  const int slices = min(heads, max(1, GROUPS / n)), per = (heads + slices - 1) / slices;
+  for (int item = threadIdx.x / LANES; item < n * slices; item += GROUPS) {
+    const int tl = item / slices, h0 = (item - tl * slices) * per, h1 = min(heads, h0 + per);
+    E* o = to(tl);
+    if (!o) continue;
+    o += h0 * dst_h;
+    const E* p = src + tl * src_t + h0 * src_h;
+    float4 c0 = {}, c1 = {};
+    if (turned) {
+      const float4* cs = reinterpret_cast<const float4*>(turns + tl * turns_t) + 2 * e;
+      c0 = cs[0];
+      c1 = cs[1];
+    }
+    for (int h = h0; h < h1; h += U) {
+      Four<TX> x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u < h1) {
+          x[u].load(p + d);
+          y[u].load(p + d2);
+        }
+        p += src_h;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u < h1) {
+          if (turned) {
+            float a[4], b[4];
+            x[u].get(a);
+            y[u].get(b);
+            if (interleaved) {
+              x[u].set(fmaf(a[0], c0.x, -(a[1] * c0.y)), fmaf(a[1], c0.x, a[0] * c0.y),
+                       fmaf(a[2], c0.z, -(a[3] * c0.w)), fmaf(a[3], c0.z, a[2] * c0.w));
+              y[u].set(fmaf(b[0], c1.x, -(b[1] * c1.y)), fmaf(b[1], c1.x, b[0] * c1.y),
+                       fmaf(b[2], c1.z, -(b[3] * c1.w)), fmaf(b[3], c1.z, b[2] * c1.w));
+            } else {
+              x[u].set(fmaf(a[0], c0.x, -(b[0] * c0.y)), fmaf(a[1], c0.z, -(b[1] * c0.w)),
+                       fmaf(a[2], c1.x, -(b[2] * c1.y)), fmaf(a[3], c1.z, -(b[3] * c1.w)));
+              y[u].set(fmaf(b[0], c0.x, a[0] * c0.y), fmaf(b[1], c0.z, a[1] * c0.w),
+                       fmaf(b[2], c1.x, a[2] * c1.y), fmaf(b[3], c1.z, a[3] * c1.w));
+            }
+          }
+          x[u].store(o + d);
+          y[u].store(o + d2);
+        }
+        o += dst_h;
+      }
+    }
+  }
+}
+
+// The rows Q of the CTA's tokens, turned into QO.
+template <int TX, int LANES>
+__device__ __forceinline__ void turn_rows(const RowsView& Q, const RowsView& QO, const Rope& rope,
+                                          const int64_t* places, const float2* turns, int t0,
+                                          int n, bool vec) {
+  using E = elem_t<TX>;
+  const E* const from = static_cast<const E*>(Q.data) + (int64_t)t0 * Q.sT;
+  E* const to = static_cast<E*>(QO.data) + (int64_t)t0 * QO.sT;
+  const int e = threadIdx.x % LANES, Dh = Q.Dh;
+  if (vec && rope.pairs % 4 == 0) {
+    move_rows<TX, LANES>(
+        from, Q.sT, Q.sH, [&](int tl) { return places[tl] == -2 ? nullptr : to + tl * QO.sT; },
+        QO.sH, Q.heads, Dh, rope.pairs, rope.interleaved, turns, rope.pairs, n);
+    return;
+  }
+  const unsigned mask =
+      LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+  for (Walk at(threadIdx.x / LANES, kThreads / LANES, Q.heads); at.tl < n; at.next()) {
+    if (places[at.tl] == -2) continue;
+    const E* p = from + at.tl * Q.sT + at.kvh * Q.sH;
+    const Eight<E> raw = load8(p, 8 * e, Dh, vec);
+    const Eight<E> out = turned8(p, raw, rope, 8 * e, Dh, vec, turns + at.tl * rope.pairs);
+    __syncwarp(mask);  // a row may be turned in place: all have read
+    store8(to + at.tl * QO.sT + at.kvh * QO.sH, 8 * e, Dh, vec, out);
+  }
 }
 
 // One vector per group of LANES lanes at a time: the CTAs of an SM keep enough
 // reads going, and more registers would cost some of those (prompts of 11.7k tokens
 // to e4m3 and back: 61 us; 79 with two vectors in flight, 80 with four).
+// With ROPE the first q_ctas CTAs take Q's rows, the others K and V.
 template <int TX, int TC, int LANES, bool ROPE>
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const RowsView K, const RowsView V, const RowsView Q, const RowsView QO,
-                  const KvPages pg, const SeqTable sq, const Rope rope, const int tokens,
-                  const bool vec, int* index_status) {
+                  const KvPages pg, const SeqTable sq, const Rope rope, const int q_ctas,
+                  const int tokens, const bool vec, int* index_status) {
   using EX = elem_t<TX>;
   using EC = elem_t<TC>;
   constexpr bool CODED = elem_coded(TC);
   __shared__ int64_t places[kMaxTokens], position[ROPE ? kMaxTokens : 1];
-  extern __shared__ float2 turns[];
+  extern __shared__ __align__(16) float2 turns[];
   const int e = threadIdx.x % LANES, d = e * 8;
   const int Dh = pg.Dh;
   grid_dep_wait();
-  const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
+  const bool is_q = ROPE && (int)blockIdx.x < q_ctas;
+  const int t0 = (blockIdx.x - (is_q ? 0 : q_ctas)) * tokens, n = min(tokens, sq.total - t0);
   find_places(sq, pg, t0, n, places, index_status, ROPE ? position : nullptr);
   if constexpr (ROPE) {
     turn_angles(rope, position, n, turns);
     __syncthreads();
+    if (is_q) {
+      turn_rows<TX, LANES>(Q, QO, rope, places, turns, t0, n, vec);
+      return;
+    }
+    if constexpr (TC == TX) {
+      if (vec && rope.pairs % 4 == 0) {
+        const int64_t head = (int64_t)Dh << pg.page_shift;
+        auto move = [&](const RowsView& src, void* pages, int pairs) {
+          move_rows<TX, LANES>(
+              static_cast<const EX*>(src.data) + (int64_t)t0 * src.sT, src.sT, src.sH,
+              [&](int tl) {
+                return places[tl] < 0 ? nullptr : static_cast<EX*>(pages) + places[tl] * Dh;
+              },
+              head, pg.H, Dh, pairs, rope.interleaved, turns, rope.pairs, n);
+        };
+        move(K, pg.k, rope.pairs);
+        move(V, pg.v, 0);
+        return;
+      }
+    }
   }
   // A group's lanes share their vector; the other groups of the warp may have left.
   const unsigned mask =
       LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
-  float co[8], si[8];
-  int turned = -1;  // the token that they are of
-  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H + (ROPE ? Q.heads : 0)); at.tl < n;
-       at.next()) {
-    const int64_t first = places[at.tl];
-    const int64_t t = t0 + at.tl;
-    const bool is_q = ROPE && at.kvh >= 2 * pg.H;
-    if (first < (is_q ? -1 : 0)) continue;  // Q's rows are turned wherever K may go
+  for (Walk at(threadIdx.x / LANES, kThreads / LANES, 2 * pg.H); at.tl < n; at.next()) {
     const bool is_v = at.kvh >= pg.H;
-    const int h = is_q ? at.kvh - 2 * pg.H : is_v ? at.kvh - pg.H : at.kvh;
-    const RowsView& src = is_q ? Q : is_v ? V : K;
-    const EX* row = static_cast<const EX*>(src.data) + t * src.sT + (int64_t)h * src.sH;
+    const int h = is_v ? at.kvh - pg.H : at.kvh;
+    const int64_t first = places[at.tl];
+    if (first < 0) continue;
+    const EX* row = static_cast<const EX*>(is_v ? V.data : K.data) +
+                    (int64_t)(t0 + at.tl) * (is_v ? V.sT : K.sT) +
+                    (int64_t)h * (is_v ? V.sH : K.sH);
     Eight<EX> raw = load8(row, d, Dh, vec);
-    if constexpr (ROPE) {
-      if (is_q || !is_v) {
-        if (turned != at.tl) {
-          turned = at.tl;
-          lane_turns(rope, turns + at.tl * rope.pairs, d, co, si);
-        }
-        raw = turned8(row, raw, rope, d, Dh, vec, co, si);
-      }
-      if (is_q) {
-        __syncwarp(mask);
-        store8(static_cast<EX*>(QO.data) + t * QO.sT + (int64_t)h * QO.sH, d, Dh, vec, raw);
-        continue;
-      }
-    }
+    if (ROPE && !is_v) raw = turned8(row, raw, rope, d, Dh, vec, turns + at.tl * rope.pairs);
     const int64_t place = first + ((int64_t)h << pg.page_shift);
     if constexpr (TC == kI4) {
       float x[8], top = 0.f;
@@ -530,7 +672,7 @@ void kv_pages_append_launch(const RowsView& K, const RowsView& V, const KvPages&
     constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
     ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, false>,
                           dim3((sq.total + tokens - 1) / tokens), dim3(kThreads), 0, s, K, V,
-                          RowsView{}, RowsView{}, pg, sq, Rope{}, tokens, vec, index_status));
+                          RowsView{}, RowsView{}, pg, sq, Rope{}, 0, tokens, vec, index_status));
   });
 }
 
@@ -544,10 +686,10 @@ void kv_pages_append_rope_launch(const RowsView& Q, const RowsView& QO, const Ro
   ProfScope prof("kv_pages", s);
   dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
     constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;
-    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, true>,
-                          dim3((sq.total + tokens - 1) / tokens), dim3(kThreads),
+    const int ctas = (sq.total + tokens - 1) / tokens, q_ctas = Q.heads ? ctas : 0;
+    ATTNB_CUDA(launch_pdl(append_kernel<TX, TC, LN, true>, dim3(ctas + q_ctas), dim3(kThreads),
                           tokens * rope.pairs * sizeof(float2), s, K, V, Q, QO, pg, sq, rope,
-                          tokens, vec, index_status));
+                          q_ctas, tokens, vec, index_status));
   });
 }
 
