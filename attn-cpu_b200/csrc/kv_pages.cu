@@ -169,46 +169,51 @@ struct Walk {
 };
 
 // The share of one lane (dimensions d to d + 7) in 4 bits: its eight codes and its
-// group's factor.  top: the vector's largest magnitude, finite.  All lanes of
-// `mask` call.
+// group's factor.  own, top: the largest magnitudes of the group and of the vector,
+// finite.
 template <int TX>
-__device__ __forceinline__ uint32_t i4_codes(const float (&x)[8], float top, unsigned mask,
-                                             int& factor) {
+__device__ __forceinline__ uint32_t i4_codes(const float (&x)[8], float own, float top, int& factor) {
   // 16-bit values: products exact in fp32, once the vector is brought near 1.
   using Wide = std::conditional_t<TX == kF32, double, float>;
   float near = 1.f;
   if (TX != kF16) near = top > 0x1p60f ? 0x1p-64f : top < 0x1p-60f ? 0x1p64f : 1.f;
-  float y[8], own = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    y[j] = fabsf(x[j]) * near;
-    own = fmaxf(own, y[j]);
-  }
-  own = fmaxf(own, __shfl_xor_sync(mask, own, 1));  // 32 dimensions are four lanes
-  own = fmaxf(own, __shfl_xor_sync(mask, own, 2));
   factor = 0;
   if (!(own > 0.f)) return 0x88888888u;
   const float a = top * near;
-  int r = min(max((int)ceilf(own / a * 255.f), 1), 255);
+  own *= near;
+  int r = min(max((int)ceilf(__fdividef(own, a) * 255.f), 1), 255);
   const Wide want = (Wide)own * (Wide)255;
   if ((Wide)(r - 1) * (Wide)a >= want) --r;
   if ((Wide)r * (Wide)a < want) ++r;
   factor = r;
   const Wide ar = (Wide)a * (Wide)r;
-  const float inv = 1785.f / (float)ar;
-  uint32_t codes = 0;
+  const float inv = __fdividef(1785.f, (float)ar);
+  // Candidates by an addition that leaves code + 8 in the last bits; each is right unless
+  // its remainder is half a step or more.
+  constexpr float kMagic = 12582912.f + 8.f;
+  constexpr uint32_t kMagicBits = 0x4b400000u;  // of 12582912
+  uint32_t bits[8];
+  bool off = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    // A whole number next below the quotient (or, where that is next to a whole number,
-    // that one: both round the same way), and which side of the tie above it
-    // the quotient is on.
-    const float m = floorf(y[j] * inv);
-    const Wide p = (Wide)y[j] * (Wide)3570, tie = (Wide)(2.f * m + 1.f) * ar;
-    int c = (int)m;
-    if (p > tie || (p == tie && (c & 1))) ++c;
-    codes |= (uint32_t)(x[j] < 0.f ? 8 - c : 8 + c) << (4 * j);
+    const float y = x[j] * near, f = fmaf(y, inv, kMagic);
+    bits[j] = __float_as_uint(f);
+    const Wide rest = (Wide)y * (Wide)1785 - (Wide)(f - kMagic) * ar;
+    off |= (Wide)2 * (rest < (Wide)0 ? -rest : rest) >= ar;
   }
-  return codes;
+  if (off) {  // a tie, or next to one
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = (int)(bits[j] - kMagicBits) - 8;
+      const Wide rest = (Wide)(x[j] * near) * (Wide)1785 - (Wide)c * ar;
+      const Wide two = (Wide)2 * (rest < (Wide)0 ? -rest : rest);
+      if (two > ar || (two == ar && (c & 1))) bits[j] += rest < (Wide)0 ? ~0u : 1u;
+    }
+  }
+  uint32_t codes = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) codes = codes * 16u + bits[j];
+  return codes - kMagicBits * 0x11111111u;
 }
 
 // cos and sin of every token and pair of the CTA, [n][pairs].
@@ -411,7 +416,7 @@ __device__ __forceinline__ void turn_rows(const RowsView& Q, const RowsView& QO,
 // to e4m3 and back: 61 us; 79 with two vectors in flight, 80 with four).
 // With ROPE the first q_ctas CTAs take Q's rows, the others K and V.
 template <int TX, int TC, int LANES, bool ROPE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ROPE ? 4 : 1)
     append_kernel(const RowsView K, const RowsView V, const RowsView Q, const RowsView QO,
                   const KvPages pg, const SeqTable sq, const Rope rope, const int q_ctas,
                   const int tokens, const bool vec, int* index_status) {
@@ -465,29 +470,29 @@ __global__ void __launch_bounds__(kThreads)
     if (ROPE && !is_v) raw = turned8(row, raw, rope, d, Dh, vec, turns + at.tl * rope.pairs);
     const int64_t place = first + ((int64_t)h << pg.page_shift);
     if constexpr (TC == kI4) {
-      float x[8], top = 0.f;
+      float x[8], own = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = to_float(raw.e[j]);
-        top = max_nan(top, fabsf(x[j]));
+        own = max_nan(own, fabsf(x[j]));
       }
+      own = max_nan(own, __shfl_xor_sync(mask, own, 1));  // 32 dimensions are four lanes
+      own = max_nan(own, __shfl_xor_sync(mask, own, 2));
+      float top = own;
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+      for (int o = LANES / 2; o > 2; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
       const bool bad = !(top <= 3.402823466e38f);
       if (e == 0)
         (is_v ? pg.v_scale : pg.k_scale)[place] = bad ? __int_as_float(0x7fffffff) : top / 1785.f;
-      if (bad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
-      }
       int factor;
-      const uint32_t codes = i4_codes<TX>(x, top, mask, factor);
+      const uint32_t codes = i4_codes<TX>(x, bad ? 0.f : own, top, factor);
       if (d < Dh)
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(is_v ? pg.v : pg.k) +
                                      place * (Dh / 2) + d / 2) = codes;
       const int bytes = i4_group_bytes(Dh);
-      if (e % 4 == 0 && e / 4 < bytes)
-        (is_v ? pg.v_group : pg.k_group)[place * bytes + e / 4] = (uint8_t)factor;
+      if (e % 4 == 0)  // a lane of the group writes its factor, and zeros behind the last group
+        for (int g = e / 4; g < bytes; g += LANES / 4)
+          (is_v ? pg.v_group : pg.k_group)[place * bytes + g] = g == e / 4 ? (uint8_t)factor : 0;
     } else if constexpr (CODED) {
       EC* out = static_cast<EC*>(is_v ? pg.v : pg.k) + place * Dh;
       constexpr float C = TC == kE4M3 ? 448.f : 127.f;
@@ -682,7 +687,7 @@ void kv_pages_append_rope_launch(const RowsView& Q, const RowsView& QO, const Ro
                                  cudaStream_t s) {
   const bool vec = vec_rows(K) && vec_rows(V) && vec_pages(pg) &&
                    (Q.heads == 0 || (vec_rows(Q) && vec_rows(QO)));
-  const int tokens = tokens_per_cta(sq, num_sms);
+  const int tokens = tokens_per_cta(sq, Q.heads ? num_sms / 2 : num_sms);
   ProfScope prof("kv_pages", s);
   dispatch(K, pg, [&](auto tx, auto tc, auto lanes) {
     constexpr int TX = decltype(tx)::value, TC = decltype(tc)::value, LN = decltype(lanes)::value;

@@ -48,6 +48,8 @@ def _rows(g, n, H, D, dtype):
 def test_codes(cuda, dtype, D):
     new, keys, H = [60, 0, 1, 300], [60, 9, 33, 411], 3
     p = Pages(keys, H, D, 16, I4)
+    for t in (p.k, p.v, *p.kw.values()):  # whatever was there before
+        t.view(torch.uint8).fill_(0xA5)
     n = sum(new)
     g = _gen(D)
     k, v = (_rows(g, n, H, D, dtype) for _ in range(2))
