@@ -344,7 +344,7 @@ int attnb_kv_blocks_select_dev(const attnb_rows* Q, const attnb_bounds* bounds, 
     if (!workspace) invalid("Null workspace");
     DeviceCtx& c = current_ctx();
     kv_blocks_select_run(rows(Q), bounds->data, num_pages, H, shift, sq, keep_first, keep_last,
-                         blocks, take, workspace, workspace_bytes, c.index_status,
+                         blocks, take, workspace, workspace_bytes, c.index_status, c.num_sms,
                          as_stream(stream));
   });
 }

@@ -305,7 +305,7 @@ size_t kv_blocks_workspace_bytes(int tokens, int H, int max_pages);
 void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, int H,
                           int page_shift, const SeqTable& sq, int keep_first, int keep_last,
                           int32_t* blocks, int take, void* ws, size_t ws_bytes, int* index_status,
-                          cudaStream_t s);
+                          int num_sms, cudaStream_t s);
 // Lists as page numbers [tokens * H][take] and keys that they hold for their token
 // [tokens * H] (-1: a row of no sequence).
 void kv_blocks_lists_launch(const SeqTable& sq, const KvPages& pg, const int32_t* blocks, int take,

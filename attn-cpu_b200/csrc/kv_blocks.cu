@@ -25,10 +25,11 @@
 namespace attnb {
 namespace {
 
-constexpr int kBoundsThreads = 128;
+constexpr int kBoundsThreads = 256;
 constexpr int kScoreThreads = 128;
-constexpr int kScoreBlocks = 128;  // blocks of one CTA of the score kernel
+constexpr int kScoreRound = kScoreThreads / 8 * 2;  // blocks of one round of a CTA of the score kernel
 constexpr int kPickThreads = 256;
+constexpr int kPickKeys = 4096;  // held in shared memory
 constexpr size_t kScoreBytes = 64u << 20;  // workspace for scores, at most (or one token's)
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -60,15 +61,31 @@ __device__ __forceinline__ float key_value(const KvPages& pg, int64_t place, int
   }
 }
 
-// A CTA takes every gridDim.x-th of the pairs (completed block, head); a thread takes a
-// dimension, and for head sizes up to 64 every second key of it.
+// Dimensions d to d + 7 of the key at `place`; codes without their scale.
+template <int TC>
+__device__ __forceinline__ void key_eight(const KvPages& pg, int64_t place, int d, float (&x)[8]) {
+  if constexpr (TC == kI4) {
+    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(
+        static_cast<const uint8_t*>(pg.k) + place * (pg.Dh / 2) + d / 2));
+    i4_values(codes, __ldg(pg.k_group + place * i4_group_bytes(pg.Dh) + d / kI4Group), x);
+  } else {
+    const elem_t<TC>* p = static_cast<const elem_t<TC>*>(pg.k) + place * pg.Dh + d;
+    load4(p, *reinterpret_cast<float(*)[4]>(x));
+    load4(p + 4, *reinterpret_cast<float(*)[4]>(x + 4));
+  }
+}
+
+// A CTA takes every gridDim.x-th of the pairs (completed block, head).  vec: groups of 8 to
+// 32 lanes take a key, 8 dimensions a lane, so that the keys of a page are read in a few
+// rounds; else a thread takes a dimension.
 template <int TC, int TB>
 __global__ void __launch_bounds__(kBoundsThreads)
-    bounds_kernel(const KvPages pg, void* bounds, const SeqTable sq, int* index_status) {
+    bounds_kernel(const KvPages pg, void* bounds, const SeqTable sq, const bool vec,
+                  int* index_status) {
   using EB = elem_t<TB>;
   __shared__ long long warps[32];
   __shared__ int before[kBoundsThreads], block0[kBoundsThreads];
-  __shared__ float2 half[64];
+  __shared__ float2 part[kBoundsThreads / 32][256];
   const int tid = threadIdx.x, page = 1 << pg.page_shift;
   grid_dep_wait();
   for (int b0 = 0; b0 < sq.batch; b0 += kBoundsThreads) {
@@ -98,22 +115,48 @@ __global__ void __launch_bounds__(kBoundsThreads)
       if (number < 0) continue;  // the same for the whole block
       const int64_t place = ((int64_t)number * pg.H + h) << pg.page_shift;
       EB* out = static_cast<EB*>(bounds) + ((int64_t)number * pg.H + h) * 2 * pg.Dh;
-      if (pg.Dh <= 64) {
-        const int d = tid & 63;
-        float2 x = make_float2(INFINITY, -INFINITY);
+      if (vec) {
+        const int lanes = pg.Dh <= 64 ? 8 : pg.Dh <= 128 ? 16 : 32, d = tid % lanes * 8;
+        float lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          lo[e] = INFINITY;
+          hi[e] = -INFINITY;
+        }
         if (d < pg.Dh) {
 #pragma unroll 4
-          for (int key = tid >> 6; key < page; key += 2) {
-            const float v = key_value<TC>(pg, place + key, d);
-            x = make_float2(min_nan(x.x, v), max_nan(x.y, v));
+          for (int key = tid / lanes; key < page; key += kBoundsThreads / lanes) {
+            float x[8];
+            key_eight<TC>(pg, place + key, d, x);
+            const float scale = elem_coded(TC) ? __ldg(pg.k_scale + place + key) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = elem_coded(TC) ? x[e] * scale : x[e];
+              lo[e] = min_nan(lo[e], v);
+              hi[e] = max_nan(hi[e], v);
+            }
+          }
+        }
+        // The groups of a warp meet by shuffles, the warps in shared memory.
+        for (int o = 16; o >= lanes; o >>= 1) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            lo[e] = min_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+            hi[e] = max_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
           }
         }
         __syncthreads();  // the block before has been read
-        if (tid >= 64) half[d] = x;
+        if ((tid & 31) < lanes) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part[tid >> 5][d + e] = make_float2(lo[e], hi[e]);
+        }
         __syncthreads();
-        if (tid < pg.Dh) {
-          from_float(min_nan(x.x, half[d].x), out[d]);
-          from_float(max_nan(x.y, half[d].y), out[pg.Dh + d]);
+        for (int i = tid; i < pg.Dh; i += kBoundsThreads) {
+          float2 x = part[0][i];
+          for (int w = 1; w < kBoundsThreads / 32; ++w)
+            x = make_float2(min_nan(x.x, part[w][i].x), max_nan(x.y, part[w][i].y));
+          from_float(x.x, out[i]);
+          from_float(x.y, out[pg.Dh + i]);
         }
       } else {
         for (int d = tid; d < pg.Dh; d += kBoundsThreads) {
@@ -140,6 +183,7 @@ struct BlockArgs {
   int num_pages, H, G, page_shift;
   int keep_first, keep_last, take;
   int token0, tokens;     // the part of the rows that this launch takes
+  int chunk;              // blocks of one CTA of the score kernel
   uint64_t* keys;         // [tokens][H][max_pages]
   int32_t* blocks;        // [all tokens][H][take]
   int* index_status;
@@ -178,8 +222,8 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const BlockArgs a,
   int b;
   const int own = own_block(a.seqs, a.page_shift, a.token0 + t, b, a.index_status);
   if (own + 1 <= a.take) return;  // all of them
-  const int from = a.keep_first + blockIdx.x * kScoreBlocks;
-  const int to = min(own + 1 - a.keep_last, from + kScoreBlocks);
+  const int from = a.keep_first + blockIdx.x * a.chunk;
+  const int to = min(own + 1 - a.keep_last, from + a.chunk);
   if (from >= to) return;
   for (int d = tid; d < Dh; d += kScoreThreads) {
     const EB* q = static_cast<const EB*>(a.q.data) + (int64_t)(a.token0 + t) * a.q.sT +
@@ -206,44 +250,61 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const BlockArgs a,
     }
   const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
   uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages;
-  for (int j0 = from; j0 < to; j0 += kScoreThreads / 8) {
-    const int j = j0 + (tid >> 3);
-    double s = 0.0;
-    if (j < to) {
-      const int page = __ldg(table + j);
-      if (page < 0 || page >= a.num_pages) {
-        raise_index(a.index_status);  // bounds of zeros
-      } else {
-        const EB* p = static_cast<const EB*>(a.bounds) + ((int64_t)page * a.H + h) * 2 * Dh;
+  // Two blocks a group and round, both on their way before the first is summed.
+  for (int j0 = from; j0 < to; j0 += kScoreRound) {
+    const EB* p[2];
+    uint4 x[2][NU];
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          const int d = (u * 8 + e) * PER;
-          if (vec) {  // 2 Dh is a multiple of PER
-            if (d >= 2 * Dh) continue;
-            const uint4 x = *reinterpret_cast<const uint4*>(p + d);
-            const EB* v = reinterpret_cast<const EB*>(&x);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) s = fma(q[u * PER + i], (double)to_float(v[i]), s);
-          } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-              if (d + i < 2 * Dh) s = fma(q[u * PER + i], (double)to_float(p[d + i]), s);
-          }
-        }
+    for (int k = 0; k < 2; ++k) {
+      const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
+      p[k] = nullptr;
+      if (j < to) {
+        const int page = __ldg(table + j);
+        if (page < 0 || page >= a.num_pages) raise_index(a.index_status);  // bounds of zeros
+        else p[k] = static_cast<const EB*>(a.bounds) + ((int64_t)page * a.H + h) * 2 * Dh;
       }
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (e == 0 && j < to) keys[j] = sort_key(s);
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int d = (u * 8 + e) * PER;
+        x[k][u] = make_uint4(0, 0, 0, 0);
+        if (!p[k] || d >= 2 * Dh) continue;
+        if (vec) {  // 2 Dh is a multiple of PER
+          x[k][u] = *reinterpret_cast<const uint4*>(p[k] + d);
+        } else {
+          EB* v = reinterpret_cast<EB*>(&x[k][u]);
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (d + i < 2 * Dh) v[i] = p[k][d + i];
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      double s = 0.0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const EB* v = reinterpret_cast<const EB*>(&x[k][u]);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s = fma(q[u * PER + i], (double)to_float(v[i]), s);
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
+      if (e == 0 && j < to) keys[j] = sort_key(s);
+    }
   }
 }
 
 // ------------------------------------------------------------------ choice
-// One CTA for a token and a KV head.
+// One CTA for a token and a KV head.  Keys of up to kPickKeys blocks are read once.
 __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
   __shared__ int hist[256];
   __shared__ int warp_sum[kPickThreads / 32];
+  __shared__ uint64_t warp_lo[kPickThreads / 32], warp_hi[kPickThreads / 32];
   __shared__ int digit, left;
+  __shared__ uint64_t mine[kPickKeys];
   const int tid = threadIdx.x, row = blockIdx.x, t = row / a.H, h = row - t * a.H;
   const int lane = tid & 31, warp = tid >> 5;
   grid_dep_wait();
@@ -262,21 +323,49 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
   for (int i = tid; i < a.keep_last; i += kPickThreads)
     out[a.take - a.keep_last + i] = own + 1 - a.keep_last + i;
   if (want == 0) return;
-  // The top digits that the last one taken has, until as many have them as are wanted.
-  uint64_t top = 0;
-  int shift = 64, rest = want;
+  // The first bit in which they differ: digits start there.
+  uint64_t lo = ~0ull, hi = 0;
+#pragma unroll 4
+  for (int i = tid; i < n; i += kPickThreads) {
+    const uint64_t k = keys[i];
+    if (n <= kPickKeys) mine[i] = k;
+    lo = min(lo, k);
+    hi = max(hi, k);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, (uint64_t)__shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, (uint64_t)__shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (lane == 0) {
+    warp_lo[warp] = lo;
+    warp_hi[warp] = hi;
+  }
+  __syncthreads();
+  for (int w = 0; w < kPickThreads / 32; ++w) {
+    lo = min(lo, warp_lo[w]);
+    hi = max(hi, warp_hi[w]);
+  }
+  if (n <= kPickKeys) keys = mine;
+  // The top digits of the last one taken, until as many keys have them as are wanted.  All keys
+  // agree above bit `bits`.
+  int bits = 64 - (lo == hi ? 64 : __clzll((long long)(lo ^ hi))), shift = bits;
+  uint64_t top = bits == 64 ? 0 : hi >> bits;
+  int rest = want;
   while (shift > 0) {
-    shift -= 8;
+    const int wide = min(8, shift), above = shift;
+    shift -= wide;
     hist[tid] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += kPickThreads) {
       const uint64_t k = keys[i];
-      if (shift == 56 || k >> (shift + 8) == top) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+      if (above == 64 || k >> above == top)
+        atomicAdd(&hist[(int)(k >> shift) & ((1 << wide) - 1)], 1);
     }
     __syncthreads();
     // Sums from the greatest digit down: thread i has digit 255 - i.
-    const int mine = hist[255 - tid];
-    int sum = mine;
+    const int count = hist[255 - tid];
+    int sum = count;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, sum, o);
@@ -285,13 +374,13 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
     if (lane == 31) warp_sum[warp] = sum;
     __syncthreads();
     for (int i = 0; i < warp; ++i) sum += warp_sum[i];
-    if (sum >= rest && sum - mine < rest) {
+    if (sum >= rest && sum - count < rest) {
       digit = 255 - tid;
-      left = rest - (sum - mine);
+      left = rest - (sum - count);
     }
     __syncthreads();
     const bool all = hist[digit] == left;
-    top = top << 8 | (uint64_t)digit;
+    top = (above == 64 ? 0 : top << wide) | (uint64_t)digit;
     rest = left;
     __syncthreads();
     if (all) break;
@@ -373,9 +462,10 @@ size_t keys_per_token(int H, int max_pages) { return (size_t)H * std::max(max_pa
 
 void kv_blocks_bounds_launch(const KvPages& pg, void* bounds, int bounds_type, const SeqTable& sq,
                              int* index_status, int num_sms, cudaStream_t s) {
+  const bool vec = pg.Dh % 8 == 0 && reinterpret_cast<uintptr_t>(pg.k) % (4 * elem_bytes(pg.type)) == 0;
   auto go = [&](auto tc, auto tb) {
     ATTNB_CUDA(launch_pdl(bounds_kernel<decltype(tc)::value, decltype(tb)::value>,
-                          dim3(4 * num_sms), dim3(kBoundsThreads), 0, s, pg, bounds, sq,
+                          dim3(2 * num_sms), dim3(kBoundsThreads), 0, s, pg, bounds, sq, vec,
                           index_status));
   };
   with_value_type(bounds_type, [&](auto tb) {
@@ -394,7 +484,7 @@ size_t kv_blocks_workspace_bytes(int tokens, int H, int max_pages) {
 void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, int H,
                           int page_shift, const SeqTable& sq, int keep_first, int keep_last,
                           int32_t* blocks, int take, void* ws, size_t ws_bytes, int* index_status,
-                          cudaStream_t s) {
+                          int num_sms, cudaStream_t s) {
   BlockArgs a{};
   a.q = q;
   a.bounds = bounds;
@@ -415,10 +505,14 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
   if (fit == 0) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
   const int eb = elem_bytes(q.type);
   const bool vec = reinterpret_cast<uintptr_t>(bounds) % 16 == 0 && 2 * q.Dh * eb % 16 == 0;
-  const int chunks = (sq.max_pages + kScoreBlocks - 1) / kScoreBlocks;
   for (a.token0 = 0; a.token0 < sq.total; a.token0 += a.tokens) {
     a.tokens = (int)std::min<size_t>(fit, sq.total - a.token0);
     if (sq.max_pages > take) {
+      // Four CTAs an SM where there is that much to do.
+      const int64_t rounds = (sq.max_pages + kScoreRound - 1) / kScoreRound;
+      const int64_t each = std::max<int64_t>(1, rounds * a.tokens * H / (4 * num_sms));
+      a.chunk = (int)std::min(rounds, each) * kScoreRound;
+      const int chunks = (sq.max_pages + a.chunk - 1) / a.chunk;
       with_value_type(q.type, [&](auto tb) {
         constexpr int TB = decltype(tb)::value;
         constexpr int F = TB == kF32 ? 2 : 1;
