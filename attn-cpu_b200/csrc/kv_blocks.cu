@@ -26,10 +26,12 @@ namespace attnb {
 namespace {
 
 constexpr int kBoundsThreads = 256;
-constexpr int kScoreThreads = 128;
+constexpr int kScoreThreads = 256;
 constexpr int kScoreRound = kScoreThreads / 8 * 2;  // blocks of one round of a CTA of the score kernel
-constexpr int kPickThreads = 256;
-constexpr int kPickKeys = 4096;  // held in shared memory
+constexpr int kScoreMost = 8 * kScoreRound;         // blocks of one CTA
+constexpr int kPickThreads = 512;
+constexpr int kPickKeys = 4096;   // of a row, held in shared memory
+constexpr int kPickParts = 2048;  // of the scores' range
 constexpr size_t kScoreBytes = 64u << 20;  // workspace for scores, at most (or one token's)
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -38,9 +40,9 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// Tokens that sequence b holds, as far as its table goes.
-__device__ __forceinline__ int held(const SeqTable& sq, int page_shift, int b, int* index_status) {
-  const int len = __ldg(sq.lens + b);
+// Tokens that a sequence of length `len` holds, as far as its table goes.
+__device__ __forceinline__ int held(int len, const SeqTable& sq, int page_shift,
+                                    int* index_status) {
   const long long room = (long long)sq.max_pages << page_shift;
   if (len < 0 || len > room) raise_index(index_status);
   return (int)min((long long)max(len, 0), room);
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kBoundsThreads)
   for (int b0 = 0; b0 < sq.batch; b0 += kBoundsThreads) {
     int j0 = 0, count = 0;
     if (b0 + tid < sq.batch) {
-      const int b = b0 + tid, len = held(sq, pg.page_shift, b, index_status);
+      const int b = b0 + tid, len = held(__ldg(sq.lens + b), sq, pg.page_shift, index_status);
       int first, n;
       seq_rows(sq.cu, b, INT_MAX, first, n);
       j0 = (len - min(n, len)) >> pg.page_shift;
@@ -189,16 +191,41 @@ struct BlockArgs {
   int* index_status;
 };
 
-// The block that packed token t lies in, of its sequence b; -1 where there is none.
-__device__ __forceinline__ int own_block(const SeqTable& sq, int page_shift, int t, int& b,
-                                         int* index_status, int* position = nullptr) {
-  int first, count;
-  b = seq_of(sq, t, first, count);
-  if (b < 0) return -1;
-  const int pos = held(sq, page_shift, b, index_status) - count + (t - first);
-  if (pos < 0) return -1;
-  if (position) *position = pos;
-  return pos >> page_shift;
+// The place of packed token t.  `threads` threads find it side by side: each tries every so many
+// of the sequences, offsets and lengths read at once, where a search would wait for one read
+// after the other.
+struct TokenPlace {
+  int b;    // its sequence, -1: none
+  int pos;  // its position, negative where its sequence holds less than it brings
+};
+// This thread's finding, as a number of which the greatest counts; 0: none.
+__device__ __forceinline__ unsigned long long find_token(const SeqTable& sq, int page_shift, int t,
+                                                         int tid, int threads, int* index_status) {
+  unsigned long long found = 0;
+  for (int b = tid; b < sq.batch; b += threads) {
+    const int len = __ldg(sq.lens + b);
+    int first, count;
+    seq_rows(sq.cu, b, sq.total, first, count);
+    if (t >= first && t < first + count) {
+      const int pos = held(len, sq, page_shift, index_status) - count + (t - first);
+      found = (unsigned long long)(b + 1) << 32 | (unsigned)pos;
+    }
+  }
+  return found;
+}
+__device__ __forceinline__ TokenPlace token_place(unsigned long long found) {
+  return {(int)(found >> 32) - 1, (int)(unsigned)found};
+}
+// For all threads of a block.
+__device__ __forceinline__ TokenPlace block_token(const SeqTable& sq, int page_shift, int t,
+                                                  unsigned long long* sh, int* index_status) {
+  if (threadIdx.x == 0) *sh = 0;
+  __syncthreads();
+  const unsigned long long found =
+      find_token(sq, page_shift, t, threadIdx.x, blockDim.x, index_status);
+  if (found) atomicMax(sh, found);
+  __syncthreads();
+  return token_place(*sh);
 }
 
 // Unsigned numbers that sort as the scores do.
@@ -209,108 +236,126 @@ __device__ __forceinline__ uint64_t sort_key(double x) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// Eight lanes a block, each with every eighth unit of 16 bytes of its bounds and the same
-// part of the queries' sums in registers.  NU: units a lane.
+// A CTA takes up to kScoreMost blocks of a token and KV head: eight lanes a block, each with
+// every eighth unit of 16 bytes of its bounds, two blocks in flight.  The queries' sums are
+// read from shared memory: in registers they would leave too few CTAs an SM for the
+// latency of the reads that come before the bounds (32 us for 32 sequences of 8000-32768 keys).
+// NU: units a lane.
 template <int TB, int NU>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const BlockArgs a, const bool vec) {
+__global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(const BlockArgs a, const bool vec) {
   using EB = elem_t<TB>;
   constexpr int PER = 16 / sizeof(EB);
-  __shared__ double parts[512];  // q-, q+
+  __shared__ __align__(16) double parts[NU * 8 * PER];  // q-, q+, zeros
+  __shared__ int pages[kScoreMost];
+  __shared__ unsigned long long found;
   const int tid = threadIdx.x, row = blockIdx.y, t = row / a.H, h = row - t * a.H;
   const int Dh = a.q.Dh;
   grid_dep_wait();
-  int b;
-  const int own = own_block(a.seqs, a.page_shift, a.token0 + t, b, a.index_status);
+  for (int d = tid; d < NU * 8 * PER; d += kScoreThreads) {
+    const bool high = d >= Dh;
+    double sum = 0.0;
+    if (d < 2 * Dh) {
+      const EB* q = static_cast<const EB*>(a.q.data) + (int64_t)(a.token0 + t) * a.q.sT +
+                    (int64_t)h * a.G * a.q.sH + (high ? d - Dh : d);
+#pragma unroll 4
+      for (int g = 0; g < a.G; ++g) {
+        const float x = to_float(q[g * a.q.sH]);  // (a NaN goes to both)
+        sum += (double)(high ? (x < 0.f ? 0.f : x) : (x > 0.f ? 0.f : x));
+      }
+    }
+    parts[d] = sum;
+  }
+  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
+  if (at.b < 0 || at.pos < 0) return;
+  const int own = at.pos >> a.page_shift;
   if (own + 1 <= a.take) return;  // all of them
   const int from = a.keep_first + blockIdx.x * a.chunk;
   const int to = min(own + 1 - a.keep_last, from + a.chunk);
   if (from >= to) return;
-  for (int d = tid; d < Dh; d += kScoreThreads) {
-    const EB* q = static_cast<const EB*>(a.q.data) + (int64_t)(a.token0 + t) * a.q.sT +
-                  (int64_t)h * a.G * a.q.sH + d;
-    double lo = 0.0, hi = 0.0;
-    for (int g = 0; g < a.G; ++g) {
-      const float x = to_float(q[g * a.q.sH]);
-      // (a NaN goes to both)
-      lo += (double)(x > 0.f ? 0.f : x);
-      hi += (double)(x < 0.f ? 0.f : x);
+  for (int j = from + tid; j < to; j += kScoreThreads) {
+    int page = __ldg(a.seqs.table + at.b * a.seqs.table_stride + j);
+    if (page < 0 || page >= a.num_pages) {
+      raise_index(a.index_status);  // bounds of zeros
+      page = -1;
     }
-    parts[d] = lo;
-    parts[Dh + d] = hi;
+    pages[j - from] = page;
   }
   __syncthreads();
   const int e = tid & 7;
-  double q[NU * PER];
-#pragma unroll
-  for (int u = 0; u < NU; ++u)
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int d = (u * 8 + e) * PER + i;
-      q[u * PER + i] = d < 2 * Dh ? parts[d] : 0.0;
-    }
-  const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
   uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages;
-  // Two blocks a group and round, both on their way before the first is summed.
   for (int j0 = from; j0 < to; j0 += kScoreRound) {
-    const EB* p[2];
-    uint4 x[2][NU];
+    uint4 y[2][NU];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
-      p[k] = nullptr;
-      if (j < to) {
-        const int page = __ldg(table + j);
-        if (page < 0 || page >= a.num_pages) raise_index(a.index_status);  // bounds of zeros
-        else p[k] = static_cast<const EB*>(a.bounds) + ((int64_t)page * a.H + h) * 2 * Dh;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
+      const int page = j < to ? pages[j - from] : -1;
+      const EB* p = static_cast<const EB*>(a.bounds) + ((int64_t)page * a.H + h) * 2 * Dh;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int d = (u * 8 + e) * PER;
-        x[k][u] = make_uint4(0, 0, 0, 0);
-        if (!p[k] || d >= 2 * Dh) continue;
-        if (vec) {  // 2 Dh is a multiple of PER
-          x[k][u] = *reinterpret_cast<const uint4*>(p[k] + d);
-        } else {
-          EB* v = reinterpret_cast<EB*>(&x[k][u]);
+        y[k][u] = make_uint4(0, 0, 0, 0);
+        if (page >= 0 && d < 2 * Dh) {
+          if (vec) {  // 2 Dh is a multiple of PER
+            y[k][u] = *reinterpret_cast<const uint4*>(p + d);
+          } else {
+            EB* v = reinterpret_cast<EB*>(&y[k][u]);
 #pragma unroll
-          for (int i = 0; i < PER; ++i)
-            if (d + i < 2 * Dh) v[i] = p[k][d + i];
+            for (int i = 0; i < PER; ++i)
+              if (d + i < 2 * Dh) v[i] = p[d + i];
+          }
         }
       }
+    }
+    double s[2] = {0.0, 0.0};
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const double2* q = reinterpret_cast<const double2*>(parts + (u * 8 + e) * PER);
+#pragma unroll
+      for (int i = 0; i < PER / 2; ++i) {
+        const double2 two = q[i];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const EB* v = reinterpret_cast<const EB*>(&y[k][u]);
+          s[k] = fma(two.x, (double)to_float(v[2 * i]), s[k]);
+          s[k] = fma(two.y, (double)to_float(v[2 * i + 1]), s[k]);
+        }
+      }
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      double s = 0.0;
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const EB* v = reinterpret_cast<const EB*>(&x[k][u]);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) s = fma(q[u * PER + i], (double)to_float(v[i]), s);
-      }
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int o = 4; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
       const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
-      if (e == 0 && j < to) keys[j] = sort_key(s);
+      if (e == 0 && j < to) keys[j] = sort_key(s[k]);
     }
   }
 }
 
 // ------------------------------------------------------------------ choice
-// One CTA for a token and a KV head.  Keys of up to kPickKeys blocks are read once.
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[kPickThreads / 32];
-  __shared__ uint64_t warp_lo[kPickThreads / 32], warp_hi[kPickThreads / 32];
-  __shared__ int digit, left;
-  __shared__ uint64_t mine[kPickKeys];
+__device__ __forceinline__ double key_score(uint64_t k) {
+  return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k));
+}
+
+// One CTA for a token and a KV head; up to `hold` keys are read once.  The key that is taken last
+// is found by a histogram over equal parts of the scores' range and the ranks of the few in its
+// part; where that part is full (many equal scores, or scores far off the others) or the
+// range is not finite, by digits of 8 bits from the first bit in which keys differ.
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, const int hold) {
+  constexpr int W = kPickThreads / 32;
+  __shared__ int hist[kPickParts];
+  __shared__ int warp_sum[W], warp_eq[W];
+  __shared__ uint64_t warp_lo[W], warp_hi[W];
+  __shared__ int digit, left, few;
+  __shared__ unsigned long long found;
+  __shared__ uint64_t few_key[kPickThreads], last_key;
+  __shared__ int few_at[kPickThreads];
+  extern __shared__ uint64_t mine[];
   const int tid = threadIdx.x, row = blockIdx.x, t = row / a.H, h = row - t * a.H;
   const int lane = tid & 31, warp = tid >> 5;
   grid_dep_wait();
-  int b;
-  const int own = own_block(a.seqs, a.page_shift, a.token0 + t, b, a.index_status);
-  if (b < 0) return;  // rows of no sequence stay
+  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
+  if (at.b < 0) return;  // rows of no sequence stay
+  const int own = at.pos < 0 ? -1 : at.pos >> a.page_shift;
   int32_t* out = a.blocks + ((int64_t)(a.token0 + t) * a.H + h) * a.take;
   if (own + 1 <= a.take) {
     for (int i = tid; i < a.take; i += kPickThreads) out[i] = i <= own ? i : -1;
@@ -323,12 +368,11 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
   for (int i = tid; i < a.keep_last; i += kPickThreads)
     out[a.take - a.keep_last + i] = own + 1 - a.keep_last + i;
   if (want == 0) return;
-  // The first bit in which they differ: digits start there.
   uint64_t lo = ~0ull, hi = 0;
 #pragma unroll 4
   for (int i = tid; i < n; i += kPickThreads) {
     const uint64_t k = keys[i];
-    if (n <= kPickKeys) mine[i] = k;
+    if (n <= hold) mine[i] = k;
     lo = min(lo, k);
     hi = max(hi, k);
   }
@@ -341,31 +385,16 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
     warp_lo[warp] = lo;
     warp_hi[warp] = hi;
   }
+  if (tid == 0) few = 0;
+  for (int i = tid; i < kPickParts; i += kPickThreads) hist[i] = 0;
   __syncthreads();
-  for (int w = 0; w < kPickThreads / 32; ++w) {
+  for (int w = 0; w < W; ++w) {
     lo = min(lo, warp_lo[w]);
     hi = max(hi, warp_hi[w]);
   }
-  if (n <= kPickKeys) keys = mine;
-  // The top digits of the last one taken, until as many keys have them as are wanted.  All keys
-  // agree above bit `bits`.
-  int bits = 64 - (lo == hi ? 64 : __clzll((long long)(lo ^ hi))), shift = bits;
-  uint64_t top = bits == 64 ? 0 : hi >> bits;
-  int rest = want;
-  while (shift > 0) {
-    const int wide = min(8, shift), above = shift;
-    shift -= wide;
-    hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) {
-      const uint64_t k = keys[i];
-      if (above == 64 || k >> above == top)
-        atomicAdd(&hist[(int)(k >> shift) & ((1 << wide) - 1)], 1);
-    }
-    __syncthreads();
-    // Sums from the greatest digit down: thread i has digit 255 - i.
-    const int count = hist[255 - tid];
-    int sum = count;
+  if (n <= hold) keys = mine;
+  // Sum over the threads up to this one.
+  auto scan = [&](int sum) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, sum, o);
@@ -374,43 +403,130 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a) {
     if (lane == 31) warp_sum[warp] = sum;
     __syncthreads();
     for (int i = 0; i < warp; ++i) sum += warp_sum[i];
-    if (sum >= rest && sum - count < rest) {
-      digit = 255 - tid;
-      left = rest - (sum - count);
-    }
-    __syncthreads();
-    const bool all = hist[digit] == left;
-    top = (above == 64 ? 0 : top << wide) | (uint64_t)digit;
-    rest = left;
-    __syncthreads();
-    if (all) break;
-  }
-  // Those above, and the first `rest` of those with the same digits, in their order.
-  int taken = 0, same = 0;  // before this round
-  for (int i0 = 0; i0 < n; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const uint64_t k = i < n ? keys[i] >> shift : 0;
-    const bool above = i < n && k > top, equal = i < n && k == top;
-    const unsigned eq = __ballot_sync(0xffffffffu, equal), ab = __ballot_sync(0xffffffffu, above);
-    if (lane == 0) warp_sum[warp] = __popc(eq) | __popc(ab) << 16;
-    __syncthreads();
-    int eq_before = same + __popc(eq & ((1u << lane) - 1)), ab_before = __popc(ab & ((1u << lane) - 1));
-    int eq_all = 0, ab_all = 0;
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-      const int s = warp_sum[w];
-      if (w < warp) {
-        eq_before += s & 0xffff;
-        ab_before += s >> 16;
+    return sum;
+  };
+  // Taken are the keys with (key >> shift) > top and, of those equal to it, the first `rest`.
+  int shift = 0, rest = want;
+  uint64_t top = hi;
+  const double low = key_score(lo), range = key_score(hi) - low;
+  bool done = lo == hi;
+  if (!done && range < INFINITY && range > 0.0) {  // (false for NaN)
+    const double per = (kPickParts - 0.5) / range;
+    // Not falling in the key, whatever is rounded.
+    auto part = [&](uint64_t k) {
+      return min((int)((key_score(k) - low) * per), kPickParts - 1);
+    };
+    if (per < INFINITY) {
+      for (int i = tid; i < n; i += kPickThreads) atomicAdd(&hist[part(keys[i])], 1);
+      __syncthreads();
+      // From the greatest part down: thread i has a run of parts that ends at the i-th from above.
+      constexpr int RUN = kPickParts / kPickThreads;
+      int count = 0;
+#pragma unroll
+      for (int k = 0; k < RUN; ++k) count += hist[kPickParts - 1 - tid * RUN - k];
+      int sum = scan(count);
+      if (sum >= want && sum - count < want) {
+        sum -= count;
+        for (int k = 0; k < RUN; ++k) {
+          const int p = kPickParts - 1 - tid * RUN - k, c = hist[p];
+          if (sum + c >= want) {
+            digit = p;
+            left = want - sum;
+            break;
+          }
+          sum += c;
+        }
       }
-      eq_all += s & 0xffff;
-      ab_all += s >> 16;
+      __syncthreads();
+      const int p = digit, c = hist[p];
+      if (c <= kPickThreads) {
+        for (int i = tid; i < n; i += kPickThreads) {
+          const uint64_t k = keys[i];
+          if (part(k) == p) {
+            const int slot = atomicAdd(&few, 1);
+            few_key[slot] = k;
+            few_at[slot] = i;
+          }
+        }
+        __syncthreads();
+        if (tid < c) {
+          const uint64_t k = few_key[tid];
+          const int i = few_at[tid];
+          int above = 0, same = 0;  // before it
+          for (int f = 0; f < c; ++f) {
+            above += few_key[f] > k;
+            same += few_key[f] == k && few_at[f] < i;
+          }
+          if (above + same == left - 1) {
+            last_key = k;
+            warp_eq[0] = same + 1;
+          }
+        }
+        __syncthreads();
+        top = last_key;
+        rest = warp_eq[0];
+        done = true;
+        __syncthreads();
+      }
     }
-    if (above || (equal && eq_before < rest))
-      out[a.keep_first + taken + ab_before + min(eq_before, rest) - min(same, rest)] =
-          a.keep_first + i;
-    taken += ab_all + min(same + eq_all, rest) - min(same, rest);
-    same += eq_all;
-    __syncthreads();
+  }
+  if (!done) {
+    // All keys agree above bit `shift`.
+    shift = 64 - __clzll((long long)(lo ^ hi));
+    top = shift == 64 ? 0 : hi >> shift;
+    while (shift > 0) {
+      const int wide = min(8, shift), above = shift;
+      shift -= wide;
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += kPickThreads) {
+        const uint64_t k = keys[i];
+        if (above == 64 || k >> above == top)
+          atomicAdd(&hist[(int)(k >> shift) & ((1 << wide) - 1)], 1);
+      }
+      __syncthreads();
+      // From the greatest digit down: thread i has digit 255 - i.
+      const int count = tid < 256 ? hist[255 - tid] : 0, sum = scan(count);
+      if (sum >= rest && sum - count < rest) {
+        digit = 255 - tid;
+        left = rest - (sum - count);
+      }
+      __syncthreads();
+      const bool all = hist[digit] == left;
+      top = (above == 64 ? 0 : top << wide) | (uint64_t)digit;
+      rest = left;
+      __syncthreads();
+      if (all) break;
+    }
+  }
+  // In their order, a warp a run of them: first how many there are, then their places.
+  const int run = ((n + W - 1) / W + 31) & ~31, first = warp * run, end = min(n, first + run);
+  int above = 0, same = 0;
+  for (int i0 = first; i0 < end; i0 += 32) {
+    const uint64_t k = i0 + lane < end ? keys[i0 + lane] >> shift : 0;
+    above += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k > top));
+    same += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k == top));
+  }
+  if (lane == 0) {
+    warp_sum[warp] = above;
+    warp_eq[warp] = same;
+  }
+  __syncthreads();
+  above = same = 0;
+  for (int w = 0; w < warp; ++w) {
+    above += warp_sum[w];
+    same += warp_eq[w];
+  }
+  for (int i0 = first; i0 < end; i0 += 32) {
+    const uint64_t k = i0 + lane < end ? keys[i0 + lane] >> shift : 0;
+    const bool over = i0 + lane < end && k > top, equal = i0 + lane < end && k == top;
+    const unsigned ab = __ballot_sync(0xffffffffu, over), eq = __ballot_sync(0xffffffffu, equal);
+    const int ab_before = above + __popc(ab & ((1u << lane) - 1));
+    const int eq_before = same + __popc(eq & ((1u << lane) - 1));
+    if (over || (equal && eq_before < rest))
+      out[a.keep_first + ab_before + min(eq_before, rest)] = a.keep_first + i0 + lane;
+    above += __popc(ab);
+    same += __popc(eq);
   }
 }
 
@@ -424,8 +540,12 @@ __global__ void __launch_bounds__(256)
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   grid_dep_wait();
   if (row >= sq.total * pg.H) return;
-  int b, pos = 0;
-  const int own = own_block(sq, pg.page_shift, row / pg.H, b, index_status, &pos);
+  unsigned long long found = find_token(sq, pg.page_shift, row / pg.H, lane, 32, index_status);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    found = max(found, __shfl_xor_sync(0xffffffffu, found, o));
+  const TokenPlace at = token_place(found);
+  const int b = at.b, pos = at.pos, own = pos < 0 ? -1 : pos >> pg.page_shift;
   if (b < 0) {
     if (lane == 0) lens[row] = -1;
     return;
@@ -511,7 +631,7 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
       // Four CTAs an SM where there is that much to do.
       const int64_t rounds = (sq.max_pages + kScoreRound - 1) / kScoreRound;
       const int64_t each = std::max<int64_t>(1, rounds * a.tokens * H / (4 * num_sms));
-      a.chunk = (int)std::min(rounds, each) * kScoreRound;
+      a.chunk = (int)std::min({rounds, each, (int64_t)kScoreMost / kScoreRound}) * kScoreRound;
       const int chunks = (sq.max_pages + a.chunk - 1) / a.chunk;
       with_value_type(q.type, [&](auto tb) {
         constexpr int TB = decltype(tb)::value;
@@ -525,7 +645,9 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
         else go(std::integral_constant<int, 8 * F>{});
       });
     }
-    ATTNB_CUDA(launch_pdl(pick_kernel, dim3(a.tokens * H), dim3(kPickThreads), 0, s, a));
+    const int hold = std::min(sq.max_pages, kPickKeys);
+    ATTNB_CUDA(launch_pdl(pick_kernel, dim3(a.tokens * H), dim3(kPickThreads), (size_t)hold * 8, s,
+                          a, hold));
   }
 }
 
