@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(c
         sum += (double)(high ? (x < 0.f ? 0.f : x) : (x > 0.f ? 0.f : x));
       }
     }
-    parts[d] = sum;
+    // Pairs of the eight lanes that read at once lie side by side.
+    parts[((d / (8 * PER) * (PER / 2) + d % PER / 2) * 8 + d / PER % 8) * 2 + d % 2] = sum;
   }
   const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
   if (at.b < 0 || at.pos < 0) return;
@@ -309,10 +310,9 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(c
     double s[2] = {0.0, 0.0};
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const double2* q = reinterpret_cast<const double2*>(parts + (u * 8 + e) * PER);
 #pragma unroll
       for (int i = 0; i < PER / 2; ++i) {
-        const double2 two = q[i];
+        const double2 two = reinterpret_cast<const double2*>(parts)[(u * (PER / 2) + i) * 8 + e];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const EB* v = reinterpret_cast<const EB*>(&y[k][u]);
@@ -336,6 +336,96 @@ __device__ __forceinline__ double key_score(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k));
 }
 
+// The parts of a list that need no score; how many of the n others are wanted, 0 if the list is
+// complete.  `who` of `all` threads call.
+__device__ __forceinline__ int plain_part(const BlockArgs& a, const TokenPlace& at, int row,
+                                          int32_t*& out, int& n, int who, int all) {
+  if (at.b < 0) return 0;  // rows of no sequence stay
+  const int t = row / a.H, h = row - t * a.H;
+  const int own = at.pos < 0 ? -1 : at.pos >> a.page_shift;
+  out = a.blocks + ((int64_t)(a.token0 + t) * a.H + h) * a.take;
+  if (own + 1 <= a.take) {
+    for (int i = who; i < a.take; i += all) out[i] = i <= own ? i : -1;
+    return 0;
+  }
+  for (int i = who; i < a.keep_first; i += all) out[i] = i;
+  for (int i = who; i < a.keep_last; i += all)
+    out[a.take - a.keep_last + i] = own + 1 - a.keep_last + i;
+  out += a.keep_first;
+  n = own + 1 - a.keep_first - a.keep_last;
+  return a.take - a.keep_first - a.keep_last;  // < n
+}
+
+// Up to kWarpKeys blocks a row: a warp for a token and a KV head, keys in registers.  The key that
+// is taken last is built from its first bit that not all keys share, each bit set if enough
+// keys are still at or above; it ends where as many are as are wanted.  (1064 rows of 80-310
+// keys: 23 us with a CTA each.)
+constexpr int kWarpKeys = 512;
+__global__ void __launch_bounds__(128) pick_warp_kernel(const BlockArgs a) {
+  constexpr int EACH = kWarpKeys / 32;
+  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  grid_dep_wait();
+  if (row >= a.tokens * a.H) return;
+  unsigned long long found =
+      find_token(a.seqs, a.page_shift, a.token0 + row / a.H, lane, 32, a.index_status);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) found = max(found, __shfl_xor_sync(0xffffffffu, found, o));
+  int32_t* out = nullptr;
+  int n = 0;
+  const int want = plain_part(a, token_place(found), row, out, n, lane, 32);
+  if (want == 0) return;
+  const uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first;
+  uint64_t k[EACH], lo = ~0ull, hi = 0;  // no key is 0
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    k[i] = i * 32 + lane < n ? keys[i * 32 + lane] : 0;
+    if (k[i]) lo = min(lo, k[i]);
+    hi = max(hi, k[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, (uint64_t)__shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, (uint64_t)__shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  uint64_t last = hi;
+  int rest = want;  // of the keys equal to it
+  if (lo != hi) {
+    int bit = 63 - __clzll((long long)(lo ^ hi)), count = 0;
+    last = bit == 63 ? 0 : hi >> (bit + 1) << (bit + 1);
+    for (; bit >= 0; --bit) {
+      const uint64_t next = last | 1ull << bit;
+      unsigned c = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) c += k[i] >= next;
+      count = (int)__reduce_add_sync(0xffffffffu, c);
+      if (count >= want) last = next;
+      if (count == want) break;
+    }
+    if (bit < 0) {
+      unsigned c = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) c += k[i] > last;
+      rest -= (int)__reduce_add_sync(0xffffffffu, c);
+    } else {
+      --last;  // all above it, and none of its equals
+      rest = 0;
+    }
+  }
+  const unsigned before = (1u << lane) - 1;
+  int at = 0, same = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (i * 32 >= n) break;
+    const bool equal = k[i] == last;
+    const unsigned eq = __ballot_sync(0xffffffffu, equal);
+    const bool taken = k[i] > last || (equal && same + __popc(eq & before) < rest);
+    const unsigned tk = __ballot_sync(0xffffffffu, taken);
+    if (taken) out[at + __popc(tk & before)] = a.keep_first + i * 32 + lane;
+    at += __popc(tk);
+    same += __popc(eq);
+  }
+}
+
 // One CTA for a token and a KV head; up to `hold` keys are read once.  The key that is taken last
 // is found by a histogram over equal parts of the scores' range and the ranks of the few in its
 // part; where that part is full (many equal scores, or scores far off the others) or the
@@ -350,24 +440,15 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
   __shared__ uint64_t few_key[kPickThreads], last_key;
   __shared__ int few_at[kPickThreads];
   extern __shared__ uint64_t mine[];
-  const int tid = threadIdx.x, row = blockIdx.x, t = row / a.H, h = row - t * a.H;
-  const int lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dep_wait();
-  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
-  if (at.b < 0) return;  // rows of no sequence stay
-  const int own = at.pos < 0 ? -1 : at.pos >> a.page_shift;
-  int32_t* out = a.blocks + ((int64_t)(a.token0 + t) * a.H + h) * a.take;
-  if (own + 1 <= a.take) {
-    for (int i = tid; i < a.take; i += kPickThreads) out[i] = i <= own ? i : -1;
-    return;
-  }
-  const uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first;
-  const int n = own + 1 - a.keep_first - a.keep_last;
-  const int want = a.take - a.keep_first - a.keep_last;  // < n
-  for (int i = tid; i < a.keep_first; i += kPickThreads) out[i] = i;
-  for (int i = tid; i < a.keep_last; i += kPickThreads)
-    out[a.take - a.keep_last + i] = own + 1 - a.keep_last + i;
+  const TokenPlace at =
+      block_token(a.seqs, a.page_shift, a.token0 + row / a.H, &found, a.index_status);
+  int32_t* out = nullptr;
+  int n = 0;
+  const int want = plain_part(a, at, row, out, n, tid, kPickThreads);
   if (want == 0) return;
+  const uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first;
   uint64_t lo = ~0ull, hi = 0;
 #pragma unroll 4
   for (int i = tid; i < n; i += kPickThreads) {
@@ -524,7 +605,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
     const int ab_before = above + __popc(ab & ((1u << lane) - 1));
     const int eq_before = same + __popc(eq & ((1u << lane) - 1));
     if (over || (equal && eq_before < rest))
-      out[a.keep_first + ab_before + min(eq_before, rest)] = a.keep_first + i0 + lane;
+      out[ab_before + min(eq_before, rest)] = a.keep_first + i0 + lane;
     above += __popc(ab);
     same += __popc(eq);
   }
@@ -630,7 +711,7 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
     if (sq.max_pages > take) {
       // Four CTAs an SM where there is that much to do.
       const int64_t rounds = (sq.max_pages + kScoreRound - 1) / kScoreRound;
-      const int64_t each = std::max<int64_t>(1, rounds * a.tokens * H / (4 * num_sms));
+      const int64_t each = (rounds * a.tokens * H + 4 * num_sms - 1) / (4 * num_sms);
       a.chunk = (int)std::min({rounds, each, (int64_t)kScoreMost / kScoreRound}) * kScoreRound;
       const int chunks = (sq.max_pages + a.chunk - 1) / a.chunk;
       with_value_type(q.type, [&](auto tb) {
@@ -645,9 +726,11 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
         else go(std::integral_constant<int, 8 * F>{});
       });
     }
-    const int hold = std::min(sq.max_pages, kPickKeys);
-    ATTNB_CUDA(launch_pdl(pick_kernel, dim3(a.tokens * H), dim3(kPickThreads), (size_t)hold * 8, s,
-                          a, hold));
+    const int hold = std::min(sq.max_pages, kPickKeys), rows = a.tokens * H;
+    if (sq.max_pages <= kWarpKeys)
+      ATTNB_CUDA(launch_pdl(pick_warp_kernel, dim3((rows + 3) / 4), dim3(128), 0, s, a));
+    else
+      ATTNB_CUDA(launch_pdl(pick_kernel, dim3(rows), dim3(kPickThreads), (size_t)hold * 8, s, a, hold));
   }
 }
 

@@ -204,11 +204,12 @@ __device__ __noinline__ float step_by_key(RowState& st, uint32_t sb, int kb0, in
 }
 
 template <int TQ, int TK, int DHP>
-__global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS, 1)
+__global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
     seq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ SeqAttnArgs a,
                   const bool qtma, const bool qvec, const bool ovec) {
-  constexpr bool CODED = TK == kE4M3 || TK == kI8;
+  constexpr bool CODED = elem_coded(TK), I4 = TK == kI4;
+  constexpr int ROWB = I4 ? DHP / 2 : 128;  // codes: bytes of a row as it comes
   using Cfg = TcCfg<CODED, DHP>;
   using EQ = elem_t<TQ>;
   constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
@@ -320,11 +321,11 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           const uint32_t bar = smem_addr(&rfull[ring.stage]);
           const int key0 = (hj >> 2) * BN + (hj & 1) * 64;
           int page = 0;  // of this lane's copy
-          uint32_t bytes = 64 * 128;
+          uint32_t bytes = 64 * ROWB;
           for (int i = 0; i < copies; ++i) {
             const int p = win.get(a, w.b, (key0 + i * box) >> shift, used);
             if (lane == i) page = p;
-            if (!is_v && p < a.pages.num_pages) bytes += 2 * box * 4;
+            if (p < a.pages.num_pages) bytes += ((is_v ? 0 : 2) + (I4 ? 1 : 0)) * box * 4;
           }
           const int my_key = key0 + lane * box;
           const bool there = page < a.pages.num_pages;
@@ -338,9 +339,13 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
           if (lane < copies) {
-            tma_load_4d(st + lane * box * 128, is_v ? &tmV : &tmK, bar, 0, my_key & mask, w.h, page);
+            tma_load_4d(st + lane * box * ROWB, is_v ? &tmV : &tmK, bar, 0, my_key & mask, w.h,
+                        page);
+            const int64_t at = (((int64_t)page * a.pages.H + w.h) << shift) + (my_key & mask);
+            if (I4 && there)
+              bulk_load(st + 64 * 128 + 512 + lane * box * 4,
+                        (is_v ? a.pages.v_group : a.pages.k_group) + at * 4, box * 4, bar);
             if (!is_v && there) {
-              const int64_t at = (((int64_t)page * a.pages.H + w.h) << shift) + (my_key & mask);
               bulk_load(st + 64 * 128 + lane * box * 4, a.pages.k_scale + at, box * 4, bar);
               bulk_load(st + 64 * 128 + 256 + lane * box * 4, a.pages.v_scale + at, box * 4, bar);
             }
@@ -703,6 +708,29 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
               const uint8_t* from = mem + Cfg::OFF_RAW + ring.stage * Cfg::RAW;
               const int r = hf * 64 + row;
               const bool gone = row >= w.s.L - j * BN - hf * 64;  // stale
+              if constexpr (I4) {
+                // 32 codes of one group; pairs of dimensions (0, 4), (1, 5), (2, 6), (3, 7) of
+                // each eight, the order that Q and the outputs follow.
+                const uint32_t factors =
+                    gone ? 0u : reinterpret_cast<const uint32_t*>(from + 64 * 128 + 512)[row];
+#pragma unroll 1
+                for (int i = 0; i < DHP / 64; ++i) {
+                  const int u = part * (DHP / 64) + i;
+                  const uint4 x = *reinterpret_cast<const uint4*>(from + sw_rows<ROWB>(row, u));
+                  const I4Factors f = i4_factors(__byte_perm(factors >> (8 * u), 0, 0x4040));
+                  const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                  uint8_t* ch = to + (u >> 1) * Cfg::CHUNK;
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const uint32_t lo = xs[k], hi = xs[k] >> 8;
+                    *reinterpret_cast<uint4*>(ch + sw128(r, (u & 1) * 4 + k)) =
+                        make_uint4(fma_f16x2(lo & kI4Low, f.low, f.add),
+                                   fma_f16x2(lo & kI4High, f.high, f.add),
+                                   fma_f16x2(hi & kI4Low, f.low, f.add),
+                                   fma_f16x2(hi & kI4High, f.high, f.add));
+                  }
+                }
+              } else
 #pragma unroll 1  // (the instruction cache, see the softmax)
               for (int i = 0; i < DHP / 32; ++i) {
                 const int u = part * (DHP / 32) + i;  // 16 codes
@@ -784,17 +812,18 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
             for (int b = 0; b < 8; ++b) top = fmaxf(top, fabsf(to_float(e[b])));
           }
           f = row_scale(top);
-          scale = a.scale_log2 / f;
+          scale = a.scale_log2 * (I4 ? kI4Unit : 1.f) / f;
         }
 #pragma unroll 4
         for (int u = 0; u < DHP / 8; ++u) {
           uint4 x = unit(u);
           if constexpr (CODED) {
             const EQ* e = reinterpret_cast<const EQ*>(&x);
-            x = make_uint4(pack_f16(to_float(e[0]) * f, to_float(e[1]) * f),
-                           pack_f16(to_float(e[2]) * f, to_float(e[3]) * f),
-                           pack_f16(to_float(e[4]) * f, to_float(e[5]) * f),
-                           pack_f16(to_float(e[6]) * f, to_float(e[7]) * f));
+            auto two = [&](int b) {  // 4-bit codes: dimensions b / 2 and b / 2 + 4
+              return pack_f16(to_float(e[I4 ? b / 2 : b]) * f,
+                              to_float(e[I4 ? b / 2 + 4 : b + 1]) * f);
+            };
+            x = make_uint4(two(0), two(2), two(4), two(6));
           }
           *reinterpret_cast<uint4*>(qt + (u >> 3) * Cfg::CHUNK + sw128(r, u & 7)) = x;
         }
@@ -989,6 +1018,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
         // Two factors: 2^rho may lie below the smallest fp32 number.
         const float half_rho = CODED ? fast_exp2(0.5f * rho) : 1.f;
         mulo *= half_rho;
+        if constexpr (I4) mulo *= kI4Unit;
         const int* ps = reinterpret_cast<const int*>(mem + Cfg::OFF_X) + (piece % kPoison) * 3 * DHP;
         const bool hit = !CODED && *(volatile int*)&poison_set[piece % kPoison] != 0;
         const int64_t prow = (int64_t)slot * a.rows + c * half + r;
@@ -1013,6 +1043,13 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
           for (int i = 0; i < 32; ++i) {
             const float x = __uint_as_float(o[i]);
             o[i] = __float_as_uint((CODED ? x * half_rho : x) * mulo);
+          }
+          if constexpr (I4) {  // in the order of the dimensions
+            uint32_t t[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) t[i] = o[(i & ~7) + (i & 3) * 2 + ((i >> 2) & 1)];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = t[i];
           }
           if (hit) {
 #pragma unroll
@@ -1092,7 +1129,7 @@ __global__ void __launch_bounds__(TcCfg<TK == kE4M3 || TK == kI8, DHP>::THREADS,
 template <int TQ, int TK, int DHP>
 void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& q, const CUtensorMap& k,
             const CUtensorMap& v, bool qtma, bool qvec, bool ovec, cudaStream_t s) {
-  using Cfg = TcCfg<TK == kE4M3 || TK == kI8, DHP>;
+  using Cfg = TcCfg<elem_coded(TK), DHP>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   ATTNB_CUDA(cudaGetDevice(&dev));
@@ -1128,7 +1165,6 @@ CUtensorMap rows_map(const RowsView& r, int heads, int tokens) {
 }  // namespace
 
 bool seq_tc_supported(const SeqAttnArgs& a) {
-  if (a.pages.k && a.pages.type == kI4) return false;
   if (a.q.type == kF32 || a.G > BM || a.q.Dh > 128 || a.q.Dh % 8 != 0) return false;
   if (a.pages.k) return seq_pages_tma(a);
   return map_allowed(a.k) && map_allowed(a.v);
@@ -1155,6 +1191,7 @@ void seq_tc_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   with_value_type(a.q.type, [&](auto tq) {
     if (a.pages.k && a.pages.type == kE4M3) go(tq, std::integral_constant<int, kE4M3>{});
     else if (a.pages.k && a.pages.type == kI8) go(tq, std::integral_constant<int, kI8>{});
+    else if (a.pages.k && a.pages.type == kI4) go(tq, std::integral_constant<int, kI4>{});
     else go(tq, tq);
   });
 }

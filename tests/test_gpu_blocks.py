@@ -181,40 +181,44 @@ def test_one_long_context(cuda, dtype, kind, new):
         _attended(p, q, blocks, [new], keys, dtype, 0.1)
 
 
-def test_ties_go_to_the_lower_block(cuda):
-    """Blocks of equal bounds, more than a round of the selection holds, and all of them zero."""
-    keys, page, D = [16 * 700], 16, 64
+@pytest.mark.parametrize("n", [300, 512, 513, 700, 5000])
+def test_ties_go_to_the_lower_block(cuda, n):
+    """Blocks of equal bounds, as many as each form of the selection takes, and all of them zero."""
+    keys, page, D = [16 * n], 16, 64
     p = _filled(keys, 1, D, page, BF16, BF16)
     _bound(p, keys)
     q = _randn(_gen(2), 1, 2, D, dtype=BF16)
     at = p.table[0].long()
     p.bounds[at] = p.bounds[at[0]].clone()
-    p.bounds[at[500]] += 1  # a better one, and a worse one
+    p.bounds[at[200]] += 1  # a better one, and a worse one
     p.bounds[at[3]] -= 1
-    s = more.scores(q[0], *p.bounds[at[[0, 500, 3]], 0].unbind(1))
+    s = more.scores(q[0], *p.bounds[at[[0, 200, 3]], 0].unbind(1))
     better, worse = (s[1] > s[0]), (s[2] < s[0])
-    blocks = _select(p, q, [1], 300, 1, 1)[0, 0].tolist()
-    assert blocks == _wanted(p, q, [1], keys, 300, 1, 1)[0, 0].tolist()
-    assert (500 in blocks) == bool(better) and (3 not in blocks) == bool(worse)
+    blocks = _select(p, q, [1], 150, 1, 1)[0, 0].tolist()
+    assert blocks == _wanted(p, q, [1], keys, 150, 1, 1)[0, 0].tolist()
+    assert (200 in blocks) == bool(better) and (3 not in blocks) == bool(worse)
     p.bounds.zero_()
-    assert _select(p, q, [1], 9, 2, 3)[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 697, 698, 699]
+    assert _select(p, q, [1], 9, 2, 3)[0, 0].tolist() == [0, 1, 2, 3, 4, 5, n - 3, n - 2, n - 1]
     p.bounds[at[[50, 60]]] = float("nan")  # the greatest
-    assert _select(p, q, [1], 9, 2, 3)[0, 0].tolist() == [0, 1, 2, 3, 50, 60, 697, 698, 699]
+    assert _select(p, q, [1], 9, 2, 3)[0, 0].tolist() == [0, 1, 2, 3, 50, 60, n - 3, n - 2, n - 1]
 
 
-def test_scores_next_to_each_other(cuda):
-    """Scores that differ in the last place of fp32 are told apart."""
-    keys, page, D = [16 * 64], 16, 64
+@pytest.mark.parametrize("n", [64, 700])
+def test_scores_next_to_each_other(cuda, n):
+    """Scores that differ in the last place of fp32 are told apart, next to one far off the others."""
+    keys, page, D = [16 * n], 16, 64
     p = _filled(keys, 1, D, page, F32, F32)
     p.bounds.zero_()
     at = p.table[0].long()
-    one = torch.full((64,), 1000.0, device="cuda")
+    one = torch.full((n,), 1000.0, device="cuda")
+    one[45] = -1e30
     one[20:40] = torch.nextafter(one[20:40], one[20:40] * 2)
     p.bounds[at, 0, :, 0] = one[:, None]
     p.bounds[at, 0, :, 1] = 16777216.0  # the same for all, far greater
     q = torch.zeros(1, 1, D, device="cuda")
     q[0, 0, :2] = 1
-    assert _select(p, q, [1], 12, 1, 1)[0, 0].tolist() == [0] + list(range(20, 30)) + [63]
+    assert _select(p, q, [1], 12, 1, 1)[0, 0].tolist() == [0] + list(range(20, 30)) + [n - 1]
+    assert _select(p, q, [1], 50, 1, 1)[0, 0].tolist() == [j for j in range(50) if j != 45] + [n - 1]
 
 
 def test_lists_of_the_callers_own(cuda):
