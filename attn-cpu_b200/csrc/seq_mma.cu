@@ -109,6 +109,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// f16 products added to (c0, c1, c0, c1) instead of d.
+__device__ __forceinline__ void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                              float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+
 // An 8 x 8 tile of 16-bit values, transposed across the warp.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t r;
@@ -419,10 +430,10 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                   // The codes as they are, 1 to 15: their sum starts at that of -8 q.
-                  const float* o = off[r][k + e];
-                  float t[4] = {o[0], o[1], o[0], o[1]};
-                  mma16816<false>(t, x & kI4Low, y & kI4Low, x & kI4High, y & kI4High,
-                                  q[r][2 * (k + e)][0], q[r][2 * (k + e)][1]);
+                  float t[4];
+                  mma16816_from(t, x & kI4Low, y & kI4Low, x & kI4High, y & kI4High,
+                                q[r][2 * (k + e)][0], q[r][2 * (k + e)][1], off[r][k + e][0],
+                                off[r][k + e][1]);
                   mma16816<false>(t, x8 & kI4Low, y8 & kI4Low, x8 & kI4High, y8 & kI4High,
                                   q[r][2 * (k + e) + 1][0], q[r][2 * (k + e) + 1][1]);
 #pragma unroll
@@ -476,13 +487,55 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         uint32_t p[NH][NR][2];
         bool moved = false;
         float alpha[NR][2];  // what acc is multiplied by
+        if constexpr (I4) {
+          // As below, with fewer instructions: the maximum is that of the scores as they are, an
+          // exponent is one FMA from the score (what m is off by is common to all weights
+          // of the row), and only tiles with a mask look for what it hides.
+          if (masked) {
+#pragma unroll
+            for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (key0 + hf * 16 + g + 8 * (e >> 1) >= seen[r][e & 1]) s[hf][r][e] = -INFINITY;
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float best = fmaxf(s[0][r][i], s[0][r][i + 2]);
+#pragma unroll
+              for (int hf = 1; hf < NH; ++hf)
+                best = fmaxf(best, fmaxf(s[hf][r][i], s[hf][r][i + 2]));
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+              const float top = fmaxf(m[r][i], best * mulq[r][i]);
+              const float use = top == -INFINITY ? 0.f : top;
+              if (m[r][i] != -INFINITY) rho[r][i] -= top - m[r][i];
+              l[r][i] *= fast_exp2(m[r][i] - use);
+              m[r][i] = top;
+              float most = -INFINITY;
+#pragma unroll
+              for (int k = 0; k < 2 * NH; ++k) {
+                float& at = s[k >> 1][r][i + 2 * (k & 1)];
+                const float x = fmaf(at, mulq[r][i], -use);
+                l[r][i] += fast_exp2(x);
+                // The scale of a masked key may be anything.
+                at = masked && x == -INFINITY ? x : x + lv[k];
+                most = fmaxf(most, at);
+              }
+              moved |= most - rho[r][i] > kRhoGap;
+            }
+        } else {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
 #pragma unroll
           for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if constexpr (CODED && !I4) s[hf][r][e] *= mulq[r][e & 1] * mulk[e >> 1];
+              if constexpr (CODED) s[hf][r][e] *= mulq[r][e & 1] * mulk[e >> 1];
               else s[hf][r][e] *= mulq[r][e & 1];
               if (masked && key0 + hf * 16 + g + 8 * (e >> 1) >= seen[r][e & 1])
                 s[hf][r][e] = -INFINITY;
@@ -522,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
               }
             }
           }
+        }
         }
         moved = __any_sync(0xffffffffu, moved);
         if constexpr (CODED) {
