@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -536,9 +537,10 @@ def _rows(t, name: str, device) -> Rows:
 
 def _offsets(t, name: str, device, n=None) -> int:
     """Device address of a contiguous int32 vector (of n entries)."""
-    if t.dtype != _torch.int32 or t.dim() != 1 or not t.is_contiguous():
+    shape = t.shape
+    if t.dtype != _torch.int32 or len(shape) != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector")
-    if n is not None and len(t) != n:
+    if n is not None and shape[0] != n:
         raise ValueError(f"{name} must have {n} entries, one more than sequences for offsets")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -546,38 +548,46 @@ def _offsets(t, name: str, device, n=None) -> int:
 
 
 def _pages(k_pages, v_pages, k_scale, v_scale, device, k_group=None, v_group=None) -> KvPages:
-    shape = k_pages.shape
-    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or dtype != v_pages.dtype:
         raise ValueError("k_pages and v_pages must be [pages, H, page_size, Dh] of one type")
     n, H, page, Dh = shape
-    ty = _TYPES.get(k_pages.dtype)
+    ty = _TYPES.get(dtype)
     if ty is None:
-        raise ValueError(f"k_pages: {k_pages.dtype} is not supported")
-    at = []
-    for t in (k_pages, v_pages, k_scale, v_scale):
-        if t is None:
-            at.append(None)
-            continue
-        if t.device != device:
-            raise ValueError(f"pages and scales must be on {device}, not on {t.device}")
-        if not t.is_contiguous():
-            raise ValueError("pages and scales must be contiguous")
-        if len(at) >= 2 and (t.dtype != _torch.float32 or t.shape != shape[:3]):
-            raise ValueError("k_scale and v_scale must be float32 [pages, H, page_size]")
-        at.append(t.data_ptr())
+        raise ValueError(f"k_pages: {dtype} is not supported")
+    ks = vs = None
+    if k_pages.device != device or v_pages.device != device:
+        raise ValueError(f"pages and scales must be on {device}, not on {k_pages.device} "
+                         f"and {v_pages.device}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("pages and scales must be contiguous")
+    if k_scale is not None:
+        ks = _scales(k_scale, (n, H, page), device)
+    if v_scale is not None:
+        vs = ks if v_scale is k_scale else _scales(v_scale, (n, H, page), device)
     if ty != _I4:
         if k_group is not None or v_group is not None:
             raise ValueError("only uint8 pages have k_group and v_group")
-        return KvPages(*at, ty, n, H, page, Dh)
+        return KvPages(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, ty, n, H, page, Dh)
     Dh *= 2
-    want = (n, H, page, i4_group_bytes(Dh))
+    want = (n, H, page, 4 * -(-Dh // 128))
     for t in (k_group, v_group):
         if t is None or t.dtype != _torch.uint8 or t.shape != want or not t.is_contiguous():
             raise ValueError(f"uint8 pages need k_group and v_group, contiguous uint8 {want}")
         if t.device != device:
             raise ValueError(f"pages and factors must be on {device}, not on {t.device}")
-        at.append(t.data_ptr())
-    return KvPages(*at[:4], ty, n, H, page, Dh, *at[4:])
+    return KvPages(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, ty, n, H, page, Dh,
+                   k_group.data_ptr(), v_group.data_ptr())
+
+
+def _scales(t, shape, device) -> int:
+    if t.device != device:
+        raise ValueError(f"pages and scales must be on {device}, not on {t.device}")
+    if not t.is_contiguous():
+        raise ValueError("pages and scales must be contiguous")
+    if t.dtype != _torch.float32 or t.shape != shape:
+        raise ValueError("k_scale and v_scale must be float32 [pages, H, page_size]")
+    return t.data_ptr()
 
 
 def i4_group_bytes(Dh: int) -> int:
@@ -586,12 +596,15 @@ def i4_group_bytes(Dh: int) -> int:
 
 
 def _seqs(cu, table, lens, device) -> Seqs:
-    if table.dtype != _torch.int32 or table.dim() != 2 or table.device != device or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != _torch.int32 or table.device != device:
         raise ValueError(f"table must be int32 [sequences, pages] on {device}, rows contiguous")
-    batch, width = table.shape
-    return Seqs(_offsets(cu, "cu", device, batch + 1), batch, table.data_ptr(), table.stride(0),
-                width, _offsets(lens, "lens", device, batch))
+    batch, width = shape
+    stride, step = table.stride()
+    if width > 1 and step != 1:
+        raise ValueError(f"table must be int32 [sequences, pages] on {device}, rows contiguous")
+    return Seqs(_offsets(cu, "cu", device, batch + 1), batch, table.data_ptr(), stride, width,
+                _offsets(lens, "lens", device, batch))
 
 
 def _workspace(device, q_heads: int, kv_heads: int, Dh: int):
@@ -743,11 +756,18 @@ def _lists(blocks, tokens: int, heads: int, device) -> int:
     return blocks.data_ptr()
 
 
-def _blocks_workspace(device, tokens, q_heads, kv_heads, Dh, take, max_pages):
+@functools.lru_cache(maxsize=4096)
+def _blocks_bytes(index, tokens, q_heads, kv_heads, Dh, take, max_pages) -> int:
     size = ctypes.c_size_t()
     check(_lib.attnb_blocks_workspace(tokens, q_heads, kv_heads, Dh, take, max_pages,
                                       ctypes.byref(size)))
-    return _torch.empty(size.value, dtype=_torch.uint8, device=device), size.value
+    return size.value
+
+
+def _blocks_workspace(device, tokens, q_heads, kv_heads, Dh, take, max_pages):
+    """As _workspace, for the selection of blocks and attention to them."""
+    n = _blocks_bytes(device.index, tokens, q_heads, kv_heads, Dh, take, max_pages)
+    return _torch.empty(n, dtype=_torch.uint8, device=device), n
 
 
 def kv_blocks_bounds_dev(k_pages, bounds, cu, table, lens, k_scale=None, k_group=None,
