@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kBoundsThreads)
   __shared__ int before[kBoundsThreads], block0[kBoundsThreads];
   __shared__ float2 part[kBoundsThreads / 32][256];
   const int tid = threadIdx.x, page = 1 << pg.page_shift;
+  grid_dep_launch();
   grid_dep_wait();
   for (int b0 = 0; b0 < sq.batch; b0 += kBoundsThreads) {
     int j0 = 0, count = 0;
@@ -364,6 +365,7 @@ constexpr int kWarpKeys = 512;
 __global__ void __launch_bounds__(128) pick_warp_kernel(const BlockArgs a) {
   constexpr int EACH = kWarpKeys / 32;
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  grid_dep_launch();
   grid_dep_wait();
   if (row >= a.tokens * a.H) return;
   unsigned long long found =
@@ -441,6 +443,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
   __shared__ int few_at[kPickThreads];
   extern __shared__ uint64_t mine[];
   const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dep_launch();
   grid_dep_wait();
   const TokenPlace at =
       block_token(a.seqs, a.page_shift, a.token0 + row / a.H, &found, a.index_status);
@@ -619,6 +622,7 @@ __global__ void __launch_bounds__(256)
     lists_kernel(const SeqTable sq, const KvPages pg, const int32_t* blocks, int take, int32_t* pages,
                  int32_t* lens, int* index_status) {
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  grid_dep_launch();
   grid_dep_wait();
   if (row >= sq.total * pg.H) return;
   unsigned long long found = find_token(sq, pg.page_shift, row / pg.H, lane, 32, index_status);

@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     tma_prefetch_desc(&tmV);
   }
   for (int i = threadIdx.x; i < 3 * DHP; i += kThreads) poison[i] = INT_MAX;
+  grid_dep_launch();
   grid_dep_wait();
   SeqPlace place;
   const bool any = seq_locate(a, sh, place);  // synchronises the block
