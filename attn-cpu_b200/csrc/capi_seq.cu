@@ -316,8 +316,7 @@ int attnb_blocks_workspace(int tokens, int q_heads, int kv_heads, int Dh, int ta
     if (tokens < 0 || max_pages < 0) invalid("tokens and max_pages must be non-negative");
     if (take <= 0) invalid("take must be positive");
     *bytes = std::max(kv_blocks_workspace_bytes(tokens, kv_heads, max_pages),
-                      seq_blocks_workspace_bytes(tokens, kv_heads, q_heads / kv_heads, Dh, take,
-                                                 current_ctx().num_sms));
+                      seq_workspace_bytes(q_heads / kv_heads, Dh, current_ctx().num_sms));
   });
 }
 

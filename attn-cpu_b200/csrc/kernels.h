@@ -266,11 +266,12 @@ struct SeqAttnArgs {
   int G;                // query heads per KV head
   int causal;
   float scale_log2;     // softmax scale times log2(e)
-  // Attention to selected blocks (sel_heads > 0, else 0): "sequence" v of the schedule is
-  // one token's query heads of one KV head, v = token * sel_heads + KV head.  Row v of
-  // seqs.table holds its pages, seqs.lens[v] how many keys they have for it (-1: no such
-  // row), and each counts for sel_tiles tiles on the line whatever it has.
-  int sel_heads, sel_tiles;
+  // Attention to selected blocks (sel_blocks given): "sequence" v of the schedule is one
+  // token's query heads of one KV head, v = token * pages.H + KV head, with the list
+  // sel_blocks + v * sel_take; each counts for sel_tiles tiles on the line whatever it
+  // has.
+  const int32_t* sel_blocks;
+  int sel_take, sel_tiles;
   // Schedule: rows per item, log2 of the keys per tile, fewest tiles per CTA,
   // tiles that an item counts for besides its own.
   int rows, kt_shift, min_tiles, extra;
@@ -291,7 +292,6 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
 
 // The same over blocks of its own for each token and KV head: blocks [tokens][H][take],
 // ascending, -1 behind the last one.  a.pages and a.seqs as for seq_attn_run.
-size_t seq_blocks_workspace_bytes(int tokens, int H, int G, int Dh, int take, int num_sms);
 void seq_attn_blocks_run(SeqAttnArgs a, const int32_t* blocks, int take, void* ws, size_t ws_bytes,
                          int num_sms, cudaStream_t s);
 
@@ -306,11 +306,6 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
                           int page_shift, const SeqTable& sq, int keep_first, int keep_last,
                           int32_t* blocks, int take, void* ws, size_t ws_bytes, int* index_status,
                           int num_sms, cudaStream_t s);
-// Lists as page numbers [tokens * H][take] and keys that they hold for their token
-// [tokens * H] (-1: a row of no sequence).
-void kv_blocks_lists_launch(const SeqTable& sq, const KvPages& pg, const int32_t* blocks, int take,
-                            int32_t* pages, int32_t* lens, int* index_status, cudaStream_t s);
-
 // The kernels (K6: any type, stride and head size up to 256).
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
 // K7: 16-bit queries over 16-bit or coded pages, 8 or 16 rows per item.

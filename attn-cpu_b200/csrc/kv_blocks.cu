@@ -237,22 +237,14 @@ __device__ __forceinline__ uint64_t sort_key(double x) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// A CTA takes up to kScoreMost blocks of a token and KV head: eight lanes a block, each with
-// every eighth unit of 16 bytes of its bounds, two blocks in flight.  The queries' sums are
-// read from shared memory: in registers they would leave too few CTAs an SM for the
-// latency of the reads that come before the bounds (32 us for 32 sequences of 8000-32768 keys).
-// NU: units a lane.
+// Sums of the queries' negative and positive parts over the query heads of a KV head: q-, q+, zeros.
+// The eight lanes that read at once find their pairs side by side.
 template <int TB, int NU>
-__global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(const BlockArgs a, const bool vec) {
+__device__ __forceinline__ void query_parts(const BlockArgs& a, int t, int h, double* parts) {
   using EB = elem_t<TB>;
   constexpr int PER = 16 / sizeof(EB);
-  __shared__ __align__(16) double parts[NU * 8 * PER];  // q-, q+, zeros
-  __shared__ int pages[kScoreMost];
-  __shared__ unsigned long long found;
-  const int tid = threadIdx.x, row = blockIdx.y, t = row / a.H, h = row - t * a.H;
   const int Dh = a.q.Dh;
-  grid_dep_wait();
-  for (int d = tid; d < NU * 8 * PER; d += kScoreThreads) {
+  for (int d = threadIdx.x; d < NU * 8 * PER; d += kScoreThreads) {
     const bool high = d >= Dh;
     double sum = 0.0;
     if (d < 2 * Dh) {
@@ -264,18 +256,23 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(c
         sum += (double)(high ? (x < 0.f ? 0.f : x) : (x > 0.f ? 0.f : x));
       }
     }
-    // Pairs of the eight lanes that read at once lie side by side.
     parts[((d / (8 * PER) * (PER / 2) + d % PER / 2) * 8 + d / PER % 8) * 2 + d % 2] = sum;
   }
-  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
-  if (at.b < 0 || at.pos < 0) return;
-  const int own = at.pos >> a.page_shift;
-  if (own + 1 <= a.take) return;  // all of them
-  const int from = a.keep_first + blockIdx.x * a.chunk;
-  const int to = min(own + 1 - a.keep_last, from + a.chunk);
-  if (from >= to) return;
+}
+
+// Scores of blocks [from, to) of sequence b, at most kScoreMost, to put(block, key): eight lanes a
+// block, each with every eighth unit of 16 bytes of its bounds, two blocks in flight.  The
+// queries' sums are read from shared memory: in registers they would leave too few CTAs an SM
+// for the latency of the reads that come before the bounds (32 us for 32 sequences of
+// 8000-32768 keys).  NU: units a lane.  All threads call.
+template <int TB, int NU, class Put>
+__device__ __forceinline__ void score_blocks(const BlockArgs& a, int b, int h, int from, int to,
+                                             bool vec, const double* parts, int* pages, Put put) {
+  using EB = elem_t<TB>;
+  constexpr int PER = 16 / sizeof(EB);
+  const int tid = threadIdx.x, e = tid & 7, Dh = a.q.Dh;
   for (int j = from + tid; j < to; j += kScoreThreads) {
-    int page = __ldg(a.seqs.table + at.b * a.seqs.table_stride + j);
+    int page = __ldg(a.seqs.table + b * a.seqs.table_stride + j);
     if (page < 0 || page >= a.num_pages) {
       raise_index(a.index_status);  // bounds of zeros
       page = -1;
@@ -283,8 +280,6 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(c
     pages[j - from] = page;
   }
   __syncthreads();
-  const int e = tid & 7;
-  uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages;
   for (int j0 = from; j0 < to; j0 += kScoreRound) {
     uint4 y[2][NU];
 #pragma unroll
@@ -327,9 +322,31 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : 1) score_kernel(c
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
       const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
-      if (e == 0 && j < to) keys[j] = sort_key(s[k]);
+      if (e == 0 && j < to) put(j, sort_key(s[k]));
     }
   }
+}
+
+// A CTA takes a.chunk blocks of a token and KV head.
+template <int TB, int NU>
+__global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : NU <= 8 ? 2 : 1)
+    score_kernel(const BlockArgs a, const bool vec) {
+  __shared__ __align__(16) double parts[NU * 8 * 16 / sizeof(elem_t<TB>)];
+  __shared__ int pages[kScoreMost];
+  __shared__ unsigned long long found;
+  const int row = blockIdx.y, t = row / a.H, h = row - t * a.H;
+  grid_dep_wait();
+  query_parts<TB, NU>(a, t, h, parts);
+  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
+  if (at.b < 0 || at.pos < 0) return;
+  const int own = at.pos >> a.page_shift;
+  if (own + 1 <= a.take) return;  // all of them
+  const int from = a.keep_first + blockIdx.x * a.chunk;
+  const int to = min(own + 1 - a.keep_last, from + a.chunk);
+  if (from >= to) return;
+  uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages;
+  score_blocks<TB, NU>(a, at.b, h, from, to, vec, parts, pages,
+                       [&](int j, uint64_t key) { keys[j] = key; });
 }
 
 // ------------------------------------------------------------------ choice
@@ -357,26 +374,15 @@ __device__ __forceinline__ int plain_part(const BlockArgs& a, const TokenPlace& 
   return a.take - a.keep_first - a.keep_last;  // < n
 }
 
-// Up to kWarpKeys blocks a row: a warp for a token and a KV head, keys in registers.  The key that
+// The `want` greatest of up to kWarpKeys keys, by one warp with the keys in registers.  The key that
 // is taken last is built from its first bit that not all keys share, each bit set if enough
 // keys are still at or above; it ends where as many are as are wanted.  (1064 rows of 80-310
 // keys: 23 us with a CTA each.)
 constexpr int kWarpKeys = 512;
-__global__ void __launch_bounds__(128) pick_warp_kernel(const BlockArgs a) {
+__device__ __forceinline__ void pick_warp(const uint64_t* keys, int n, int want, int keep_first,
+                                          int32_t* out) {
   constexpr int EACH = kWarpKeys / 32;
-  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  grid_dep_launch();
-  grid_dep_wait();
-  if (row >= a.tokens * a.H) return;
-  unsigned long long found =
-      find_token(a.seqs, a.page_shift, a.token0 + row / a.H, lane, 32, a.index_status);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) found = max(found, __shfl_xor_sync(0xffffffffu, found, o));
-  int32_t* out = nullptr;
-  int n = 0;
-  const int want = plain_part(a, token_place(found), row, out, n, lane, 32);
-  if (want == 0) return;
-  const uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first;
+  const int lane = threadIdx.x & 31;
   uint64_t k[EACH], lo = ~0ull, hi = 0;  // no key is 0
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -422,41 +428,47 @@ __global__ void __launch_bounds__(128) pick_warp_kernel(const BlockArgs a) {
     const unsigned eq = __ballot_sync(0xffffffffu, equal);
     const bool taken = k[i] > last || (equal && same + __popc(eq & before) < rest);
     const unsigned tk = __ballot_sync(0xffffffffu, taken);
-    if (taken) out[at + __popc(tk & before)] = a.keep_first + i * 32 + lane;
+    if (taken) out[at + __popc(tk & before)] = keep_first + i * 32 + lane;
     at += __popc(tk);
     same += __popc(eq);
   }
 }
 
-// One CTA for a token and a KV head; up to `hold` keys are read once.  The key that is taken last
-// is found by a histogram over equal parts of the scores' range and the ranks of the few in its
-// part; where that part is full (many equal scores, or scores far off the others) or the
-// range is not finite, by digits of 8 bits from the first bit in which keys differ.
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, const int hold) {
+// The `want` greatest of n keys, by a block; up to `hold` keys from global memory are put in `mine`
+// (null: they are read from where they are).  The key that is taken last is found by a
+// histogram over equal parts of the scores' range and the ranks of the few in its part; where that
+// part is full (many equal scores, or scores far off the others) or the range is not
+// finite, by digits of 8 bits from the first bit in which keys differ.
+template <int kPickThreads>
+struct PickShared {
+  static constexpr int W = kPickThreads / 32;
+  int hist[kPickParts];
+  int warp_sum[W], warp_eq[W];
+  uint64_t warp_lo[W], warp_hi[W];
+  uint64_t few_key[kPickThreads], last_key;
+  int few_at[kPickThreads];
+  int digit, left, few;
+};
+template <int kPickThreads>
+__device__ __forceinline__ void pick_block(const uint64_t* keys, uint64_t* mine, int hold, int n,
+                                           int want, int keep_first, int32_t* out,
+                                           PickShared<kPickThreads>& sh) {
   constexpr int W = kPickThreads / 32;
-  __shared__ int hist[kPickParts];
-  __shared__ int warp_sum[W], warp_eq[W];
-  __shared__ uint64_t warp_lo[W], warp_hi[W];
-  __shared__ int digit, left, few;
-  __shared__ unsigned long long found;
-  __shared__ uint64_t few_key[kPickThreads], last_key;
-  __shared__ int few_at[kPickThreads];
-  extern __shared__ uint64_t mine[];
-  const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_dep_launch();
-  grid_dep_wait();
-  const TokenPlace at =
-      block_token(a.seqs, a.page_shift, a.token0 + row / a.H, &found, a.index_status);
-  int32_t* out = nullptr;
-  int n = 0;
-  const int want = plain_part(a, at, row, out, n, tid, kPickThreads);
-  if (want == 0) return;
-  const uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first;
+  int(&hist)[kPickParts] = sh.hist;
+  int(&warp_sum)[W] = sh.warp_sum;
+  int(&warp_eq)[W] = sh.warp_eq;
+  uint64_t(&warp_lo)[W] = sh.warp_lo;
+  uint64_t(&warp_hi)[W] = sh.warp_hi;
+  uint64_t(&few_key)[kPickThreads] = sh.few_key;
+  int(&few_at)[kPickThreads] = sh.few_at;
+  int &digit = sh.digit, &left = sh.left, &few = sh.few;
+  uint64_t& last_key = sh.last_key;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint64_t lo = ~0ull, hi = 0;
 #pragma unroll 4
   for (int i = tid; i < n; i += kPickThreads) {
     const uint64_t k = keys[i];
-    if (n <= hold) mine[i] = k;
+    if (mine && n <= hold) mine[i] = k;
     lo = min(lo, k);
     hi = max(hi, k);
   }
@@ -476,7 +488,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
     lo = min(lo, warp_lo[w]);
     hi = max(hi, warp_hi[w]);
   }
-  if (n <= hold) keys = mine;
+  if (mine && n <= hold) keys = mine;
   // Sum over the threads up to this one.
   auto scan = [&](int sum) {
 #pragma unroll
@@ -608,57 +620,61 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
     const int ab_before = above + __popc(ab & ((1u << lane) - 1));
     const int eq_before = same + __popc(eq & ((1u << lane) - 1));
     if (over || (equal && eq_before < rest))
-      out[ab_before + min(eq_before, rest)] = a.keep_first + i0 + lane;
+      out[ab_before + min(eq_before, rest)] = keep_first + i0 + lane;
     above += __popc(ab);
     same += __popc(eq);
   }
 }
 
-// ------------------------------------------------ lists to pages, for the attention
-// A warp for a token and a KV head: its list up to the first entry that is not above the
-// one before it or lies behind the token's own block, as page numbers, and how many keys
-// these hold for it.
-__global__ void __launch_bounds__(256)
-    lists_kernel(const SeqTable sq, const KvPages pg, const int32_t* blocks, int take, int32_t* pages,
-                 int32_t* lens, int* index_status) {
-  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+// A CTA for a token and a KV head whose scores are there.
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, const int hold) {
+  __shared__ PickShared<kPickThreads> sh;
+  __shared__ unsigned long long found;
+  extern __shared__ uint64_t mine[];
+  const int row = blockIdx.x;
   grid_dep_launch();
   grid_dep_wait();
-  if (row >= sq.total * pg.H) return;
-  unsigned long long found = find_token(sq, pg.page_shift, row / pg.H, lane, 32, index_status);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    found = max(found, __shfl_xor_sync(0xffffffffu, found, o));
-  const TokenPlace at = token_place(found);
-  const int b = at.b, pos = at.pos, own = pos < 0 ? -1 : pos >> pg.page_shift;
-  if (b < 0) {
-    if (lane == 0) lens[row] = -1;
-    return;
+  const TokenPlace at =
+      block_token(a.seqs, a.page_shift, a.token0 + row / a.H, &found, a.index_status);
+  int32_t* out = nullptr;
+  int n = 0;
+  const int want = plain_part(a, at, row, out, n, threadIdx.x, kPickThreads);
+  if (want == 0) return;
+  pick_block<kPickThreads>(a.keys + (int64_t)row * a.seqs.max_pages + a.keep_first, mine, hold, n,
+                           want, a.keep_first, out, sh);
+}
+
+// Scores and choice in one: a CTA for a token and a KV head, keys in shared memory.
+template <int TB, int NU>
+__global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : NU <= 8 ? 2 : 1)
+    select_kernel(const BlockArgs a, const bool vec) {
+  __shared__ __align__(16) double parts[NU * 8 * 16 / sizeof(elem_t<TB>)];
+  __shared__ union {
+    int pages[kScoreMost];
+    PickShared<kScoreThreads> pick;
+  } sh;
+  __shared__ unsigned long long found;
+  extern __shared__ uint64_t mine[];
+  const int row = blockIdx.x, t = row / a.H, h = row - t * a.H;
+  grid_dep_launch();
+  grid_dep_wait();
+  query_parts<TB, NU>(a, t, h, parts);
+  const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);
+  int32_t* out = nullptr;
+  int n = 0;
+  const int want = plain_part(a, at, row, out, n, threadIdx.x, kScoreThreads);
+  if (want == 0) return;
+  for (int from = 0; from < n; from += kScoreMost) {
+    if (from > 0) __syncthreads();  // the pages before have been read
+    score_blocks<TB, NU>(a, at.b, h, a.keep_first + from, a.keep_first + min(n, from + kScoreMost),
+                         vec, parts, sh.pages,
+                         [&](int j, uint64_t key) { mine[j - a.keep_first] = key; });
   }
-  const int32_t* list = blocks + (int64_t)row * take;
-  int last = -1, count = 0;
-  for (int i0 = 0; own >= 0 && i0 < take; i0 += 32) {
-    const int mine = i0 + lane < take ? __ldg(list + i0 + lane) : -1;
-    int prior = __shfl_up_sync(0xffffffffu, mine, 1);
-    if (lane == 0) prior = last;
-    const bool good = mine > prior && mine <= own;
-    const unsigned bad = __ballot_sync(0xffffffffu, !good);
-    const int n = bad ? __ffs(bad) - 1 : 32;
-    if (lane < n) {
-      const int page = seq_page(sq, pg, b, mine << pg.page_shift, index_status);
-      pages[(int64_t)row * take + i0 + lane] = page;
-    }
-    count += n;
-    if (n > 0) last = __shfl_sync(0xffffffffu, mine, n - 1);
-    if (n < 32) {
-      if (lane == n && i0 + lane < take && mine != -1) raise_index(index_status);
-      break;
-    }
-  }
-  if (lane == 0)
-    lens[row] = (count << pg.page_shift) -
-                (last == own && count > 0 ? (1 << pg.page_shift) - 1 - (pos & ((1 << pg.page_shift) - 1))
-                                          : 0);
+  __syncthreads();
+  if (n > kWarpKeys)
+    pick_block<kScoreThreads>(mine, nullptr, 0, n, want, a.keep_first, out, sh.pick);
+  else if (threadIdx.x < 32)
+    pick_warp(mine, n, want, a.keep_first, out);
 }
 
 size_t keys_per_token(int H, int max_pages) { return (size_t)H * std::max(max_pages, 1) * 8; }
@@ -712,37 +728,40 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
   const bool vec = reinterpret_cast<uintptr_t>(bounds) % 16 == 0 && 2 * q.Dh * eb % 16 == 0;
   for (a.token0 = 0; a.token0 < sq.total; a.token0 += a.tokens) {
     a.tokens = (int)std::min<size_t>(fit, sq.total - a.token0);
+    const int rows = a.tokens * H;
+    // f(type, units of 16 bytes a lane).
+    auto with_units = [&](auto&& f) {
+      with_value_type(q.type, [&](auto tb) {
+        constexpr int F = decltype(tb)::value == kF32 ? 2 : 1;
+        if (q.Dh <= 64) f(tb, std::integral_constant<int, 2 * F>{});
+        else if (q.Dh <= 128) f(tb, std::integral_constant<int, 4 * F>{});
+        else f(tb, std::integral_constant<int, 8 * F>{});
+      });
+    };
+    // One CTA a row where rows are short, or so many that they fill the machine; else the
+    // blocks of a row are spread over several.  (4 rows of 4096 blocks: 16 us against
+    // 40; 256 rows of 125-512: the other way round, 26 against 17.)
+    if (sq.max_pages <= kWarpKeys || (rows >= 2 * num_sms && sq.max_pages <= kPickKeys)) {
+      with_units([&](auto tb, auto nu) {
+        ATTNB_CUDA(launch_pdl(select_kernel<decltype(tb)::value, decltype(nu)::value>, dim3(rows),
+                              dim3(kScoreThreads), (size_t)sq.max_pages * 8, s, a, vec));
+      });
+      continue;
+    }
     if (sq.max_pages > take) {
       // Four CTAs an SM where there is that much to do.
       const int64_t rounds = (sq.max_pages + kScoreRound - 1) / kScoreRound;
-      const int64_t each = (rounds * a.tokens * H + 4 * num_sms - 1) / (4 * num_sms);
+      const int64_t each = (rounds * rows + 4 * num_sms - 1) / (4 * num_sms);
       a.chunk = (int)std::min({rounds, each, (int64_t)kScoreMost / kScoreRound}) * kScoreRound;
       const int chunks = (sq.max_pages + a.chunk - 1) / a.chunk;
-      with_value_type(q.type, [&](auto tb) {
-        constexpr int TB = decltype(tb)::value;
-        constexpr int F = TB == kF32 ? 2 : 1;
-        auto go = [&](auto nu) {
-          ATTNB_CUDA(launch_pdl(score_kernel<TB, decltype(nu)::value>, dim3(chunks, a.tokens * H),
-                                dim3(kScoreThreads), 0, s, a, vec));
-        };
-        if (q.Dh <= 64) go(std::integral_constant<int, 2 * F>{});
-        else if (q.Dh <= 128) go(std::integral_constant<int, 4 * F>{});
-        else go(std::integral_constant<int, 8 * F>{});
+      with_units([&](auto tb, auto nu) {
+        ATTNB_CUDA(launch_pdl(score_kernel<decltype(tb)::value, decltype(nu)::value>,
+                              dim3(chunks, rows), dim3(kScoreThreads), 0, s, a, vec));
       });
     }
-    const int hold = std::min(sq.max_pages, kPickKeys), rows = a.tokens * H;
-    if (sq.max_pages <= kWarpKeys)
-      ATTNB_CUDA(launch_pdl(pick_warp_kernel, dim3((rows + 3) / 4), dim3(128), 0, s, a));
-    else
-      ATTNB_CUDA(launch_pdl(pick_kernel, dim3(rows), dim3(kPickThreads), (size_t)hold * 8, s, a, hold));
+    const int hold = std::min(sq.max_pages, kPickKeys);
+    ATTNB_CUDA(launch_pdl(pick_kernel, dim3(rows), dim3(kPickThreads), (size_t)hold * 8, s, a, hold));
   }
-}
-
-void kv_blocks_lists_launch(const SeqTable& sq, const KvPages& pg, const int32_t* blocks, int take,
-                            int32_t* pages, int32_t* lens, int* index_status, cudaStream_t s) {
-  const int rows = sq.total * pg.H;
-  ATTNB_CUDA(launch_pdl(lists_kernel, dim3((rows + 7) / 8), dim3(256), 0, s, sq, pg, blocks, take,
-                        pages, lens, index_status));
 }
 
 }  // namespace attnb

@@ -17,7 +17,8 @@
 // not grow with the batch.
 //
 // Attention to selected blocks runs on the same line, with a "sequence" for each
-// token and KV head that has pages of its own.  These are many and much the same,
+// token and KV head: the keys of the blocks in its list, one block after the other.  These
+// are many and much the same,
 // so that each counts for as many tiles as the longest may have: a CTA finds its
 // place by one division, where the sum over their own lengths would cost more than
 // it evens out.
@@ -77,14 +78,6 @@ __device__ __forceinline__ int seq_of(const SeqTable& sq, int t, int& first, int
 
 __device__ __forceinline__ SeqInfo seq_info(const SeqAttnArgs& a, int b) {
   SeqInfo i;
-  if (a.sel_heads) {
-    const int len = __ldg(a.seqs.lens + b);
-    i.q0 = b / a.sel_heads;
-    i.n = len >= 0 ? 1 : 0;
-    i.k0 = 0;
-    i.L = max(len, 0);
-    return i;
-  }
   seq_rows(a.seqs.cu, b, a.seqs.total, i.q0, i.n);
   if (a.pages.k) {
     const int len = __ldg(a.seqs.lens + b);
@@ -219,11 +212,68 @@ __device__ __forceinline__ int sel_items(const SeqAttnArgs& a) {
 }
 __device__ __forceinline__ int sel_span(const SeqAttnArgs& a) { return a.sel_tiles + a.extra; }
 
+// What a token and KV head (row v of the lists) attend to.
+struct SelRow {
+  int b, L;  // sequence (-1: a row of none) and number of keys
+};
+
+// All lanes of a warp call.  The list ends at its first entry that is not above the one
+// before it or lies behind the token's own block; any but -1 there is told.
+__device__ __forceinline__ SelRow sel_row(const SeqAttnArgs& a, int v) {
+  const int lane = threadIdx.x & 31, t = v / a.pages.H, shift = a.pages.page_shift;
+  // The first entries of the list are on their way while the token's sequence is found.
+  const int32_t* list = a.sel_blocks + (int64_t)v * a.sel_take;
+  int mine = lane < a.sel_take ? __ldg(list + lane) : -1;
+  SelRow r{-1, 0};
+  int first = 0, count = 0;
+  if (a.seqs.batch <= 64) {  // two sequences a lane at most, all at once
+    for (int b0 = 0; b0 < a.seqs.batch && r.b < 0; b0 += 32) {
+      int f = 0, c = 0;
+      if (b0 + lane < a.seqs.batch) seq_rows(a.seqs.cu, b0 + lane, a.seqs.total, f, c);
+      const unsigned hit = __ballot_sync(0xffffffffu, t >= f && t < f + c);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        r.b = b0 + src;
+        first = __shfl_sync(0xffffffffu, f, src);
+        count = __shfl_sync(0xffffffffu, c, src);
+      }
+    }
+  } else {
+    r.b = seq_of(a.seqs, t, first, count);
+  }
+  if (r.b < 0) return r;
+  const int len = __ldg(a.seqs.lens + r.b);
+  const long long room = (long long)a.seqs.max_pages << shift;
+  if (len < 0 || len > room) raise_index(a.index_status);
+  const int pos = (int)min((long long)max(len, 0), room) - count + (t - first);
+  if (pos < 0) return r;
+  const int own = pos >> shift;
+  int last = -1, blocks = 0;
+  for (int i0 = 0;; ) {
+    int prior = __shfl_up_sync(0xffffffffu, mine, 1);
+    if (lane == 0) prior = last;
+    const unsigned bad = __ballot_sync(0xffffffffu, !(mine > prior && mine <= own));
+    const int n = bad ? __ffs(bad) - 1 : 32;
+    blocks += n;
+    if (n > 0) last = __shfl_sync(0xffffffffu, mine, n - 1);
+    if (n < 32) {
+      if (lane == n && i0 + lane < a.sel_take && mine != -1) raise_index(a.index_status);
+      break;
+    }
+    i0 += 32;
+    if (i0 >= a.sel_take) break;
+    mine = i0 + lane < a.sel_take ? __ldg(list + i0 + lane) : -1;
+  }
+  r.L = blocks << shift;
+  if (blocks > 0 && last == own) r.L -= (1 << shift) - 1 - (pos & ((1 << shift) - 1));
+  return r;
+}
+
 // All threads of the block; false when the CTA has nothing to do.
 __device__ inline bool seq_locate(const SeqAttnArgs& a, SeqShared& sh, SeqPlace& p) {
-  if (a.sel_heads) {
+  if (a.sel_blocks) {
     const int M = sel_items(a), span = sel_span(a);
-    const long long total = (long long)a.seqs.batch * M * span;
+    const long long total = (long long)a.seqs.total * a.pages.H * M * span;
     p.quota = max((long long)a.min_tiles, (long long)udiv(total + gridDim.x - 1, gridDim.x));
     p.t0 = p.quota * blockIdx.x;
     p.t1 = min(total, p.t0 + p.quota);
@@ -232,7 +282,7 @@ __device__ inline bool seq_locate(const SeqAttnArgs& a, SeqShared& sh, SeqPlace&
     const long long item = (long long)udiv(p.t0, span);
     p.b = (int)udiv(item, M);
     p.m = (int)(item - (long long)p.b * M);
-    p.h = p.b % a.sel_heads;
+    p.h = p.b % a.pages.H;
     p.item0 = item * span;
     p.j = (int)(p.t0 - p.item0);
     return true;
@@ -307,6 +357,7 @@ struct SeqPiece {
   SeqInfo s;
   int b, h, m, j0, j1, nt;
   int row0, rows;  // its rows [row0, row0 + rows) of the sequence's n * G
+  int v;           // selected blocks: row of the lists
   bool head;       // of the item that the CTA's first tile lies in
 };
 
@@ -329,7 +380,7 @@ struct SeqIterOf {
     fresh = head = true;
   }
   __device__ __forceinline__ bool next(const SeqAttnArgs& a, SeqPiece& w) {
-    if (SEL && a.sel_heads) return next_selected(a, w);
+    if (SEL && a.sel_blocks) return next_selected(a, w);
     while (t < t1) {
       if (fresh) {
         s = seq_info(a, b);
@@ -369,8 +420,10 @@ struct SeqIterOf {
   __device__ __forceinline__ bool next_selected(const SeqAttnArgs& a, SeqPiece& w) {
     const int span = sel_span(a), M = sel_items(a);
     while (t < t1) {
-      w.s = seq_info(a, b);
-      w.b = b;
+      const SelRow r = sel_row(a, b);
+      w.s = SeqInfo{b / a.pages.H, r.b >= 0 ? 1 : 0, 0, r.L};
+      w.b = r.b;
+      w.v = b;
       w.h = h;
       w.m = m;
       w.nt = seq_tiles(a, w.s, m);
@@ -386,7 +439,7 @@ struct SeqIterOf {
       if (++m == M) {
         m = 0;
         ++b;
-        if (++h == a.sel_heads) h = 0;
+        if (++h == a.pages.H) h = 0;
       }
       if (w.j1 > w.j0) return true;
     }
@@ -407,13 +460,19 @@ __device__ __forceinline__ int seq_slot(const SeqPiece& w) {
   return w.j0 == 0 && w.j1 == w.nt ? -1 : 2 * (int)blockIdx.x + (w.head ? 0 : 1);
 }
 
-// One thread of every CTA, those without work included.
+// The first warp of every CTA, those without work included.
 __device__ __forceinline__ void seq_write_split(const SeqAttnArgs& a, bool any,
                                                 const SeqPlace& p) {
   SeqSplit d{};
   d.extra = a.extra;
   if (any && p.j > a.extra) {
-    const SeqInfo s = seq_info(a, p.b);
+    SeqInfo s;
+    if (a.sel_blocks) {
+      const SelRow r = sel_row(a, p.b);
+      s = SeqInfo{p.b / a.pages.H, r.b >= 0 ? 1 : 0, 0, r.L};
+    } else {
+      s = seq_info(a, p.b);
+    }
     d.item0 = p.item0 + a.extra;
     d.item1 = d.item0 + seq_tiles(a, s, p.m);
     d.continues = s.n > 0 && p.t0 < d.item1;
@@ -423,7 +482,12 @@ __device__ __forceinline__ void seq_write_split(const SeqAttnArgs& a, bool any,
     d.row_token = s.q0;
     d.kv_head = p.h;
   }
-  reinterpret_cast<SeqSplit*>(a.ws_split)[blockIdx.x] = d;
+  if (threadIdx.x == 0) reinterpret_cast<SeqSplit*>(a.ws_split)[blockIdx.x] = d;
+}
+
+// The slot in its sequence's table that slot `i` of the piece's keys is.
+__device__ __forceinline__ int piece_slot(const SeqAttnArgs& a, const SeqPiece& w, int i) {
+  return a.sel_blocks ? __ldg(a.sel_blocks + (int64_t)w.v * a.sel_take + i) : i;
 }
 
 // The page that holds position `pos` of sequence b, or -1.

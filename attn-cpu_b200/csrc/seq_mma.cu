@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
   grid_dep_wait();
   SeqPlace place;
   const bool any = seq_locate(a, sh, place);  // synchronises the block
-  if (threadIdx.x == 0) seq_write_split(a, any, place);
+  if (threadIdx.x < 32) seq_write_split(a, any, place);
   if (!any) return;
   __syncthreads();
 
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         for (int i = 0; i < kKeys / 16; ++i) {
           if (i >= copies) break;
           const int at = j * kKeys + i * box;
-          page[i] = win.get(a, w.b, at >> shift, used);
+          page[i] = win.get<true>(a, w, at >> shift, used);
           if constexpr (CODED) {
             if (page[i] < a.pages.num_pages) {
               bytes += (I4 ? 4 : 2) * box * 4;

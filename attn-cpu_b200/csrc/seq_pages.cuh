@@ -11,19 +11,22 @@ namespace attnb {
 // The page numbers of a sequence, 32 at a time in the lanes of one warp: a tile
 // then costs no read of the table that anything waits for.
 struct PageWindow {
-  int b = -1, first = 0;  // window of sequence b from this slot on
+  int b = -1, first = 0;  // window of sequence b (selected blocks: of list b) from this slot on
   int page;               // this lane's slot
   // Number of the page at `slot` (the same for the whole warp; all lanes
   // call), num_pages, which lies outside the pool and reads as zeros, for slots
   // past `used` and for bad numbers.
-  __device__ __forceinline__ int get(const SeqAttnArgs& a, int seq, int slot, int used) {
-    if (seq != b || slot < first || slot >= first + 32) {
-      b = seq;
+  template <bool SEL>
+  __device__ __forceinline__ int get(const SeqAttnArgs& a, const SeqPiece& w, int slot, int used) {
+    const int of = SEL && a.sel_blocks ? w.v : w.b;
+    if (of != b || slot < first || slot >= first + 32) {
+      b = of;
       first = slot;
       const int mine = slot + (int)(threadIdx.x & 31);
       page = a.pages.num_pages;
       if (mine < used) {
-        const int p = __ldg(a.seqs.table + seq * a.seqs.table_stride + mine);
+        const int at = SEL ? piece_slot(a, w, mine) : mine;
+        const int p = __ldg(a.seqs.table + w.b * a.seqs.table_stride + at);
         if (p >= 0 && p < a.pages.num_pages) page = p;
         else raise_index(a.index_status);
       }

@@ -187,29 +187,18 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   run(a, kind, rows, at, at + ws_bytes, num_sms, s);
 }
 
-size_t seq_blocks_workspace_bytes(int tokens, int H, int G, int Dh, int take, int num_sms) {
-  return (size_t)tokens * H * ((size_t)take + 1) * 4 + 256 + seq_workspace_bytes(G, Dh, num_sms);
-}
-
 void seq_attn_blocks_run(SeqAttnArgs a, const int32_t* blocks, int take, void* ws, size_t ws_bytes,
                          int num_sms, cudaStream_t s) {
   if (a.seqs.batch == 0 || a.seqs.total == 0) return;
-  const uintptr_t end = reinterpret_cast<uintptr_t>(ws) + ws_bytes;
-  const size_t rows = (size_t)a.seqs.total * a.pages.H;
-  uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
-  int32_t* const pages = reinterpret_cast<int32_t*>(p);
-  int32_t* const lens = pages + rows * take;
-  p += rows * (take + 1) * 4;
-  if (p > end) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
-  kv_blocks_lists_launch(a.seqs, a.pages, blocks, take, pages, lens, a.index_status, s);
   // K6 or K7 take any number of rows; a token has few.
   const Kind kind = seq_mma_supported(a) ? kMma : kSimt;
-  a.sel_heads = a.pages.H;
   const int kt = kind == kMma ? seq_mma_key_shift(a) : 6;
+  a.sel_blocks = blocks;
+  a.sel_take = take;
   a.sel_tiles = (int)((((int64_t)take << a.pages.page_shift) + (1 << kt) - 1) >> kt);
-  a.causal = 0;  // the lengths are the token's own
-  a.seqs = SeqTable{nullptr, (int)rows, a.seqs.total, pages, take, take, lens};
-  run(a, kind, a.G, p, end, num_sms, s);
+  a.causal = 0;  // a list's keys are those that its token sees
+  const uintptr_t at = reinterpret_cast<uintptr_t>(ws);
+  run(a, kind, a.G, at, at + ws_bytes, num_sms, s);
 }
 
 }  // namespace attnb

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
   grid_dep_wait();
   SeqPlace place;
   const bool any = seq_locate(a, sh, place);
-  if (threadIdx.x == 0) seq_write_split(a, any, place);
+  if (threadIdx.x < 32) seq_write_split(a, any, place);
   if (!any) return;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -132,7 +132,9 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
         vs[u] = 1.f;
         if (key < w.s.L) {
           if (paged) {
-            const int page = seq_page(a.seqs, a.pages, w.b, key, a.index_status);
+            const int at_key = piece_slot(a, w, key >> a.pages.page_shift)
+                               << a.pages.page_shift;
+            const int page = seq_page(a.seqs, a.pages, w.b, at_key, a.index_status);
             if (page >= 0) {  // a bad page reads as zeros
               const int64_t at =
                   (((int64_t)page * a.pages.H + w.h) << a.pages.page_shift) + (key & page_mask);

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
   grid_dep_wait();
   SeqPlace place;
   const bool any = seq_locate(a, sh, place);  // synchronises the block
-  if (threadIdx.x == 0) seq_write_split(a, any, place);
+  if (threadIdx.x < 32) seq_write_split(a, any, place);
   if (!any) return;
   if (warp == 1) {
     tmem_alloc(smem_addr(&tmem_slot), 512);
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
           int page = 0;  // of this lane's copy
           uint32_t bytes = 64 * ROWB;
           for (int i = 0; i < copies; ++i) {
-            const int p = win.get(a, w.b, (key0 + i * box) >> shift, used);
+            const int p = win.get<false>(a, w, (key0 + i * box) >> shift, used);
             if (lane == i) page = p;
             if (p < a.pages.num_pages) bytes += ((is_v ? 0 : 2) + (I4 ? 1 : 0)) * box * 4;
           }
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
         int page = 0;
         if (paged)
           for (int i = 0; i < copies; ++i) {
-            const int p = win.get(a, w.b, (j * BN + i * box) >> shift, used);
+            const int p = win.get<false>(a, w, (j * BN + i * box) >> shift, used);
             if (lane == i) page = p;
           }
         if (lane == 0) mbar_arrive_expect_tx(bar, Cfg::TILE);

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dep_wait();
   SeqPlace place;
   const bool any = seq_locate(a, sh, place);
-  if (threadIdx.x == 0) seq_write_split(a, any, place);
+  if (threadIdx.x < 32) seq_write_split(a, any, place);
   if (!any) return;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
