@@ -89,7 +89,6 @@ __global__ void __launch_bounds__(kBoundsThreads)
   __shared__ int before[kBoundsThreads], block0[kBoundsThreads];
   __shared__ float2 part[kBoundsThreads / 32][256];
   const int tid = threadIdx.x, page = 1 << pg.page_shift;
-  grid_dep_launch();
   grid_dep_wait();
   for (int b0 = 0; b0 < sq.batch; b0 += kBoundsThreads) {
     int j0 = 0, count = 0;
@@ -632,7 +631,6 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const BlockArgs a, c
   __shared__ unsigned long long found;
   extern __shared__ uint64_t mine[];
   const int row = blockIdx.x;
-  grid_dep_launch();
   grid_dep_wait();
   const TokenPlace at =
       block_token(a.seqs, a.page_shift, a.token0 + row / a.H, &found, a.index_status);
@@ -656,7 +654,6 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : NU <= 8 ? 2 : 1)
   __shared__ unsigned long long found;
   extern __shared__ uint64_t mine[];
   const int row = blockIdx.x, t = row / a.H, h = row - t * a.H;
-  grid_dep_launch();
   grid_dep_wait();
   query_parts<TB, NU>(a, t, h, parts);
   const TokenPlace at = block_token(a.seqs, a.page_shift, a.token0 + t, &found, a.index_status);

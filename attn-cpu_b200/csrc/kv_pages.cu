@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(kThreads, ROPE ? 4 : 1)
   extern __shared__ __align__(16) float2 turns[];
   const int e = threadIdx.x % LANES, d = e * 8;
   const int Dh = pg.Dh;
-  grid_dep_launch();
   grid_dep_wait();
   const bool is_q = ROPE && (int)blockIdx.x < q_ctas;
   const int t0 = (blockIdx.x - (is_q ? 0 : q_ctas)) * tokens, n = min(tokens, sq.total - t0);
@@ -591,7 +590,6 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int64_t places[kMaxTokens];
   const int d = threadIdx.x % LANES * 8;
   const int Dh = pg.Dh;
-  grid_dep_launch();
   grid_dep_wait();
   const int t0 = blockIdx.x * tokens, n = min(tokens, sq.total - t0);
   find_places(sq, pg, t0, n, places, index_status);

@@ -269,9 +269,12 @@ __device__ __forceinline__ SelRow sel_row(const SeqAttnArgs& a, int v) {
   return r;
 }
 
-// All threads of the block; false when the CTA has nothing to do.
+// All threads of the block; false when the CTA has nothing to do.  SEL here and below: in a
+// kernel that selected blocks may come to (K7 has two forms: their code costs steps over all
+// keys 5 us of 61).
+template <bool SEL = false>
 __device__ inline bool seq_locate(const SeqAttnArgs& a, SeqShared& sh, SeqPlace& p) {
-  if (a.sel_blocks) {
+  if (SEL && a.sel_blocks) {
     const int M = sel_items(a), span = sel_span(a);
     const long long total = (long long)a.seqs.total * a.pages.H * M * span;
     p.quota = max((long long)a.min_tiles, (long long)udiv(total + gridDim.x - 1, gridDim.x));
@@ -362,7 +365,6 @@ struct SeqPiece {
 };
 
 // Steps through a CTA's pieces; every role of a kernel runs one of its own.
-// SEL: in a kernel that selected blocks may come to.
 template <bool SEL>
 struct SeqIterOf {
   long long t, t1;
@@ -461,13 +463,14 @@ __device__ __forceinline__ int seq_slot(const SeqPiece& w) {
 }
 
 // The first warp of every CTA, those without work included.
+template <bool SEL = false>
 __device__ __forceinline__ void seq_write_split(const SeqAttnArgs& a, bool any,
                                                 const SeqPlace& p) {
   SeqSplit d{};
   d.extra = a.extra;
   if (any && p.j > a.extra) {
     SeqInfo s;
-    if (a.sel_blocks) {
+    if (SEL && a.sel_blocks) {
       const SelRow r = sel_row(a, p.b);
       s = SeqInfo{p.b / a.pages.H, r.b >= 0 ? 1 : 0, 0, r.L};
     } else {

@@ -127,8 +127,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return r;
 }
 
-// TQ: type of Q and O; TK: TQ or codes; DHP: head size padded to 64 or 128.
-template <int TQ, int TK, int DHP, int NR>
+// TQ: type of Q and O; TK: TQ or codes; DHP: head size padded to 64 or 128; SEL: over selected
+// blocks.
+template <int TQ, int TK, int DHP, int NR, bool SEL>
 __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     seq_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ SeqAttnArgs a) {
@@ -164,15 +165,14 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
     tma_prefetch_desc(&tmV);
   }
   for (int i = threadIdx.x; i < 3 * DHP; i += kThreads) poison[i] = INT_MAX;
-  grid_dep_launch();
   grid_dep_wait();
   SeqPlace place;
-  const bool any = seq_locate(a, sh, place);  // synchronises the block
-  if (threadIdx.x < 32) seq_write_split(a, any, place);
+  const bool any = seq_locate<SEL>(a, sh, place);  // synchronises the block
+  if (threadIdx.x < 32) seq_write_split<SEL>(a, any, place);
   if (!any) return;
   __syncthreads();
 
-  SeqIterOf<true> it;
+  SeqIterOf<SEL> it;
   it.start(place);
   SeqPiece w;
   if (warp == kWarps) {
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         for (int i = 0; i < kKeys / 16; ++i) {
           if (i >= copies) break;
           const int at = j * kKeys + i * box;
-          page[i] = win.get<true>(a, w, at >> shift, used);
+          page[i] = win.get<SEL>(a, w, at >> shift, used);
           if constexpr (CODED) {
             if (page[i] < a.pages.num_pages) {
               bytes += (I4 ? 4 : 2) * box * 4;
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
   }
 }
 
-template <int TQ, int TK, int DHP, int NR>
+template <int TQ, int TK, int DHP, int NR, bool SEL>
 void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensorMap& v,
             cudaStream_t s) {
   using Cfg = MmaCfg<TK, DHP, NR>;
@@ -792,11 +792,11 @@ void launch(const SeqAttnArgs& a, int ctas, const CUtensorMap& k, const CUtensor
   ATTNB_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load() & bit)) {
-    ATTNB_CUDA(cudaFuncSetAttribute(seq_mma_kernel<TQ, TK, DHP, NR>,
+    ATTNB_CUDA(cudaFuncSetAttribute(seq_mma_kernel<TQ, TK, DHP, NR, SEL>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     configured.fetch_or(bit);
   }
-  ATTNB_CUDA(launch_pdl(seq_mma_kernel<TQ, TK, DHP, NR>, dim3(ctas), dim3(kThreads), Cfg::SMEM, s,
+  ATTNB_CUDA(launch_pdl(seq_mma_kernel<TQ, TK, DHP, NR, SEL>, dim3(ctas), dim3(kThreads), Cfg::SMEM, s,
                         k, v, a));
 }
 
@@ -836,12 +836,18 @@ void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
   auto go = [&](auto tq, auto tk) {
     constexpr int TQ = decltype(tq)::value, TK = decltype(tk)::value;
     if constexpr (TQ != kF32) {
-      if (a.rows == 8) {
-        if (a.q.Dh <= 64) launch<TQ, TK, 64, 1>(a, ctas, k, v, s);
-        else launch<TQ, TK, 128, 1>(a, ctas, k, v, s);
+      auto run = [&](auto dhp, auto nr) {
+        constexpr int DHP = decltype(dhp)::value, NR = decltype(nr)::value;
+        if (a.sel_blocks) launch<TQ, TK, DHP, NR, true>(a, ctas, k, v, s);
+        else launch<TQ, TK, DHP, NR, false>(a, ctas, k, v, s);
+      };
+      using std::integral_constant;
+      if (a.q.Dh <= 64) {
+        if (a.rows == 8) run(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+        else run(integral_constant<int, 64>{}, integral_constant<int, 2>{});
       } else {
-        if (a.q.Dh <= 64) launch<TQ, TK, 64, 2>(a, ctas, k, v, s);
-        else launch<TQ, TK, 128, 2>(a, ctas, k, v, s);
+        if (a.rows == 8) run(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+        else run(integral_constant<int, 128>{}, integral_constant<int, 2>{});
       }
     }
   };

@@ -24,7 +24,6 @@ __global__ void __launch_bounds__(kMergeThreads) seq_merge_kernel(const SeqAttnA
   constexpr int kChunk = 256;  // pieces whose weights are held at a time
   __shared__ float weight[kChunk];
   __shared__ float red[kMergeThreads];
-  grid_dep_launch();
   grid_dep_wait();
   const int c = blockIdx.x + 1;
   const SeqSplit d = reinterpret_cast<const SeqSplit*>(a.ws_split)[c];

@@ -78,11 +78,10 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 3 : 1) seq_simt_kernel(cons
   __shared__ float sm_acc[kThreads / 32][R][D];
   __shared__ float2 sm_ml[kThreads / 32][R];
 
-  grid_dep_launch();
   grid_dep_wait();
   SeqPlace place;
-  const bool any = seq_locate(a, sh, place);
-  if (threadIdx.x < 32) seq_write_split(a, any, place);
+  const bool any = seq_locate<true>(a, sh, place);
+  if (threadIdx.x < 32) seq_write_split<true>(a, any, place);
   if (!any) return;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
