@@ -227,9 +227,8 @@ CUtensorMap make_tmap_nd(const void* base, int elem_bytes, int rank, const uint6
                          const uint64_t* strides, const uint32_t* box) {
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
     fail(ATTNB_ERR_RUNTIME, "TMA base address is not 16-byte aligned");
-  const uint32_t width = box[0] * elem_bytes;
-  if ((width != 128 && width != 64 && width != 32) || rank < 2 || rank > 5)
-    fail(ATTNB_ERR_RUNTIME, "TMA box must be 32, 64 or 128 bytes wide, of rank 2 to 5");
+  if (box[0] * elem_bytes != 128 || rank < 2 || rank > 5)
+    fail(ATTNB_ERR_RUNTIME, "TMA box must be 128 bytes wide, of rank 2 to 5");
   cuuint64_t d[5], st[4];
   cuuint32_t bx[5], es[5];
   for (int i = 0; i < rank; ++i) {
@@ -247,10 +246,8 @@ CUtensorMap make_tmap_nd(const void* base, int elem_bytes, int rank, const uint6
   const CUresult r = encode_fn()(
       &m, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, rank,
       const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      width == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-      : width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                    : CU_TENSOR_MAP_SWIZZLE_32B,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     fail(ATTNB_ERR_CUDA, "cuTensorMapEncodeTiled (n-D) failed (" + std::to_string((int)r) + ")");
   return m;

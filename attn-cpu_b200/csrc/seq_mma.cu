@@ -58,7 +58,7 @@ struct MmaCfg {
   static constexpr int CTAS = NR == 1 ? 3 : 2;         // per SM
   static constexpr int KEYS = I4 ? 128 : 64;           // of a tile
   static constexpr int HALVES = KEYS / (16 * kWarps);  // 16 keys each, of a warp
-  static constexpr int ROWB = I4 ? DHP / 2 : 128;      // bytes of a row in a tile
+  static constexpr int ROWB = I4 ? DHP / 2 : 128;      // bytes of a row in a tile, at most
   static constexpr int CHUNKS = CODED ? 1 : DHP / 64;  // such pieces of a row
   static constexpr int CHUNK = KEYS * ROWB;
   static constexpr int TILE = CHUNKS * CHUNK;          // K or V
@@ -191,40 +191,31 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         if (!__shfl_sync(0xffffffffu, got, 0)) goto drained;
         const uint32_t st = base + ring.stage * Cfg::STAGE;
         const uint32_t bar = smem_addr(&full[ring.stage]);
-        int page[kKeys / 16];
-        uint32_t bytes = 2 * Cfg::TILE;
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i) {
-          if (i >= copies) break;
-          const int at = j * kKeys + i * box;
-          page[i] = win.get<SEL>(a, w, at >> shift, used);
-          if constexpr (CODED) {
-            if (page[i] < a.pages.num_pages) {
-              bytes += (I4 ? 4 : 2) * box * 4;
-            } else if (lane < 2) {  // no such page: codes 0 with a scale of 0
-              float* sc = reinterpret_cast<float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
-              for (int k = 0; k < box; ++k) sc[lane * kKeys + i * box + k] = 0.f;
-              fence_proxy_async_smem();
-            }
+        if constexpr (I4) {
+          // Up to eight copies, of a page's part each: K, V, both scales, both factors by lanes of
+          // their own.
+          const int i = lane & 7, part = lane >> 3, key = j * kKeys + i * box;
+          const int page = win.get_eight<SEL>(a, w, (j * kKeys) >> shift,
+                                              max(1, kKeys >> shift), used);
+          // (pages of 128 keys: one copy; smaller ones: one each)
+          const bool mine = i < copies, there = mine && page < a.pages.num_pages;
+          if (part == 2 && mine && !there) {  // no such page: scales of 0
+            float* sc = reinterpret_cast<float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
+            for (int k = 0; k < box; ++k) sc[i * box + k] = sc[kKeys + i * box + k] = 0.f;
+            fence_proxy_async_smem();
           }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-        __syncwarp();
-        if constexpr (I4) {  // up to eight pages: K, V, both scales, both factors by lanes of their own
-          const int i = lane & 7, part = lane >> 3;
-          int mine = page[0];
-#pragma unroll
-          for (int k = 1; k < kKeys / 16; ++k)
-            if (k == i) mine = page[k];
-          if (i < copies) {
-            const int in_page = (j * kKeys + i * box) & ((1 << shift) - 1);
-            const int64_t at = (((int64_t)mine * a.pages.H + w.h) << shift) + in_page;
+          const int good = __popc(__ballot_sync(0xffffffffu, there) & 0xffu);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(bar, kKeys * a.q.Dh + good * 4 * box * 4);
+          __syncwarp();
+          if (mine) {
+            const int in_page = key & ((1 << shift) - 1);
+            const int64_t at = (((int64_t)page * a.pages.H + w.h) << shift) + in_page;
             const uint32_t side = st + 2 * Cfg::TILE + i * box * 4;
             if (part < 2) {
-              tma_load_4d(st + part * Cfg::TILE + i * box * Cfg::ROWB, part ? &tmV : &tmK, bar, 0,
-                          in_page, w.h, mine);
-            } else if (mine < a.pages.num_pages) {
+              tma_load_4d(st + part * Cfg::TILE + i * box * (a.q.Dh / 2), part ? &tmV : &tmK, bar, 0,
+                          in_page * a.q.Dh / 256, w.h, page);
+            } else if (there) {
               const bool scales = part == 2;
               const void* kp = scales ? (const void*)(a.pages.k_scale + at) : a.pages.k_group + at * 4;
               const void* vp = scales ? (const void*)(a.pages.v_scale + at) : a.pages.v_group + at * 4;
@@ -233,21 +224,43 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
               bulk_load(to + 4 * kKeys, vp, box * 4, bar);
             }
           }
-        } else if (lane < 2) {  // lane 0: K, lane 1: V
-          const CUtensorMap* map = lane ? &tmV : &tmK;
-          const float* sc = lane ? a.pages.v_scale : a.pages.k_scale;
+        } else {
+          int page[kKeys / 16];
+          uint32_t bytes = 2 * Cfg::TILE;
 #pragma unroll
           for (int i = 0; i < kKeys / 16; ++i) {
             if (i >= copies) break;
-            const int in_page = (j * kKeys + i * box) & ((1 << shift) - 1);
-            const uint32_t dst = st + lane * Cfg::TILE + i * box * 128;
+            const int at = j * kKeys + i * box;
+            page[i] = win.get<SEL>(a, w, at >> shift, used);
+            if constexpr (CODED) {
+              if (page[i] < a.pages.num_pages) {
+                bytes += 2 * box * 4;
+              } else if (lane < 2) {  // no such page: codes 0 with a scale of 0
+                float* sc = reinterpret_cast<float*>(mem + ring.stage * Cfg::STAGE + 2 * Cfg::TILE);
+                for (int k = 0; k < box; ++k) sc[lane * kKeys + i * box + k] = 0.f;
+                fence_proxy_async_smem();
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
+          if (lane < 2) {  // lane 0: K, lane 1: V
+            const CUtensorMap* map = lane ? &tmV : &tmK;
+            const float* sc = lane ? a.pages.v_scale : a.pages.k_scale;
 #pragma unroll
-            for (int c = 0; c < Cfg::CHUNKS; ++c)
-              tma_load_4d(dst + c * Cfg::CHUNK, map, bar, c * 64, in_page, w.h, page[i]);
-            if (CODED && page[i] < a.pages.num_pages)
-              bulk_load(st + 2 * Cfg::TILE + (lane * kKeys + i * box) * 4,
-                        sc + ((((int64_t)page[i] * a.pages.H + w.h) << shift) + in_page), box * 4,
-                        bar);
+            for (int i = 0; i < kKeys / 16; ++i) {
+              if (i >= copies) break;
+              const int in_page = (j * kKeys + i * box) & ((1 << shift) - 1);
+              const uint32_t dst = st + lane * Cfg::TILE + i * box * 128;
+#pragma unroll
+              for (int c = 0; c < Cfg::CHUNKS; ++c)
+                tma_load_4d(dst + c * Cfg::CHUNK, map, bar, c * 64, in_page, w.h, page[i]);
+              if (CODED && page[i] < a.pages.num_pages)
+                bulk_load(st + 2 * Cfg::TILE + (lane * kKeys + i * box) * 4,
+                          sc + ((((int64_t)page[i] * a.pages.H + w.h) << shift) + in_page), box * 4,
+                          bar);
+            }
           }
         }
         ring.note_issue();
@@ -267,6 +280,13 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
   const int g = lane >> 2, c = lane & 3;  // fragment row and column group
   Ring<ST> ring;
   bool ok = true;
+  uint32_t unit[NH][I4 ? KS / 4 : 1];  // 4-bit codes: where this lane's matrix rows are in a tile
+#pragma unroll
+  for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+    for (int k = 0; k < (I4 ? KS / 4 : 1); ++k)
+      unit[hf][k] = i4_unit((warp * (16 * NH) + hf * 16 + (lane & 15)) * (a.q.Dh / 32) + 2 * k +
+                            (lane >> 4));
   while (it.next(a, w)) {
     // Q^T as B fragments: row 8 r + g, by step of 16 dimensions.  16-bit keys:
     // dimensions 2c, 2c+1 and 2c+8, 2c+9 of the step; codes: 4c .. 4c+3, as a
@@ -424,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
 #pragma unroll
             for (int k = 0; k < KS / 2; k += 2) {
               uint32_t b[4];
-              ldsm4(st + sw_rows<Cfg::ROWB>(kr + hf * 16, k + (lane >> 4)), b);
+              ldsm4(st + unit[hf][k / 2], b);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const uint32_t x = b[2 * e], y = b[2 * e + 1], x8 = x >> 8, y8 = y >> 8;
@@ -493,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           // exponent is one FMA from the score (what m is off by is common to all weights
           // of the row), and only tiles with a mask look for what it hides.
           if (masked) {
+            asm volatile("" ::: "memory");  // a branch: as predicates they cost every tile 25 instructions
 #pragma unroll
             for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
@@ -656,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
 #pragma unroll
             for (int u = 0; u < KS / 2; u += 2) {
               uint32_t b[4];
-              ldsm4_t(st + Cfg::TILE + sw_rows<Cfg::ROWB>(kr + hf * 16, u + (lane >> 4)), b);
+              ldsm4_t(st + Cfg::TILE + unit[hf][u / 2], b);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 // keys 2c, 2c + 1 (and 8 more) in the halves, dimensions 4g .. 4g + 3 in a half
@@ -814,11 +835,12 @@ bool seq_pages_tma(const SeqAttnArgs& a) {
 
 CUtensorMap seq_pages_map(const KvPages& p, const void* base, int rows) {
   const uint64_t eb = elem_bytes(p.type), page = 1u << p.page_shift;
-  const uint64_t row = vector_bytes(p.type, p.Dh);
-  const uint64_t dims[4] = {row / eb, page, (uint64_t)p.H, (uint64_t)p.num_pages};
-  const uint64_t strides[3] = {row, row * page, row * page * p.H};
-  const uint32_t wide = p.type == kI4 ? (p.Dh <= 64 ? 32 : 64) : 128 / eb;
-  const uint32_t box[4] = {wide, (uint32_t)std::min<uint64_t>(page, rows), 1, 1};
+  const uint64_t row = vector_bytes(p.type, p.Dh), most = std::min<uint64_t>(page, rows);
+  const bool i4 = p.type == kI4;  // in rows of 128 bytes whatever a vector's are
+  const uint64_t dims[4] = {i4 ? 128 : row / eb, i4 ? page * row / 128 : page, (uint64_t)p.H,
+                            (uint64_t)p.num_pages};
+  const uint64_t strides[3] = {i4 ? 128 : row, row * page, row * page * p.H};
+  const uint32_t box[4] = {(uint32_t)(128 / eb), (uint32_t)(i4 ? most * row / 128 : most), 1, 1};
   return make_tmap_nd(base, (int)eb, 4, dims, strides, box);
 }
 

@@ -34,6 +34,18 @@ struct PageWindow {
     const int p = __shfl_sync(0xffffffffu, page, slot - first);
     return slot < used ? p : a.pages.num_pages;
   }
+  // The same of slots `slot` to `slot` + count - 1 (count <= 8) at once: lane i has that of
+  // slot + (i & 7).
+  template <bool SEL>
+  __device__ __forceinline__ int get_eight(const SeqAttnArgs& a, const SeqPiece& w, int slot,
+                                           int count, int used) {
+    const int of = SEL && a.sel_blocks ? w.v : w.b;
+    if (of != b || slot < first || slot + count > first + 32) b = -1;  // all of them in one window
+    get<SEL>(a, w, slot, used);
+    const int mine = slot + (int)(threadIdx.x & 7);
+    const int p = __shfl_sync(0xffffffffu, page, mine - first);
+    return mine < used ? p : a.pages.num_pages;
+  }
 };
 
 // 128-byte rows with the TMA's 128-byte swizzle: byte offset of 16-byte unit u
@@ -42,15 +54,10 @@ __device__ __forceinline__ uint32_t sw128(int r, int u) {
   return (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
 }
 
-// The same for rows of 64 bytes with the 64-byte swizzle and of 32 bytes with the
-// 32-byte one (tile base 512-byte aligned): eight rows at one unit lie in
-// different banks.
-template <int ROW>
-__device__ __forceinline__ uint32_t sw_rows(int r, int u) {
-  if constexpr (ROW == 128) return sw128(r, u);
-  else if constexpr (ROW == 64) return (uint32_t)(r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
-  else return (uint32_t)(r * 32 + ((u ^ ((r >> 2) & 1)) << 4));
-}
+// 4-bit codes lie as they do in a page, vector after vector (Dh / 32 units of 16 bytes each), in
+// such rows: byte offset of unit i.  Rows of their own for the vectors, of 64 bytes, are copied
+// 4 us of 88 more slowly.  (Eight vectors' units are in different banks for Dh 64 and 128.)
+__device__ __forceinline__ uint32_t i4_unit(int i) { return sw128(i >> 3, i & 7); }
 
 // a * b + c of two pairs of f16.
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {

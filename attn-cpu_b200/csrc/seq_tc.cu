@@ -209,7 +209,6 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ SeqAttnArgs a,
                   const bool qtma, const bool qvec, const bool ovec) {
   constexpr bool CODED = elem_coded(TK), I4 = TK == kI4;
-  constexpr int ROWB = I4 ? DHP / 2 : 128;  // codes: bytes of a row as it comes
   using Cfg = TcCfg<CODED, DHP>;
   using EQ = elem_t<TQ>;
   constexpr bool BF16 = TQ == kBF16 && !CODED;  // type of the products
@@ -310,6 +309,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
     if constexpr (CODED) {
       Ring<RST> ring;
       const int box = min(1 << shift, 64), copies = 64 / box;
+      const int row = I4 ? a.q.Dh / 2 : 128;  // bytes of a key as it comes
       while (ok && it.next(a, w)) {
         const int used = (w.s.L + mask) >> shift;
         for (int hj = 4 * w.j0; ok && hj < 4 * w.j1; ++hj) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
           const uint32_t bar = smem_addr(&rfull[ring.stage]);
           const int key0 = (hj >> 2) * BN + (hj & 1) * 64;
           int page = 0;  // of this lane's copy
-          uint32_t bytes = 64 * ROWB;
+          uint32_t bytes = 64 * row;
           for (int i = 0; i < copies; ++i) {
             const int p = win.get<false>(a, w, (key0 + i * box) >> shift, used);
             if (lane == i) page = p;
@@ -339,8 +339,9 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
           if (lane < copies) {
-            tma_load_4d(st + lane * box * ROWB, is_v ? &tmV : &tmK, bar, 0, my_key & mask, w.h,
-                        page);
+            const int in_page = my_key & mask;
+            tma_load_4d(st + lane * box * row, is_v ? &tmV : &tmK, bar, 0,
+                        I4 ? in_page * row / 128 : in_page, w.h, page);
             const int64_t at = (((int64_t)page * a.pages.H + w.h) << shift) + (my_key & mask);
             if (I4 && there)
               bulk_load(st + 64 * 128 + 512 + lane * box * 4,
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
 #pragma unroll 1
                 for (int i = 0; i < DHP / 64; ++i) {
                   const int u = part * (DHP / 64) + i;
-                  const uint4 x = *reinterpret_cast<const uint4*>(from + sw_rows<ROWB>(row, u));
+                  const uint4 x = *reinterpret_cast<const uint4*>(from + i4_unit(row * (a.q.Dh / 32) + u));
                   const I4Factors f = i4_factors(__byte_perm(factors >> (8 * u), 0, 0x4040));
                   const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
                   uint8_t* ch = to + (u >> 1) * Cfg::CHUNK;
