@@ -55,7 +55,9 @@ template <int TK, int DHP, int NR>
 struct MmaCfg {
   static constexpr bool CODED = elem_coded(TK), I4 = TK == kI4;
   static constexpr int ROWS = 8 * NR;
-  static constexpr int CTAS = NR == 1 ? 3 : 2;         // per SM
+  // Per SM.  4-bit codes at head sizes over 64 need the registers (64 sequences of 1000-8192
+  // keys: 110 us, with three CTAs and 128 registers 117, with four 149).
+  static constexpr int CTAS = NR == 1 && !(I4 && DHP == 128) ? 3 : 2;
   static constexpr int KEYS = I4 ? 128 : 64;           // of a tile
   static constexpr int HALVES = KEYS / (16 * kWarps);  // 16 keys each, of a warp
   static constexpr int ROWB = I4 ? DHP / 2 : 128;      // bytes of a row in a tile, at most
@@ -65,7 +67,7 @@ struct MmaCfg {
   // Behind them the scales of K and V, and I4's factors.
   static constexpr int STAGE = 2 * TILE + (I4 ? KEYS * 16 : CODED ? 1024 : 0);
   // Together the CTAs of an SM have about 190 KB of copies in flight.
-  static constexpr int STAGES = I4 ? (DHP == 128 ? 3 : 5) + (NR == 1 ? 0 : 2)
+  static constexpr int STAGES = I4 ? (DHP == 128 || NR == 1 ? 5 : 8)
                                 : CODED ? (NR == 1 ? 3 : 5)
                                 : (DHP == 128 ? (NR == 1 ? 2 : 3) : (NR == 1 ? 4 : 6));
   // I4, of a warp's 32 keys: factor times K scale by key and group, factors of V in f16 by
@@ -869,7 +871,7 @@ void seq_mma_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s) {
         else run(integral_constant<int, 64>{}, integral_constant<int, 2>{});
       } else {
         if (a.rows == 8) run(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-        else run(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+        else if constexpr (TK != kI4) run(integral_constant<int, 128>{}, integral_constant<int, 2>{});
       }
     }
   };

@@ -114,9 +114,13 @@ Space simt_space(int Dh, int64_t rows, int num_sms) {
 }
 // Rows of a KV head in one item: 8 for a step of up to 8 query heads, else 16 (32
 // sequences of 4096 bf16 keys: 4 rows 91 us against 94, e4m3 59 against 90; 16
-// rows 169 us against 103, e4m3 99 against 98).
-Space mma_space(int64_t rows, int num_sms) {
-  return rows <= 8 ? Space{8, 3 * num_sms} : Space{16, 2 * num_sms};
+// rows 169 us against 103, e4m3 99 against 98).  Over 4-bit pages at head sizes over 64
+// always 8, two CTAs an SM, for want of registers (16 rows the same way 101 us
+// against 139).
+Space mma_space(int type, int Dh, int64_t rows, int num_sms) {
+  const bool large = type == kI4 && Dh > 64;
+  if (rows > 8 && !large) return {16, 2 * num_sms};
+  return {8, (large ? 2 : 3) * num_sms};
 }
 Space tc_space(int G, int num_sms) { return {seq_tc_rows(G), num_sms}; }
 Space tf32_space(int num_sms) { return {128, num_sms}; }
@@ -124,7 +128,8 @@ Space tf32_space(int num_sms) { return {128, num_sms}; }
 }  // namespace
 
 size_t seq_workspace_bytes(int G, int Dh, int num_sms) {
-  size_t n = std::max(simt_space(Dh, 4, num_sms).bytes(Dh), mma_space(16, num_sms).bytes(Dh));
+  size_t n = std::max({simt_space(Dh, 4, num_sms).bytes(Dh), mma_space(kF16, Dh, 16, num_sms).bytes(Dh),
+                       mma_space(kF16, Dh, 8, num_sms).bytes(Dh)});
   if (Dh <= 128) n = std::max(n, tf32_space(num_sms).bytes(Dh));
   if (G <= 128 && Dh <= 128) n = std::max(n, tc_space(G, num_sms).bytes(Dh));
   return n + 256;
@@ -137,7 +142,7 @@ enum Kind { kSimt, kMma, kTc, kTf32 };
 static void run(SeqAttnArgs a, Kind kind, int64_t rows, uintptr_t ws, uintptr_t ws_end, int num_sms,
                 cudaStream_t s) {
   const Space sp = kind == kTc     ? tc_space(a.G, num_sms)
-                   : kind == kMma  ? mma_space(rows, num_sms)
+                   : kind == kMma  ? mma_space(a.pages.type, a.q.Dh, rows, num_sms)
                    : kind == kTf32 ? tf32_space(num_sms)
                                    : simt_space(a.q.Dh, rows, num_sms);
   a.rows = sp.rows;
@@ -174,11 +179,14 @@ void seq_attn_run(SeqAttnArgs a, int max_new, void* ws, size_t ws_bytes, int num
   // Rows of one KV head and sequence.  16-bit pages: K7 up to 32 rows, K8 beyond (32
   // sequences of 4096 keys, 8 KV heads of 128: 16 rows 102 us against 193, 32 rows
   // 186 against 184, 48 rows 271 against 189); codes, which K8 converts in four
-  // warps: up to 48 (e4m3: 48 rows 267 us against 282, 64 rows 347 against 284).  In
+  // warps: up to 48 (e4m3: 48 rows 267 us against 282, 64 rows 347 against 284; 4 bits:
+  // 259 against 306, 337 against 307), 4 bits of head sizes up to 64 up to 96 (64 rows
+  // 187 us against 268, 96 rows 269 against 273).  In
   // fp32, K9 over 16 rows (8 sequences of 2000 keys, 4 KV heads of 64: 16 rows 53 us
   // both, 64 rows 62 us against K6's 169).
+  const int64_t few = a.pages.type == kI4 && a.q.Dh <= 64 ? 96 : elem_coded(a.pages.type) ? 48 : 32;
   Kind kind = kSimt;
-  if (seq_mma_supported(a) && rows <= (elem_coded(a.pages.type) ? 48 : 32)) kind = kMma;
+  if (seq_mma_supported(a) && rows <= few) kind = kMma;
   else if (seq_tc_supported(a)) kind = kTc;
   else if (seq_mma_supported(a)) kind = kMma;
   else if (a.q.Dh <= 128 && rows > 16) kind = kTf32;
