@@ -858,8 +858,11 @@ class PagedKVCacheDev:
         if dtype == torch.uint8 and Dh % 32:
             raise ValueError("pages of 4 bits need a head size that is a multiple of 32")
         coded = dtype in (torch.float8_e4m3fn, torch.int8, torch.uint8)
-        if not isinstance(bounds, bool) and bounds is not None and not coded and bounds != dtype:
-            raise ValueError("bounds of uncoded pages have their type")
+        if not isinstance(bounds, bool) and bounds is not None:
+            if not coded and bounds != dtype:
+                raise ValueError("bounds of uncoded pages have their type")
+            if bounds not in (torch.float32, torch.bfloat16, torch.float16):
+                raise ValueError("bounds must be float32, bfloat16 or float16")
         wide = Dh // 2 if dtype == torch.uint8 else Dh
         self.k_pages, self.v_pages = (torch.empty(num_pages, H, page_size, wide, dtype=dtype,
                                                   device=device) for _ in range(2))

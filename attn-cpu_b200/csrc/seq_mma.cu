@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float f = 256.f * row_scale(top);  // room below for the sixteenths
+        const float f = kI4Rows * row_scale(top);
 #pragma unroll
         for (int k = 0; k < KS / 2; ++k) {
           float sum = 0.f;
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          mulq[r][i] = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, f, (2 * c + i) * 4);
+          mulq[r][i] =
+              a.scale_log2 / __shfl_sync(0xffffffffu, f * (0x1p-5f / kI4Rows), (2 * c + i) * 4);
       } else if constexpr (CODED) {
         float x[KS][4], top = 0.f;
 #pragma unroll
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
           const float* scales = reinterpret_cast<const float*>(side);
           const uint32_t* factors = reinterpret_cast<const uint32_t*>(side + 8 * kKeys);
           const uint32_t kf = factors[key];
-          const float ks = scales[key];
+          const float ks = scales[key] * (0x1p19f / kI4Rows);  // the codes' unit, but for 2^5
           // (2^23 + r has r as its last bits)
           auto times = [&](int i) {
             return (__uint_as_float(__byte_perm(kf, 0x4b000000u, 0x7540 + i)) - 8388608.f) * ks;

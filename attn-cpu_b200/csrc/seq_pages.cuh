@@ -72,6 +72,10 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
 // exact: a multiple of 2^-19 below 2^-8, in one FMA of two.
 constexpr uint32_t kI4Low = 0x000f000fu, kI4High = 0x00f000f0u;
 constexpr float kI4Unit = 0x1p19f;  // what such values are to be multiplied by
+// Against such small values queries are brought up to 2^14 (2^15 next to overflow): room
+// below for sixteenths of them, and little left of the unit for the factors of scores, which
+// stay finite for queries and keys up to 2^124.
+constexpr float kI4Rows = 0x1p13f;
 struct I4Factors {
   uint32_t low, high, add;  // pairs of f16: r 2^5, r 2^1, -r 2^-16
 };

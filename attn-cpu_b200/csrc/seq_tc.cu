@@ -813,7 +813,8 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
             for (int b = 0; b < 8; ++b) top = fmaxf(top, fabsf(to_float(e[b])));
           }
           f = row_scale(top);
-          scale = a.scale_log2 * (I4 ? kI4Unit : 1.f) / f;
+          scale = a.scale_log2 * (I4 ? kI4Unit / kI4Rows : 1.f) / f;
+          if (I4) f *= kI4Rows;
         }
 #pragma unroll 4
         for (int u = 0; u < DHP / 8; ++u) {

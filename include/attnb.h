@@ -449,7 +449,7 @@ ATTNB_API int attnb_kv_pages_read_dev(const attnb_kv_pages* pages, const attnb_r
 /* Attention of the packed rows (new tokens, one and up per sequence) over the
  * lens[b] tokens that the pages hold, their own among them (append first);
  * otherwise as attnb_attn_packed_dev.  Q and O have one type; the pages have
- * that type or are E4M3, I8 or I4.  max_new: the most rows of one sequence, as far
+ * that type or are E4M3, I8 or I4 (16-bit queries over I4: queries and keys below 2^124).  max_new: the most rows of one sequence, as far
  * as the caller knows (0: unknown); it steers the choice of kernel only. */
 ATTNB_API int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pages,
                                    const attnb_rows* O, const attnb_seqs* seqs, int max_new,

@@ -157,6 +157,34 @@ def test_values_of_any_size(cuda, new):
         _against(p, q, [new], keys, BF16)
 
 
+@pytest.mark.parametrize("new", [1, 5, 200])
+@pytest.mark.parametrize("by", [(115, -115), (100, -100), (-100, 100), (-110, 118), (60, -50)])
+def test_queries_and_keys_of_any_size(cuda, new, by):
+    """Large queries over small keys and the other way round, scores of ordinary size or one far above
+    the others."""
+    keys, H, D = [500], 1, 128
+    g = _gen(9)
+    p = Pages(keys, H, D, 64, I4)
+    k, v = (_randn(g, 500, H, D) for _ in range(2))
+    k = (k * 2.0 ** by[1]).to(BF16)
+    capi.kv_pages_append_dev(k, v.to(BF16), p.k, p.v, *p.where(keys), **p.kw)
+    q = (_randn(g, new, 4, D) * 2.0 ** by[0]).to(BF16)
+    if by[0] + by[1] <= 0:
+        _against(p, q, [new], keys, BF16, new)
+        return
+    # Rows whose best key is 30 above the next have no other: 500 e^-30 is below 2^-34.  They get that
+    # key's value.
+    ks, vs = _held(p, "k", 0, 500), _held(p, "v", 0, 500)
+    s = torch.einsum("ihd,jd->ihj", q.double().cpu(), ks[:, 0])
+    s = s.masked_fill(~torch.ones(new, 500, dtype=torch.bool).tril(500 - new)[:, None], -torch.inf)
+    o = _attend(p, q, [new], new).double().cpu()
+    top = s.topk(2, -1)
+    sure = (top.values[..., 0] - top.values[..., 1]) * D ** -0.5 > 30
+    assert sure.any() and torch.isfinite(o).all()
+    want = vs[:, 0][top.indices[..., 0]]
+    assert ((o - want).abs()[sure] <= 2.0 ** -7 * want.abs()[sure] + 1e-6).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 100])
 def test_stale_pages_stay_out(cuda, dtype, new):
@@ -241,3 +269,83 @@ def test_cache_object(cuda):
             held[2 + b] = torch.cat([held[2 + b], x])
             step_size = held[2 + b].float().abs().amax(-1, keepdim=True) / 7
             assert ((vs[b] - held[2 + b].float()).abs() <= step_size * 0.51).all()
+
+
+def test_captured_attend_is_replayed_after_later_appends(cuda):
+    """A generation step of the cache object through one graph, as the context grows over pages."""
+    H, heads, D = 2, 4, 64
+    cache = capi.PagedKVCacheDev(2, H, D, num_pages=20, page_size=16, dtype=torch.uint8)
+    k, v = (_randn(_gen(i), 90, H, D, dtype=BF16) for i in (1, 2))
+    cache.append(k, v, [60, 30])
+    q, graph = torch.empty(2, heads, D, dtype=BF16, device="cuda"), None
+    o = torch.empty_like(q)
+    for step in range(40):
+        kn, vn = (_randn(_gen(100 * step + i), 2, H, D, dtype=BF16) for i in (3, 4))
+        cache.append(kn, vn, [1, 1])
+        q.copy_(_randn(_gen(step), 2, heads, D, dtype=BF16))
+        if graph is None:
+            cache.attend(q, o)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                cache.attend(q, o)
+        o.fill_(float("nan"))
+        graph.replay()
+        want = torch.full_like(o, float("nan"))
+        cache.attend(q, want)
+        assert torch.equal(o, want)
+    ks, vs = [], []
+    for b in range(2):
+        pair = [torch.empty(cache.lengths[b], H, D, device="cuda") for _ in range(2)]
+        cache.read(b, *pair)
+        ks.append(pair[0])
+        vs.append(pair[1])
+    ref, mag = seq_ref.attention(q, ks, vs, [1, 1])
+    smax = float(q.double().norm(dim=-1).max() * max(x.double().norm(dim=-1).max() for x in ks)) * D ** -0.5
+    _check(o, ref, mag, BF16, smax, True, 100, more.weight_floor(q, ks, vs, [1, 1]))
+
+
+def test_long_pool_offsets_pass_32_bits(cuda):
+    """The pages that are used lie more than 2^31 bytes of codes into the pool."""
+    H, page, D, n = 8, 128, 128, 300
+    num = 2 ** 31 // (H * page * D // 2) + 20
+    pools = [torch.empty(num, H, page, D // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    kw = {x + "_scale": torch.zeros(num, H, page, device="cuda") for x in "kv"}
+    kw |= {x + "_group": torch.zeros(num, H, page, 4, dtype=torch.uint8, device="cuda") for x in "kv"}
+    table = torch.arange(num - 1, num - 4, -1, dtype=torch.int32, device="cuda")[None]
+    where = seq_ref.starts([n]), table, torch.tensor([n], dtype=torch.int32, device="cuda")
+    k, v = (_randn(_gen(i), n, H, D, dtype=BF16) for i in (1, 2))
+    capi.kv_pages_append_dev(k, v, *pools, *where, **kw)
+    back = [torch.empty_like(k, dtype=F32), torch.empty_like(v, dtype=F32)]
+    capi.kv_pages_read_dev(*pools, *back, *where, **kw)
+    for x, y in zip((k, v), back):
+        assert ((x.float() - y).abs() <= x.float().abs().amax(-1, keepdim=True) / 7 * 0.51).all()
+    for new in (1, 100):
+        q = _randn(_gen(3), new, 16, D, dtype=BF16)
+        o = torch.empty_like(q)
+        w = seq_ref.starts([new]), *where[1:]
+        capi.attn_paged_dev(q, *pools, o, *w, new, **kw)
+        ref, mag = seq_ref.attention(q, [back[0]], [back[1]], [new])
+        smax = float(q.double().norm(dim=-1).max() * back[0].double().norm(dim=-1).max()) * D ** -0.5
+        _check(o, ref, mag, BF16, smax, True, n, more.weight_floor(q, [back[0]], [back[1]], [new]))
+    bounds = torch.zeros(num, H, 2, D, dtype=BF16, device="cuda")
+    capi.kv_blocks_bounds_dev(pools[0], bounds, *where, kw["k_scale"], kw["k_group"])
+    want = torch.stack([back[0][:128].amin(0), back[0][:128].amax(0)], 1).to(BF16)
+    assert torch.equal(bounds[num - 1], want)
+
+
+def test_two_streams_at_once(cuda):
+    """Two calls over one cache in flight together have workspaces of their own."""
+    keys = [5000]
+    p = _filled(keys, 2, 128, 64, BF16)
+    qs = [_randn(_gen(i), 1, 8, 128, dtype=BF16) for i in range(6)]
+    want = [_attend(p, q, [1], 1) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [torch.empty_like(q) for q in qs]
+    for _ in range(20):
+        for i, q in enumerate(qs):
+            with torch.cuda.stream(streams[i % 2]):
+                capi.attn_paged_dev(q, p.k, p.v, got[i], *p.where([1]), 1, **p.kw)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

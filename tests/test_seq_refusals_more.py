@@ -201,3 +201,5 @@ def test_cache_object():
         capi.PagedKVCacheDev(1, 2, 80, 4, dtype=torch.uint8, device="cpu")
     with pytest.raises(ValueError, match="have their type"):
         capi.PagedKVCacheDev(1, 2, 64, 4, dtype=torch.float16, device="cpu", bounds=torch.bfloat16)
+    with pytest.raises(ValueError, match="bounds must be float32"):
+        capi.PagedKVCacheDev(1, 2, 64, 4, dtype=torch.int8, device="cpu", bounds=torch.int8)
