@@ -1,5 +1,6 @@
 // seq_simt.cu -- K6: attention of packed query rows over packed keys or pages on
-// CUDA cores, for every type, stride and head size up to 256 (and all of fp32).
+// CUDA cores, for every type, stride and head size up to 256 (and all of fp32); the keys may be
+// those of the blocks in a token's list.
 //
 // For a query row i and the keys j that it sees,
 //     s_j = scale * kscale_j * q . k_j,   o = sum_j 2^(s_j - m) vscale_j v_j / sum_j 2^(s_j - m)

@@ -26,6 +26,10 @@
 //   1.03 ms (578 TFLOP/s: the conversion of codes shares the SM's issue slots; with
 //   the scales in the f16 tiles 0.98 ms, and two roundings of every K and V more).
 //
+// 4-bit codes come as r (code - 8) 2^-19, exact in f16, 32 at a time of one group, with the
+// dimensions of each eight in the order (0, 4, 1, 5, 2, 6, 3, 7), which Q follows on its way in
+// and O on its way out.  The same chunks over 4-bit pages take 1.04 ms.
+//
 // The running maximum moves only when it grows by more than 8 (weights stay
 // below 2^8, which f16 and bf16 hold); O and the sum are rescaled then.  Weights
 // are rounded to 16 bits once, to nearest; maxima, sums and O are fp32.
