@@ -391,3 +391,79 @@ def test_cache_object(cuda):
         assert ((o.float() - full.float()).abs() <= 2.0 ** -6 * full.float().abs() + 2.0 ** -7).all()
     with pytest.raises(ValueError, match="bounds"):
         capi.PagedKVCacheDev(1, H, D, num_pages=2, dtype=BF16).attend_blocks(q, o, take=4)
+
+
+@pytest.mark.parametrize("dtype,kind,D,page,n,H,new", [
+    (BF16, BF16, 64, 16, 700, 2, 160),  # rows enough to fill the machine, more keys than a warp chooses from
+    (F32, F32, 256, 16, 1300, 1, 300),
+    (F16, I4, 128, 32, 600, 8, 40),
+])
+def test_many_rows_of_many_blocks(cuda, dtype, kind, D, page, n, H, new):
+    keys = [page * n - 3]
+    p = _filled(keys, H, D, page, dtype, kind)
+    _bound(p, keys)
+    q = _randn(_gen(3), new, 2 * H, D, dtype=dtype)
+    for take in (30, 590):
+        blocks = _select(p, q, [new], take, 2, 1)
+        assert torch.equal(blocks.cpu(), _wanted(p, q, [new], keys, take, 2, 1))
+
+
+@pytest.mark.parametrize("batch", [65, 300, 700])
+def test_many_sequences(cuda, batch):
+    """More sequences than lanes of a warp and threads of a CTA, some without a token."""
+    keys = [20 + 37 * i % 300 for i in range(batch)]
+    new = [i % 3 for i in range(batch)]
+    p = _filled(keys, 1, 64, 16, BF16, BF16)
+    _bound(p, keys)
+    q = _randn(_gen(4), sum(new), 2, 64, dtype=BF16)
+    blocks = _select(p, q, new, 5)
+    assert torch.equal(blocks.cpu(), _wanted(p, q, new, keys, 5, 1, 1))
+    _attended(p, q, blocks, new, keys, BF16)
+    capi.stream_status()
+
+
+def test_rows_in_several_launches(cuda):
+    """A table so wide that the scores of all rows would not fit the workspace: the call goes in parts.
+    Its pages are a few that repeat, so that nearly all scores are equal to many others."""
+    page, D, width, new, few, take = 16, 64, 200_000, 70, 50, 100
+    p = Pages([page * few], 1, D, page, BF16)
+    k = _randn(_gen(5), page * few, 1, D, dtype=BF16)
+    capi.kv_pages_append_dev(k, k, p.k, p.v, *p.where([page * few]))
+    p.bounds = torch.zeros(p.k.shape[0], 1, 2, D, dtype=BF16, device="cuda")
+    _bound(p, [page * few])
+    own = p.table[0, :few].clone()
+    g = torch.Generator().manual_seed(6)
+    slot = torch.randint(0, few, (width,), generator=g)
+    p.table = own[slot.cuda()][None].contiguous()
+    L = page * width - 5
+    p.lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    q = _randn(_gen(7), new, 2, D, dtype=BF16)
+    blocks = _select(p, q, [new], take, 1, 2).cpu()
+    low, high = p.bounds[own.long(), 0].unbind(1)
+    for i in (0, 1, 30, 39, 40, 41, 42, 43, 69):
+        n = (L - new + i) // page + 1
+        s = more.scores(q[i], low, high)[slot[:n]]
+        assert blocks[i, 0].tolist() == more.select(s, take, 1, 2), i
+    o = torch.empty_like(q)
+    capi.attn_blocks_dev(q, p.k, p.v, o, blocks.cuda(), *p.where([new]))
+    ks = k.view(few, page, 1, D)
+    for i in (0, 69):
+        at, pos = blocks[i, 0].long(), L - new + i
+        x = ks[slot[at].cuda()].flatten(0, 1)
+        x = x[: len(x) - (page - 1 - pos % page)]
+        ref, mag = seq_ref.attention(q[i:i + 1], [x], [x], [1])
+        _check(o[i:i + 1], ref, mag, BF16, float(q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max()) / 8, L=1600)
+    capi.stream_status()
+
+
+@pytest.mark.parametrize("dtype,kind,D", [(BF16, BF16, 80), (BF16, I4, 128), (F16, I4, 64), (F32, F32, 64), (F16, I8, 96)])
+@pytest.mark.parametrize("G", [9, 20])
+def test_many_query_heads(cuda, dtype, kind, D, G):
+    """More query heads of a KV head than an item has rows."""
+    new, keys, page = [2, 1, 3], [700, 40, 333], 16
+    p = _filled(keys, 2, D, page, dtype, kind)
+    _bound(p, keys)
+    q = _randn(_gen(G), 6, 2 * G, D, dtype=dtype)
+    blocks = _select(p, q, new, 7, 1, 2)
+    assert torch.equal(blocks.cpu(), _wanted(p, q, new, keys, 7, 1, 2))
+    _attended(p, q, blocks, new, keys, dtype)

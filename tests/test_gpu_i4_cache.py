@@ -349,3 +349,41 @@ def test_two_streams_at_once(cuda):
                 capi.attn_paged_dev(q, p.k, p.v, got[i], *p.where([1]), 1, **p.kw)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_off_their_alignment(cuda, dtype):
+    """Rows one element off and with gaps give the same codes, and are read back the same."""
+    keys, H, D = [70, 3], 2, 96
+    n = sum(keys)
+    x = _randn(_gen(1), n, 2 * H, D, dtype=dtype)
+    got = []
+    for shift in (0, 1):
+        wide = torch.empty(n * (2 * H + 1) * D + 1, dtype=dtype, device="cuda")[shift: shift + n * (2 * H + 1) * D]
+        rows = wide.view(n, 2 * H + 1, D)
+        rows[:, : 2 * H] = x
+        p = Pages(keys, H, D, 16, I4)
+        capi.kv_pages_append_dev(rows[:, :H], rows[:, H:2 * H], p.k, p.v, *p.where(keys), **p.kw)
+        back = torch.full_like(wide, 7).view(n, 2 * H + 1, D)
+        capi.kv_pages_read_dev(p.k, p.v, back[:, :H], back[:, H:2 * H], *p.where(keys), **p.kw)
+        assert (back[:, 2 * H] == 7).all()
+        got.append(p.bits() + [back[:, : 2 * H].clone()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("new", [1, 40, 200])
+def test_pages_off_16_bytes(cuda, new):
+    """Pages and factors on 4-byte boundaries only: another kernel, the same attention."""
+    keys = [400]
+    p = _filled(keys, 2, 64, 16, BF16)
+    q = _randn(_gen(3), new, 8, 64, dtype=BF16)
+
+    def moved(t):
+        return torch.empty(t.numel() + 4, dtype=t.dtype, device="cuda")[4:].view_as(t).copy_(t)
+
+    p.k, p.v = moved(p.k), moved(p.v)
+    p.kw = {name: moved(t) if t.dtype == torch.uint8 else t for name, t in p.kw.items()}
+    _against(p, q, [new], keys, BF16, new)
+    p.k = torch.empty(p.k.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(p.k)
+    with pytest.raises(capi.AttnbError, match="4-byte boundaries"):
+        _attend(p, q, [new], new)

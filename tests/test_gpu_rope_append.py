@@ -209,3 +209,40 @@ def test_captured_and_replayed(cuda):
     capi.kv_pages_append_rope_dev(k, v, p.k, p.v, *where, f, False, q, out, stream=stream)
     stream.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", [None, E4M3, I4])
+@pytest.mark.parametrize("pairs,interleaved", [(32, False), (32, True), (20, False)])
+def test_coded_rows_off_their_alignment(cuda, kind, pairs, interleaved):
+    new, keys, D, H = [40, 3], [300, 3], 64, 2
+    n = sum(new)
+    x = _randn(_gen(9), n, 4 * H, D, dtype=BF16)
+    got = []
+    for shift in (0, 1):
+        rows = torch.empty(n * 4 * H * D + 1, dtype=BF16, device="cuda")[shift: shift + n * 4 * H * D].view(n, 4 * H, D)
+        rows.copy_(x)
+        p = Pages(keys, H, D, 16, kind or BF16)
+        out = torch.empty(n, 2 * H, D, dtype=BF16, device="cuda")
+        capi.kv_pages_append_rope_dev(rows[:, :H], rows[:, H:2 * H], p.k, p.v, *p.where(new), _freq(pairs), interleaved,
+                                      rows[:, 2 * H:], out, **p.kw)
+        got.append(p.bits() + [out])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_more_tokens_than_a_cta_takes(cuda):
+    """Thousands of tokens of many sequences, some without any, and few heads."""
+    g = torch.Generator().manual_seed(1)
+    new = torch.randint(0, 90, (300,), generator=g).tolist()
+    keys = [n + int(k) for n, k in zip(new, torch.randint(0, 40, (300,), generator=g))]
+    p = Pages(keys, 1, 64, 16, BF16)
+    n = sum(new)
+    q, k, v = (_randn(_gen(i), n, 1, 64, dtype=BF16) for i in (1, 2, 3))
+    out, f = torch.empty_like(q), _freq(32)
+    capi.kv_pages_append_rope_dev(k, v, p.k, p.v, *p.where(new), f, True, q, out)
+    ref, bound = more.rotate(q, _positions(new, keys), f, True)
+    assert ((out.double().cpu() - ref).abs() <= bound).all()
+    back = [torch.empty_like(k), torch.empty_like(v)]
+    capi.kv_pages_read_dev(p.k, p.v, *back, *p.where(new))
+    ref, bound = more.rotate(k, _positions(new, keys), f, True)
+    assert ((back[0].double().cpu() - ref).abs() <= bound).all() and torch.equal(back[1], v)
+    capi.stream_status()
