@@ -568,6 +568,8 @@ __device__ __forceinline__ void pick_block(const uint64_t* keys, uint64_t* mine,
         rest = warp_eq[0];
         done = true;
         __syncthreads();
+      } else {
+        __syncthreads();  // all have read hist[p], which the digits start by clearing
       }
     }
   }
