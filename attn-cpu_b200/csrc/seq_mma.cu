@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, (MmaCfg<TK, DHP, NR>::CTAS))
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float f = kI4Rows * row_scale(top);
+        const float f = i4_row_scale(top);
 #pragma unroll
         for (int k = 0; k < KS / 2; ++k) {
           float sum = 0.f;

@@ -75,7 +75,7 @@ constexpr float kI4Unit = 0x1p19f;  // what such values are to be multiplied by
 // Against such small values queries are brought up to 2^14 (2^15 next to overflow): room
 // below for sixteenths of them, and little left of the unit for the factors of scores, which
 // stay finite for queries and keys up to 2^124.
-constexpr float kI4Rows = 0x1p13f;
+constexpr float kI4Rows = 0x1p13f;  // (i4_row_scale has the exponent too)
 struct I4Factors {
   uint32_t low, high, add;  // pairs of f16: r 2^5, r 2^1, -r 2^-16
 };
@@ -114,6 +114,15 @@ __device__ __forceinline__ float row_scale(float top) {
   const int e = (int)(__float_as_uint(top) >> 23);  // top >= 0
   if (e == 0 || e == 255) return 1.f;
   return __uint_as_float((uint32_t)max(254 - e, 1) << 23);  // [2, 4) next to overflow
+}
+
+// kI4Rows times that, for queries over 4-bit codes.  At most 2^127, so that it stays finite: rows that are
+// smaller than 2^-114 come out below 2^13, and as exactly, since bf16's values are multiples of
+// 2^-133.
+__device__ __forceinline__ float i4_row_scale(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23);
+  if (top == 0.f || e == 255) return kI4Rows;
+  return __uint_as_float((uint32_t)min(max(254 - e, 1) + 13, 254) << 23);
 }
 
 // The larger one, or NaN where one of them is.

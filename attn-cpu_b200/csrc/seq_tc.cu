@@ -816,9 +816,8 @@ __global__ void __launch_bounds__(TcCfg<elem_coded(TK), DHP>::THREADS, 1)
 #pragma unroll
             for (int b = 0; b < 8; ++b) top = fmaxf(top, fabsf(to_float(e[b])));
           }
-          f = row_scale(top);
-          scale = a.scale_log2 * (I4 ? kI4Unit / kI4Rows : 1.f) / f;
-          if (I4) f *= kI4Rows;
+          f = I4 ? i4_row_scale(top) : row_scale(top);
+          scale = I4 ? a.scale_log2 * (kI4Unit / kI4Rows) / (f / kI4Rows) : a.scale_log2 / f;
         }
 #pragma unroll 4
         for (int u = 0; u < DHP / 8; ++u) {
