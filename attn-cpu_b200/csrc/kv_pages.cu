@@ -187,6 +187,8 @@ __device__ __forceinline__ uint32_t i4_codes(const float (&x)[8], float own, flo
   if (!(own > 0.f)) return 0x88888888u;
   const float a = top * near;
   own *= near;
+  factor = 1;
+  if (own == 0.f) return 0x88888888u;  // brought below fp32's least: under 2^-146 of the largest
   int r = min(max((int)ceilf(__fdividef(own, a) * 255.f), 1), 255);
   const Wide want = (Wide)own * (Wide)255;
   if ((Wide)(r - 1) * (Wide)a >= want) --r;
