@@ -7,7 +7,8 @@
 // heads that read the KV head.  It is linear in the positive and the negative part of
 // the queries: with q- = sum over heads of min(q, 0) and q+ = sum of max(q, 0),
 //     score = q- . least + q+ . greatest,
-// one product of 2 Dh numbers for all heads.  Sums are in 64 bits: products of 16-bit or
+// one product of 2 Dh numbers for all heads.  (That holds for finite numbers; where the result is not
+// finite the score is made anew by its definition.)  Sums are in 64 bits: products of 16-bit or
 // fp32 values and their sum are then off by 2^-53 or so, and which of two blocks is
 // better does not hang on the order of a sum.
 //
@@ -242,6 +243,10 @@ __device__ __forceinline__ uint64_t sort_key(double x) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
+__device__ __forceinline__ double key_score(uint64_t k) {
+  return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k));
+}
+
 // Sums of the queries' negative and positive parts over the query heads of a KV head: q-, q+, zeros.
 // The eight lanes that read at once find their pairs side by side.
 template <int TB, int NU>
@@ -265,14 +270,35 @@ __device__ __forceinline__ void query_parts(const BlockArgs& a, int t, int h, do
   }
 }
 
-// Scores of blocks [from, to) of sequence b, at most kScoreMost, to put(block, key): eight lanes a
+// The score of a block as it is defined, from its bounds (null: zeros) and the G queries from q on.  The
+// eight lanes of a block call, and all have it.
+template <class EB>
+__device__ __noinline__ double defined_score(const EB* q, int64_t stride, int G, int Dh,
+                                             const EB* bounds) {
+  double sum = 0.0;
+  for (int d = threadIdx.x & 7; d < Dh; d += 8) {
+    const double least = bounds ? (double)to_float(bounds[d]) : 0.0;
+    const double greatest = bounds ? (double)to_float(bounds[Dh + d]) : 0.0;
+    for (int g = 0; g < G; ++g) {
+      const double x = (double)to_float(q[g * stride + d]), lo = x * least, hi = x * greatest;
+      sum += lo != lo || lo > hi ? lo : hi;  // a NaN of either one
+    }
+  }
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+  return sum;
+}
+
+// Scores of blocks [from, to) of sequence b, at most kScoreMost, to keys: eight lanes a
 // block, each with every eighth unit of 16 bytes of its bounds, two blocks in flight.  The
 // queries' sums are read from shared memory: in registers they would leave too few CTAs an SM
 // for the latency of the reads that come before the bounds (32 us for 32 sequences of
 // 8000-32768 keys).  NU: units a lane.  All threads call.
-template <int TB, int NU, class Put>
-__device__ __forceinline__ void score_blocks(const BlockArgs& a, int b, int h, int from, int to,
-                                             bool vec, const double* parts, int* pages, Put put) {
+template <int TB, int NU>
+__device__ __forceinline__ void score_blocks(const BlockArgs& a, int b, int t, int h, int from,
+                                             int to, bool vec, const double* parts, int* pages,
+                                             uint64_t* keys) {
   using EB = elem_t<TB>;
   constexpr int PER = 16 / sizeof(EB);
   const int tid = threadIdx.x, e = tid & 7, Dh = a.q.Dh;
@@ -285,6 +311,7 @@ __device__ __forceinline__ void score_blocks(const BlockArgs& a, int b, int h, i
     pages[j - from] = page;
   }
   __syncthreads();
+  bool odd = false;
   for (int j0 = from; j0 < to; j0 += kScoreRound) {
     uint4 y[2][NU];
 #pragma unroll
@@ -327,8 +354,25 @@ __device__ __forceinline__ void score_blocks(const BlockArgs& a, int b, int h, i
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
       const int j = j0 + k * (kScoreRound / 2) + (tid >> 3);
-      if (e == 0 && j < to) put(j, sort_key(s[k]));
+      odd |= !(fabs(s[k]) < INFINITY) && j < to;
+      if (e == 0 && j < to) keys[j - from] = sort_key(s[k]);
     }
+  }
+  // Where bounds or queries are infinite the products above may have had an infinity and the zero of
+  // the other sign's part: what is not finite is made anew.  (Within the loop this would cost it
+  // registers.)
+  if (!__any_sync(0xffffffffu, odd)) return;
+  __syncwarp();  // keys that a group's first lane wrote are read by all of it
+  const EB* q = static_cast<const EB*>(a.q.data) + (int64_t)(a.token0 + t) * a.q.sT +
+                (int64_t)h * a.G * a.q.sH;
+  for (int j = from + (tid >> 3); j < to; j += kScoreThreads / 8) {
+    if (fabs(key_score(keys[j - from])) < INFINITY) continue;  // the same for all eight lanes
+    const int page = pages[j - from];
+    const double score = defined_score(
+        q, a.q.sH, a.G, Dh,
+        page < 0 ? nullptr
+                 : static_cast<const EB*>(a.bounds) + ((int64_t)page * a.H + h) * 2 * Dh);
+    if (e == 0) keys[j - from] = sort_key(score);
   }
 }
 
@@ -349,16 +393,11 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : NU <= 8 ? 2 : 1)
   const int from = a.keep_first + blockIdx.x * a.chunk;
   const int to = min(own + 1 - a.keep_last, from + a.chunk);
   if (from >= to) return;
-  uint64_t* keys = a.keys + (int64_t)row * a.seqs.max_pages;
-  score_blocks<TB, NU>(a, at.b, h, from, to, vec, parts, pages,
-                       [&](int j, uint64_t key) { keys[j] = key; });
+  score_blocks<TB, NU>(a, at.b, t, h, from, to, vec, parts, pages,
+                       a.keys + (int64_t)row * a.seqs.max_pages + from);
 }
 
 // ------------------------------------------------------------------ choice
-__device__ __forceinline__ double key_score(uint64_t k) {
-  return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k));
-}
-
 // The parts of a list that need no score; how many of the n others are wanted, 0 if the list is
 // complete.  `who` of `all` threads call.
 __device__ __forceinline__ int plain_part(const BlockArgs& a, const TokenPlace& at, int row,
@@ -671,9 +710,8 @@ __global__ void __launch_bounds__(kScoreThreads, NU <= 4 ? 4 : NU <= 8 ? 2 : 1)
   if (want == 0) return;
   for (int from = 0; from < n; from += kScoreMost) {
     if (from > 0) __syncthreads();  // the pages before have been read
-    score_blocks<TB, NU>(a, at.b, h, a.keep_first + from, a.keep_first + min(n, from + kScoreMost),
-                         vec, parts, sh.pages,
-                         [&](int j, uint64_t key) { mine[j - a.keep_first] = key; });
+    score_blocks<TB, NU>(a, at.b, t, h, a.keep_first + from, a.keep_first + min(n, from + kScoreMost),
+                         vec, parts, sh.pages, mine + from);
   }
   __syncthreads();
   if (n > kWarpKeys)
