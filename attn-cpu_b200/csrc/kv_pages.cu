@@ -29,7 +29,9 @@
 // Rotation: x' = x cos t -+ y sin t with y the other one of the pair and t = position *
 // inv_freq.  The angle is reduced to a fraction of a turn in 64 bits (at
 // position 100000 an fp32 product is off by 0.004), once per token and
-// pair of a CTA for all heads; then everything is fp32.  The result is rounded to the rows'
+// pair of a CTA for all heads.  Sine and cosine are those of the fraction in fp32, turned by
+// what its rounding left over (up to 9.4e-8, as much as their own last place); then everything is
+// fp32.  The result is rounded to the rows'
 // type once and stored as that: the same numbers as rotating first and
 // appending then.
 //
@@ -230,10 +232,13 @@ __device__ __forceinline__ void turn_angles(const Rope& rope, const int64_t* pos
   for (int i = threadIdx.x; i < n * rope.pairs; i += kThreads) {
     const int t = i / rope.pairs, p = i - t * rope.pairs;
     const double turn = (double)position[t] * (double)__ldg(rope.inv_freq + p) * 0.15915494309189535;
-    const float part = (float)(turn - rint(turn));  // of a turn, at most a half
-    float2 cs;
-    sincospif(2.f * part, &cs.y, &cs.x);
-    turns[i] = cs;
+    const double rest = turn - rint(turn);  // of a turn, at most a half
+    const float part = (float)rest;
+    float s, c;
+    sincospif(2.f * part, &s, &c);
+    // What part is off by, up to 2^-26 of a turn, turns the two by a small angle.
+    const float small = (float)(rest - (double)part) * 6.28318531f;
+    turns[i] = make_float2(fmaf(-s, small, c), fmaf(c, small, s));
   }
 }
 
