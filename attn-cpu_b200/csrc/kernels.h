@@ -308,6 +308,7 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
                           int num_sms, cudaStream_t s);
 // The kernels (K6: any type, stride and head size up to 256).
 void seq_simt_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);
+void seq_simt_blocks_launch(const SeqAttnArgs& a, int ctas, cudaStream_t s);  // of a.sel_blocks
 // K7: 16-bit queries over 16-bit or coded pages, 8 or 16 rows per item.
 bool seq_mma_supported(const SeqAttnArgs& a);
 // log2 of the keys of a tile.

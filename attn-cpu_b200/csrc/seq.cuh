@@ -270,8 +270,8 @@ __device__ __forceinline__ SelRow sel_row(const SeqAttnArgs& a, int v) {
 }
 
 // All threads of the block; false when the CTA has nothing to do.  SEL here and below: in a
-// kernel that selected blocks may come to (K7 has two forms: their code costs steps over all
-// keys 5 us of 61).
+// kernel that selected blocks may come to (K6 and K7 have two forms: their code costs steps over
+// all keys 5 us of 61).
 template <bool SEL = false>
 __device__ inline bool seq_locate(const SeqAttnArgs& a, SeqShared& sh, SeqPlace& p) {
   if (SEL && a.sel_blocks) {
