@@ -727,6 +727,7 @@ size_t keys_per_token(int H, int max_pages) { return (size_t)H * std::max(max_pa
 void kv_blocks_bounds_launch(const KvPages& pg, void* bounds, int bounds_type, const SeqTable& sq,
                              int* index_status, int num_sms, cudaStream_t s) {
   const bool vec = pg.Dh % 8 == 0 && reinterpret_cast<uintptr_t>(pg.k) % (4 * elem_bytes(pg.type)) == 0;
+  ProfScope prof("kv_blocks", s);
   auto go = [&](auto tc, auto tb) {
     ATTNB_CUDA(launch_pdl(bounds_kernel<decltype(tc)::value, decltype(tb)::value>,
                           dim3(2 * num_sms), dim3(kBoundsThreads), 0, s, pg, bounds, sq, vec,
@@ -769,6 +770,7 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
   if (fit == 0) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
   const int eb = elem_bytes(q.type);
   const bool vec = reinterpret_cast<uintptr_t>(bounds) % 16 == 0 && 2 * q.Dh * eb % 16 == 0;
+  ProfScope prof("kv_blocks", s);
   for (a.token0 = 0; a.token0 < sq.total; a.token0 += a.tokens) {
     a.tokens = (int)std::min<size_t>(fit, sq.total - a.token0);
     const int rows = a.tokens * H;
