@@ -863,6 +863,11 @@ class PagedKVCacheDev:
                 raise ValueError("bounds of uncoded pages have their type")
             if bounds not in (torch.float32, torch.bfloat16, torch.float16):
                 raise ValueError("bounds must be float32, bfloat16 or float16")
+        most = num_pages * page_size if max_tokens is None else max_tokens
+        width = max(1, -(-most // page_size))
+        # (as kv_blocks_bounds_dev would, but behind an append that has run)
+        if bounds and (width * page_size >= 1 << 30 or batch * width >= 1 << 31):
+            raise ValueError("bounds need max_tokens below 2^30, and fewer than 2^31 pages in the table")
         wide = Dh // 2 if dtype == torch.uint8 else Dh
         self.k_pages, self.v_pages = (torch.empty(num_pages, H, page_size, wide, dtype=dtype,
                                                   device=device) for _ in range(2))
@@ -877,8 +882,6 @@ class PagedKVCacheDev:
         if bounds:
             kind = (torch.bfloat16 if coded else dtype) if bounds is True else bounds
             self.bounds = torch.empty(num_pages, H, 2, Dh, dtype=kind, device=device)
-        most = num_pages * page_size if max_tokens is None else max_tokens
-        width = max(1, -(-most // page_size))
         self._free = list(range(num_pages - 1, -1, -1))
         self._held = [[] for _ in range(batch)]
         self.lengths = [0] * batch
