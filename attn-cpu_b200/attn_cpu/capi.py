@@ -765,7 +765,7 @@ def _blocks_bytes(index, tokens, q_heads, kv_heads, Dh, take, max_pages) -> int:
 
 
 def _blocks_workspace(device, tokens, q_heads, kv_heads, Dh, take, max_pages):
-    """As _workspace, for the selection of blocks and attention to them."""
+    """As _workspace, for the selection of blocks."""
     n = _blocks_bytes(device.index, tokens, q_heads, kv_heads, Dh, take, max_pages)
     return _torch.empty(n, dtype=_torch.uint8, device=device), n
 
@@ -825,7 +825,7 @@ def attn_blocks_dev(Q, k_pages, v_pages, O, blocks, cu, table, lens, scale=None,
     pg = _pages(k_pages, v_pages, k_scale, v_scale, dev, k_group, v_group)
     sq = _seqs(cu, table, lens, dev)
     at, take = _lists(blocks, q.tokens, pg.H, dev), blocks.shape[2]
-    ws, size = _blocks_workspace(dev, q.tokens, q.heads, pg.H, q.Dh, take, sq.max_pages)
+    ws, size = _workspace(dev, q.heads, pg.H, q.Dh)  # no scores here
     check(_lib.attnb_attn_blocks_dev(q, pg, o, sq, at, take, _scale(scale), ws.data_ptr(), size,
                                      _raw_stream(dev.index)))
 
