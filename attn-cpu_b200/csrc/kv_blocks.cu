@@ -742,6 +742,7 @@ void kv_blocks_bounds_launch(const KvPages& pg, void* bounds, int bounds_type, c
 }
 
 size_t kv_blocks_workspace_bytes(int tokens, int H, int max_pages) {
+  if (max_pages <= kWarpKeys) return 256;  // keys in shared memory, however many rows there are
   const size_t each = keys_per_token(H, max_pages);
   return std::min<size_t>(each * std::max(tokens, 1), std::max(each, kScoreBytes)) + 256;
 }
@@ -766,7 +767,9 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
   const uintptr_t p = (reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255;
   a.keys = reinterpret_cast<uint64_t*>(p);
   const size_t room = reinterpret_cast<uintptr_t>(ws) + ws_bytes - std::min(p, reinterpret_cast<uintptr_t>(ws) + ws_bytes);
-  const size_t fit = std::min<size_t>(room / keys_per_token(H, sq.max_pages), 65535 / H);
+  const bool in_shared = sq.max_pages <= kWarpKeys;
+  const size_t held = in_shared ? SIZE_MAX : room / keys_per_token(H, sq.max_pages);  // tokens
+  const size_t fit = std::min<size_t>(held, 65535 / H);
   if (fit == 0) fail(ATTNB_ERR_INVALID_ARGUMENT, "workspace too small");
   const int eb = elem_bytes(q.type);
   const bool vec = reinterpret_cast<uintptr_t>(bounds) % 16 == 0 && 2 * q.Dh * eb % 16 == 0;
@@ -786,7 +789,7 @@ void kv_blocks_select_run(const RowsView& q, const void* bounds, int num_pages, 
     // One CTA a row where rows are short, or so many that they fill the machine; else the
     // blocks of a row are spread over several.  (256 rows of 125-512 blocks 22 us against 25,
     // 1064 rows of 80-310 28 against 41; 4 rows of 4096 88 against 16.)
-    if (sq.max_pages <= kWarpKeys || (rows >= 2 * num_sms && sq.max_pages <= kPickKeys)) {
+    if (in_shared || (rows >= 2 * num_sms && sq.max_pages <= kPickKeys)) {
       with_units([&](auto tb, auto nu) {
         ATTNB_CUDA(launch_pdl(select_kernel<decltype(tb)::value, decltype(nu)::value>, dim3(rows),
                               dim3(kScoreThreads), (size_t)sq.max_pages * 8, s, a, vec));

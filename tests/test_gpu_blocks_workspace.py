@@ -1,11 +1,13 @@
-"""Memory that attention over lists takes besides its arguments."""
+"""Memory that the choice of blocks and attention over lists take besides their arguments."""
 from __future__ import annotations
 
-import torch
+import ctypes
+
 import pytest
+import torch
 
 from attn_cpu import capi
-from test_gpu_blocks import _filled
+from test_gpu_blocks import _bound, _filled, _select, _wanted
 from test_gpu_seq_ops import BF16, F32, _gen, _randn
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +36,19 @@ def test_no_more_than_attention_to_all_keys(cuda, dtype, D):
 
     all_keys = peak(lambda: capi.attn_paged_dev(q, p.k, p.v, o, *where))
     assert peak(lambda: capi.attn_blocks_dev(q, p.k, p.v, o, blocks, *where)) <= all_keys
+
+
+@pytest.mark.parametrize("width", [100, 512])
+def test_choice_from_short_tables_holds_no_scores(cuda, width):
+    """Rows of up to 512 blocks have their scores in shared memory: what attention takes is enough for both calls."""
+    new, H, take = 200, 4, 6
+    keys = [16 * width]
+    p = _filled(keys, H, 64, 16, BF16, BF16)
+    _bound(p, keys)
+    q = _randn(_gen(1), new, H, 64, dtype=BF16)
+    both, attention = ctypes.c_size_t(), ctypes.c_size_t()
+    capi.check(capi.lib().attnb_blocks_workspace(new * 1000, H, H, 64, take, width, ctypes.byref(both)))
+    capi.check(capi.lib().attnb_seq_workspace(H, H, 64, ctypes.byref(attention)))
+    assert both.value == attention.value
+    blocks = _select(p, q, [new], take, 1, 2)
+    assert torch.equal(blocks.cpu(), _wanted(p, q, [new], keys, take, 1, 2))
