@@ -2,7 +2,8 @@
 //
 // A block is one page of a sequence.  Its bounds are the least and the greatest
 // value of its keys in each dimension, so that for a query q
-//     q . k <= sum_d max(q_d least_d, q_d greatest_d)     for every key k of the block.
+//     q . k <= sum_d max(q_d least_d, q_d greatest_d)     for every key k of the block
+// (the bounds of coded pages are rounded to nearest, and the sum may be below by as much).
 // The score of a block for a token and a KV head is that bound summed over the query
 // heads that read the KV head.  It is linear in the positive and the negative part of
 // the queries: with q- = sum over heads of min(q, 0) and q+ = sum of max(q, 0),

@@ -395,7 +395,7 @@ typedef struct attnb_seqs {
   const int32_t* lens;
 } attnb_seqs;
 
-/* Bytes of device workspace for the two attention calls below, enough for any
+/* Bytes of device workspace for the attention calls below, enough for any
  * number of sequences and tokens with these head counts on the current device.
  * Calls that may run at the same time need workspaces of their own. */
 ATTNB_API int attnb_seq_workspace(int q_heads, int kv_heads, int Dh, size_t* bytes);
@@ -434,10 +434,10 @@ typedef struct attnb_rope {
 
 /* attnb_kv_pages_append_dev with K rotated by its tokens' positions in their
  * sequences on the way, and the rows Q (K's type, tokens and Dh, any number of
- * heads) rotated into QO, which may be Q itself, with the same strides.  Q and QO
- * may be NULL.  A rotated vector is rounded to the rows' type and stored as that.  Q's
- * rows are written for every token of a sequence, also where a page number is out of
- * range; rows of no sequence stay. */
+ * heads) rotated into QO, which may be Q itself, with the same strides, and shares
+ * no other memory with the call's rows.  Q and QO may be NULL.  A rotated vector is
+ * rounded to the rows' type and stored as that.  Q's rows are written for every token
+ * of a sequence, also where a page number is out of range; rows of no sequence stay. */
 ATTNB_API int attnb_kv_pages_append_rope_dev(const attnb_rows* Q, const attnb_rows* QO,
                                              const attnb_rows* K, const attnb_rows* V,
                                              const attnb_kv_pages* pages, const attnb_seqs* seqs,
@@ -450,8 +450,9 @@ ATTNB_API int attnb_kv_pages_read_dev(const attnb_kv_pages* pages, const attnb_r
 /* Attention of the packed rows (new tokens, one and up per sequence) over the
  * lens[b] tokens that the pages hold, their own among them (append first);
  * otherwise as attnb_attn_packed_dev.  Q and O have one type; the pages have
- * that type or are E4M3, I8 or I4 (16-bit queries over I4: queries and keys below 2^124).  max_new: the most rows of one sequence, as far
- * as the caller knows (0: unknown); it steers the choice of kernel only. */
+ * that type or are E4M3, I8 or I4 (16-bit queries over I4: queries and keys below
+ * 2^124).  max_new: the most rows of one sequence, as far as the caller knows (0:
+ * unknown); it steers the choice of kernel only. */
 ATTNB_API int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pages,
                                    const attnb_rows* O, const attnb_seqs* seqs, int max_new,
                                    int causal, float scale, void* workspace,
@@ -460,7 +461,8 @@ ATTNB_API int attnb_attn_paged_dev(const attnb_rows* Q, const attnb_kv_pages* pa
 /* Attention to selected blocks of a long context.  A block is one page of a
  * sequence: block j holds tokens j * page_size to (j + 1) * page_size - 1.  Its
  * bounds are the least and the greatest value of its keys in each dimension,
- * rounded to `type` (F32, BF16 or F16): data is [num_pages, H, 2, Dh], dense. */
+ * rounded to `type` (F32, BF16 or F16) to nearest: data is [num_pages, H, 2, Dh],
+ * dense.  F16 bounds of coded pages are infinite past 65504. */
 typedef struct attnb_bounds {
   void* data;
   int type;
@@ -473,8 +475,9 @@ typedef struct attnb_bounds {
 ATTNB_API int attnb_kv_blocks_bounds_dev(const attnb_kv_pages* pages, const attnb_bounds* bounds,
                                          const attnb_seqs* seqs, void* stream);
 
-/* Bytes of device workspace for the two calls below with these sizes on the current
- * device (as with attnb_seq_workspace, one for each call in flight). */
+/* Bytes of device workspace for either of the two calls below with these sizes on the
+ * current device (as with attnb_seq_workspace, one for each call in flight).  For
+ * the second what attnb_seq_workspace gives is enough. */
 ATTNB_API int attnb_blocks_workspace(int tokens, int q_heads, int kv_heads, int Dh, int take,
                                      int max_pages, size_t* bytes);
 
@@ -484,8 +487,9 @@ ATTNB_API int attnb_blocks_workspace(int tokens, int q_heads, int kv_heads, int 
  * else the first keep_first, the last keep_last (1 at least, its own among them)
  * and, of the others, those with the greatest scores, the lower one of equal ones.
  * The score is the sum over the query heads that read the KV head, and over the
- * dimensions, of max(q least, q greatest): an upper bound of the sum of q . k for
- * every key of the block.  Sums are in 64 bits; NaN is the greatest.  Q has the
+ * dimensions, of max(q least, q greatest), NaN where one of the two is: an upper bound
+ * of the sum of q . k for every key of the block, for coded pages but for the rounding
+ * of their bounds.  Sums are in 64 bits; NaN is the greatest.  Q has the
  * bounds' type.  The pages are [num_pages, H, page_size, Dh]; rows of no
  * sequence stay as they are. */
 ATTNB_API int attnb_kv_blocks_select_dev(const attnb_rows* Q, const attnb_bounds* bounds,
